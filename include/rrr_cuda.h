@@ -384,6 +384,94 @@ int rrr_position_advance(rrr_ctx* ctx, int* d_pos, int delta, void* stream);
 int rrr_embed_rows(rrr_ctx* ctx, int ggml_type, const void* table, int64_t n_rows, int d,
                    const int32_t* tokens, int n_tokens, float* out, void* stream);
 
+/* ---- packed rows of a batch of sequences, and a 4-bit KV cache ----------------------
+ * The reference serves one sequence over f16 caches (phi4.rs:1284-1309, 1656-1690); these
+ * operators serve a batch. Rows of several sequences lie one after another ("packed"): a
+ * device array cu of n_seqs + 1 ascending int32 gives sequence s the rows cu[s] ..
+ * cu[s+1]-1; rows from cu[n_seqs] on belong to none and are left as they were. Lengths,
+ * positions and page numbers are read on the device when the kernel runs, so a captured
+ * graph replays with others. Values outside their range are recorded in the device error
+ * flag (code 6) and nothing is read or written for them. Element types are GGML type ids;
+ * strides count elements; the values of a head are contiguous. */
+enum { RRR_F32 = 0, RRR_F16 = 1, RRR_BF16 = 30 };
+
+/* QKV rows [Q heads | K heads | V heads] -> rows of q, k and v in out_type: each query and
+ * key head is normed (x * gamma / sqrt(mean(x^2) + eps), gamma f32[head_dim]; NULL: not
+ * normed) and its first a->rope_dim values are rotated for the row's position (device
+ * int32[rows], 0 <= position < a->max_seq; a row outside is left as it was), in one pass,
+ * rounded once. Frequencies as in apply_rope_cfg (phi4.rs:238-256), but the angle is not
+ * rounded to 32 bits before its sine (exact to 2^-24 turns at any position). halves = 0
+ * rotates the pairs (2i, 2i+1) as rrr_rope_kv_store does, 1 the pairs (i, i + rope_dim/2)
+ * (rope_dim then a multiple of head_dim/16). V is copied; v = NULL leaves it out. q, k, v
+ * may lie in their own place in qkv (same type and stride), and overlap nothing else. */
+int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_type, const void* qkv,
+                     int64_t row_stride, int rows, const int32_t* positions, const float* q_gamma,
+                     const float* k_gamma, float eps, int halves, int out_type, void* q,
+                     int64_t q_stride, void* k, int64_t k_stride, void* v, int64_t v_stride,
+                     void* stream);
+
+/* A KV cache in 4 bits: pages of 64 rows, each page one block of 80*head_dim bytes per KV
+ * head. Every 32 consecutive values of a head are held as d*code + m, code 0..15, with d and
+ * m in f16: m = f16(min), d = f16((max - min) / 15), code = round((x - m) / d) (f32, ties to
+ * even) within 0..15, 0 when d = 0; a min beyond f16's range is held at its end, and a group
+ * with an infinity or a NaN reads back as NaN. 5 bits a value. Row p of sequence s is row
+ * p % 64 of page page_table[s * table_stride + p / 64]; pages may be shared by sequences that
+ * only read them. A block is [K codes 32*hd | K d 4*hd | K m 4*hd | V codes 32*hd | V d 4*hd
+ * | V m 4*hd] bytes; with J = min(hd/32, 4), plane P, group j = P*J + i:
+ *   K codes  u32 [P][row][t 4][i J]: nibble n = element 32j + 8t + n
+ *   V codes  u32 [P][row/16][(row%16)/8][g 8][t 4][i J], t = (row%8)/2: low half the even
+ *            row, high half the odd row; nibble n of a half = element 32j + 8n + g
+ *   K d, K m, V d  f16 [row][hd/32];  V m  f16 [row/2][hd/32][row%2]
+ * (the order in which the tensor-core fragments of rrr_attention_kv4 read them). */
+typedef struct rrr_kv4_cache {
+  void* pages;               /* device, n_pages * n_kv_heads * 80 * head_dim bytes, 16-byte aligned */
+  int64_t n_pages;
+  int n_kv_heads, head_dim;  /* head_dim 64/128/256 */
+  const int32_t* page_table; /* device int32 [n_seqs][table_stride] */
+  int n_seqs, max_pages;     /* max_pages: pages a sequence can have (<= table_stride) */
+  int64_t table_stride;
+} rrr_kv4_cache;
+/* Stores packed rows of K and V (n_kv_heads*head_dim values each, `type`): sequence s has
+ * kv_lens[s] rows once they are stored, and its packed rows are its last ones. Rows of the
+ * pages that are not stored keep their values. */
+int rrr_kv4_store(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, const void* k, int64_t k_stride,
+                  const void* v, int64_t v_stride, int rows, const int32_t* cu_rows,
+                  const int32_t* kv_lens, void* stream);
+/* The reverse: the last rows of every sequence, as the values they stand for, into packed
+ * rows (the prefix of a continued prompt for rrr_attention_packed). k or v may be NULL. */
+int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_t k_stride, void* v,
+                 int64_t v_stride, int rows, const int32_t* cu_rows, const int32_t* kv_lens,
+                 void* stream);
+/* Attention of one query row per sequence over its kv_lens[s] cached rows: out[s][h] = sum_p
+ * softmax_p(scale * q[s][h] . k[p][g]) v[p][g], g = h / (n_heads / n_kv_heads), at most 8
+ * query heads per KV head; scale 0 = 1/sqrt(head_dim). q, out: rows of n_heads*head_dim values
+ * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros. Scores and sums
+ * carry 32-bit accuracy whatever the type. workspace: rrr_kv4_workspace bytes of device
+ * memory, zeroed once before its first use (the kernel leaves its counters zero); calls
+ * that can run at the same time, replays of captured graphs among them, need one each. */
+int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t* bytes);
+int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int type, const void* q,
+                      int64_t q_stride, const int32_t* kv_lens, float scale, void* out,
+                      int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of packed prompts with grouped heads: query row i of sequence s over the
+ * sequence's KV rows, out_i = sum_j softmax_j(scale * q_i . k_j) v_j. causal: row i of Lq sees
+ * the rows j <= i + Lk - Lq (the queries are the last of the Lk rows), so without a prefix
+ * Lk = Lq and cu_kv = cu_q; a row that sees nothing gives zeros. 16-bit types; scores and
+ * softmax statistics in 32 bits, the weights rounded to the type for the second product.
+ * Pointers 16-byte aligned; strides multiples of 8 elements. out overlaps no input. */
+typedef struct rrr_packed_desc {
+  int type;                           /* RRR_F16 or RRR_BF16: q, k, v and out */
+  int n_heads, n_kv_heads, head_dim;  /* head_dim 64/128/256 */
+  int n_seqs, causal;
+  float scale;                        /* 0 = 1/sqrt(head_dim) */
+  int64_t q_rows, kv_rows;            /* rows of q and out, of k and v */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head; /* strides */
+} rrr_packed_desc;
+int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, const void* q, const void* k,
+                         const void* v, const int32_t* cu_q, const int32_t* cu_kv, void* out,
+                         void* stream);
+
 /* ---- Phi-4-mini-shape decode step (replaces forward_gpu, phi4.rs:1099-1196) --------
  * max_seq == 0: one token at position 0 (attention output = V, see RRR_X_GQA_V): per layer
  *   h += Wo . expand(V(Wqkv . rms(h)*g_attn)); h += Wdown . (silu(g) * u),

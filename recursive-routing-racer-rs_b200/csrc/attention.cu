@@ -726,9 +726,7 @@ cudaError_t launch_pos_advance(const LaunchEnv& env, int* d_pos, int delta) {
 
 using namespace rrr;
 
-namespace {
-
-int check_attn_desc(rrr_ctx* ctx, const rrr_attn_desc* a, const char* fn) {
+int rrr::check_attn_desc(rrr_ctx* ctx, const rrr_attn_desc* a, const char* fn) {
   if (!a) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null descriptor", fn);
   if (a->n_heads < 1 || a->n_kv_heads < 1 || a->n_heads % a->n_kv_heads ||
       a->n_heads / a->n_kv_heads > kMaxHpk ||
@@ -741,6 +739,8 @@ int check_attn_desc(rrr_ctx* ctx, const rrr_attn_desc* a, const char* fn) {
                      fn);
   return RRR_OK;
 }
+
+namespace {
 
 int check_rows(rrr_ctx* ctx, const rrr_attn_desc* a, int rows, int pos0, const int* d_pos,
                const char* fn) {

@@ -50,4 +50,6 @@ rrr_comm* tp_comm_p2p_of(rrr_tp_comm* c);
 // with N = F).
 int check_gemv(rrr_ctx* ctx, int qtype, const void* w, const float* x, float* y, int K, int N,
                const float* residual, const rrr_gemv_prologue* pro, bool swiglu);
+// Argument rules of an rrr_attn_desc (heads, head_dim, rope_dim, max_seq).
+int check_attn_desc(rrr_ctx* ctx, const rrr_attn_desc* a, const char* fn);
 }  // namespace rrr

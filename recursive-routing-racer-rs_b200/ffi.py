@@ -21,6 +21,7 @@ STATUS = {
     -8: "RRR_ERR_OOM", -9: "RRR_ERR_UNSUPPORTED", -10: "RRR_ERR_IO", -11: "RRR_ERR_BUFFER_TOO_SMALL",
 }
 Q4_K, Q5_K, Q6_K = 12, 13, 14
+F32, F16, BF16 = 0, 1, 30  # GGML type ids of the packed rows
 X_PLAIN, X_RMSNORM, X_SILU_GATE, X_GQA_V = 0, 1, 2, 3
 
 
@@ -70,6 +71,21 @@ class AttnDesc(ctypes.Structure):
     _fields_ = [("n_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("rope_dim", c_int),
                 ("rope_theta", c_float), ("rope_attn_factor", c_float), ("rope_factors", c_void_p),
                 ("n_rope_factors", c_int), ("max_seq", c_int)]
+
+
+class PackedDesc(ctypes.Structure):
+    """rrr_packed_desc: attention of packed prompts."""
+    _fields_ = [("type", c_int), ("n_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int),
+                ("n_seqs", c_int), ("causal", c_int), ("scale", c_float), ("q_rows", c_int64),
+                ("kv_rows", c_int64), ("q_row", c_int64), ("q_head", c_int64), ("k_row", c_int64),
+                ("k_head", c_int64), ("v_row", c_int64), ("v_head", c_int64), ("out_row", c_int64),
+                ("out_head", c_int64)]
+
+
+class KV4Desc(ctypes.Structure):
+    """rrr_kv4_cache: pages of the 4-bit KV cache."""
+    _fields_ = [("pages", c_void_p), ("n_pages", c_int64), ("n_kv_heads", c_int), ("head_dim", c_int),
+                ("page_table", c_void_p), ("n_seqs", c_int), ("max_pages", c_int), ("table_stride", c_int64)]
 
 
 vp = c_void_p
@@ -155,6 +171,14 @@ PROTOS = {
     "rrr_rope_kv_store": (c_int, [vp, POINTER(AttnDesc), vp, c_int64, c_int, c_int, vp, vp, vp, vp]),
     "rrr_attention_f16kv": (c_int, [vp, POINTER(AttnDesc), vp, c_int64, c_int, c_int, vp, vp, vp, vp, vp]),
     "rrr_rope_attention_f16kv": (c_int, [vp, POINTER(AttnDesc), vp, c_int, vp, vp, vp, vp, vp]),
+    "rrr_qk_norm_rope": (c_int, [vp, POINTER(AttnDesc), c_int, vp, c_int64, c_int, vp, vp, vp, c_float, c_int,
+                                 c_int, vp, c_int64, vp, c_int64, vp, c_int64, vp]),
+    "rrr_kv4_store": (c_int, [vp, POINTER(KV4Desc), c_int, vp, c_int64, vp, c_int64, c_int, vp, vp, vp]),
+    "rrr_kv4_load": (c_int, [vp, POINTER(KV4Desc), c_int, vp, c_int64, vp, c_int64, c_int, vp, vp, vp]),
+    "rrr_kv4_workspace": (c_int, [vp, POINTER(KV4Desc), c_int, POINTER(c_int64)]),
+    "rrr_attention_kv4": (c_int, [vp, POINTER(KV4Desc), c_int, c_int, vp, c_int64, vp, c_float, vp, c_int64,
+                                  vp, c_int64, vp]),
+    "rrr_attention_packed": (c_int, [vp, POINTER(PackedDesc), vp, vp, vp, vp, vp, vp, vp]),
     "rrr_embed_rows": (c_int, [vp, c_int, vp, c_int64, c_int, vp, c_int, vp, vp]),
     "rrr_fill_kquant_random": (c_int, [vp, c_int, vp, c_int64, c_uint64, vp]),
     "rrr_fill_f32_normal": (c_int, [vp, vp, c_int64, c_float, c_float, c_uint64, vp]),
