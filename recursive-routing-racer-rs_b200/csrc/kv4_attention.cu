@@ -3,16 +3,21 @@
 // for a batch of sequences of different lengths on pages.
 //
 // Mathematics. A key is k = d_j code + m_j in groups j of 32 values, so q . k = sum_j d_j (q_j .
-// code_j) + m_j (sum q_j): the products with the codes run on mma.m16n8k16 (f16 in, f32
-// accumulate) with the codes themselves as the B operand, and d_j multiplies each group's
-// accumulator in f32. A 4-bit code in the low bits of an f16 is the subnormal code * 2^-24 (four
-// bits further up, code * 2^-20), so one AND makes two operands out of a word and the powers of
-// two leave with the scales. The A operand has 16 rows for at most 8 query heads: rows 0-7 hold
-// the f16 part hi of the (power-of-two scaled) query, rows 8-15 the remainder (q - hi) * 2^11, so
-// a score carries 22 bits of the query at no further instruction. The second product is alike: A
-// holds p_i d_ij (one rescaled row set per group j, split hi and lo), B the V codes, and one
-// more product of p itself with the m_ij. The softmax runs online in base 2, with 32-bit maxima and
-// sums; scores, weights and sums keep f32 accuracy throughout.
+// (code_j - 7.5)) + (m_j + 7.5 d_j) (sum q_j). The products with the codes run on mma.m16n8k16
+// (f16 in, f32 accumulate): 16 rows of codes are the A operand, and the B operand's eight columns
+// are four query heads as (hi, lo) pairs: the f16 part of the (power-of-two scaled) query and
+// the remainder (q - hi) * 2^11, so a score carries 22 bits of the query. A code shifted into the
+// top of an f16's mantissa is 1 + code / 16 (a shift and an AND-OR for two operands); the
+// accumulators start at -(1 + 7.5 / 16) sum q_j, the power of two leaves with the scales and d_j
+// multiplies them in f32. (The code in the low bits would be the subnormal code * 2^-24 for fewer
+// instructions, but the tensor core aligns a subnormal's products as if they were normal: they
+// lost 6 bits, an error of 1e-6 in the scores.) The second product is alike: A holds
+// V's codes, B the weights p_i d_ij of group j as (hi, lo), and one more product of p itself takes
+// the m_ij + 7.5 d_ij. V's codes are centred, code - 7.5: over a long context the weighted values
+// nearly cancel, and sums of the codes themselves would be hundreds of times the result (measured:
+// an error of 1.2e-3 at 131,000 rows). The tensor core truncates its sums, so they are moved to
+// shared memory, rounded, every kFlush pages. The softmax runs online in base 2, with 32-bit maxima
+// and sums; scores, weights and sums keep f32 accuracy throughout.
 //
 // Work. A unit is one page (64 rows) of one (sequence, KV head). The CTAs share all units of the
 // batch evenly, in order, whatever the lengths are (read on the device): CTA c of G takes the
@@ -34,6 +39,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxStages = 16;
 constexpr int kMaxHpk = 8;
 constexpr float kLo = 1.f / 2048.f;
+constexpr int kFlush = 16;  // pages whose products one set of accumulators takes
 
 struct Kv4Params {
   const uint8_t* pages;
@@ -59,8 +65,10 @@ struct Segment {  // beside each stage
   int first_page;  // of this CTA's segment
 };
 
-template <int HD>
-constexpr int ctas_per_sm() { return HD == 256 ? 1 : 2; }
+// CTAs of an SM by what its registers hold: HD/4 accumulators and HD/8 of the query per column tile
+// (NT = 1: up to four query heads per KV head, 2: up to eight).
+template <int HD, int NT>
+constexpr int ctas_per_sm() { return HD * NT >= 512 ? 1 : HD * NT >= 256 ? 2 : 3; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -83,7 +91,21 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ float half_of(uint32_t w, int i) {
-  return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xffffu)));
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return i ? __high2float(h) : __low2float(h);
+}
+
+// 1 + code / 16 of the four bits at 6..9 of both halves of w
+__device__ __forceinline__ uint32_t from_one(uint32_t w) { return (w & 0x03C003C0u) | 0x3C003C00u; }
+// 16 (code - 7.5) of the four bits at 4..7 of both halves of w: 1024 + 16 code - 1144, exact
+__device__ __forceinline__ uint32_t centred(uint32_t w) {
+  const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0xe478)));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+// The f16 pair (m + 7.5 d) of a pair of rows, as hi and lo
+__device__ __forceinline__ void middle(uint32_t d, uint32_t m, uint32_t& hi, uint32_t& lo) {
+  split2(fmaf(7.5f, half_of(d, 0), half_of(m, 0)), fmaf(7.5f, half_of(d, 1), half_of(m, 1)), hi, lo);
 }
 
 // N words at p (N a power of two; p aligned to min(16, 4 N))
@@ -121,19 +143,20 @@ struct ConsumerSync {
   }
 };
 
-template <int HD, typename T>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
   using B = Kv4Block<HD>;
   constexpr int G = B::kGroups, J = B::kJ;
+  constexpr int PITCH = HD + 8;  // floats between the heads of a warp's sums
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], cons_bar;
   __shared__ Segment seg[kMaxStages];
   __shared__ float wm[kConsumers][kMaxHpk], wl[kConsumers][kMaxHpk];
-  __shared__ long long prefix[kThreads];
+  __shared__ long long warp_units[kConsumers + 1];
   __shared__ long long first_base;  // unit of the first sequence's first page
   __shared__ int first_seq, is_last;
-  float* wo = reinterpret_cast<float*>(smem + (size_t)p.stages * p.stage_bytes);  // [warp][hpk][HD]
+  float* wo = reinterpret_cast<float*>(smem + (size_t)p.stages * p.stage_bytes);  // [warp][hpk][PITCH]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -161,12 +184,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
   const int my0 = min(p.n_seqs, (int)threadIdx.x * per), my1 = min(p.n_seqs, my0 + per);
   long long mine = 0;
   for (int s = my0; s < my1; ++s) mine += (long long)pages_of(seq_len(s)) * p.nkv;
-  prefix[threadIdx.x] = mine;
+  long long upto = mine;  // units of this warp's threads up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_units[warp] = upto;
   __syncthreads();
-  long long before = 0, U = 0;
-  for (int i = 0; i < kThreads; ++i) {
-    if (i == (int)threadIdx.x) before = U;
-    U += prefix[i];
+  long long before = upto - mine, U = 0;
+#pragma unroll
+  for (int w = 0; w <= kConsumers; ++w) {
+    if (w < warp) before += warp_units[w];
+    U += warp_units[w];
   }
   const long long grid = U < (long long)gridDim.x ? U : (long long)gridDim.x;  // CTAs with units
   if ((long long)blockIdx.x >= grid) return;
@@ -246,14 +276,56 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
     return;
   }
 
-  // ---------------- consumers
+  // ---------------- consumers: warp w takes rows 16w .. 16w + 15 of every page
+  // Fragments of lane (g, t): A rows g and g + 8, k slots 2t, + 1 and 2t + 8, + 9; B the same
+  // slots of column g, that is of head g / 2's hi (g even) or lo part; C rows g, g + 8 of columns
+  // 2t, 2t + 1, that is of head t. Tile n holds the heads 4n .. 4n + 3.
   const int g = lane >> 2, t = lane & 3;
+  const bool odd = g & 1;
   ConsumerSync sync{&cons_bar, 0, p.err};
-  uint32_t qa[G][8], qm[4];  // A fragments: two k steps per group; the groups' sums
-  float kscale = 0.f;
-  float m = -INFINITY, l = 0.f;
-  float o[4 * G][4], om[4];
+  uint32_t qb[NT][G][4];                       // B: two k steps per group
+  float qh[NT][G], ql[NT][G], qs[NT][G];       // head t: -(1 + 7.5 / 16) times the sums of hi and lo; sums of q
+  float kscale[NT], m[NT], l[NT], m_held[NT];  // head t; m_held: of what shared memory holds
+  float o[NT][2 * G][4], om[NT][4];            // values: [16 u + (g, g + 8)] of group j; middles
+  bool held = false;
+  int since = 0;
   int it = 0;
+
+  // adds this warp's accumulators to its sums in shared memory, and clears them
+  auto flush = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m_use = m[n] == -INFINITY ? 0.f : m[n];
+      const float keep = ex2(m_held[n] - m_use);
+      const int h = 4 * n + t;
+      // group g's middles: row g holds the hi, row g + 8 the lo parts
+      const float mine_m = fmaf(om[n][1] + om[n][2], kLo, om[n][0]);
+      float* dst = wo + ((size_t)warp * p.hpk + h) * PITCH;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const float mid = __shfl_sync(0xffffffffu, mine_m, 4 * j + t);
+        if (h < p.hpk) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float* c = o[n][2 * j + u] + 2 * r;
+              float* d = dst + 32 * j + 16 * u + 8 * r + g;
+              const float v = fmaf(fmaf(c[1], kLo, c[0]), 0.0625f, mid);
+              *d = held ? fmaf(*d, keep, v) : v;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][2 * j][i] = o[n][2 * j + 1][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) om[n][i] = 0.f;
+      m_held[n] = m[n];
+    }
+    held = true;
+    since = 0;
+  };
+
   for (long long u = u0; u < u1; ++u, ++it) {
     const int st = it % p.stages;
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[st], (uint32_t)(it / p.stages) & 1u, p.err, kDevErrFullTimeout)))
@@ -261,150 +333,189 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
     const uint8_t* blk = smem + (size_t)st * p.stage_bytes;
     const Segment sg = seg[st];
     if (sg.flags & 1) {
-      // the query of head row g: scaled by a power of two to below 2^10, split, its group sums
-      float x[G][8];
-      float top = 0.f;
-      const T* q = reinterpret_cast<const T*>(blk + B::kBytes) + g * HD + 8 * t;
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        if (g < p.hpk) {
-          load_vec<T, 8>(q + 32 * j, x[j]);
-        } else {
+      for (int n = 0; n < NT; ++n) {
+        // head g / 2 of the tile, scaled by a power of two to below 2^10, and its group sums
+        const int h = 4 * n + (g >> 1);
+        float x[G][8];
+        float top = 0.f;
+        const T* q = reinterpret_cast<const T*>(blk + B::kBytes) + h * HD + 8 * t;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+        for (int j = 0; j < G; ++j) {
+          if (h < p.hpk) {
+            load_vec<T, 8>(q + 32 * j, x[j]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
         }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int sh = min(120, 9 - ((int)(__float_as_uint(top) >> 23) - 127));
+        const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+        // head t's numbers lie in the lanes of g = 2t
+        kscale[n] = p.scale * __uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, sh, 8 * t)) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
+        for (int j = 0; j < G; ++j) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[j][i] *= up;
+          float sum_hi = 0.f, sum_lo = 0.f;
+          // k slots of a lane: elements 0, 4 | 1, 5 and 2, 6 | 3, 7
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t hi, lo;
+            split2(x[j][i], x[j][i + 4], hi, lo);
+            qb[n][j][i] = odd ? lo : hi;
+            sum_hi += half_of(hi, 0) + half_of(hi, 1);
+            sum_lo += half_of(lo, 0) + half_of(lo, 1);
+          }
+          sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, 1);
+          sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, 1);
+          sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, 2);
+          sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, 2);
+          sum_hi = __shfl_sync(0xffffffffu, sum_hi, 8 * t);
+          sum_lo = __shfl_sync(0xffffffffu, sum_lo, 8 * t);
+          qh[n][j] = sum_hi * -1.46875f;
+          ql[n][j] = sum_lo * -1.46875f;
+          qs[n][j] = fmaf(sum_lo, kLo, sum_hi);
+        }
+        m[n] = m_held[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) om[n][k] = 0.f;
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int sh = min(120, 9 - ((int)(__float_as_uint(top) >> 23) - 127));
-      const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-      kscale = p.scale * __uint_as_float((uint32_t)(127 - sh) << 23);
-      float sum[G];
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        sum[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[j][i] *= up;
-          sum[j] += x[j][i];
-        }
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-        // k slots of a lane: elements 0, 4 | 1, 5 (codes times 16) and 2, 6 | 3, 7 (times 16)
-        split2(x[j][0], x[j][4], qa[j][0], qa[j][1]);
-        split2(x[j][1] * 0.0625f, x[j][5] * 0.0625f, qa[j][2], qa[j][3]);
-        split2(x[j][2], x[j][6], qa[j][4], qa[j][5]);
-        split2(x[j][3] * 0.0625f, x[j][7] * 0.0625f, qa[j][6], qa[j][7]);
-      }
-      float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-      for (int j = 0; j < G; j += 2)
-        if (j == 2 * t) {
-          s0 = sum[j];
-          s1 = sum[j + 1];
-        }
-      split2(s0, s1, qm[0], qm[1]);
-      qm[2] = qm[3] = 0;
-      m = -INFINITY;
-      l = 0.f;
-#pragma unroll
-      for (int n = 0; n < 4 * G; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) om[i] = 0.f;
+      held = false;
+      since = 0;
     }
     const int r0 = 16 * warp;
     if (r0 < sg.valid) {
-      // ---- scores of rows r0 + 8n + 2t, + 1 for head row g
-      float s[2][2];
+      const bool whole = r0 + 16 <= sg.valid;
+      // ---- scores of rows r0 + g, r0 + 8 + g for head t of every tile
+      float s[NT][2], e[NT][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int rg = r0 + 8 * n + g, rt = r0 + 8 * n + 2 * t;
-        float cm[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t mins =
-            2 * t < G ? *reinterpret_cast<const uint32_t*>(blk + B::kCodes + B::kScales + 2 * B::scale(rg, 2 * t)) : 0u;
-        mma_f16(cm, qm, mins, 0u);
-        uint32_t d[G];  // f16 d of rows rt, rt + 1: [row][group]
-        lds_words<G>(blk + B::kCodes + 2 * B::scale(rt, 0), d);
-        float a0 = 0.f, a1 = 0.f;
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = e[n][0] = e[n][1] = 0.f;
+      {
+        const int ra = r0 + g, rb = ra + 8;
+        uint32_t da[G / 2], db[G / 2], ma[G / 2], mb[G / 2];  // f16 pairs of groups
+        lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(ra, 0), da);
+        lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(rb, 0), db);
+        lds_words<G / 2>(blk + B::kCodes + B::kScales + 2 * B::scale(ra, 0), ma);
+        lds_words<G / 2>(blk + B::kCodes + B::kScales + 2 * B::scale(rb, 0), mb);
 #pragma unroll
         for (int P = 0; P < B::kPlanes; ++P) {
-          uint32_t w[J];
-          lds_words<J>(blk + 4 * B::k_word(rg, P * J, t), w);
+          uint32_t wa[J], wb[J];
+          lds_words<J>(blk + 4 * B::k_word(ra, P * J, t), wa);
+          lds_words<J>(blk + 4 * B::k_word(rb, P * J, t), wb);
 #pragma unroll
           for (int i = 0; i < J; ++i) {
             const int j = P * J + i;
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(c, &qa[j][0], w[i] & 0x000F000Fu, w[i] & 0x00F000F0u);
-            const uint32_t w8 = w[i] >> 8;
-            mma_f16(c, &qa[j][4], w8 & 0x000F000Fu, w8 & 0x00F000F0u);
-            a0 = fmaf(half_of(d[j / 2], j & 1), fmaf(c[2], kLo, c[0]), a0);
-            a1 = fmaf(half_of(d[(G + j) / 2], j & 1), fmaf(c[3], kLo, c[1]), a1);
+            const uint32_t a0[4] = {from_one(wa[i] << 6), from_one(wb[i] << 6), from_one(wa[i] << 2), from_one(wb[i] << 2)};
+            const uint32_t a1[4] = {from_one(wa[i] >> 2), from_one(wb[i] >> 2), from_one(wa[i] >> 6), from_one(wb[i] >> 6)};
+            const float d0 = half_of(da[j / 2], j & 1), d1 = half_of(db[j / 2], j & 1);
+            const float c0 = fmaf(7.5f, d0, half_of(ma[j / 2], j & 1)), c1 = fmaf(7.5f, d1, half_of(mb[j / 2], j & 1));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float c[4] = {qh[n][j], ql[n][j], qh[n][j], ql[n][j]};
+              mma_f16(c, a0, qb[n][j][0], qb[n][j][1]);
+              mma_f16(c, a1, qb[n][j][2], qb[n][j][3]);
+              s[n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[n][0]);
+              s[n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[n][1]);
+              e[n][0] = fmaf(c0, qs[n][j], e[n][0]);
+              e[n][1] = fmaf(c1, qs[n][j], e[n][1]);
+            }
           }
         }
-        s[n][0] = fmaf(a0, 16777216.f, fmaf(cm[2], kLo, cm[0])) * kscale;
-        s[n][1] = fmaf(a1, 16777216.f, fmaf(cm[3], kLo, cm[1])) * kscale;
       }
-      const bool whole = r0 + 16 <= sg.valid;
-      if (!whole) {
+      // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
+      // rows 2t, 2t + 1 of the first (g even) or second eight rows
+      float pa[NT], pb[NT];
+      bool grow = false;
+      float m_use[NT], alpha[NT];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (r0 + 8 * n + 2 * t + i >= sg.valid) s[n][i] = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          s[n][i] = fmaf(s[n][i], 16.f, e[n][i]) * kscale[n];
+          if (!whole && r0 + 8 * i + g >= sg.valid) s[n][i] = -INFINITY;
+        }
+        float top = fmaxf(s[n][0], s[n][1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const float m_new = fmaxf(m[n], top);
+        m_use[n] = m_new == -INFINITY ? 0.f : m_new;
+        alpha[n] = ex2(m[n] - m_use[n]);
+        grow |= m_new > m[n];
+        m[n] = m_new;
+        const float p0 = ex2(s[n][0] - m_use[n]), p1 = ex2(s[n][1] - m_use[n]);
+        l[n] = fmaf(l[n], alpha[n], p0 + p1);
+        const int from = 8 * t + (g >> 1);
+        const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
+        const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
+        pa[n] = odd ? a1 : a0;
+        pb[n] = odd ? b1 : b0;
       }
-      // ---- online softmax
-      float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float m_new = fmaxf(m, top);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      if (__any_sync(0xffffffffu, m_new > m)) {
-        const float alpha = ex2(m - m_use);
-        l *= alpha;
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int n = 0; n < 4 * G; ++n)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][i] *= alpha;
+          for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) om[i] *= alpha;
-        m = m_new;
-      }
-      float pr[2][2];
+            for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha[n];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) pr[n][i] = ex2(s[n][i] - m_use);
-      l += (pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]);
-      // ---- weighted rows
-      const uint8_t* vb = blk + B::kHalf;
-      uint32_t d0[G], d1[G];  // f16 d of rows r0 + 2t, + 1 and r0 + 8 + 2t, + 1
-      lds_words<G>(vb + B::kCodes + 2 * B::scale(r0 + 2 * t, 0), d0);
-      lds_words<G>(vb + B::kCodes + 2 * B::scale(r0 + 8 + 2 * t, 0), d1);
-      uint32_t pa[4];
-      split2(pr[0][0], pr[0][1], pa[0], pa[1]);
-      split2(pr[1][0], pr[1][1], pa[2], pa[3]);
-      uint32_t v0 = 0, v1 = 0;
-      if (g < G) {
-        v0 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 2 * t, g));
-        v1 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 8 + 2 * t, g));
-      }
-      if (!whole) {  // rows that hold nothing yet: what their d and m are does not count
-        const int n0 = sg.valid - (r0 + 2 * t), n1 = n0 - 8;
-        const uint32_t k0 = n0 >= 2 ? 0xffffffffu : n0 == 1 ? 0xffffu : 0u;
-        const uint32_t k1 = n1 >= 2 ? 0xffffffffu : n1 == 1 ? 0xffffu : 0u;
-        v0 &= k0;
-        v1 &= k1;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          if (i < G / 2 ? n0 < 1 : n0 < 2) d0[i] = 0u;
-          if (i < G / 2 ? n1 < 1 : n1 < 2) d1[i] = 0u;
+          for (int k = 0; k < 4; ++k) om[n][k] *= alpha[n];
         }
       }
-      mma_f16(om, pa, v0, v1);
+      // ---- weighted rows
+      const uint8_t* vb = blk + B::kHalf;
+      const int rw = r0 + 2 * t + (odd ? 8 : 0);  // rows of pa, pb
+      uint32_t dw[G];  // f16 d of those rows: [row][group]
+      lds_words<G>(vb + B::kCodes + 2 * B::scale(rw, 0), dw);
+      // A of the middles: group g of rows r0 + 2t, + 1 and r0 + 8 + 2t, + 1
+      uint32_t v0 = 0, v1 = 0, e0 = 0, e1 = 0;
+      if (g < G) {
+        const uint8_t* d16 = vb + B::kCodes + 2 * B::scale(r0 + 2 * t, g);
+        v0 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 2 * t, g));
+        v1 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 8 + 2 * t, g));
+        e0 = *reinterpret_cast<const uint16_t*>(d16) | (uint32_t)*reinterpret_cast<const uint16_t*>(d16 + 2 * G) << 16;
+        e1 = *reinterpret_cast<const uint16_t*>(d16 + 16 * G) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(d16 + 18 * G) << 16;
+      }
+      if (!whole) {  // rows that hold nothing yet: what their d and m are does not count
+        auto keep = [&](int r) { return sg.valid - r >= 2 ? 0xffffffffu : sg.valid - r == 1 ? 0xffffu : 0u; };
+        v0 &= keep(r0 + 2 * t);
+        e0 &= keep(r0 + 2 * t);
+        v1 &= keep(r0 + 8 + 2 * t);
+        e1 &= keep(r0 + 8 + 2 * t);
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+          if (sg.valid - rw < (i < G / 2 ? 1 : 2)) dw[i] = 0u;
+      }
+      // hi and lo of the weights (a, b) of this lane's head to the lanes of B's columns
+      auto columns = [&](float a, float b, uint32_t& b0, uint32_t& b1) {
+        uint32_t hi, lo;
+        split2(a, b, hi, lo);
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? hi : lo, 4);
+        b0 = odd ? got : hi;
+        b1 = odd ? lo : got;
+      };
+      {
+        uint32_t a[4];
+        middle(e0, v0, a[0], a[1]);
+        middle(e1, v1, a[2], a[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t b0, b1;
+          columns(pa[n], pb[n], b0, b1);
+          mma_f16(om[n], a, b0, b1);
+        }
+      }
 #pragma unroll
       for (int P = 0; P < B::kPlanes; ++P) {
         uint32_t w0[J], w1[J];
@@ -413,45 +524,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
 #pragma unroll
         for (int i = 0; i < J; ++i) {
           const int j = P * J + i;
-          uint32_t a[4];
-          split2(pr[0][0] * half_of(d0[j / 2], j & 1), pr[0][1] * half_of(d0[(G + j) / 2], j & 1), a[0], a[1]);
-          split2(pr[1][0] * half_of(d1[j / 2], j & 1), pr[1][1] * half_of(d1[(G + j) / 2], j & 1), a[2], a[3]);
-          mma_f16(o[4 * j], a, w0[i] & 0x000F000Fu, w1[i] & 0x000F000Fu);
-          mma_f16(o[4 * j + 1], a, w0[i] & 0x00F000F0u, w1[i] & 0x00F000F0u);
-          const uint32_t x0 = w0[i] >> 8, x1 = w1[i] >> 8;
-          mma_f16(o[4 * j + 2], a, x0 & 0x000F000Fu, x1 & 0x000F000Fu);
-          mma_f16(o[4 * j + 3], a, x0 & 0x00F000F0u, x1 & 0x00F000F0u);
+          const uint32_t a0[4] = {centred(w0[i] << 4), centred(w0[i]), centred(w1[i] << 4), centred(w1[i])};
+          const uint32_t a1[4] = {centred(w0[i] >> 4), centred(w0[i] >> 8), centred(w1[i] >> 4), centred(w1[i] >> 8)};
+          const float da = half_of(dw[j / 2], j & 1), db = half_of(dw[(G + j) / 2], j & 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t b0, b1;
+            columns(pa[n] * da, pb[n] * db, b0, b1);
+            mma_f16(o[n][2 * j], a0, b0, b1);
+            mma_f16(o[n][2 * j + 1], a1, b0, b1);
+          }
         }
       }
+      if (++since == kFlush) flush();
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[st]);
     if (!(sg.flags & 2)) continue;
 
     // ---------------- end of the segment: join the warps in order
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t == 0 && g < p.hpk) {
-      wm[warp][g] = m;
-      wl[warp][g] = l;
-    }
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      // group j's sum of p m sits in lane t = j / 2 (columns 2t, 2t + 1)
-      const float mine_m = j & 1 ? fmaf(om[3], kLo, om[1]) : fmaf(om[2], kLo, om[0]);
-      const float mins = __shfl_sync(0xffffffffu, mine_m, (lane & ~3) | (j / 2));
-      if (g < p.hpk) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = r & 1 ? 1048576.f : 16777216.f;
-          const float* c = o[4 * j + r];
-          float2 v;
-          v.x = fmaf(fmaf(c[2], kLo, c[0]), f, mins);
-          v.y = fmaf(fmaf(c[3], kLo, c[1]), f, mins);
-          *reinterpret_cast<float2*>(wo + ((size_t)warp * p.hpk + g) * HD + 32 * j + 8 * r + 2 * t) = v;
-        }
+    for (int n = 0; n < NT; ++n) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+      if (g == 0 && 4 * n + t < p.hpk) {
+        wm[warp][4 * n + t] = m[n];
+        wl[warp][4 * n + t] = l[n];
       }
     }
+    flush();
     if (!sync()) return;
     // participants of this (sequence, head)
     const long long last_unit = sg.base + sg.pages - 1;
@@ -470,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
 #pragma unroll
       for (int w = 0; w < kConsumers; ++w) {
         const float e = ex2(wm[w][h] - Mu);
-        v = fmaf(e, wo[(size_t)w * p.hpk * HD + i], v);
+        v = fmaf(e, wo[((size_t)w * p.hpk + h) * PITCH + i % HD], v);
         L = fmaf(e, wl[w][h], L);
       }
       if (alone) {
@@ -493,21 +595,45 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
       }
       if (!sync()) return;
       if (is_last) {
-        for (int i = threadIdx.x; i < p.hpk * HD; i += 32 * kConsumers) {
-          const int h = i / HD;
-          float M = -INFINITY, v = 0.f, L = 0.f;
-          for (int c = c0; c <= c1; ++c) {
-            // the part that starts the (sequence, head) is its CTA's slot 1, the others slot 0
-            const float* q = p.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * part_floats;
-            const float pm = __ldcg(q + p.hpk * HD + h), pl = __ldcg(q + p.hpk * HD + p.hpk + h);
-            const float pv = __ldcg(q + i);
-            const float Mn = fmaxf(M, pm), Mu = Mn == -INFINITY ? 0.f : Mn;
-            const float e0 = ex2(M - Mu), e1 = ex2(pm - Mu);
-            v = fmaf(v, e0, pv * e1);
-            L = fmaf(L, e0, pl * e1);
-            M = Mn;
+        // the parts in order (the one that starts the (sequence, head) is its CTA's slot 1, the
+        // others slot 0): a warp per head finds the maximum and the sum, then every thread joins
+        // four values, eight parts' loads in flight
+        const float* first = p.parts + (size_t)(2 * c0 + 1) * part_floats;
+        const float* rest = p.parts + (size_t)(2 * c0) * part_floats;
+        auto part_of = [&](int i) { return i == 0 ? first : rest + (size_t)(2 * i) * part_floats; };
+        const int n = c1 - c0 + 1, stat = p.hpk * HD;
+        for (int h = warp; h < p.hpk; h += kConsumers) {
+          float M = -INFINITY, L = 0.f;
+          for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(part_of(i) + stat + h));
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+          const float Mu = M == -INFINITY ? 0.f : M;
+          for (int i = lane; i < n; i += 32)
+            L = fmaf(ex2(__ldcg(part_of(i) + stat + h) - Mu), __ldcg(part_of(i) + stat + p.hpk + h), L);
+          L = warp_sum(L);
+          if (lane == 0) {
+            wm[0][h] = Mu;
+            wl[0][h] = L;
           }
-          out[i] = from_f32<T>(L == 0.f ? 0.f : v / L);
+        }
+        if (!sync()) return;
+        for (int e = 4 * threadIdx.x; e < stat; e += 4 * 32 * kConsumers) {
+          const int h = e / HD;
+          const float Mu = wm[0][h], L = wl[0][h];
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+          for (int i = 0; i < n; ++i) {
+            const float* q = part_of(i);
+            const float w = ex2(__ldcg(q + stat + h) - Mu);
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(q + e)), y = __ldcg(reinterpret_cast<const float2*>(q + e + 2));
+            v[0] = fmaf(w, x.x, v[0]);
+            v[1] = fmaf(w, x.y, v[1]);
+            v[2] = fmaf(w, y.x, v[2]);
+            v[3] = fmaf(w, y.y, v[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = L == 0.f ? 0.f : v[i] / L;
+          store_vec<T, 4>(out + e, v);
         }
       }
     }
@@ -515,28 +641,33 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD>())
   }
 }
 
-template <int HD, typename T>
-cudaError_t launch(const LaunchEnv& env, Kv4Params p, int max_ctas) {
-  constexpr int kBudget = (ctas_per_sm<HD>() == 2 ? 113 : 226) * 1024 - 6144;  // static and reserved shared memory
+template <int HD, int NT, typename T>
+cudaError_t launch(const LaunchEnv& env, Kv4Params p) {
+  constexpr int kCtas = ctas_per_sm<HD, NT>();
+  constexpr int kBudget = 227 * 1024 / kCtas - 1024 - 2560;  // the system's and the static shared memory
   p.stage_bytes = Kv4Block<HD>::kBytes + p.hpk * HD * (int)sizeof(T);
-  const int join = kConsumers * p.hpk * HD * 4;
+  const int join = kConsumers * p.hpk * (HD + 8) * 4;
   p.stages = (kBudget - join) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = p.stages * p.stage_bytes + join;
-  auto kern = kv4_attention_kernel<HD, T>;
+  auto kern = kv4_attention_kernel<HD, NT, T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)p.n_seqs * p.nkv * (p.max_pages > 0 ? p.max_pages : 1);
-  const int grid = (int)(units < max_ctas ? units : max_ctas);
+  const int ctas = env.sm_count * kCtas;
+  const int grid = (int)(units < ctas ? units : ctas);
   return rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl, p);
+}
+template <int HD, typename T>
+cudaError_t launch_tiles(const LaunchEnv& env, const Kv4Params& p) {
+  return p.hpk <= 4 ? launch<HD, 1, T>(env, p) : launch<HD, 2, T>(env, p);
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, const Kv4Params& p) {
-  const int ctas = env.sm_count * ctas_per_sm<HD>();
   switch (type) {
-    case RRR_F32: return launch<HD, float>(env, p, ctas);
-    case RRR_F16: return launch<HD, __half>(env, p, ctas);
-    default: return launch<HD, __nv_bfloat16>(env, p, ctas);
+    case RRR_F32: return launch_tiles<HD, float>(env, p);
+    case RRR_F16: return launch_tiles<HD, __half>(env, p);
+    default: return launch_tiles<HD, __nv_bfloat16>(env, p);
   }
 }
 
@@ -562,7 +693,7 @@ int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t
   int rc = check_kv4_cache(ctx, c, fn);
   if (rc || (rc = check_heads(ctx, c, n_heads, fn))) return rc;
   if (!bytes) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
-  const int64_t parts = 2 * 2 * (int64_t)ctx->sm_count;  // two per CTA, at most two CTAs per SM
+  const int64_t parts = 2 * 3 * (int64_t)ctx->sm_count;  // two per CTA, at most three CTAs per SM
   *bytes = counter_bytes(c) + parts * (n_heads / c->n_kv_heads) * (c->head_dim + 2) * 4;
   return RRR_OK;
 }
