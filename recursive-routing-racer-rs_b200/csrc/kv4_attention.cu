@@ -3,17 +3,17 @@
 // for a batch of sequences of different lengths on pages.
 //
 // Mathematics. A key is k = d_j code + m_j in groups j of 32 values, so q . k = sum_j d_j (q_j .
-// (code_j - 7.5)) + (m_j + 7.5 d_j) (sum q_j). The products with the codes run on mma.m16n8k16
+// code_j) + m_j (sum q_j). The products with the codes run on mma.m16n8k16
 // (f16 in, f32 accumulate): 16 rows of codes are the A operand, and the B operand's eight columns
 // are four query heads as (hi, lo) pairs: the f16 part of the (power-of-two scaled) query and
 // the remainder (q - hi) * 2^11, so a score carries 22 bits of the query. A code shifted into the
 // top of an f16's mantissa is 1 + code / 16 (a shift and an AND-OR for two operands); the
-// accumulators start at -(1 + 7.5 / 16) sum q_j, the power of two leaves with the scales and d_j
-// multiplies them in f32. (The code in the low bits would be the subnormal code * 2^-24 for fewer
+// accumulators start at -sum q_j, the power of two leaves with the scales and d_j multiplies them
+// in f32. One more product takes the m_j. (The code in the low bits would be the subnormal code * 2^-24 for fewer
 // instructions, but the tensor core aligns a subnormal's products as if they were normal: they
 // lost 6 bits, an error of 1e-6 in the scores.) The second product is alike: A holds
-// V's codes, B the weights p_i d_ij of group j as (hi, lo), and one more product of p itself takes
-// the m_ij + 7.5 d_ij. V's codes are centred, code - 7.5: over a long context the weighted values
+// V's codes, B the weights p_i d_ij of group j as (hi, lo), and the sums of p_i (m_ij + 7.5 d_ij)
+// run beside it in f32. V's codes are centred, code - 7.5: over a long context the weighted values
 // nearly cancel, and sums of the codes themselves would be hundreds of times the result (measured:
 // an error of 1.2e-3 at 131,000 rows). The tensor core truncates its sums, so they are moved to
 // shared memory, rounded, every kFlush pages. The softmax runs online in base 2, with 32-bit maxima
@@ -28,6 +28,8 @@
 // other CTAs share goes to the workspace, and the CTA that finishes last joins the parts in
 // order (so results do not depend on which one that is) and leaves the counter at zero.
 #include <math.h>
+
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -57,12 +59,12 @@ struct Kv4Params {
   int* err;
 };
 
-struct Segment {  // beside each stage
+struct Segment {  // beside each stage: this CTA's run of pages of one (sequence, head)
   long long base;  // unit of the (sequence, head)'s first page
   int seq, head, pages;
   int valid;       // rows of this page that count
-  int flags;       // 1: first page of this CTA's segment, 2: last
-  int first_page;  // of this CTA's segment
+  int first_page;  // of the run
+  int first, left; // whether this page is the run's first; its pages from this one on
 };
 
 // CTAs of an SM by what its registers hold: HD/4 accumulators and HD/8 of the query per column tile
@@ -70,6 +72,14 @@ struct Segment {  // beside each stage
 template <int HD, int NT>
 constexpr int ctas_per_sm() { return HD * NT >= 512 ? 1 : HD * NT >= 256 ? 2 : 3; }
 
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1,
+                                        const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -83,10 +93,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // a, b as f16 pairs hi and lo = (x - hi) * 2^11
+__device__ __forceinline__ float from_half(__half h, float x) {  // h - x
+  float r;
+  asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(r) : "h"(__half_as_ushort(h)), "f"(x));
+  return r;
+}
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn((a - f.x) * 2048.f, (b - f.y) * 2048.f);
+  const __half2 l = __floats2half2_rn(from_half(__low2half(h), a) * -2048.f, from_half(__high2half(h), b) * -2048.f);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -95,19 +109,26 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {
   return i ? __high2float(h) : __low2float(h);
 }
 
-// 1 + code / 16 of the four bits at 6..9 of both halves of w
-__device__ __forceinline__ uint32_t from_one(uint32_t w) { return (w & 0x03C003C0u) | 0x3C003C00u; }
+// (w & mask) | bits in one instruction: `bits` comes in a register, an instruction has room for
+// one constant (with both as constants each pair of operands cost two: 16 % more time)
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(mask), "r"(bits));
+  return x;
+}
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+// 1 + code / 16 of the four bits at 6..9 of both halves of w (one: 0x3C003C00)
+__device__ __forceinline__ uint32_t from_one(uint32_t w, uint32_t one) { return and_or(w, 0x03C003C0u, one); }
 // 16 (code - 7.5) of the four bits at 4..7 of both halves of w: 1024 + 16 code - 1144, exact
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
-  const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
+// (big: 0x64006400)
+__device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t big) {
+  const uint32_t x = and_or(w, 0x00F000F0u, big);
   const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0xe478)));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-// The f16 pair (m + 7.5 d) of a pair of rows, as hi and lo
-__device__ __forceinline__ void middle(uint32_t d, uint32_t m, uint32_t& hi, uint32_t& lo) {
-  split2(fmaf(7.5f, half_of(d, 0), half_of(m, 0)), fmaf(7.5f, half_of(d, 1), half_of(m, 1)), hi, lo);
-}
-
 // N words at p (N a power of two; p aligned to min(16, 4 N))
 template <int N>
 __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -221,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     int len = seq_len(s), np = pages_of(len);
     int head = (int)((u0 - base) / np), page = (int)((u0 - base) % np);
     int first_page = page, ids_at = -1, id = 0;
-    int it = 0;
+    int it = 0, st = 0;
+    uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
     bool ok = true;
     const uint32_t q_bytes = (uint32_t)(p.hpk * HD * sizeof(T));
     for (long long u = u0; u < u1; ++u, ++it) {
@@ -248,15 +270,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         if (lane == 0) flag_position(p.err);
         valid = 0;
       }
-      const int st = it % p.stages;
-      if (it >= p.stages) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], (uint32_t)(it / p.stages - 1) & 1u, p.err,
-                                                       kDevErrEmptyTimeout));
-        if (!ok) break;
-      }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], phase, p.err, kDevErrEmptyTimeout));
+      if (!ok) break;
       if (lane == 0) {
-        const bool first = u == u0 || page == 0, last = u + 1 == u1 || page + 1 == np;
-        seg[st] = Segment{base + (long long)head * np, s, head, np, valid, (first ? 1 : 0) | (last ? 2 : 0), first_page};
+        const bool first = u == u0 || page == 0;
+        const int left = (int)(u1 - u < np - page ? u1 - u : np - page);
+        seg[st] = Segment{base + (long long)head * np, s, head, np, valid, first_page, first ? 1 : 0, left};
         uint8_t* dst = smem + (size_t)st * p.stage_bytes;
         mbar_arrive_expect_tx(&full[st], (valid ? (uint32_t)B::kBytes : 0u) + (first ? q_bytes : 0u));
         if (first)
@@ -266,30 +285,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       }
       __syncwarp();
       ++page;
+      if (++st == p.stages) {
+        st = 0;
+        phase ^= 1;
+      }
     }
     // after a wait that gave up, the copies in flight land before the CTA leaves
     if (!ok)
-      for (int st = 0; st < p.stages && st < it; ++st) {
-        const int uses = (it - st + p.stages - 1) / p.stages;
-        mbar_wait_bounded(&full[st], (uint32_t)(uses - 1) & 1u, p.err, kDevErrDrainTimeout);
+      for (int i = 0; i < p.stages && i < it; ++i) {
+        const int uses = (it - i + p.stages - 1) / p.stages;
+        mbar_wait_bounded(&full[i], (uint32_t)(uses - 1) & 1u, p.err, kDevErrDrainTimeout);
       }
     return;
   }
 
-  // ---------------- consumers: warp w takes rows 16w .. 16w + 15 of every page
+  // ---------------- consumers: warp w takes rows 16w .. 16w + 15 of every page, of two pages at a
+  // time where the run has them
   // Fragments of lane (g, t): A rows g and g + 8, k slots 2t, + 1 and 2t + 8, + 9; B the same
   // slots of column g, that is of head g / 2's hi (g even) or lo part; C rows g, g + 8 of columns
   // 2t, 2t + 1, that is of head t. Tile n holds the heads 4n .. 4n + 3.
   const int g = lane >> 2, t = lane & 3;
   const bool odd = g & 1;
+  const uint32_t one = opaque(0x3C003C00u), big = opaque(0x64006400u);
   ConsumerSync sync{&cons_bar, 0, p.err};
-  uint32_t qb[NT][G][4];                       // B: two k steps per group
-  float qh[NT][G], ql[NT][G], qs[NT][G];       // head t: -(1 + 7.5 / 16) times the sums of hi and lo; sums of q
+  uint32_t qb[NT][G][4], qm[NT];  // B: two k steps per group; the groups' sums of q
+  float qi[NT][G][2];             // head t: minus the sums of hi and lo
   float kscale[NT], m[NT], l[NT], m_held[NT];  // head t; m_held: of what shared memory holds
-  float o[NT][2 * G][4], om[NT][4];            // values: [16 u + (g, g + 8)] of group j; middles
+  float o[NT][2 * G][4];          // values: [16 u + (g, g + 8)] of group j, head t
+  float om[NT][G];                // middles of group j, head g / 2, this lane's rows
   bool held = false;
   int since = 0;
-  int it = 0;
 
   // adds this warp's accumulators to its sums in shared memory, and clears them
   auto flush = [&]() {
@@ -298,12 +323,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       const float m_use = m[n] == -INFINITY ? 0.f : m[n];
       const float keep = ex2(m_held[n] - m_use);
       const int h = 4 * n + t;
-      // group g's middles: row g holds the hi, row g + 8 the lo parts
-      const float mine_m = fmaf(om[n][1] + om[n][2], kLo, om[n][0]);
       float* dst = wo + ((size_t)warp * p.hpk + h) * PITCH;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        const float mid = __shfl_sync(0xffffffffu, mine_m, 4 * j + t);
+        float mid = om[n][j];
+        mid += __shfl_xor_sync(0xffffffffu, mid, 1);
+        mid += __shfl_xor_sync(0xffffffffu, mid, 2);
+        mid += __shfl_xor_sync(0xffffffffu, mid, 4);
+        mid = __shfl_sync(0xffffffffu, mid, 8 * t);
         if (h < p.hpk) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -317,29 +344,190 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[n][2 * j][i] = o[n][2 * j + 1][i] = 0.f;
+        om[n][j] = 0.f;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) om[n][i] = 0.f;
       m_held[n] = m[n];
     }
     held = true;
     since = 0;
   };
 
-  for (long long u = u0; u < u1; ++u, ++it) {
-    const int st = it % p.stages;
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[st], (uint32_t)(it / p.stages) & 1u, p.err, kDevErrFullTimeout)))
-      return;
-    const uint8_t* blk = smem + (size_t)st * p.stage_bytes;
+  // hi and lo of the weights (a, b) of this lane's head g / 2 to the lanes of B's columns
+  auto columns = [&](float a, float b, uint32_t& b0, uint32_t& b1) {
+    uint32_t hi, lo;
+    split2(a, b, hi, lo);
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? hi : lo, 4);
+    b0 = odd ? got : hi;
+    b1 = odd ? lo : got;
+  };
+
+  // this warp's rows of NS pages
+  auto rows = [&](auto ns, const uint8_t* const* blocks, const int* valid) {
+    constexpr int NS = decltype(ns)::value;
+    const int r0 = 16 * warp;
+    // ---- scores of rows r0 + g, r0 + 8 + g for head t of every tile
+    float s[NS][NT][2];
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+      const uint8_t* blk = blocks[x];
+      const int ra = r0 + g, rb = ra + 8;
+      uint32_t da[G / 2], db[G / 2];  // f16 pairs of groups
+      lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(ra, 0), da);
+      lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(rb, 0), db);
+      uint32_t ma[4] = {0u, 0u, 0u, 0u};
+      if (2 * t < G) {
+        ma[0] = *reinterpret_cast<const uint32_t*>(blk + B::kCodes + B::kScales + 2 * B::scale(ra, 2 * t));
+        ma[1] = *reinterpret_cast<const uint32_t*>(blk + B::kCodes + B::kScales + 2 * B::scale(rb, 2 * t));
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[x][n][0] = s[x][n][1] = 0.f;
+#pragma unroll
+      for (int P = 0; P < B::kPlanes; ++P) {
+        uint32_t wa[J], wb[J];
+        lds_words<J>(blk + 4 * B::k_word(ra, P * J, t), wa);
+        lds_words<J>(blk + 4 * B::k_word(rb, P * J, t), wb);
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+          const int j = P * J + i;
+          const uint32_t a0[4] = {from_one(wa[i] << 6, one), from_one(wb[i] << 6, one), from_one(wa[i] << 2, one),
+                                  from_one(wb[i] << 2, one)};
+          const uint32_t a1[4] = {from_one(wa[i] >> 2, one), from_one(wb[i] >> 2, one), from_one(wa[i] >> 6, one),
+                                  from_one(wb[i] >> 6, one)};
+          const float d0 = half_of(da[j / 2], j & 1), d1 = half_of(db[j / 2], j & 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float init[4] = {qi[n][j][0], qi[n][j][1], qi[n][j][0], qi[n][j][1]};
+            float c[4];
+            mma_f16(c, a0, qb[n][j][0], qb[n][j][1], init);
+            mma_f16(c, a1, qb[n][j][2], qb[n][j][3]);
+            s[x][n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[x][n][0]);
+            s[x][n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[x][n][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        float c[4];
+        mma_f16(c, ma, qm[n], 0u, zero);
+        s[x][n][0] = fmaf(s[x][n][0], 16.f, fmaf(c[1], kLo, c[0])) * kscale[n];
+        s[x][n][1] = fmaf(s[x][n][1], 16.f, fmaf(c[3], kLo, c[2])) * kscale[n];
+      }
+      if (r0 + 16 > valid[x]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (r0 + 8 * i + g >= valid[x]) s[x][n][i] = -INFINITY;
+      }
+    }
+    // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
+    // rows 2t, 2t + 1 of the first (g even) or second eight rows
+    float pa[NS][NT], pb[NS][NT], alpha[NT];
+    bool grow = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top = fmaxf(s[0][n][0], s[0][n][1]);
+      if constexpr (NS == 2) top = fmaxf(top, fmaxf(s[1][n][0], s[1][n][1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const float m_new = fmaxf(m[n], top), m_use = m_new == -INFINITY ? 0.f : m_new;
+      alpha[n] = ex2(m[n] - m_use);
+      grow |= m_new > m[n];
+      m[n] = m_new;
+      l[n] *= alpha[n];
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const float p0 = ex2(s[x][n][0] - m_use), p1 = ex2(s[x][n][1] - m_use);
+        l[n] += p0 + p1;
+        const int from = 8 * t + (g >> 1);
+        const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
+        const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
+        pa[x][n] = odd ? a1 : a0;
+        pb[x][n] = odd ? b1 : b0;
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha[n];
+        const float al = __shfl_sync(0xffffffffu, alpha[n], g >> 1);
+#pragma unroll
+        for (int j = 0; j < G; ++j) om[n][j] *= al;
+      }
+    }
+    // ---- weighted rows
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+      const uint8_t* vb = blocks[x] + B::kHalf;
+      const int rw = r0 + 2 * t + (odd ? 8 : 0);  // rows of pa, pb
+      uint32_t dw[G], mw[G];                      // f16 d [row][group]; m [group][row]
+      lds_words<G>(vb + B::kCodes + 2 * B::scale(rw, 0), dw);
+      lds_words<G>(vb + B::kCodes + B::kScales + 2 * B::v_min(rw, 0), mw);
+      if (r0 + 16 > valid[x]) {  // rows that hold nothing yet: what their d and m are does not count
+        const int n = valid[x] - rw;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          if (n < (i < G / 2 ? 1 : 2)) dw[i] = 0u;
+          mw[i] &= n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u;
+        }
+      }
+#pragma unroll
+      for (int P = 0; P < B::kPlanes; ++P) {
+        uint32_t w0[J], w1[J];
+        lds_words<J>(vb + 2 * B::v_half(r0 + 2 * t, P * J, g), w0);
+        lds_words<J>(vb + 2 * B::v_half(r0 + 8 + 2 * t, P * J, g), w1);
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+          const int j = P * J + i;
+          const uint32_t a0[4] = {centred(w0[i] << 4, big), centred(w0[i], big), centred(w1[i] << 4, big),
+                                  centred(w1[i], big)};
+          const uint32_t a1[4] = {centred(w0[i] >> 4, big), centred(w0[i] >> 8, big), centred(w1[i] >> 4, big),
+                                  centred(w1[i] >> 8, big)};
+          const float da = half_of(dw[j / 2], j & 1), db = half_of(dw[(G + j) / 2], j & 1);
+          const float ca = fmaf(7.5f, da, half_of(mw[j], 0)), cb = fmaf(7.5f, db, half_of(mw[j], 1));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t b0, b1;
+            columns(pa[x][n] * da, pb[x][n] * db, b0, b1);
+            mma_f16(o[n][2 * j], a0, b0, b1);
+            mma_f16(o[n][2 * j + 1], a1, b0, b1);
+            om[n][j] = fmaf(pa[x][n], ca, fmaf(pb[x][n], cb, om[n][j]));
+          }
+        }
+      }
+    }
+  };
+
+  int st = 0;
+  uint32_t phase = 0;
+  auto landed = [&]() {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], phase, p.err, kDevErrFullTimeout));
+  };
+  auto next = [&]() {
+    if (++st == p.stages) {
+      st = 0;
+      phase ^= 1;
+    }
+  };
+  for (long long u = u0; u < u1;) {
+    if (!landed()) return;
     const Segment sg = seg[st];
-    if (sg.flags & 1) {
+    const int at0 = st, take = sg.left > 1 ? 2 : 1;
+    const uint8_t* blocks[2] = {smem + (size_t)st * p.stage_bytes, nullptr};
+    int valid[2] = {sg.valid, 0};
+    if (sg.first) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         // head g / 2 of the tile, scaled by a power of two to below 2^10, and its group sums
         const int h = 4 * n + (g >> 1);
         float x[G][8];
         float top = 0.f;
-        const T* q = reinterpret_cast<const T*>(blk + B::kBytes) + h * HD + 8 * t;
+        const T* q = reinterpret_cast<const T*>(blocks[0] + B::kBytes) + h * HD + 8 * t;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           if (h < p.hpk) {
@@ -357,6 +545,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
         // head t's numbers lie in the lanes of g = 2t
         kscale[n] = p.scale * __uint_as_float((uint32_t)(127 - __shfl_sync(0xffffffffu, sh, 8 * t)) << 23);
+        float s0 = 0.f, s1 = 0.f;  // sums of groups 2t, 2t + 1
 #pragma unroll
         for (int j = 0; j < G; ++j) {
 #pragma unroll
@@ -375,172 +564,49 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, 1);
           sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, 2);
           sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, 2);
-          sum_hi = __shfl_sync(0xffffffffu, sum_hi, 8 * t);
-          sum_lo = __shfl_sync(0xffffffffu, sum_lo, 8 * t);
-          qh[n][j] = sum_hi * -1.46875f;
-          ql[n][j] = sum_lo * -1.46875f;
-          qs[n][j] = fmaf(sum_lo, kLo, sum_hi);
+          const float sum = fmaf(sum_lo, kLo, sum_hi);
+          if (j == 2 * t) s0 = sum;
+          if (j == 2 * t + 1) s1 = sum;
+          qi[n][j][0] = -__shfl_sync(0xffffffffu, sum_hi, 8 * t);
+          qi[n][j][1] = -__shfl_sync(0xffffffffu, sum_lo, 8 * t);
+          om[n][j] = 0.f;
         }
+        uint32_t hi, lo;
+        split2(s0, s1, hi, lo);
+        qm[n] = odd ? lo : hi;
         m[n] = m_held[n] = -INFINITY;
         l[n] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) om[n][k] = 0.f;
       }
       held = false;
       since = 0;
     }
-    const int r0 = 16 * warp;
-    if (r0 < sg.valid) {
-      const bool whole = r0 + 16 <= sg.valid;
-      // ---- scores of rows r0 + g, r0 + 8 + g for head t of every tile
-      float s[NT][2], e[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = e[n][0] = e[n][1] = 0.f;
-      {
-        const int ra = r0 + g, rb = ra + 8;
-        uint32_t da[G / 2], db[G / 2], ma[G / 2], mb[G / 2];  // f16 pairs of groups
-        lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(ra, 0), da);
-        lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(rb, 0), db);
-        lds_words<G / 2>(blk + B::kCodes + B::kScales + 2 * B::scale(ra, 0), ma);
-        lds_words<G / 2>(blk + B::kCodes + B::kScales + 2 * B::scale(rb, 0), mb);
-#pragma unroll
-        for (int P = 0; P < B::kPlanes; ++P) {
-          uint32_t wa[J], wb[J];
-          lds_words<J>(blk + 4 * B::k_word(ra, P * J, t), wa);
-          lds_words<J>(blk + 4 * B::k_word(rb, P * J, t), wb);
-#pragma unroll
-          for (int i = 0; i < J; ++i) {
-            const int j = P * J + i;
-            const uint32_t a0[4] = {from_one(wa[i] << 6), from_one(wb[i] << 6), from_one(wa[i] << 2), from_one(wb[i] << 2)};
-            const uint32_t a1[4] = {from_one(wa[i] >> 2), from_one(wb[i] >> 2), from_one(wa[i] >> 6), from_one(wb[i] >> 6)};
-            const float d0 = half_of(da[j / 2], j & 1), d1 = half_of(db[j / 2], j & 1);
-            const float c0 = fmaf(7.5f, d0, half_of(ma[j / 2], j & 1)), c1 = fmaf(7.5f, d1, half_of(mb[j / 2], j & 1));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float c[4] = {qh[n][j], ql[n][j], qh[n][j], ql[n][j]};
-              mma_f16(c, a0, qb[n][j][0], qb[n][j][1]);
-              mma_f16(c, a1, qb[n][j][2], qb[n][j][3]);
-              s[n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[n][0]);
-              s[n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[n][1]);
-              e[n][0] = fmaf(c0, qs[n][j], e[n][0]);
-              e[n][1] = fmaf(c1, qs[n][j], e[n][1]);
-            }
-          }
-        }
-      }
-      // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
-      // rows 2t, 2t + 1 of the first (g even) or second eight rows
-      float pa[NT], pb[NT];
-      bool grow = false;
-      float m_use[NT], alpha[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[n][i] = fmaf(s[n][i], 16.f, e[n][i]) * kscale[n];
-          if (!whole && r0 + 8 * i + g >= sg.valid) s[n][i] = -INFINITY;
-        }
-        float top = fmaxf(s[n][0], s[n][1]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const float m_new = fmaxf(m[n], top);
-        m_use[n] = m_new == -INFINITY ? 0.f : m_new;
-        alpha[n] = ex2(m[n] - m_use[n]);
-        grow |= m_new > m[n];
-        m[n] = m_new;
-        const float p0 = ex2(s[n][0] - m_use[n]), p1 = ex2(s[n][1] - m_use[n]);
-        l[n] = fmaf(l[n], alpha[n], p0 + p1);
-        const int from = 8 * t + (g >> 1);
-        const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
-        const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
-        pa[n] = odd ? a1 : a0;
-        pb[n] = odd ? b1 : b0;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int i = 0; i < 2 * G; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha[n];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) om[n][k] *= alpha[n];
-        }
-      }
-      // ---- weighted rows
-      const uint8_t* vb = blk + B::kHalf;
-      const int rw = r0 + 2 * t + (odd ? 8 : 0);  // rows of pa, pb
-      uint32_t dw[G];  // f16 d of those rows: [row][group]
-      lds_words<G>(vb + B::kCodes + 2 * B::scale(rw, 0), dw);
-      // A of the middles: group g of rows r0 + 2t, + 1 and r0 + 8 + 2t, + 1
-      uint32_t v0 = 0, v1 = 0, e0 = 0, e1 = 0;
-      if (g < G) {
-        const uint8_t* d16 = vb + B::kCodes + 2 * B::scale(r0 + 2 * t, g);
-        v0 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 2 * t, g));
-        v1 = *reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales + 2 * B::v_min(r0 + 8 + 2 * t, g));
-        e0 = *reinterpret_cast<const uint16_t*>(d16) | (uint32_t)*reinterpret_cast<const uint16_t*>(d16 + 2 * G) << 16;
-        e1 = *reinterpret_cast<const uint16_t*>(d16 + 16 * G) |
-             (uint32_t)*reinterpret_cast<const uint16_t*>(d16 + 18 * G) << 16;
-      }
-      if (!whole) {  // rows that hold nothing yet: what their d and m are does not count
-        auto keep = [&](int r) { return sg.valid - r >= 2 ? 0xffffffffu : sg.valid - r == 1 ? 0xffffu : 0u; };
-        v0 &= keep(r0 + 2 * t);
-        e0 &= keep(r0 + 2 * t);
-        v1 &= keep(r0 + 8 + 2 * t);
-        e1 &= keep(r0 + 8 + 2 * t);
-#pragma unroll
-        for (int i = 0; i < G; ++i)
-          if (sg.valid - rw < (i < G / 2 ? 1 : 2)) dw[i] = 0u;
-      }
-      // hi and lo of the weights (a, b) of this lane's head to the lanes of B's columns
-      auto columns = [&](float a, float b, uint32_t& b0, uint32_t& b1) {
-        uint32_t hi, lo;
-        split2(a, b, hi, lo);
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? hi : lo, 4);
-        b0 = odd ? got : hi;
-        b1 = odd ? lo : got;
-      };
-      {
-        uint32_t a[4];
-        middle(e0, v0, a[0], a[1]);
-        middle(e1, v1, a[2], a[3]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint32_t b0, b1;
-          columns(pa[n], pb[n], b0, b1);
-          mma_f16(om[n], a, b0, b1);
-        }
-      }
-#pragma unroll
-      for (int P = 0; P < B::kPlanes; ++P) {
-        uint32_t w0[J], w1[J];
-        lds_words<J>(vb + 2 * B::v_half(r0 + 2 * t, P * J, g), w0);
-        lds_words<J>(vb + 2 * B::v_half(r0 + 8 + 2 * t, P * J, g), w1);
-#pragma unroll
-        for (int i = 0; i < J; ++i) {
-          const int j = P * J + i;
-          const uint32_t a0[4] = {centred(w0[i] << 4), centred(w0[i]), centred(w1[i] << 4), centred(w1[i])};
-          const uint32_t a1[4] = {centred(w0[i] >> 4), centred(w0[i] >> 8), centred(w1[i] >> 4), centred(w1[i] >> 8)};
-          const float da = half_of(dw[j / 2], j & 1), db = half_of(dw[(G + j) / 2], j & 1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b0, b1;
-            columns(pa[n] * da, pb[n] * db, b0, b1);
-            mma_f16(o[n][2 * j], a0, b0, b1);
-            mma_f16(o[n][2 * j + 1], a1, b0, b1);
-          }
-        }
-      }
-      if (++since == kFlush) flush();
+    next();
+    const int at1 = st;
+    if (take == 2) {
+      if (!landed()) return;
+      valid[1] = seg[st].valid;
+      blocks[1] = smem + (size_t)st * p.stage_bytes;
+      next();
     }
+    if (16 * warp < valid[1])
+      rows(std::integral_constant<int, 2>{}, blocks, valid);
+    else if (16 * warp < valid[0])
+      rows(std::integral_constant<int, 1>{}, blocks, valid);
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
-    if (!(sg.flags & 2)) continue;
+    if (lane == 0) {
+      mbar_arrive(&empty[at0]);
+      if (take == 2) mbar_arrive(&empty[at1]);
+    }
+    u += take;
+    since += take;
+    if (sg.left > take) {
+      if (since >= kFlush) flush();
+      continue;
+    }
 
     // ---------------- end of the segment: join the warps in order
 #pragma unroll
