@@ -447,8 +447,8 @@ int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_
  * query heads per KV head; scale 0 = 1/sqrt(head_dim). q, out: rows of n_heads*head_dim values
  * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros. Scores and sums
  * carry 32-bit accuracy whatever the type. workspace: rrr_kv4_workspace bytes of device
- * memory, zeroed once before its first use (the kernel leaves its counters zero); calls
- * that can run at the same time, replays of captured graphs among them, need one each. */
+ * memory, whatever they hold; calls that can run at the same time, replays of captured
+ * graphs among them, need one each. */
 int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t* bytes);
 int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int type, const void* q,
                       int64_t q_stride, const int32_t* kv_lens, float scale, void* out,

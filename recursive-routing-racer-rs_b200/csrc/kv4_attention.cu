@@ -25,11 +25,10 @@
 // contiguous, with bulk copies into a ring of stages, the segment's query row with its first
 // page; four consumer warps take 16 rows of a page each and keep their own softmax state. At
 // the end of a (sequence, head) segment the warps' states are joined in order; a segment that
-// other CTAs share goes to the workspace, and the CTA that finishes last joins the parts in
-// order (so results do not depend on which one that is) and leaves the counter at zero.
+// other CTAs share goes to the workspace, and a second small kernel joins the parts in order. (The
+// CTA that finishes last did that first, found by a counter: 6 of 14 us at one short sequence,
+// most of it instructions that no SM had executed before, by one CTA per head.)
 #include <math.h>
-
-#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -53,8 +52,8 @@ struct Kv4Params {
   int64_t q_stride, out_stride;
   const int* lens;
   float scale;  // with log2(e)
-  unsigned* counters;
-  float* parts;
+  int2* runs;    // [seq][head]: first CTA and CTAs of its pages
+  float* parts;  // [CTA][2][hpk * (HD + 2)]: sums, maxima, weights' sums
   int stages, stage_bytes;
   int* err;
 };
@@ -150,6 +149,22 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// The producer's wait for a free stage, bounded: with several stages ahead it is in no hurry, and
+// a wait that polls takes issue slots from the consumers (measured: a third of all
+// instructions), so it sleeps between its polls.
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(err);
+  for (;;) {
+    __nanosleep(400);
+    if (mbar_try_wait(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > limit) {
+      if (err) atomicCAS(err, 0, code);
+      return false;
+    }
+  }
+}
+
 // The consumer warps' barrier, bounded.
 struct ConsumerSync {
   uint64_t* bar;
@@ -176,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   __shared__ float wm[kConsumers][kMaxHpk], wl[kConsumers][kMaxHpk];
   __shared__ long long warp_units[kConsumers + 1];
   __shared__ long long first_base;  // unit of the first sequence's first page
-  __shared__ int first_seq, is_last;
+  __shared__ int first_seq;
   float* wo = reinterpret_cast<float*>(smem + (size_t)p.stages * p.stage_bytes);  // [warp][hpk][PITCH]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         if (lane == 0) flag_position(p.err);
         valid = 0;
       }
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], phase, p.err, kDevErrEmptyTimeout));
+      ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)wait_asleep(&empty[st], phase, p.err, kDevErrEmptyTimeout) : 0, 0);
       if (!ok) break;
       if (lane == 0) {
         const bool first = u == u0 || page == 0;
@@ -299,8 +314,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     return;
   }
 
-  // ---------------- consumers: warp w takes rows 16w .. 16w + 15 of every page, of two pages at a
-  // time where the run has them
+  // ---------------- consumers: warp w takes rows 16w .. 16w + 15 of every page
   // Fragments of lane (g, t): A rows g and g + 8, k slots 2t, + 1 and 2t + 8, + 9; B the same
   // slots of column g, that is of head g / 2's hi (g even) or lo part; C rows g, g + 8 of columns
   // 2t, 2t + 1, that is of head t. Tile n holds the heads 4n .. 4n + 3.
@@ -361,15 +375,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     b1 = odd ? lo : got;
   };
 
-  // this warp's rows of NS pages
-  auto rows = [&](auto ns, const uint8_t* const* blocks, const int* valid) {
-    constexpr int NS = decltype(ns)::value;
+  // this warp's rows of a page (two pages at a time, for more independent work, measured 7 %
+  // slower: the loop outgrows the instruction cache)
+  auto rows = [&](const uint8_t* blk, int valid) {
     const int r0 = 16 * warp;
     // ---- scores of rows r0 + g, r0 + 8 + g for head t of every tile
-    float s[NS][NT][2];
-#pragma unroll
-    for (int x = 0; x < NS; ++x) {
-      const uint8_t* blk = blocks[x];
+    float s[NT][2];
+    {
       const int ra = r0 + g, rb = ra + 8;
       uint32_t da[G / 2], db[G / 2];  // f16 pairs of groups
       lds_words<G / 2>(blk + B::kCodes + 2 * B::scale(ra, 0), da);
@@ -380,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         ma[1] = *reinterpret_cast<const uint32_t*>(blk + B::kCodes + B::kScales + 2 * B::scale(rb, 2 * t));
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[x][n][0] = s[x][n][1] = 0.f;
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = 0.f;
 #pragma unroll
       for (int P = 0; P < B::kPlanes; ++P) {
         uint32_t wa[J], wb[J];
@@ -400,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
             float c[4];
             mma_f16(c, a0, qb[n][j][0], qb[n][j][1], init);
             mma_f16(c, a1, qb[n][j][2], qb[n][j][3]);
-            s[x][n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[x][n][0]);
-            s[x][n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[x][n][1]);
+            s[n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[n][0]);
+            s[n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[n][1]);
           }
         }
       }
@@ -410,25 +422,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         float c[4];
         mma_f16(c, ma, qm[n], 0u, zero);
-        s[x][n][0] = fmaf(s[x][n][0], 16.f, fmaf(c[1], kLo, c[0])) * kscale[n];
-        s[x][n][1] = fmaf(s[x][n][1], 16.f, fmaf(c[3], kLo, c[2])) * kscale[n];
+        s[n][0] = fmaf(s[n][0], 16.f, fmaf(c[1], kLo, c[0])) * kscale[n];
+        s[n][1] = fmaf(s[n][1], 16.f, fmaf(c[3], kLo, c[2])) * kscale[n];
       }
-      if (r0 + 16 > valid[x]) {
+      if (r0 + 16 > valid) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (r0 + 8 * i + g >= valid[x]) s[x][n][i] = -INFINITY;
+            if (r0 + 8 * i + g >= valid) s[n][i] = -INFINITY;
       }
     }
     // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
     // rows 2t, 2t + 1 of the first (g even) or second eight rows
-    float pa[NS][NT], pb[NS][NT], alpha[NT];
+    float pa[NT], pb[NT], alpha[NT];
     bool grow = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top = fmaxf(s[0][n][0], s[0][n][1]);
-      if constexpr (NS == 2) top = fmaxf(top, fmaxf(s[1][n][0], s[1][n][1]));
+      float top = fmaxf(s[n][0], s[n][1]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -436,16 +447,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       alpha[n] = ex2(m[n] - m_use);
       grow |= m_new > m[n];
       m[n] = m_new;
-      l[n] *= alpha[n];
-#pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        const float p0 = ex2(s[x][n][0] - m_use), p1 = ex2(s[x][n][1] - m_use);
-        l[n] += p0 + p1;
+      {
+        const float p0 = ex2(s[n][0] - m_use), p1 = ex2(s[n][1] - m_use);
+        l[n] = fmaf(l[n], alpha[n], p0 + p1);
         const int from = 8 * t + (g >> 1);
         const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
         const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
-        pa[x][n] = odd ? a1 : a0;
-        pb[x][n] = odd ? b1 : b0;
+        pa[n] = odd ? a1 : a0;
+        pb[n] = odd ? b1 : b0;
       }
     }
     if (__any_sync(0xffffffffu, grow)) {
@@ -461,15 +470,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       }
     }
     // ---- weighted rows
-#pragma unroll
-    for (int x = 0; x < NS; ++x) {
-      const uint8_t* vb = blocks[x] + B::kHalf;
+    {
+      const uint8_t* vb = blk + B::kHalf;
       const int rw = r0 + 2 * t + (odd ? 8 : 0);  // rows of pa, pb
       uint32_t dw[G], mw[G];                      // f16 d [row][group]; m [group][row]
       lds_words<G>(vb + B::kCodes + 2 * B::scale(rw, 0), dw);
       lds_words<G>(vb + B::kCodes + B::kScales + 2 * B::v_min(rw, 0), mw);
-      if (r0 + 16 > valid[x]) {  // rows that hold nothing yet: what their d and m are does not count
-        const int n = valid[x] - rw;
+      if (r0 + 16 > valid) {  // rows that hold nothing yet: what their d and m are does not count
+        const int n = valid - rw;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
           if (n < (i < G / 2 ? 1 : 2)) dw[i] = 0u;
@@ -493,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             uint32_t b0, b1;
-            columns(pa[x][n] * da, pb[x][n] * db, b0, b1);
+            columns(pa[n] * da, pb[n] * db, b0, b1);
             mma_f16(o[n][2 * j], a0, b0, b1);
             mma_f16(o[n][2 * j + 1], a1, b0, b1);
-            om[n][j] = fmaf(pa[x][n], ca, fmaf(pb[x][n], cb, om[n][j]));
+            om[n][j] = fmaf(pa[n], ca, fmaf(pb[n], cb, om[n][j]));
           }
         }
       }
@@ -514,12 +522,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       phase ^= 1;
     }
   };
-  for (long long u = u0; u < u1;) {
+  for (long long u = u0; u < u1; ++u) {
     if (!landed()) return;
     const Segment sg = seg[st];
-    const int at0 = st, take = sg.left > 1 ? 2 : 1;
-    const uint8_t* blocks[2] = {smem + (size_t)st * p.stage_bytes, nullptr};
-    int valid[2] = {sg.valid, 0};
+    const uint8_t* blk = smem + (size_t)st * p.stage_bytes;
     if (sg.first) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -527,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         const int h = 4 * n + (g >> 1);
         float x[G][8];
         float top = 0.f;
-        const T* q = reinterpret_cast<const T*>(blocks[0] + B::kBytes) + h * HD + 8 * t;
+        const T* q = reinterpret_cast<const T*>(blk + B::kBytes) + h * HD + 8 * t;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           if (h < p.hpk) {
@@ -584,27 +590,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       held = false;
       since = 0;
     }
-    next();
-    const int at1 = st;
-    if (take == 2) {
-      if (!landed()) return;
-      valid[1] = seg[st].valid;
-      blocks[1] = smem + (size_t)st * p.stage_bytes;
-      next();
-    }
-    if (16 * warp < valid[1])
-      rows(std::integral_constant<int, 2>{}, blocks, valid);
-    else if (16 * warp < valid[0])
-      rows(std::integral_constant<int, 1>{}, blocks, valid);
+    if (16 * warp < sg.valid) rows(blk, sg.valid);
     __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(&empty[at0]);
-      if (take == 2) mbar_arrive(&empty[at1]);
-    }
-    u += take;
-    since += take;
-    if (sg.left > take) {
-      if (since >= kFlush) flush();
+    if (lane == 0) mbar_arrive(&empty[st]);
+    next();
+    if (sg.left > 1) {
+      if (++since == kFlush) flush();
       continue;
     }
 
@@ -621,9 +612,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     }
     flush();
     if (!sync()) return;
-    // participants of this (sequence, head)
+    // the CTAs of this (sequence, head)
     const long long last_unit = sg.base + sg.pages - 1;
     const int c0 = (int)(((sg.base + 1) * grid - 1) / U), c1 = (int)(((last_unit + 1) * grid - 1) / U);
+    if (sg.first_page == 0 && threadIdx.x == 0) p.runs[(size_t)sg.seq * p.nkv + sg.head] = make_int2(c0, c1 - c0 + 1);
     const bool alone = c0 == c1;
     const size_t part_floats = (size_t)p.hpk * (HD + 2);
     float* part = p.parts + (size_t)(2 * blockIdx.x + (sg.first_page == 0 ? 1 : 0)) * part_floats;
@@ -651,59 +643,82 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         }
       }
     }
-    if (!alone) {
-      __threadfence();
-      if (!sync()) return;
-      if (threadIdx.x == 0) {
-        const unsigned n = (unsigned)(c1 - c0);
-        is_last = atomicInc(&p.counters[(size_t)sg.seq * p.nkv + sg.head], n) == n;
-        __threadfence();
-      }
-      if (!sync()) return;
-      if (is_last) {
-        // the parts in order (the one that starts the (sequence, head) is its CTA's slot 1, the
-        // others slot 0): a warp per head finds the maximum and the sum, then every thread joins
-        // four values, eight parts' loads in flight
-        const float* first = p.parts + (size_t)(2 * c0 + 1) * part_floats;
-        const float* rest = p.parts + (size_t)(2 * c0) * part_floats;
-        auto part_of = [&](int i) { return i == 0 ? first : rest + (size_t)(2 * i) * part_floats; };
-        const int n = c1 - c0 + 1, stat = p.hpk * HD;
-        for (int h = warp; h < p.hpk; h += kConsumers) {
-          float M = -INFINITY, L = 0.f;
-          for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(part_of(i) + stat + h));
-#pragma unroll
-          for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-          const float Mu = M == -INFINITY ? 0.f : M;
-          for (int i = lane; i < n; i += 32)
-            L = fmaf(ex2(__ldcg(part_of(i) + stat + h) - Mu), __ldcg(part_of(i) + stat + p.hpk + h), L);
-          L = warp_sum(L);
-          if (lane == 0) {
-            wm[0][h] = Mu;
-            wl[0][h] = L;
-          }
-        }
-        if (!sync()) return;
-        for (int e = 4 * threadIdx.x; e < stat; e += 4 * 32 * kConsumers) {
-          const int h = e / HD;
-          const float Mu = wm[0][h], L = wl[0][h];
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-          for (int i = 0; i < n; ++i) {
-            const float* q = part_of(i);
-            const float w = ex2(__ldcg(q + stat + h) - Mu);
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(q + e)), y = __ldcg(reinterpret_cast<const float2*>(q + e + 2));
-            v[0] = fmaf(w, x.x, v[0]);
-            v[1] = fmaf(w, x.y, v[1]);
-            v[2] = fmaf(w, y.x, v[2]);
-            v[3] = fmaf(w, y.y, v[3]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = L == 0.f ? 0.f : v[i] / L;
-          store_vec<T, 4>(out + e, v);
-        }
-      }
-    }
     if (!sync()) return;  // the joined states are read: the next segment may write its own
+  }
+}
+
+// Joins the parts of one (sequence, head) per CTA: 128 threads take four values each, kGroups such
+// groups each kGroups-th part, many loads in flight; the groups' sums are added in order.
+constexpr int kGroups = 4;
+template <typename T>
+__global__ void __launch_bounds__(128 * kGroups) kv4_join_kernel(const __grid_constant__ Kv4Params p, int hd) {
+  __shared__ float wm[kMaxHpk], wl[kMaxHpk];
+  __shared__ float4 sums[kGroups][128];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int2 run = p.runs[blockIdx.x];
+  const int n = run.y, stat = p.hpk * hd;
+  if (n < 2) return;
+  const size_t part_floats = (size_t)p.hpk * (hd + 2);
+  // the part that starts the (sequence, head) is its CTA's slot 1, the others slot 0
+  const float* base = p.parts + (size_t)2 * run.x * part_floats;
+  auto part_of = [&](int i) { return base + (size_t)(2 * i + (i == 0 ? 1 : 0)) * part_floats; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < p.hpk) {
+    float M = -INFINITY, L = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float pm = __ldcg(part_of(i) + stat + warp), pl = __ldcg(part_of(i) + stat + p.hpk + warp);
+      const float Mn = fmaxf(M, pm), Mu = Mn == -INFINITY ? 0.f : Mn;
+      L = fmaf(L, ex2(M - Mu), pl * ex2(pm - Mu));
+      M = Mn;
+    }
+    float top = M;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float Mu = top == -INFINITY ? 0.f : top;
+    L = warp_sum(L * ex2(M - Mu));
+    if (lane == 0) {
+      wm[warp] = Mu;
+      wl[warp] = L;
+    }
+  }
+  __syncthreads();
+  const int col = threadIdx.x & 127, group = threadIdx.x >> 7;
+  const int seq = blockIdx.x / p.nkv, head = blockIdx.x % p.nkv;
+  T* out = static_cast<T*>(p.out) + seq * p.out_stride + (int64_t)head * stat;
+  for (int e0 = 0; e0 < stat; e0 += 512) {
+    const int e = e0 + 4 * col, h = e / hd;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (e < stat) {
+      const float Mu = wm[h];
+#pragma unroll 8
+      for (int i = group; i < n; i += kGroups) {
+        const float* q = part_of(i);
+        const float w = ex2(__ldcg(q + stat + h) - Mu);
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(q + e)), y = __ldcg(reinterpret_cast<const float2*>(q + e + 2));
+        v[0] = fmaf(w, x.x, v[0]);
+        v[1] = fmaf(w, x.y, v[1]);
+        v[2] = fmaf(w, y.x, v[2]);
+        v[3] = fmaf(w, y.y, v[3]);
+      }
+      sums[group][col] = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    __syncthreads();
+    if (group == 0 && e < stat) {
+#pragma unroll
+      for (int k = 1; k < kGroups; ++k) {
+        const float4 x = sums[k][col];
+        v[0] += x.x;
+        v[1] += x.y;
+        v[2] += x.z;
+        v[3] += x.w;
+      }
+      const float L = wl[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = L == 0.f ? 0.f : v[i] / L;
+      store_vec<T, 4>(out + e, v);
+    }
+    __syncthreads();
   }
 }
 
@@ -722,7 +737,9 @@ cudaError_t launch(const LaunchEnv& env, Kv4Params p) {
   const int64_t units = (int64_t)p.n_seqs * p.nkv * (p.max_pages > 0 ? p.max_pages : 1);
   const int ctas = env.sm_count * kCtas;
   const int grid = (int)(units < ctas ? units : ctas);
-  return rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl, p);
+  e = rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl, p);
+  if (e != cudaSuccess || p.max_pages < 2) return e;  // a single page is one CTA's
+  return rrr_launch_pdl(kv4_join_kernel<T>, dim3(p.n_seqs * p.nkv), dim3(128 * kGroups), 0, env.stream, env.pdl, p, HD);
 }
 template <int HD, typename T>
 cudaError_t launch_tiles(const LaunchEnv& env, const Kv4Params& p) {
@@ -737,7 +754,7 @@ cudaError_t launch_type(const LaunchEnv& env, int type, const Kv4Params& p) {
   }
 }
 
-int64_t counter_bytes(const rrr_kv4_cache* c) { return ((int64_t)c->n_seqs * c->n_kv_heads * 4 + 255) / 256 * 256; }
+int64_t run_bytes(const rrr_kv4_cache* c) { return ((int64_t)c->n_seqs * c->n_kv_heads * 8 + 255) / 256 * 256; }
 
 int check_heads(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, const char* fn) {
   if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > kMaxHpk)
@@ -760,7 +777,7 @@ int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t
   if (rc || (rc = check_heads(ctx, c, n_heads, fn))) return rc;
   if (!bytes) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t parts = 2 * 3 * (int64_t)ctx->sm_count;  // two per CTA, at most three CTAs per SM
-  *bytes = counter_bytes(c) + parts * (n_heads / c->n_kv_heads) * (c->head_dim + 2) * 4;
+  *bytes = run_bytes(c) + parts * (n_heads / c->n_kv_heads) * (c->head_dim + 2) * 4;
   return RRR_OK;
 }
 
@@ -808,8 +825,8 @@ int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int typ
   p.out_stride = out_stride;
   p.lens = kv_lens;
   p.scale = (scale == 0.f ? 1.f / sqrtf((float)c->head_dim) : scale) * 1.4426950408889634f;
-  p.counters = static_cast<unsigned*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(c));
+  p.runs = static_cast<int2*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + run_bytes(c));
   p.err = env.d_err;
   cudaError_t e;
   switch (c->head_dim) {

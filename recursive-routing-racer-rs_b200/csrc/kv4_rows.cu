@@ -20,10 +20,11 @@ int check_kv4_cache(rrr_ctx* ctx, const rrr_kv4_cache* c, const char* fn) {
   if (!c || !c->pages || !c->page_table) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   if ((c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) || c->n_kv_heads < 1 ||
       c->n_kv_heads > 65535 || c->n_pages < 0 || c->n_seqs < 0 || c->max_pages < 0 ||
-      c->max_pages > INT32_MAX / kPageRows || c->table_stride < c->max_pages)
+      c->max_pages > INT32_MAX / kPageRows || c->table_stride < c->max_pages ||
+      (int64_t)c->n_seqs * c->n_kv_heads > INT32_MAX)
     return set_error(ctx, RRR_ERR_BAD_SHAPE,
                      "%s: need head_dim 64/128/256, 1 <= n_kv_heads <= 65535, counts >= 0, table_stride >= "
-                     "max_pages and at most 2^31 - 64 rows per sequence",
+                     "max_pages, at most 2^31 - 64 rows per sequence and 2^31 - 1 sequences times heads",
                      fn);
   if (!aligned_to(c->pages, 16) || !aligned_to(c->page_table, 4))
     return set_error(ctx, RRR_ERR_MISALIGNED, "%s: pages must be 16-byte aligned", fn);

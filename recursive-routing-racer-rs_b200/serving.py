@@ -160,11 +160,11 @@ class KV4Cache:
                                               _stream(stream)))
 
     def workspace(self, n_heads: int):
-        """A zeroed workspace for `attention`; calls that can run at the same time need one each."""
+        """A workspace for `attention`; calls that can run at the same time need one each."""
         import torch
         n = c_int64()
         self.ctx.check(ffi.lib().rrr_kv4_workspace(self.ctx.h, byref(self.desc), n_heads, byref(n)))
-        return torch.zeros(n.value, dtype=torch.uint8, device=self.pages.device)
+        return torch.empty(n.value, dtype=torch.uint8, device=self.pages.device)
 
     def attention(self, q, kv_lens, out, workspace, scale: float = 0.0, stream=None):
         """rrr_attention_kv4: q, out [n_seqs, n_heads, hd], one query row per sequence."""
