@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include "serve_common.cuh"
+#include "tile_common.cuh"
 
 namespace rrr {
 namespace {
@@ -39,12 +40,11 @@ struct Tile {
   int seq, q0, q1, row0;  // the sequence's query rows [q0, q1), the tile's first
   int k0, k1;             // its KV rows
 };
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(const PackedParams& p, int x, Tile& t) {
-  int lo = 0, hi = p.n_seqs - 1;  // the last s with cu[s] / ROWS + s <= x
+__device__ __forceinline__ bool find_tile(const PackedParams& p, int rows, int x, Tile& t) {
+  int lo = 0, hi = p.n_seqs - 1;  // the last s with cu[s] / rows + s <= x
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] / ROWS + mid <= x)
+    if (p.cu_q[mid] / rows + mid <= x)
       lo = mid;
     else
       hi = mid - 1;
@@ -58,7 +58,7 @@ __device__ __forceinline__ bool find_tile(const PackedParams& p, int x, Tile& t)
     if (threadIdx.x == 0) flag_position(p.err);
     return false;
   }
-  const int64_t row0 = t.q0 + (int64_t)ROWS * (x - (t.q0 / ROWS + lo));
+  const int64_t row0 = t.q0 + (int64_t)rows * (x - (t.q0 / rows + lo));
   if (row0 < t.q0 || row0 >= t.q1) return false;
   t.row0 = (int)row0;
   return true;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const __grid_constant_
   pdl_launch_dependents();
   pdl_wait();
   Tile t;
-  if (!find_tile<kQRows>(p, (int)(gridDim.x - 1 - blockIdx.x), t)) return;
+  if (!find_tile(p, kQRows, (int)(gridDim.x - 1 - blockIdx.x), t)) return;
   const int head = blockIdx.y, kv = head / p.hpk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int rows = min(kQRows, t.q1 - t.row0);
@@ -280,6 +280,413 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const __grid_constant_
   }
 }
 
+// ---- head_dim 64 and 128: tcgen05 ---------------------------------------------------------
+//
+// A CTA takes two tiles of 128 (query row, head) pairs that share a KV head, heads innermost:
+// floor(128 / hpk) rows of hpk heads each, one TMA box; so grouped heads fill the tensor
+// core's 128 rows whatever their number, and the rows of a tile end near the same KV row.
+// Warps 0-3 and 4-7 are the tiles' softmax (one thread per tile row), warp 8 issues the MMAs,
+// warp 9 the copies. Per 128 KV rows and tile: S = Q K^T (128 x 128 f32 in TMEM); a thread
+// reads its row of S, takes its maximum, writes p in 16 bits over S, packed two a column, as
+// the A operand of O += P V, whose accumulator stays in TMEM. The MMA thread alternates the
+// tiles (P0 V, next S0, P1 V, next S1), so that one tile's products run during the other's
+// softmax. O is rescaled only when a row's maximum has grown by over 2^kLazy since its last
+// rescale: until then the weights are at most 2^kLazy, which neither 16-bit type rounds worse
+// than values up to one.
+// V rows behind the sequence are zeroed in shared memory before their product: other
+// sequences' values, or none, may be anything.
+constexpr int kTcThreads = 384;  // warps 10 and 11 only complete the third warpgroup
+constexpr int kTile = 128;   // MMA rows, and KV rows per block
+constexpr float kLazy = 8.f;
+
+struct TcParams {
+  PackedParams a;
+  int tokens;       // query rows per tile
+  int stages;
+  uint32_t idesc_s, idesc_o;
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  umma_bf16(d_tmem, a_desc, b_desc, idesc, accumulate);  // kind::f16: the types are in idesc
+}
+// The same with A in TMEM: 128 lanes, two 16-bit elements of K per 32-bit column
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of an operand whose rows (K) of 64 elements lie 128 bytes apart, 128-byte swizzled
+// (N contiguous): 8 rows every 1024 bytes (stride offset), the next 64 elements of N after
+// `lead` bytes (leading offset).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+      : "memory");
+}
+// 32 columns of this thread's TMEM lane, without the wait
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcParams tp) {
+  constexpr int kChunks = HD / 64;                  // 128-byte wide pieces of a head
+  constexpr uint32_t kPiece = kTile * 128;          // bytes of one
+  constexpr uint32_t kOperand = kChunks * kPiece;   // a tile of Q, K or V
+  constexpr int kMaxStages = 4;
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint64_t q_full, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  __shared__ uint64_t s_full[2], p_full[2], o_full[2], fin;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const PackedParams& p = tp.a;
+  uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
+  uint8_t* qs = smem;
+  uint8_t* ks = smem + 2 * kOperand;
+  uint8_t* vs = ks + (size_t)tp.stages * kOperand;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  Tile t;
+  const int both = 2 * tp.tokens, nkv = p.nh / p.hpk;
+  if (!find_tile(p, both, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
+  const int kv = blockIdx.x % nkv;
+  const int rows = min(both, t.q1 - t.row0);
+  // blocks of KV rows of each tile: up to what its last row sees
+  int blocks[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min(rows, (i + 1) * tp.tokens) - 1;
+    blocks[i] = last >= i * tp.tokens ? (seen_by(p, t, t.row0 + last) + kTile - 1) / kTile : 0;
+  }
+  const int n = max(blocks[0], blocks[1]);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < tp.stages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(&fin, 1);
+    abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 8) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t s_col[2] = {tmem, tmem + kTile}, o_col[2] = {tmem + 2 * kTile, tmem + 2 * kTile + HD};
+
+  // registers: 384 x 168 at launch = 256 x 232 + 128 x 40
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  if (warp == 9) {
+    // ---------------- copies
+    int issued = 0;
+    bool ok = true;
+    if (lane == 0 && n > 0) {
+      const uint32_t box = (uint32_t)(tp.tokens * p.hpk) * 128u;
+      mbar_arrive_expect_tx(&q_full, 2 * kChunks * box);
+      for (int i = 0; i < 2; ++i)
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d(qs + i * kOperand + c * kPiece, &qmap, 64 * c, kv * p.hpk, t.row0 + i * tp.tokens, &q_full);
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const int s = j % tp.stages;
+      const uint32_t ph = (uint32_t)(j / tp.stages + 1) & 1u;  // the first round finds the stages free
+      for (int which = 0; which < 2; ++which) {
+        uint64_t* empty = which ? &v_empty[s] : &k_empty[s];
+        ok = !warp_aborted(&abort_flag) && warp_wait(empty, ph, p.err);
+        if (!ok) {
+          abort_flag = 1;
+          break;
+        }
+        if (lane == 0) {
+          uint64_t* full = which ? &v_full[s] : &k_full[s];
+          uint8_t* dst = (which ? vs : ks) + (size_t)s * kOperand;
+          mbar_arrive_expect_tx(full, kOperand);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(dst + c * kPiece, which ? &vmap : &kmap, 64 * c, kv, t.k0 + j * kTile, full);
+        }
+        __syncwarp();
+        ++issued;
+      }
+    }
+    // copies in flight land before the CTA leaves
+    if (n > 0) warp_wait(&q_full, 0, p.err);
+    for (int s = 0; s < tp.stages; ++s) {
+      const int ki = (issued + 1) / 2, vi = issued / 2;  // issued K and V tiles
+      const int ku = ki > s ? (ki - s + tp.stages - 1) / tp.stages : 0;
+      const int vu = vi > s ? (vi - s + tp.stages - 1) / tp.stages : 0;
+      if (ku) warp_wait(&k_full[s], (uint32_t)(ku - 1) & 1u, p.err);
+      if (vu) warp_wait(&v_full[s], (uint32_t)(vu - 1) & 1u, p.err);
+    }
+  } else if (warp == 8) {
+    // ---------------- products
+    if (lane == 0) {
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!abort_flag && mbar_wait_bounded(bar, parity, p.err, kDevErrTileWait)) return true;
+        abort_flag = 1;
+        return false;
+      };
+      auto scores = [&](int i, int j) {  // S_i = Q_i K_j^T
+        const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ks + (size_t)(j % tp.stages) * kOperand);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk / 4) * kPiece + 32u * (kk % 4);
+          umma_f16(s_col[i], sw128_desc(qa + off), sw128_desc(ka + off), tp.idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[i]);
+      };
+      bool ok = n == 0 || (wait(&q_full, 0) && wait(&k_full[0], 0));
+      if (ok && n > 0) {
+        tc_fence_after();
+        for (int i = 0; i < 2; ++i)
+          if (blocks[i] > 0) scores(i, 0);
+        umma_commit(&k_empty[0]);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int s = j % tp.stages, s1 = (j + 1) % tp.stages;
+        ok = (j + 1 >= n || wait(&k_full[s1], (uint32_t)((j + 1) / tp.stages) & 1u)) &&
+             wait(&v_full[s], (uint32_t)(j / tp.stages) & 1u);
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j >= blocks[i]) continue;
+          ok = wait(&p_full[i], (uint32_t)j & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = smem_addr(vs + (size_t)s * kOperand);
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            umma_f16_ta(o_col[i], s_col[i] + 8u * kk, sw128_desc_mn(va + 2048u * kk, kPiece), tp.idesc_o,
+                        j > 0 || kk > 0 ? 1u : 0u);
+          if (j + 1 < blocks[i])
+            scores(i, j + 1);
+          else
+            umma_commit(&o_full[i]);
+        }
+        if (ok) {
+          umma_commit(&v_empty[s]);
+          if (j + 1 < n) umma_commit(&k_empty[s1]);
+        }
+      }
+      umma_commit(&fin);
+    }
+    __syncwarp();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // ---------------- softmax of tile i: thread r = row r
+    const int i = warp >> 2, r = threadIdx.x & 127;
+    const int token = r / p.hpk, head = kv * p.hpk + r % p.hpk;
+    const int row = t.row0 + i * tp.tokens + token;  // query row
+    const bool mine = token < tp.tokens && i * tp.tokens + token < rows;
+    const int seen = mine ? seen_by(p, t, row) : 0;
+    const int lk = t.k1 - t.k0;
+    const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t sc = s_col[i] + sub, oc = o_col[i] + sub;
+    const int end_block = (lk - 1) / kTile;
+    const bool zeroes = lk % kTile != 0 && i == (blocks[0] > end_block ? 0 : 1);
+    float m = -INFINITY;             // scaled, as of the last rescale
+    float2 l = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int j = 0; j < blocks[i]; ++j) {
+      if (warp_aborted(&abort_flag) || !warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
+        abort_flag = 1;
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t x[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) tmem_ld32(sc + c, x + c);
+      tmem_wait_ld();
+      float* s = reinterpret_cast<float*>(x);
+      if (__any_sync(0xffffffffu, (j + 1) * kTile > seen)) {
+#pragma unroll
+        for (int c = 0; c < kTile; ++c)
+          if (j * kTile + c >= seen) s[c] = -INFINITY;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kTile; c += 4)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[c + k]);
+      const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
+      if (__any_sync(0xffffffffu, m_new > m + kLazy || (m == -INFINITY && m_new > m))) {
+        const bool grow = m_new > m;
+        const float next = grow ? m_new : m;
+        const float alpha = grow ? ex2(m - next) : 1.f;
+        m = next;
+        l.x *= alpha;
+        l.y *= alpha;
+        if (j > 0) {
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(oc + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+            tmem_st32(oc + c, v);
+          }
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m;
+      const float2 scale2 = make_float2(p.scale, p.scale), neg2 = make_float2(neg, neg);
+      uint32_t w[32];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float2 e = __ffma2_rn(make_float2(s[64 * half + 2 * c], s[64 * half + 2 * c + 1]), scale2, neg2);
+          const float2 q = make_float2(ex2(e.x), ex2(e.y));
+          l = __fadd2_rn(l, q);
+          w[c] = Mma<T>::pack(q.x, q.y);
+        }
+        tmem_st32(sc + 32 * half, w);
+      }
+      if (zeroes && j == end_block) {
+        // V rows behind the sequence
+        if (!warp_wait(&v_full[j % tp.stages], (uint32_t)(j / tp.stages) & 1u, p.err)) {
+          abort_flag = 1;
+          ok = false;
+          break;
+        }
+        uint8_t* v = vs + (size_t)(j % tp.stages) * kOperand;
+        const int from = lk - j * kTile;
+        for (int c = 0; c < kChunks; ++c)
+          for (int k = (threadIdx.x & 127); k < (kTile - from) * 8; k += 128)
+            *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[i]);
+    }
+    // ---------------- out
+    if (ok && i * tp.tokens < rows) {
+      const float sum = l.x + l.y;
+      const float inv = seen > 0 ? 1.f / sum : 0.f;
+      T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head;
+      bool bad = false;
+      if (blocks[i] > 0) {
+        ok = warp_wait(&o_full[i], 0, p.err);
+        if (!ok) abort_flag = 1;
+      }
+      if (ok) {
+        tc_fence_after();
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t v[32];
+          if (blocks[i] > 0) {
+            tmem_ld32(oc + c, v);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float a = seen > 0 ? __uint_as_float(v[k + 2 * e]) * inv : 0.f;
+              const float b = seen > 0 ? __uint_as_float(v[k + 2 * e + 1]) * inv : 0.f;
+              bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
+              o[e] = Mma<T>::pack(a, b);
+            }
+            if (mine) *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        unsigned again = __ballot_sync(0xffffffffu, bad && mine);
+        while (again) {
+          const int from = __ffs(again) - 1;
+          again &= again - 1;
+          __syncwarp();
+          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, head, from));
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    warp_wait(&fin, 0u, p.err);  // no product still runs when its TMEM is freed
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Tensor map of rows of heads: {head_dim, heads, rows}, boxes of 64 x box_heads x box_rows.
+bool encode_heads(CUtensorMap* map, int type, const void* base, int hd, int64_t heads, int64_t rows, int64_t head_stride,
+                  int64_t row_stride, int box_heads, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, estr[3] = {1, 1, 1};
+  return fn(map, type == RRR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, typename T>
+cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
+  TcParams tp{};
+  tp.a = p;
+  tp.tokens = kTile / p.hpk;
+  constexpr int kOperand = kTile * HD * 2;
+  tp.stages = HD == 128 ? 2 : 4;
+  const int smem = (2 + 2 * tp.stages) * kOperand + 1024;
+  const uint32_t fmt = type == RRR_F16 ? 0u : 1u;
+  // f32 accumulator, A and B of the type, B of the second product N-contiguous, N / 8, M / 16
+  tp.idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+  tp.idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) |
+               ((uint32_t)(kTile >> 4) << 24);
+  CUtensorMap qmap, kmap, vmap;
+  const int64_t nkv = p.nh / p.hpk;
+  if (!encode_heads(&qmap, type, p.q, HD, p.nh, p.q_rows, p.q_head, p.q_row, p.hpk, tp.tokens) ||
+      !encode_heads(&kmap, type, p.k, HD, nkv, p.kv_rows, p.k_head, p.k_row, 1, kTile) ||
+      !encode_heads(&vmap, type, p.v, HD, nkv, p.kv_rows, p.v_head, p.v_row, 1, kTile))
+    return cudaErrorInvalidValue;
+  auto kern = packed_tc_kernel<HD, T>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int64_t slots = p.q_rows / (2 * tp.tokens) + p.n_seqs;
+  if (nkv * slots > INT32_MAX) return cudaErrorInvalidConfiguration;
+  return rrr_launch_pdl(kern, dim3((unsigned)(nkv * slots)), dim3(kTcThreads), (size_t)smem, env.stream, env.pdl,
+                        qmap, kmap, vmap, tp);
+}
+
 template <int HD, typename T>
 cudaError_t launch(const LaunchEnv& env, const PackedParams& p) {
   auto kern = packed_kernel<HD, T>;
@@ -291,6 +698,9 @@ cudaError_t launch(const LaunchEnv& env, const PackedParams& p) {
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, const PackedParams& p) {
+  if constexpr (HD < 256)
+    if (p.hpk <= kTile && p.kv_rows > 0)
+      return type == RRR_F16 ? launch_tc<HD, __half>(env, type, p) : launch_tc<HD, __nv_bfloat16>(env, type, p);
   return type == RRR_F16 ? launch<HD, __half>(env, p) : launch<HD, __nv_bfloat16>(env, p);
 }
 
