@@ -299,10 +299,15 @@ constexpr int kTcThreads = 384;  // warps 10 and 11 only complete the third warp
 constexpr int kTile = 128;   // MMA rows, and KV rows per block
 constexpr float kLazy = 8.f;
 
+// Stages of the ring of K and V tiles beside the two of Q: what fits. (Two stages of K and two of
+// V left the MMA thread waiting for copies half of the time: a copy had one block's time, and
+// 64 KB from the L2 take about that.)
+template <int HD>
+constexpr int tc_stages() { return HD == 128 ? 5 : 10; }
+
 struct TcParams {
   PackedParams a;
-  int tokens;       // query rows per tile
-  int stages;
+  int tokens;  // query rows per tile
   uint32_t idesc_s, idesc_o;
 };
 
@@ -354,17 +359,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int kChunks = HD / 64;                  // 128-byte wide pieces of a head
   constexpr uint32_t kPiece = kTile * 128;          // bytes of one
   constexpr uint32_t kOperand = kChunks * kPiece;   // a tile of Q, K or V
-  constexpr int kMaxStages = 4;
+  constexpr int kStages = tc_stages<HD>();          // one ring of K0, V0, K1, V1, ...
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ uint64_t q_full, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  __shared__ uint64_t q_full, full[kStages], empty[kStages];
   __shared__ uint64_t s_full[2], p_full[2], o_full[2], fin;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const PackedParams& p = tp.a;
   uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
   uint8_t* qs = smem;
-  uint8_t* ks = smem + 2 * kOperand;
-  uint8_t* vs = ks + (size_t)tp.stages * kOperand;
+  uint8_t* ring = smem + 2 * kOperand;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
@@ -385,11 +389,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    for (int s = 0; s < tp.stages; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -412,8 +414,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 9) {
     // ---------------- copies
-    int issued = 0;
-    bool ok = true;
     if (lane == 0 && n > 0) {
       const uint32_t box = (uint32_t)(tp.tokens * p.hpk) * 128u;
       mbar_arrive_expect_tx(&q_full, 2 * kChunks * box);
@@ -421,35 +421,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < kChunks; ++c)
           tma_load_3d(qs + i * kOperand + c * kPiece, &qmap, 64 * c, kv * p.hpk, t.row0 + i * tp.tokens, &q_full);
     }
-    for (int j = 0; j < n && ok; ++j) {
-      const int s = j % tp.stages;
-      const uint32_t ph = (uint32_t)(j / tp.stages + 1) & 1u;  // the first round finds the stages free
-      for (int which = 0; which < 2; ++which) {
-        uint64_t* empty = which ? &v_empty[s] : &k_empty[s];
-        ok = !warp_aborted(&abort_flag) && warp_wait(empty, ph, p.err);
-        if (!ok) {
-          abort_flag = 1;
-          break;
-        }
-        if (lane == 0) {
-          uint64_t* full = which ? &v_full[s] : &k_full[s];
-          uint8_t* dst = (which ? vs : ks) + (size_t)s * kOperand;
-          mbar_arrive_expect_tx(full, kOperand);
-          for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(dst + c * kPiece, which ? &vmap : &kmap, 64 * c, kv, t.k0 + j * kTile, full);
-        }
-        __syncwarp();
-        ++issued;
+    int issued = 0, s = 0;
+    uint32_t phase = 1;  // the first round finds the stages free
+    for (; issued < 2 * n; ++issued) {
+      if (warp_aborted(&abort_flag) || !warp_wait(&empty[s], phase, p.err)) {
+        abort_flag = 1;
+        break;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[s], kOperand);
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d(ring + (size_t)s * kOperand + c * kPiece, issued & 1 ? &vmap : &kmap, 64 * c, kv,
+                      t.k0 + (issued >> 1) * kTile, &full[s]);
+      }
+      __syncwarp();
+      if (++s == kStages) {
+        s = 0;
+        phase ^= 1;
       }
     }
     // copies in flight land before the CTA leaves
     if (n > 0) warp_wait(&q_full, 0, p.err);
-    for (int s = 0; s < tp.stages; ++s) {
-      const int ki = (issued + 1) / 2, vi = issued / 2;  // issued K and V tiles
-      const int ku = ki > s ? (ki - s + tp.stages - 1) / tp.stages : 0;
-      const int vu = vi > s ? (vi - s + tp.stages - 1) / tp.stages : 0;
-      if (ku) warp_wait(&k_full[s], (uint32_t)(ku - 1) & 1u, p.err);
-      if (vu) warp_wait(&v_full[s], (uint32_t)(vu - 1) & 1u, p.err);
+    for (int i = 0; i < kStages; ++i) {
+      const int uses = issued > i ? (issued - i + kStages - 1) / kStages : 0;
+      if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
     }
   } else if (warp == 8) {
     // ---------------- products
@@ -459,8 +454,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         abort_flag = 1;
         return false;
       };
-      auto scores = [&](int i, int j) {  // S_i = Q_i K_j^T
-        const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ks + (size_t)(j % tp.stages) * kOperand);
+      auto scores = [&](int i, int stage) {  // S_i = Q_i K^T
+        const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ring + (size_t)stage * kOperand);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = (uint32_t)(kk / 4) * kPiece + 32u * (kk % 4);
@@ -468,35 +463,53 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         umma_commit(&s_full[i]);
       };
-      bool ok = n == 0 || (wait(&q_full, 0) && wait(&k_full[0], 0));
+      int s = 0;
+      uint32_t phase = 0;
+      auto next = [&]() {
+        if (++s == kStages) {
+          s = 0;
+          phase ^= 1;
+        }
+      };
+      bool ok = n == 0 || (wait(&q_full, 0) && wait(&full[0], 0));
       if (ok && n > 0) {
         tc_fence_after();
         for (int i = 0; i < 2; ++i)
           if (blocks[i] > 0) scores(i, 0);
-        umma_commit(&k_empty[0]);
+        umma_commit(&empty[0]);
+        next();
       }
       for (int j = 0; j < n && ok; ++j) {
-        const int s = j % tp.stages, s1 = (j + 1) % tp.stages;
-        ok = (j + 1 >= n || wait(&k_full[s1], (uint32_t)((j + 1) / tp.stages) & 1u)) &&
-             wait(&v_full[s], (uint32_t)(j / tp.stages) & 1u);
+        ok = wait(&full[s], phase);
+        const int vst = s;
+        next();
+        bool have_k = false;
         for (int i = 0; i < 2 && ok; ++i) {
           if (j >= blocks[i]) continue;
           ok = wait(&p_full[i], (uint32_t)j & 1u);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t va = smem_addr(vs + (size_t)s * kOperand);
+          const uint32_t va = smem_addr(ring + (size_t)vst * kOperand);
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
             umma_f16_ta(o_col[i], s_col[i] + 8u * kk, sw128_desc_mn(va + 2048u * kk, kPiece), tp.idesc_o,
                         j > 0 || kk > 0 ? 1u : 0u);
-          if (j + 1 < blocks[i])
-            scores(i, j + 1);
-          else
+          if (j + 1 < blocks[i]) {
+            if (!have_k) ok = wait(&full[s], phase);
+            if (!ok) break;
+            tc_fence_after();
+            have_k = true;
+            scores(i, s);
+          } else {
             umma_commit(&o_full[i]);
+          }
         }
         if (ok) {
-          umma_commit(&v_empty[s]);
-          if (j + 1 < n) umma_commit(&k_empty[s1]);
+          umma_commit(&empty[vst]);
+          if (j + 1 < n) {
+            umma_commit(&empty[s]);
+            next();
+          }
         }
       }
       umma_commit(&fin);
@@ -576,12 +589,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (zeroes && j == end_block) {
         // V rows behind the sequence
-        if (!warp_wait(&v_full[j % tp.stages], (uint32_t)(j / tp.stages) & 1u, p.err)) {
+        const int item = 2 * j + 1;
+        if (!warp_wait(&full[item % kStages], (uint32_t)(item / kStages) & 1u, p.err)) {
           abort_flag = 1;
           ok = false;
           break;
         }
-        uint8_t* v = vs + (size_t)(j % tp.stages) * kOperand;
+        uint8_t* v = ring + (size_t)(item % kStages) * kOperand;
         const int from = lk - j * kTile;
         for (int c = 0; c < kChunks; ++c)
           for (int k = (threadIdx.x & 127); k < (kTile - from) * 8; k += 128)
@@ -665,8 +679,7 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
   tp.a = p;
   tp.tokens = kTile / p.hpk;
   constexpr int kOperand = kTile * HD * 2;
-  tp.stages = HD == 128 ? 2 : 4;
-  const int smem = (2 + 2 * tp.stages) * kOperand + 1024;
+  const int smem = (2 + tc_stages<HD>()) * kOperand + 1024;
   const uint32_t fmt = type == RRR_F16 ? 0u : 1u;
   // f32 accumulator, A and B of the type, B of the second product N-contiguous, N / 8, M / 16
   tp.idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
