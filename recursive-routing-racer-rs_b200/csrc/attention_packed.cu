@@ -311,6 +311,14 @@ struct TcParams {
   uint32_t idesc_s, idesc_o;
 };
 
+// One lane of a converged warp. (Under this predicate the compiler keeps descriptors in uniform
+// registers: 64 products of 128 x 128 x 16 took 8 x 577 clocks against 8 x 676 issued by a
+// branch on the lane number, 8 x 512 being the tensor core's own time.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          uint32_t accumulate) {
   umma_bf16(d_tmem, a_desc, b_desc, idesc, accumulate);  // kind::f16: the types are in idesc
@@ -447,73 +455,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
     }
   } else if (warp == 8) {
-    // ---------------- products
-    if (lane == 0) {
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!abort_flag && mbar_wait_bounded(bar, parity, p.err, kDevErrTileWait)) return true;
-        abort_flag = 1;
-        return false;
-      };
-      auto scores = [&](int i, int stage) {  // S_i = Q_i K^T
-        const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ring + (size_t)stage * kOperand);
+    // ---------------- products. A commit holds up the products behind it by some 120 clocks, so
+    // there are two per block: each tile's S, which stands for the PV before it too; the softmax
+    // frees the ring's stages on it.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!warp_aborted(&abort_flag) && warp_wait(bar, parity, p.err)) return true;
+      abort_flag = 1;
+      return false;
+    };
+    auto scores = [&](int i, int stage) {  // S_i = Q_i K^T
+      const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ring + (size_t)stage * kOperand);
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = (uint32_t)(kk / 4) * kPiece + 32u * (kk % 4);
           umma_f16(s_col[i], sw128_desc(qa + off), sw128_desc(ka + off), tp.idesc_s, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[i]);
-      };
-      int s = 0;
-      uint32_t phase = 0;
-      auto next = [&]() {
-        if (++s == kStages) {
-          s = 0;
-          phase ^= 1;
-        }
-      };
-      bool ok = n == 0 || (wait(&q_full, 0) && wait(&full[0], 0));
-      if (ok && n > 0) {
-        tc_fence_after();
-        for (int i = 0; i < 2; ++i)
-          if (blocks[i] > 0) scores(i, 0);
-        umma_commit(&empty[0]);
-        next();
       }
-      for (int j = 0; j < n && ok; ++j) {
-        ok = wait(&full[s], phase);
-        const int vst = s;
-        next();
-        bool have_k = false;
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j >= blocks[i]) continue;
-          ok = wait(&p_full[i], (uint32_t)j & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = smem_addr(ring + (size_t)vst * kOperand);
+      __syncwarp();
+    };
+    int s = 0;
+    uint32_t phase = 0;
+    auto next = [&]() {
+      if (++s == kStages) {
+        s = 0;
+        phase ^= 1;
+      }
+    };
+    bool ok = n == 0 || (wait(&q_full, 0) && wait(&full[0], 0));
+    if (ok && n > 0) {
+      tc_fence_after();
+      for (int i = 0; i < 2; ++i)
+        if (blocks[i] > 0) scores(i, 0);
+      next();
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      ok = wait(&full[s], phase);
+      const int vst = s;
+      next();
+      bool have_k = false;
+      for (int i = 0; i < 2 && ok; ++i) {
+        if (j >= blocks[i]) continue;
+        ok = wait(&p_full[i], (uint32_t)j & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_addr(ring + (size_t)vst * kOperand);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
             umma_f16_ta(o_col[i], s_col[i] + 8u * kk, sw128_desc_mn(va + 2048u * kk, kPiece), tp.idesc_o,
                         j > 0 || kk > 0 ? 1u : 0u);
-          if (j + 1 < blocks[i]) {
-            if (!have_k) ok = wait(&full[s], phase);
-            if (!ok) break;
-            tc_fence_after();
-            have_k = true;
-            scores(i, s);
-          } else {
-            umma_commit(&o_full[i]);
-          }
+          if (j + 1 >= blocks[i]) umma_commit(&o_full[i]);
         }
-        if (ok) {
-          umma_commit(&empty[vst]);
-          if (j + 1 < n) {
-            umma_commit(&empty[s]);
-            next();
-          }
+        __syncwarp();
+        if (j + 1 < blocks[i]) {
+          if (!have_k) ok = wait(&full[s], phase);
+          if (!ok) break;
+          tc_fence_after();
+          have_k = true;
+          scores(i, s);
         }
       }
-      umma_commit(&fin);
+      if (j + 1 < n) next();
     }
+    if (elect_one()) umma_commit(&fin);
     __syncwarp();
   }
   } else {
@@ -529,6 +535,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t sc = s_col[i] + sub, oc = o_col[i] + sub;
     const int end_block = (lk - 1) / kTile;
     const bool zeroes = lk % kTile != 0 && i == (blocks[0] > end_block ? 0 : 1);
+    const bool frees = i == (blocks[1] > 0 ? 1 : 0);  // the tile whose products come last
     float m = -INFINITY;             // scaled, as of the last rescale
     float2 l = make_float2(0.f, 0.f);
     bool ok = true;
@@ -539,6 +546,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         break;
       }
       tc_fence_after();
+      if (frees && threadIdx.x % 128 == 0) {  // S_j is done, and with it PV of block j - 1, of both tiles
+        mbar_arrive(&empty[2 * j % kStages]);
+        if (j > 0) mbar_arrive(&empty[(2 * j - 1) % kStages]);
+      }
       uint32_t x[kTile];
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) tmem_ld32(sc + c, x + c);
