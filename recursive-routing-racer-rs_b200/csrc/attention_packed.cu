@@ -360,6 +360,21 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
 template <int HD, typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -411,6 +426,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == 8) tmem_alloc(&tmem_slot, 512);
+  // tile rows past the last whole query row: zeros, so that their scores are
+  for (int k = tp.tokens * p.hpk * 8 + threadIdx.x; k < kTile * 8; k += kTcThreads)
+    for (int c = 0; c < 2 * kChunks; ++c) *reinterpret_cast<uint4*>(qs + c * kPiece + 16 * k) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -459,7 +478,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // there are two per block: each tile's S, which stands for the PV before it too; the softmax
     // frees the ring's stages on it.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (!warp_aborted(&abort_flag) && warp_wait(bar, parity, p.err)) return true;
+      if (warp_wait(bar, parity, p.err)) return true;
       abort_flag = 1;
       return false;
     };
@@ -530,6 +549,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int row = t.row0 + i * tp.tokens + token;  // query row
     const bool mine = token < tp.tokens && i * tp.tokens + token < rows;
     const int seen = mine ? seen_by(p, t, row) : 0;
+    const int open = mine ? seen : INT32_MAX;  // tile rows of no query mask nothing
     const int lk = t.k1 - t.k0;
     const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sc = s_col[i] + sub, oc = o_col[i] + sub;
@@ -539,64 +559,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float m = -INFINITY;             // scaled, as of the last rescale
     float2 l = make_float2(0.f, 0.f);
     bool ok = true;
+    const float2 scale2 = make_float2(p.scale, p.scale);
+    uint32_t x[kTile];
+    float* s = reinterpret_cast<float*>(x);
+    // the weights of columns 32 part .. + 31 under the maximum m, stored over S; their sum to l
+    auto weights = [&](int part) {
+      const float neg = m == -INFINITY ? 0.f : -m;
+      const float2 neg2 = make_float2(neg, neg);
+      float2 sum = make_float2(0.f, 0.f);
+      uint32_t w[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const int at = 32 * part + 2 * c;
+        const float2 e = __ffma2_rn(make_float2(s[at], s[at + 1]), scale2, neg2);
+        const float2 q = make_float2(ex2(e.x), ex2(e.y));
+        sum = __fadd2_rn(sum, q);
+        w[c] = Mma<T>::pack(q.x, q.y);
+      }
+      l = __fadd2_rn(l, sum);
+      tmem_st16(sc + 16 * part, w);
+    };
+    auto top_of = [&](int part) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 32 * part; c < 32 * part + 32; c += 4) {
+        top[0] = fmaxf(top[0], fmaxf(s[c], s[c + 1]));
+        top[1] = fmaxf(top[1], fmaxf(s[c + 2], s[c + 3]));
+      }
+      return fmaxf(top[0], top[1]);
+    };
     for (int j = 0; j < blocks[i]; ++j) {
-      if (warp_aborted(&abort_flag) || !warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
+      if (!warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
         abort_flag = 1;
         ok = false;
         break;
       }
       tc_fence_after();
-      if (frees && threadIdx.x % 128 == 0) {  // S_j is done, and with it PV of block j - 1, of both tiles
+      if (frees && r == 0) {  // S_j is done, and with it PV of block j - 1, of both tiles
         mbar_arrive(&empty[2 * j % kStages]);
         if (j > 0) mbar_arrive(&empty[(2 * j - 1) % kStages]);
-      }
-      uint32_t x[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld32(sc + c, x + c);
-      tmem_wait_ld();
-      float* s = reinterpret_cast<float*>(x);
-      if (__any_sync(0xffffffffu, (j + 1) * kTile > seen)) {
-#pragma unroll
-        for (int c = 0; c < kTile; ++c)
-          if (j * kTile + c >= seen) s[c] = -INFINITY;
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < kTile; c += 4)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[c + k]);
-      const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
-      if (__any_sync(0xffffffffu, m_new > m + kLazy || (m == -INFINITY && m_new > m))) {
-        const bool grow = m_new > m;
-        const float next = grow ? m_new : m;
-        const float alpha = grow ? ex2(m - next) : 1.f;
-        m = next;
-        l.x *= alpha;
-        l.y *= alpha;
-        if (j > 0) {
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t v[32];
-            tmem_ld32(oc + c, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
-            tmem_st32(oc + c, v);
-          }
-        }
-      }
-      const float neg = m == -INFINITY ? 0.f : -m;
-      const float2 scale2 = make_float2(p.scale, p.scale), neg2 = make_float2(neg, neg);
-      uint32_t w[32];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float2 e = __ffma2_rn(make_float2(s[64 * half + 2 * c], s[64 * half + 2 * c + 1]), scale2, neg2);
-          const float2 q = make_float2(ex2(e.x), ex2(e.y));
-          l = __fadd2_rn(l, q);
-          w[c] = Mma<T>::pack(q.x, q.y);
-        }
-        tmem_st32(sc + 32 * half, w);
       }
       if (zeroes && j == end_block) {
         // V rows behind the sequence
@@ -612,6 +613,56 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int k = (threadIdx.x & 127); k < (kTile - from) * 8; k += 128)
             *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
+      }
+      tmem_ld32(sc, x);
+      tmem_wait_ld();
+      const bool masked = __any_sync(0xffffffffu, (j + 1) * kTile > open);
+      bool done = false;
+      if (j > 0 && !masked) {
+        // the weights under the old maximum; the new one is found meanwhile
+        const float2 before = l;
+        float top = -INFINITY;
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+          if (part < 3) tmem_ld32(sc + 32 * (part + 1), x + 32 * (part + 1));
+          weights(part);
+          top = fmaxf(top, top_of(part));
+          if (part < 3) tmem_wait_ld();
+        }
+        done = !__any_sync(0xffffffffu, top * p.scale > m + kLazy);
+        if (!done) l = before;
+      } else {
+#pragma unroll
+        for (int c = 32; c < kTile; c += 32) tmem_ld32(sc + c, x + c);
+        tmem_wait_ld();
+      }
+      if (!done) {
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c)
+            if (j * kTile + c >= open) s[c] = -INFINITY;
+        }
+        const float m_new = fmaxf(fmaxf(top_of(0), top_of(1)), fmaxf(top_of(2), top_of(3))) * p.scale;
+        if (__any_sync(0xffffffffu, m_new > m + kLazy)) {
+          const bool grow = m_new > m;
+          const float next = grow ? m_new : m;
+          const float alpha = grow ? ex2(m - next) : 1.f;
+          m = next;
+          l.x *= alpha;
+          l.y *= alpha;
+          if (j > 0) {
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t v[16];
+              tmem_ld16(oc + c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+              tmem_st16(oc + c, v);
+            }
+          }
+        }
+#pragma unroll
+        for (int part = 0; part < 4; ++part) weights(part);
       }
       tmem_wait_st();
       tc_fence_before();
