@@ -55,7 +55,7 @@ __device__ __forceinline__ bool find_tile(const PackedParams& p, int rows, int x
   t.k0 = p.cu_kv[lo];
   t.k1 = p.cu_kv[lo + 1];
   if (t.q0 < 0 || t.q1 < t.q0 || t.q1 > p.q_rows || t.k0 < 0 || t.k1 < t.k0 || t.k1 > p.kv_rows) {
-    if (threadIdx.x == 0) flag_position(p.err);
+    if ((threadIdx.x & 31) == 0) flag_position(p.err);
     return false;
   }
   const int64_t row0 = t.q0 + (int64_t)rows * (x - (t.q0 / rows + lo));
@@ -375,6 +375,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
       : "r"(taddr)
       : "memory");
 }
+// 32 bytes of a row of out: every lane writes another row, so a store costs what it has of rows
+__device__ __forceinline__ void store_32(void* p, const uint32_t (&a)[4], const uint32_t (&b)[4], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a[0]), "r"(a[1]), "r"(a[2]),
+                 "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(a[0], a[1], a[2], a[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(b[0], b[1], b[2], b[3]);
+  }
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -401,12 +413,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (!find_tile(p, both, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
   const int kv = blockIdx.x % nkv;
   const int rows = min(both, t.q1 - t.row0);
-  // blocks of KV rows of each tile: up to what its last row sees
-  int blocks[2];
+  // KV rows that each tile's last row sees, and the blocks of 128 of them
+  int sees[2], blocks[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int last = min(rows, (i + 1) * tp.tokens) - 1;
-    blocks[i] = last >= i * tp.tokens ? (seen_by(p, t, t.row0 + last) + kTile - 1) / kTile : 0;
+    sees[i] = last >= i * tp.tokens ? seen_by(p, t, t.row0 + last) : 0;
+    blocks[i] = (sees[i] + kTile - 1) / kTile;
   }
   const int n = max(blocks[0], blocks[1]);
 
@@ -482,13 +495,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       abort_flag = 1;
       return false;
     };
-    auto scores = [&](int i, int stage) {  // S_i = Q_i K^T
+    // columns of block j that tile i's last row sees, in steps of the products' 16
+    auto columns = [&](int i, int j) { return min(kTile, (sees[i] - j * kTile + 15) & ~15); };
+    auto scores = [&](int i, int j, int stage) {  // S_i = Q_i K^T
+      const uint32_t idesc = tp.idesc_s | ((uint32_t)(columns(i, j) >> 3) << 17);
       const uint32_t qa = smem_addr(qs + i * kOperand), ka = smem_addr(ring + (size_t)stage * kOperand);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = (uint32_t)(kk / 4) * kPiece + 32u * (kk % 4);
-          umma_f16(s_col[i], sw128_desc(qa + off), sw128_desc(ka + off), tp.idesc_s, kk > 0 ? 1u : 0u);
+          umma_f16(s_col[i], sw128_desc(qa + off), sw128_desc(ka + off), idesc, kk > 0 ? 1u : 0u);
         }
         umma_commit(&s_full[i]);
       }
@@ -506,7 +522,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (ok && n > 0) {
       tc_fence_after();
       for (int i = 0; i < 2; ++i)
-        if (blocks[i] > 0) scores(i, 0);
+        if (blocks[i] > 0) scores(i, 0, 0);
       next();
     }
     for (int j = 0; j < n && ok; ++j) {
@@ -520,11 +536,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const uint32_t va = smem_addr(ring + (size_t)vst * kOperand);
+        const int steps = columns(i, j) / 16;
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            if (kk >= steps) break;
             umma_f16_ta(o_col[i], s_col[i] + 8u * kk, sw128_desc_mn(va + 2048u * kk, kPiece), tp.idesc_o,
                         j > 0 || kk > 0 ? 1u : 0u);
+          }
           if (j + 1 >= blocks[i]) umma_commit(&o_full[i]);
         }
         __syncwarp();
@@ -533,7 +552,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!ok) break;
           tc_fence_after();
           have_k = true;
-          scores(i, s);
+          scores(i, j + 1, s);
         }
       }
       if (j + 1 < n) next();
@@ -550,6 +569,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool mine = token < tp.tokens && i * tp.tokens + token < rows;
     const int seen = mine ? seen_by(p, t, row) : 0;
     const int open = mine ? seen : INT32_MAX;  // tile rows of no query mask nothing
+    const int all_see = (int)__reduce_min_sync(0xffffffffu, (unsigned)open);    // every row of the warp,
+    const int none_sees = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);  // and none from here on
     const int lk = t.k1 - t.k0;
     const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sc = s_col[i] + sub, oc = o_col[i] + sub;
@@ -560,18 +581,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float2 l = make_float2(0.f, 0.f);
     bool ok = true;
     const float2 scale2 = make_float2(p.scale, p.scale);
-    uint32_t x[kTile];
-    float* s = reinterpret_cast<float*>(x);
-    // the weights of columns 32 part .. + 31 under the maximum m, stored over S; their sum to l
-    auto weights = [&](int part) {
+    // the weights of 32 scores under the maximum m, stored over S as columns 32 part .. + 31; their
+    // sum to l
+    auto weights = [&](const float* v, int part) {
       const float neg = m == -INFINITY ? 0.f : -m;
       const float2 neg2 = make_float2(neg, neg);
       float2 sum = make_float2(0.f, 0.f);
       uint32_t w[16];
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
-        const int at = 32 * part + 2 * c;
-        const float2 e = __ffma2_rn(make_float2(s[at], s[at + 1]), scale2, neg2);
+        const float2 e = __ffma2_rn(make_float2(v[2 * c], v[2 * c + 1]), scale2, neg2);
         const float2 q = make_float2(ex2(e.x), ex2(e.y));
         sum = __fadd2_rn(sum, q);
         w[c] = Mma<T>::pack(q.x, q.y);
@@ -579,14 +598,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       l = __fadd2_rn(l, sum);
       tmem_st16(sc + 16 * part, w);
     };
-    auto top_of = [&](int part) {
+    auto top_of = [&](const float* v) {
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 32 * part; c < 32 * part + 32; c += 4) {
-        top[0] = fmaxf(top[0], fmaxf(s[c], s[c + 1]));
-        top[1] = fmaxf(top[1], fmaxf(s[c + 2], s[c + 3]));
+      for (int c = 0; c < 32; c += 4) {
+        top[0] = fmaxf(top[0], fmaxf(v[c], v[c + 1]));
+        top[1] = fmaxf(top[1], fmaxf(v[c + 2], v[c + 3]));
       }
       return fmaxf(top[0], top[1]);
+    };
+    // takes over a larger maximum where a row's has grown by more than kLazy; whether any has
+    auto rescale = [&](float m_new, bool has_o) {
+      if (!__any_sync(0xffffffffu, m_new > m + kLazy)) return false;
+      const bool grow = m_new > m;
+      const float next = grow ? m_new : m;
+      const float alpha = grow ? ex2(m - next) : 1.f;
+      m = next;
+      l.x *= alpha;
+      l.y *= alpha;
+      if (has_o) {
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(oc + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+          tmem_st16(oc + c, v);
+        }
+      }
+      return true;
     };
     for (int j = 0; j < blocks[i]; ++j) {
       if (!warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
@@ -614,55 +655,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
-      tmem_ld32(sc, x);
-      tmem_wait_ld();
-      const bool masked = __any_sync(0xffffffffu, (j + 1) * kTile > open);
-      bool done = false;
-      if (j > 0 && !masked) {
-        // the weights under the old maximum; the new one is found meanwhile
+      if (j > 0 && (j + 1) * kTile <= all_see) {
+        // the weights under the old maximum; the new one is found meanwhile, and where it is too
+        // large for the old one they are computed again
+        uint32_t x[kTile];
+        const float* v = reinterpret_cast<const float*>(x);
+        tmem_ld32(sc, x);
+        tmem_wait_ld();
         const float2 before = l;
         float top = -INFINITY;
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
           if (part < 3) tmem_ld32(sc + 32 * (part + 1), x + 32 * (part + 1));
-          weights(part);
-          top = fmaxf(top, top_of(part));
+          weights(v + 32 * part, part);
+          top = fmaxf(top, top_of(v + 32 * part));
           if (part < 3) tmem_wait_ld();
         }
-        done = !__any_sync(0xffffffffu, top * p.scale > m + kLazy);
-        if (!done) l = before;
-      } else {
+        const float2 after = l;
+        l = before;
+        if (rescale(top * p.scale, true)) {
 #pragma unroll
-        for (int c = 32; c < kTile; c += 32) tmem_ld32(sc + c, x + c);
-        tmem_wait_ld();
-      }
-      if (!done) {
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < kTile; ++c)
-            if (j * kTile + c >= open) s[c] = -INFINITY;
+          for (int part = 0; part < 4; ++part) weights(v + 32 * part, part);
+        } else {
+          l = after;
         }
-        const float m_new = fmaxf(fmaxf(top_of(0), top_of(1)), fmaxf(top_of(2), top_of(3))) * p.scale;
-        if (__any_sync(0xffffffffu, m_new > m + kLazy)) {
-          const bool grow = m_new > m;
-          const float next = grow ? m_new : m;
-          const float alpha = grow ? ex2(m - next) : 1.f;
-          m = next;
-          l.x *= alpha;
-          l.y *= alpha;
-          if (j > 0) {
-            for (int c = 0; c < HD; c += 16) {
-              uint32_t v[16];
-              tmem_ld16(oc + c, v);
-              tmem_wait_ld();
+      } else {
+        // the first block, or one with masked columns: the maximum first. A part of 32 columns
+        // that no row of the warp sees has no weights, one that every row sees no mask.
+        auto load = [&](int part, uint32_t* x) {
+          const int at = j * kTile + 32 * part;
+          tmem_ld32(sc + 32 * part, x);
+          tmem_wait_ld();
+          if (at + 32 > all_see) {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
-              tmem_st16(oc + c, v);
-            }
+            for (int c = 0; c < 32; ++c)
+              if (c >= open - at) x[c] = 0xff800000u;
+          }
+        };
+        const int parts = min(4, (none_sees - j * kTile + 31) / 32);
+        float m_new = -INFINITY;
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) {
+          uint32_t x[32];
+          load(part, x);
+          m_new = fmaxf(m_new, top_of(reinterpret_cast<const float*>(x)));
+        }
+        rescale(m_new * p.scale, j > 0);
+#pragma unroll 1
+        for (int part = 0; part < 4; ++part) {
+          uint32_t x[32];
+          if (part < parts) {
+            load(part, x);
+            weights(reinterpret_cast<const float*>(x), part);
+          } else {
+            const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            tmem_st16(sc + 16 * part, zero);
           }
         }
-#pragma unroll
-        for (int part = 0; part < 4; ++part) weights(part);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -675,6 +724,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float inv = seen > 0 ? 1.f / sum : 0.f;
       T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head;
       bool bad = false;
+      const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.out_row % 16 == 0 && p.out_head % 16 == 0;
       if (blocks[i] > 0) {
         ok = warp_wait(&o_full[i], 0, p.err);
         if (!ok) abort_flag = 1;
@@ -687,6 +737,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_ld32(oc + c, v);
             tmem_wait_ld();
           }
+          uint32_t pair[4];
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             uint32_t o[4];
@@ -697,7 +748,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
               o[e] = Mma<T>::pack(a, b);
             }
-            if (mine) *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(o[0], o[1], o[2], o[3]);
+            if (k % 16 == 0) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pair[e] = o[e];
+            } else if (mine) {
+              store_32(dst + c + k - 8, pair, o, wide);
+            }
           }
         }
         unsigned again = __ballot_sync(0xffffffffu, bad && mine);
@@ -744,7 +800,7 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
   const int smem = (2 + tc_stages<HD>()) * kOperand + 1024;
   const uint32_t fmt = type == RRR_F16 ? 0u : 1u;
   // f32 accumulator, A and B of the type, B of the second product N-contiguous, N / 8, M / 16
-  tp.idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+  tp.idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTile >> 4) << 24);  // N / 8: as wide as the block
   tp.idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) |
                ((uint32_t)(kTile >> 4) << 24);
   CUtensorMap qmap, kmap, vmap;

@@ -802,3 +802,22 @@ def test_two_streams_with_a_workspace_each(rrr, ctx):
     torch.cuda.synchronize()
     for i in range(2):
         check_decode(outs[i], q[i], kv, 1 / math.sqrt(128), torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(128, 3, 1), (64, 8, 2), (256, 2, 2)])
+def test_attention_packed_many_sequences(rrr, ctx, hd, nh, nkv):
+    """More sequences than one search over lengths takes, and more items than the GPU has SMs."""
+    r = np.random.default_rng(hd)
+    lq = [int(x) for x in r.integers(0, 90, 300)]
+    lk = [int(x) + int(y) for x, y in zip(lq, r.integers(0, 200, 300))]
+    g, t = gen(hd), torch.bfloat16
+    q, k, v = (normal(g, sum(n), h, hd, dtype=t) for n, h in ((lq, nh), (lk, nkv), (lk, nkv)))
+    out = torch.full_like(q, 3.0)
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), out)
+    check_packed(out, q, k, v, lq, lk, True, 1 / math.sqrt(hd))
+    lq, lk = lq[:40] + [1500], lk[:40] + [2100]
+    q, k, v = (normal(g, sum(n), h, hd, dtype=t) for n, h in ((lq, nh), (lk, nkv), (lk, nkv)))
+    out = torch.full_like(q, 3.0)
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), out)
+    check_packed(out, q, k, v, lq, lk, True, 1 / math.sqrt(hd))
