@@ -7,9 +7,16 @@
 // The value read back is d*code + m: d*code is exact in f32 (11 + 4 bits), so it carries one
 // rounding.
 //
-// Bound by memory: 2 bytes (16-bit rows) in and 5/8 out per value, or the reverse. One warp
-// takes one (row, KV head): lane l holds the values D*l .. D*l + D - 1 of the head (D =
-// head_dim / 32), a group is 32 / D lanes.
+// Bound by memory (2 bytes of a 16-bit row in and 5/8 out per value, or the reverse), and not far
+// from it by instructions. One warp takes the rows of one block of 16 (aligned in the page, where
+// V's codes of 16 rows lie together) of K or V of one head. K: a lane takes 8 consecutive values,
+// which are one word of codes. V: a lane takes the values 32i + 8n + g, + 1 (n = 0..3, g even) of
+// both rows of a pair, which are two words. A quotient is first taken by the reciprocal, and the
+// lane's quotients are divided out where one comes close to a rounding border, which the first
+// misses by less than 4e-6 of a code. (max - min) / 15 is rounded right by one correction of the
+// product with 1/15 (Markstein's method), which the tests compare with the division.
+// (First version: a warp per row with codes shuffled together and a division per value, 58 us for
+// 13,000 rows of 8 x 128 stored and read back, against 10 us of bytes.)
 #include <math.h>
 
 #include "kv4.cuh"
@@ -34,12 +41,14 @@ int check_kv4_cache(rrr_ctx* ctx, const rrr_kv4_cache* c, const char* fn) {
 namespace {
 
 constexpr int kRowWarps = 8;
+constexpr int kBlockRows = 16;
 
 struct Kv4RowParams {
   uint8_t* pages;
   int64_t n_pages, table_stride;
   const int* table;
   int n_seqs, max_pages, nkv, rows;
+  int slots;  // blocks of 16 rows, with room for the sequences' ends
   void* k;
   void* v;
   int64_t k_stride, v_stride;
@@ -48,116 +57,213 @@ struct Kv4RowParams {
   int* err;
 };
 
-// The block and the row in it of packed row `row`, KV head h; null when it has none.
+// The rows of a warp: packed rows [row0, row0 + n) are the rows first .. first + n - 1 (first < 16)
+// of 16-row block `block` of a page.
+struct RowBlock {
+  uint8_t* blk;
+  int64_t row0;
+  int block, first, n;
+};
+
+// Slot x belongs to the last sequence s with cu[s] / 16 + 2 s <= x (sequences get disjoint runs
+// of slots that are long enough), searched by the warp 32 sequences at a time.
 template <int HD>
-__device__ __forceinline__ uint8_t* find_row(const Kv4RowParams& p, int row, int h, int lane, int& in_page) {
-  const int s = seq_of_row(p.cu, p.n_seqs, row);
-  if (s < 0) return nullptr;  // behind the last sequence
-  const int64_t pos = (int64_t)p.lens[s] - (p.cu[s + 1] - row);
-  if (pos >= 0 && pos < (int64_t)p.max_pages * kPageRows) {
-    const int page = p.table[(int64_t)s * p.table_stride + pos / kPageRows];
-    if (page >= 0 && page < p.n_pages) {
-      in_page = (int)(pos % kPageRows);
-      return p.pages + ((int64_t)page * p.nkv + h) * Kv4Block<HD>::kBytes;
-    }
+__device__ __forceinline__ bool find_rows(const Kv4RowParams& p, int x, int h, RowBlock& b) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.n_seqs;  // the sequence lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+    const bool at = s < hi && p.cu[s] / kBlockRows + 2 * s <= x;
+    const unsigned below = __ballot_sync(0xffffffffu, at);
+    lo += below ? (31 - __clz(below)) * step : 0;
+    hi = min(hi, lo + step);
   }
-  if (lane == 0) flag_position(p.err);
-  return nullptr;
+  const int r0 = p.cu[lo], r1 = p.cu[lo + 1], len = p.lens[lo];
+  if (r0 < 0 || r1 < r0 || r1 > p.rows) {
+    if (lane == 0) flag_position(p.err);
+    return false;
+  }
+  const int64_t pos0 = (int64_t)len - (r1 - r0);  // position of the sequence's first packed row
+  if (r1 > r0 && (pos0 < 0 || len > (int64_t)p.max_pages * kPageRows) && lane == 0) flag_position(p.err);
+  // (rows at positions that do not exist are left out)
+  int64_t at = pos0 >= 0 ? pos0 : 0;
+  const int64_t end = min((int64_t)len, (int64_t)p.max_pages * kPageRows);
+  const int64_t q = at / kBlockRows + (x - (r0 / kBlockRows + 2 * lo));  // 16-row block of the sequence
+  const int64_t from = max(at, q * kBlockRows), to = min(end, (q + 1) * kBlockRows);
+  if (q < 0 || from >= to) return false;
+  const int page = p.table[(int64_t)lo * p.table_stride + from / kPageRows];
+  if (page < 0 || page >= p.n_pages) {
+    if (lane == 0) flag_position(p.err);
+    return false;
+  }
+  b.blk = p.pages + ((int64_t)page * p.nkv + h) * Kv4Block<HD>::kBytes;
+  b.row0 = r0 + (from - pos0);
+  b.block = (int)(from % kPageRows) / kBlockRows;
+  b.first = (int)(from % kBlockRows);
+  b.n = (int)(to - from);
+  return true;
 }
 
-// This lane's values of a head row as codes (4 bits each, value i at bit 4i) and the group's
-// d and m, which every lane of the group gets.
-template <int D>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[D], __half& d16, __half& m16) {
-  constexpr int L = 32 / D;  // lanes per group
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+// Codes of four values by the division itself (out of line: rarely called)
+__device__ __noinline__ uint32_t divided(float a, float b, float c, float e, float m, float d) {
+  auto code = [&](float x) {
+    return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, m), d)), 0.f), 15.f);
+  };
+  return code(a) | code(b) << 4 | code(c) << 8 | code(e) << 12;
+}
+// Eight values of a group of 32, which four neighbouring lanes hold: their codes, value i at bit
+// 4i, and the group's d and m.
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, __half& m16) {
+  const float inf = __int_as_float(0x7f800000);
+  float lo = x[0], hi = x[0], zero = 0.f;
 #pragma unroll
-  for (int i = 0; i < D; ++i) {
+  for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+    zero = fmaf(x[i], 0.f, zero);
   }
+  if (zero != 0.f) hi = inf;  // an infinity or a NaN among them
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
+  for (int o = 1; o < 4; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const unsigned lanes = __ballot_sync(0xffffffffu, bad) >> ((threadIdx.x & 31) & ~(L - 1));
-  const bool any_bad = (lanes & (L == 32 ? 0xffffffffu : (1u << L) - 1u)) != 0;
+  // (hi - lo) / 15 by the product with 1/15 and its remainder
+  const float range = __fsub_rn(hi, lo), first = __fmul_rn(range, 1.f / 15.f);
+  const float step = fmaf(fmaf(-15.f, first, range), 1.f / 15.f, first);
   m16 = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  d16 = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 65504.f));
-  if (any_bad) d16 = __ushort_as_half(0x7fff);
+  d16 = hi == inf ? __ushort_as_half(0x7fff) : __float2half_rn(fminf(range > 1e6f ? 65504.f : step, 65504.f));
   const float d = __half2float(d16), m = __half2float(m16);
-  uint32_t codes = 0;
+  const float inv = d > 0.f ? __fdividef(1.f, d) : 0.f;
+  uint32_t w = 0;
+  bool near = false;
 #pragma unroll
-  for (int i = 0; i < D; ++i) {
-    const float c = d > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], m), d)) : 0.f;
-    codes |= (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+  for (int i = 0; i < 8; ++i) {
+    const float q = __fsub_rn(x[i], m) * inv;
+    const float t = fminf(fmaxf(q, 0.f), 15.f) + 12582912.f;  // the nearest integer in the low bits
+    near |= fabsf(q - (t - 12582912.f)) > 0.49999f;
+    w += __float_as_uint(t) << (4 * i);
   }
-  return codes;
+  // what 12582912's own bits added
+  w -= 0x4b400000u + 0xb4000000u + 0x40000000u;
+  if (near && d > 0.f)
+    w = divided(x[0], x[1], x[2], x[3], m, d) | divided(x[4], x[5], x[6], x[7], m, d) << 16;
+  return w;
 }
+// The same eight values back
+__device__ __forceinline__ void dequantise(uint32_t w, float d, float m, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    x[i] = fmaf(__uint_as_float(((w >> (4 * i)) & 15u) | 0x4b000000u) - 8388608.f, d, m);
+}
+
+template <int HD>
+struct Lanes {  // of a warp: groups at once, and rows (K) or pairs of rows (V) at once
+  static constexpr int kGroups = Kv4Block<HD>::kGroups;
+  static constexpr int kRows = 32 / (4 * kGroups);
+  static constexpr int kAhead = kBlockRows / kRows < 4 ? kBlockRows / kRows : 4;  // rows in flight
+  static constexpr int kPairsAhead = kRows >= 4 ? 1 : 2;
+};
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_store_kernel(const __grid_constant__ Kv4RowParams p) {
   using B = Kv4Block<HD>;
-  constexpr int D = HD / 32, L = 32 / D;
+  using L = Lanes<HD>;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  const int64_t row = item / p.nkv;
-  if (row >= p.rows) return;
-  const int h = (int)(item - row * p.nkv);
-  int r;
-  uint8_t* blk = find_row<HD>(p, (int)row, h, lane, r);
-  if (!blk) return;
-  const int j = lane / L, lg = lane % L;  // this lane's group and its place in it
-  float x[D];
-  __half d, m;
-  load_vec<T, D>(static_cast<const T*>(p.k) + row * p.k_stride + (int64_t)h * HD + D * lane, x);
-  uint32_t c = quantise<D>(x, d, m);
-  {
-    // the 8 elements of a word are 8 / D lanes
-    uint8_t* codes = blk;
-    const int t = lg * D / 8;
-    if constexpr (D == 8)
-      reinterpret_cast<uint32_t*>(codes)[B::k_word(r, j, t)] = c;
-    else if constexpr (D == 4)
-      reinterpret_cast<uint16_t*>(codes)[2 * B::k_word(r, j, t) + (lg & 1)] = (uint16_t)c;
-    else
-      codes[4 * B::k_word(r, j, t) + (lg & 3)] = (uint8_t)c;
-    if (lg == 0) {
-      reinterpret_cast<__half*>(blk + B::kCodes)[B::scale(r, j)] = d;
-      reinterpret_cast<__half*>(blk + B::kCodes + B::kScales)[B::scale(r, j)] = m;
+  const int x = (int)(item / (2 * p.nkv));
+  if (x >= p.slots) return;
+  const int hv = (int)(item - (int64_t)x * 2 * p.nkv), h = hv % p.nkv;
+  RowBlock b;
+  if (!find_rows<HD>(p, x, h, b)) return;
+  const int in_page = kBlockRows * b.block + b.first;
+  const int j = lane / 4 % L::kGroups, t = lane % 4, set = lane / (4 * L::kGroups);
+  if (hv < p.nkv) {
+    const T* src = static_cast<const T*>(p.k) + (int64_t)h * HD + 32 * j + 8 * t;
+#pragma unroll 1
+    for (int r0 = set; r0 < b.n + set; r0 += L::kAhead * L::kRows) {
+      float v[L::kAhead][8];
+#pragma unroll
+      for (int a = 0; a < L::kAhead; ++a) {
+        if (r0 - set + a * L::kRows >= b.n) break;
+        const int r = min(r0 + a * L::kRows, b.n - 1);  // (rows past the last are read as it)
+        load_vec<T, 8>(src + (b.row0 + r) * p.k_stride, v[a]);
+      }
+#pragma unroll
+      for (int a = 0; a < L::kAhead; ++a) {
+        if (r0 - set + a * L::kRows >= b.n) break;
+        const int r = r0 + a * L::kRows;
+        __half d, m;
+        const uint32_t w = quantise(v[a], d, m);
+        if (r < b.n) {
+          const int row = in_page + r;
+          reinterpret_cast<uint32_t*>(b.blk)[B::k_word(row, j, t)] = w;
+          if (t == 0) {
+            reinterpret_cast<__half*>(b.blk + B::kCodes)[B::scale(row, j)] = d;
+            reinterpret_cast<__half*>(b.blk + B::kCodes + B::kScales)[B::scale(row, j)] = m;
+          }
+        }
+      }
     }
-  }
-  load_vec<T, D>(static_cast<const T*>(p.v) + row * p.v_stride + (int64_t)h * HD + D * lane, x);
-  c = quantise<D>(x, d, m);
-  blk += B::kHalf;
-  {
-    // element e = 8n + g of the group is nibble n of half word g: every lane places its codes in
-    // the eight half words (two per u32), the lanes of the group join them, and L lanes write
-    uint32_t w[4] = {0, 0, 0, 0};
+  } else {
+    uint8_t* vb = b.blk + B::kHalf;
+    const int g = 2 * t;
+    const T* src = static_cast<const T*>(p.v) + (int64_t)h * HD + 32 * j + g;
+    const int odd_first = b.first & 1, pairs = (b.n + odd_first + 1) / 2;
+#pragma unroll 1
+    for (int u0 = set; u0 < pairs + set; u0 += L::kPairsAhead * L::kRows) {
+      float v[L::kPairsAhead][2][8];  // [pair][row][2 n + (g, g + 1)]
 #pragma unroll
-    for (int i = 0; i < D; ++i) {
-      const int e = lg * D + i, g = e & 7, n = e >> 3;
-      const uint32_t v = ((c >> (4 * i)) & 15u) << (4 * n + 16 * (g & 1));
+      for (int a = 0; a < L::kPairsAhead; ++a) {
+        if (u0 - set + a * L::kRows >= pairs) break;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q == g >> 1) w[q] |= v;
-    }
+        for (int o = 0; o < 2; ++o) {
+          const int r = min(max(2 * (u0 + a * L::kRows) + o - odd_first, 0), b.n - 1);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1)
+          for (int n = 0; n < 4; ++n) {
+            float two[2];
+            load_vec<T, 2>(src + (b.row0 + r) * p.v_stride + 8 * n, two);
+            v[a][o][2 * n] = two[0];
+            v[a][o][2 * n + 1] = two[1];
+          }
+        }
+      }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) w[q] |= __shfl_xor_sync(0xffffffffu, w[q], o);
-    uint16_t* codes = reinterpret_cast<uint16_t*>(blk);
+      for (int a = 0; a < L::kPairsAhead; ++a) {
+        if (u0 - set + a * L::kRows >= pairs) break;
+        const int r = 2 * (u0 + a * L::kRows) - odd_first, row = in_page + r;  // the pair's even row
+        const bool has[2] = {r >= 0 && r < b.n, r + 1 >= 0 && r + 1 < b.n};
+        uint32_t c[2];
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
-      if (g % L == lg) codes[B::v_half(r, j, g)] = (uint16_t)(w[g >> 1] >> (16 * (g & 1)));
-    if (lg == 0) {
-      reinterpret_cast<__half*>(blk + B::kCodes)[B::scale(r, j)] = d;
-      reinterpret_cast<__half*>(blk + B::kCodes + B::kScales)[B::v_min(r, j)] = m;
+        for (int o = 0; o < 2; ++o) {
+          __half d, m;
+          c[o] = quantise(v[a][o], d, m);
+          if (t == 0 && has[o]) {
+            reinterpret_cast<__half*>(vb + B::kCodes)[B::scale(row + o, j)] = d;
+            reinterpret_cast<__half*>(vb + B::kCodes + B::kScales)[B::v_min(row + o, j)] = m;
+          }
+        }
+        // nibbles 0, 2, 4, 6 are g's, the others g + 1's: four each to a half word
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w[2];
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            uint32_t y = (c[o] >> (4 * e)) & 0x0f0f0f0fu;
+            y = (y | y >> 4) & 0x00ff00ffu;
+            w[o] = (y | y >> 8) & 0xffffu;
+          }
+          uint16_t* codes = reinterpret_cast<uint16_t*>(vb);
+          if (has[0] && has[1])
+            reinterpret_cast<uint32_t*>(vb)[B::v_half(row, j, g + e) / 2] = w[0] | w[1] << 16;
+          else if (has[0])
+            codes[B::v_half(row, j, g + e)] = (uint16_t)w[0];
+          else if (has[1])
+            codes[B::v_half(row + 1, j, g + e)] = (uint16_t)w[1];
+        }
+      }
     }
   }
 }
@@ -165,44 +271,82 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_store_kernel(const __grid_
 template <int HD, typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_load_kernel(const __grid_constant__ Kv4RowParams p) {
   using B = Kv4Block<HD>;
-  constexpr int D = HD / 32, L = 32 / D;
+  using L = Lanes<HD>;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  const int64_t row = item / p.nkv;
-  if (row >= p.rows) return;
-  const int h = (int)(item - row * p.nkv);
-  int r;
-  const uint8_t* blk = find_row<HD>(p, (int)row, h, lane, r);
-  if (!blk) return;
-  const int j = lane / L, lg = lane % L;
-  float x[D];
-  if (p.k) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(blk)[B::k_word(r, j, lg * D / 8)];
-    const float d = __half2float(reinterpret_cast<const __half*>(blk + B::kCodes)[B::scale(r, j)]);
-    const float m = __half2float(reinterpret_cast<const __half*>(blk + B::kCodes + B::kScales)[B::scale(r, j)]);
+  const int x = (int)(item / (2 * p.nkv));
+  if (x >= p.slots) return;
+  const int hv = (int)(item - (int64_t)x * 2 * p.nkv), h = hv % p.nkv;
+  if (!(hv < p.nkv ? p.k : p.v)) return;
+  RowBlock b;
+  if (!find_rows<HD>(p, x, h, b)) return;
+  const int in_page = kBlockRows * b.block + b.first;
+  const int j = lane / 4 % L::kGroups, t = lane % 4, set = lane / (4 * L::kGroups);
+  if (hv < p.nkv) {
+    T* dst = static_cast<T*>(p.k) + (int64_t)h * HD + 32 * j + 8 * t;
+#pragma unroll 1
+    for (int r0 = set; r0 < b.n; r0 += L::kAhead * L::kRows) {
+      uint32_t w[L::kAhead];
+      __half d[L::kAhead], m[L::kAhead];
 #pragma unroll
-    for (int i = 0; i < D; ++i) x[i] = fmaf((float)((w >> (4 * ((lg * D + i) & 7))) & 15u), d, m);
-    store_vec<T, D>(static_cast<T*>(p.k) + row * p.k_stride + (int64_t)h * HD + D * lane, x);
-  }
-  if (p.v) {
-    blk += B::kHalf;
-    const float d = __half2float(reinterpret_cast<const __half*>(blk + B::kCodes)[B::scale(r, j)]);
-    const float m = __half2float(reinterpret_cast<const __half*>(blk + B::kCodes + B::kScales)[B::v_min(r, j)]);
+      for (int a = 0; a < L::kAhead; ++a) {
+        const int row = in_page + min(r0 + a * L::kRows, b.n - 1);
+        w[a] = reinterpret_cast<const uint32_t*>(b.blk)[B::k_word(row, j, t)];
+        d[a] = reinterpret_cast<const __half*>(b.blk + B::kCodes)[B::scale(row, j)];
+        m[a] = reinterpret_cast<const __half*>(b.blk + B::kCodes + B::kScales)[B::scale(row, j)];
+      }
 #pragma unroll
-    for (int i = 0; i < D; ++i) {
-      const int e = lg * D + i;
-      const uint32_t w = reinterpret_cast<const uint16_t*>(blk)[B::v_half(r, j, e & 7)];
-      x[i] = fmaf((float)((w >> (4 * (e >> 3))) & 15u), d, m);
+      for (int a = 0; a < L::kAhead; ++a) {
+        const int r = r0 + a * L::kRows;
+        float v[8];
+        dequantise(w[a], __half2float(d[a]), __half2float(m[a]), v);
+        if (r < b.n) store_vec<T, 8>(dst + (b.row0 + r) * p.k_stride, v);
+      }
     }
-    store_vec<T, D>(static_cast<T*>(p.v) + row * p.v_stride + (int64_t)h * HD + D * lane, x);
+  } else {
+    const uint8_t* vb = b.blk + B::kHalf;
+    const int g = 2 * t;
+    T* dst = static_cast<T*>(p.v) + (int64_t)h * HD + 32 * j + g;
+    const int odd_first = b.first & 1, pairs = (b.n + odd_first + 1) / 2;
+#pragma unroll 1
+    for (int u0 = set; u0 < pairs; u0 += L::kPairsAhead * L::kRows) {
+      uint32_t w[L::kPairsAhead][2], m[L::kPairsAhead];
+      __half d[L::kPairsAhead][2];
+#pragma unroll
+      for (int a = 0; a < L::kPairsAhead; ++a) {
+        const int row = in_page - odd_first + 2 * min(u0 + a * L::kRows, pairs - 1);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          w[a][e] = reinterpret_cast<const uint32_t*>(vb)[B::v_half(row, j, g + e) / 2];
+          d[a][e] = reinterpret_cast<const __half*>(vb + B::kCodes)[B::scale(row + e, j)];
+        }
+        m[a] = reinterpret_cast<const uint32_t*>(vb + B::kCodes + B::kScales)[B::v_min(row, j) / 2];
+      }
+#pragma unroll
+      for (int a = 0; a < L::kPairsAhead; ++a)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int r = 2 * (u0 + a * L::kRows) + o - odd_first;
+          // nibbles n of g and of g + 1
+          const uint32_t both = __byte_perm(w[a][0], w[a][1], o ? 0x7632 : 0x5410);
+          float v[8];
+          dequantise(both, __half2float(d[a][o]), __half2float(__ushort_as_half((unsigned short)(m[a] >> (16 * o)))), v);
+          if (r >= 0 && r < b.n)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const float two[2] = {v[n], v[4 + n]};
+              store_vec<T, 2>(dst + (b.row0 + r) * p.v_stride + 8 * n, two);
+            }
+        }
+    }
   }
 }
 
 template <int HD, typename T>
 cudaError_t launch(const LaunchEnv& env, bool store, const Kv4RowParams& p) {
-  const dim3 grid((unsigned)(((int64_t)p.rows * p.nkv + kRowWarps - 1) / kRowWarps)), block(32 * kRowWarps);
+  const dim3 grid((unsigned)((2 * (int64_t)p.slots * p.nkv + kRowWarps - 1) / kRowWarps)), block(32 * kRowWarps);
   return store ? rrr_launch_pdl(kv4_store_kernel<HD, T>, grid, block, 0, env.stream, env.pdl, p)
                : rrr_launch_pdl(kv4_load_kernel<HD, T>, grid, block, 0, env.stream, env.pdl, p);
 }
@@ -225,7 +369,7 @@ int kv4_rows(rrr_ctx* ctx, const char* fn, bool store, const rrr_kv4_cache* c, i
   if ((store ? !k || !v : !k && !v) || !cu_rows || !kv_lens)
     return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
-  if (rows < 0 || (int64_t)rows * c->n_kv_heads > (int64_t)INT32_MAX * kRowWarps || (k && k_stride < width) || (v && v_stride < width))
+  if (rows < 0 || (k && k_stride < width) || (v && v_stride < width))
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows >= 0 and strides of at least n_kv_heads * head_dim", fn);
   if (!aligned_to(k, 16) || !aligned_to(v, 16) || (k && k_stride % 8) || (v && v_stride % 8) ||
       !aligned_to(cu_rows, 4) || !aligned_to(kv_lens, 4))
@@ -239,9 +383,11 @@ int kv4_rows(rrr_ctx* ctx, const char* fn, bool store, const rrr_kv4_cache* c, i
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
   if (rows == 0 || c->n_seqs == 0) return RRR_OK;
+  if (c->n_seqs > INT32_MAX / 4 || ((int64_t)rows / kBlockRows + 2 * (int64_t)c->n_seqs) * c->n_kv_heads > INT32_MAX)
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows and sequences for one call", fn);
   const LaunchEnv env = make_env(ctx, stream);
   const Kv4RowParams p{static_cast<uint8_t*>(c->pages), c->n_pages, c->table_stride, c->page_table, c->n_seqs,
-                       c->max_pages, c->n_kv_heads, rows, k, v, k_stride, v_stride, cu_rows, kv_lens, env.d_err};
+                       c->max_pages, c->n_kv_heads, rows, rows / kBlockRows + 2 * c->n_seqs, k, v, k_stride, v_stride, cu_rows, kv_lens, env.d_err};
   cudaError_t e;
   switch (c->head_dim) {
     case 64: e = launch_type<64>(env, type, store, p); break;
