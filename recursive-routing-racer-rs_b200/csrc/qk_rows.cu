@@ -15,6 +15,8 @@
 // another lane at the same place (rope_dim a multiple of 2D).
 #include <math.h>
 
+#include <type_traits>
+
 #include "serve_common.cuh"
 
 namespace rrr {
@@ -43,31 +45,32 @@ struct QkParams {
   double turns[kMaxPairs];  // theta^(-2i/rope_dim) / 2 pi
 };
 
-template <int HD, typename TIN, typename TOUT>
+template <int HD, bool HALVES, typename TIN, typename TOUT>
 __global__ void __launch_bounds__(32 * kQkWarps) qk_rows_kernel(const __grid_constant__ QkParams p) {
   constexpr int D = HD / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kQkWarps + (threadIdx.x >> 5);
-  const int64_t row = item / p.chunks;
+  const int lane = threadIdx.x & 31, e0 = D * lane;
+  const int item = blockIdx.x * kQkWarps + (threadIdx.x >> 5);
+  const int row = item / p.chunks;
   if (row >= p.rows) return;
-  const int h0 = (int)(item - row * p.chunks) * p.chunk, h1 = min(h0 + p.chunk, p.heads);
+  const int h0 = (item - row * p.chunks) * p.chunk, h1 = min(h0 + p.chunk, p.heads);
   const int pos = p.positions[row];
   if (pos < 0 || pos >= p.max_pos) {
     if (h0 == 0 && lane == 0) flag_position(p.err);
     return;
   }
-  // cos and sin of this lane's values; a value outside the rotation has (1, 0)
+  // cos and sin of this lane's values; values outside the rotation keep theirs
   float cs[D], sn[D];
-  const int e0 = D * lane;
+  bool turns[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     const int e = e0 + d;
+    turns[d] = e < 2 * p.half_dim;
     cs[d] = 1.f;
     sn[d] = 0.f;
-    if (e < 2 * p.half_dim && (p.halves || (d & 1) == 0)) {
-      const int i = p.halves ? (e < p.half_dim ? e : e - p.half_dim) : e >> 1;
+    if (turns[d] && (HALVES || (d & 1) == 0)) {
+      const int i = HALVES ? (e < p.half_dim ? e : e - p.half_dim) : e >> 1;
       double t = p.turns[i];
       if (i < p.n_factors) t /= (double)p.factors[i];
       t -= floor(t);
@@ -79,67 +82,96 @@ __global__ void __launch_bounds__(32 * kQkWarps) qk_rows_kernel(const __grid_con
       cs[d] = c * p.attn_factor;
       sn[d] = s * p.attn_factor;
       // the first of a pair subtracts its partner's product, the second adds it
-      if (p.halves && e < p.half_dim) sn[d] = -sn[d];
+      if (HALVES && e < p.half_dim) sn[d] = -sn[d];
     }
   }
   const int hop = p.half_dim / D;  // lanes between the partners of (i, i + half)
-  const int partner = lane < hop ? lane + hop : lane - hop;
-  const TIN* src = static_cast<const TIN*>(p.qkv) + row * p.row_stride;
-  for (int h = h0; h < h1; h += kBatch) {
-    float x[kBatch][D];
+  const int partner = (lane < hop ? lane + hop : lane - hop) & 31;
+  const TIN* src = static_cast<const TIN*>(p.qkv) + row * p.row_stride + e0;
+
+  // heads [a, b) of one kind; dst: where head a goes
+  auto heads = [&](auto rotate, auto norm, int a, int b, TOUT* dst, const float* gamma) {
+    float gm[D];
+    if constexpr (decltype(norm)::value) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (h + b < h1) load_vec<TIN, D>(src + (int64_t)(h + b) * HD + e0, x[b]);
+      for (int d = 0; d < D; ++d) gm[d] = gamma[e0 + d];
+    }
+#pragma unroll 1
+    for (int h = a; h < b; h += kBatch) {
+      float x[kBatch][D];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int hb = h + b;
-      if (hb >= h1) break;
-      TOUT* dst;
-      if (hb < p.nh)
-        dst = static_cast<TOUT*>(p.q) + row * p.q_stride + (int64_t)hb * HD;
-      else if (hb < p.nh + p.nkv)
-        dst = static_cast<TOUT*>(p.k) + row * p.k_stride + (int64_t)(hb - p.nh) * HD;
-      else
-        dst = static_cast<TOUT*>(p.v) + row * p.v_stride + (int64_t)(hb - p.nh - p.nkv) * HD;
-      if (hb < p.nh + p.nkv) {
-        const float* gamma = hb < p.nh ? p.q_gamma : p.k_gamma;
-        if (gamma) {
-          float sq = 0.f;
+      for (int k = 0; k < kBatch; ++k)  // (heads past the last are read as it)
+        load_vec<TIN, D>(src + (int64_t)min(h + k, b - 1) * HD, x[k]);
+      if constexpr (decltype(norm)::value) {
+        float sq[kBatch];
 #pragma unroll
-          for (int d = 0; d < D; ++d) sq = fmaf(x[b][d], x[b][d], sq);
-          const float inv = 1.f / sqrtf(warp_sum(sq) * (1.f / HD) + p.eps);
+        for (int k = 0; k < kBatch; ++k) {
+          sq[k] = 0.f;
 #pragma unroll
-          for (int d = 0; d < D; ++d) x[b][d] = (gamma[e0 + d] * x[b][d]) * inv;
+          for (int d = 0; d < D; ++d) sq[k] = fmaf(x[k][d], x[k][d], sq[k]);
         }
-        if (p.halves) {
 #pragma unroll
-          for (int d = 0; d < D; ++d) {
-            const float o = __shfl_sync(0xffffffffu, x[b][d], partner & 31);
-            if (e0 + d < 2 * p.half_dim) x[b][d] = fmaf(o, sn[d], x[b][d] * cs[d]);
-          }
-        } else {
+        for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-          for (int d = 0; d < D; d += 2)
-            if (e0 + d < 2 * p.half_dim) {
-              const float a = x[b][d], c = x[b][d + 1];
-              x[b][d] = fmaf(-c, sn[d], a * cs[d]);
-              x[b][d + 1] = fmaf(a, sn[d], c * cs[d]);
-            }
+          for (int k = 0; k < kBatch; ++k) sq[k] += __shfl_xor_sync(0xffffffffu, sq[k], o);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float inv = rsqrtf(fmaf(sq[k], 1.f / HD, p.eps));
+#pragma unroll
+          for (int d = 0; d < D; ++d) x[k][d] = (gm[d] * x[k][d]) * inv;
         }
       }
-      store_vec<TOUT, D>(dst + e0, x[b]);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if constexpr (decltype(rotate)::value && HALVES) {
+#pragma unroll
+          for (int d = 0; d < D; ++d) {
+            const float o = __shfl_sync(0xffffffffu, x[k][d], partner);
+            if (turns[d]) x[k][d] = fmaf(o, sn[d], x[k][d] * cs[d]);
+          }
+        } else if constexpr (decltype(rotate)::value) {
+#pragma unroll
+          for (int d = 0; d < D; d += 2) {
+            const float u = x[k][d], v = x[k][d + 1];
+            if (turns[d]) {
+              x[k][d] = fmaf(-v, sn[d], u * cs[d]);
+              x[k][d + 1] = fmaf(u, sn[d], v * cs[d]);
+            }
+          }
+        }
+        if (h + k < b) store_vec<TOUT, D>(dst + (int64_t)(h + k - a) * HD + e0, x[k]);
+      }
     }
-  }
+  };
+  auto rotated = [&](int first, int count, void* out, int64_t stride, const float* gamma) {
+    const int a = max(h0, first), b = min(h1, first + count);
+    if (a >= b) return;
+    TOUT* dst = static_cast<TOUT*>(out) + row * stride + (int64_t)(a - first) * HD;
+    if (gamma)
+      heads(std::true_type{}, std::true_type{}, a, b, dst, gamma);
+    else
+      heads(std::true_type{}, std::false_type{}, a, b, dst, gamma);
+  };
+  rotated(0, p.nh, p.q, p.q_stride, p.q_gamma);
+  rotated(p.nh, p.nkv, p.k, p.k_stride, p.k_gamma);
+  const int a = max(h0, p.nh + p.nkv);
+  if (a < h1)
+    heads(std::false_type{}, std::false_type{}, a, h1,
+          static_cast<TOUT*>(p.v) + row * p.v_stride + (int64_t)(a - p.nh - p.nkv) * HD, nullptr);
 }
 
+template <int HD, typename TIN, typename TOUT>
+cudaError_t launch(const LaunchEnv& env, dim3 grid, const QkParams& p) {
+  const dim3 block(32 * kQkWarps);
+  return p.halves ? rrr_launch_pdl(qk_rows_kernel<HD, true, TIN, TOUT>, grid, block, 0, env.stream, env.pdl, p)
+                  : rrr_launch_pdl(qk_rows_kernel<HD, false, TIN, TOUT>, grid, block, 0, env.stream, env.pdl, p);
+}
 template <int HD, typename TIN>
 cudaError_t launch_out(const LaunchEnv& env, int out_type, dim3 grid, const QkParams& p) {
-  const dim3 block(32 * kQkWarps);
   switch (out_type) {
-    case RRR_F32: return rrr_launch_pdl(qk_rows_kernel<HD, TIN, float>, grid, block, 0, env.stream, env.pdl, p);
-    case RRR_F16: return rrr_launch_pdl(qk_rows_kernel<HD, TIN, __half>, grid, block, 0, env.stream, env.pdl, p);
-    default:
-      return rrr_launch_pdl(qk_rows_kernel<HD, TIN, __nv_bfloat16>, grid, block, 0, env.stream, env.pdl, p);
+    case RRR_F32: return launch<HD, TIN, float>(env, grid, p);
+    case RRR_F16: return launch<HD, TIN, __half>(env, grid, p);
+    default: return launch<HD, TIN, __nv_bfloat16>(env, grid, p);
   }
 }
 template <int HD>
@@ -236,6 +268,7 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
   p.chunk = (p.chunk + kBatch - 1) / kBatch * kBatch;
   p.chunks = (p.heads + p.chunk - 1) / p.chunk;
   const int64_t blocks = ((int64_t)rows * p.chunks + kQkWarps - 1) / kQkWarps;
+  if ((blocks + 1) * kQkWarps > INT32_MAX) return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows for one call", fn);
   const LaunchEnv env = make_env(ctx, stream);
   p.err = env.d_err;
   cudaError_t e;
