@@ -34,13 +34,13 @@ def _fail(code: int, message: str):
 
 def _on(ctx: ffi.Context, t, what: str):
     """t's device address, checked to be on the context's GPU."""
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         _fail(-1, f"{what}: a tensor on cuda:{ctx.device} is needed, got one on {t.device}")
     return t.data_ptr()
 
 
 def _ints(ctx: ffi.Context, t, n: int, what: str):
-    if t.dim() != 1 or t.shape[0] != n or t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
+    if t.shape != (n,) or t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
         _fail(-3, f"{what}: a contiguous int32[{n}] is needed, got {t.dtype}{list(t.shape)}")
     return _on(ctx, t, what)
 
@@ -48,14 +48,29 @@ def _ints(ctx: ffi.Context, t, n: int, what: str):
 def _heads(ctx: ffi.Context, t, heads: int, hd: int, what: str, rows: int | None = None):
     """[rows, heads, hd] (or [rows, heads * hd]) with the heads of a row next to each other:
     (address, rows, row stride)."""
-    shape, stride = t.shape, t.stride()
-    flat = t.dim() == 2 and shape[1] == heads * hd and stride[1] == 1
-    split = t.dim() == 3 and shape[1] == heads and shape[2] == hd and stride[2] == 1 and \
-        (heads == 1 or stride[1] == hd)
-    if not (flat or split) or (rows is not None and shape[0] != rows):
+    shape = t.shape
+    n = shape[0]
+    if t.is_contiguous():  # the usual case, told in fewer calls
+        row = heads * hd
+        fine = shape == (n, heads, hd) or shape == (n, row)
+    else:
+        stride = t.stride()
+        fine = (shape == (n, heads, hd) and stride[2] == 1 and (heads == 1 or stride[1] == hd)) or \
+            (shape == (n, heads * hd) and stride[1] == 1)
+        row = stride[0] if n > 1 else heads * hd
+    if not fine or (rows is not None and n != rows):
         _fail(-3, f"{what}: rows [{'rows' if rows is None else rows}, {heads}, {hd}] with their heads next to "
-                  f"each other are needed, got {list(shape)} with strides {list(stride)}")
-    return _on(ctx, t, what), shape[0], stride[0] if shape[0] > 1 else heads * hd
+                  f"each other are needed, got {list(shape)} with strides {list(t.stride())}")
+    return _on(ctx, t, what), n, row
+
+
+def _strides(t, what: str):
+    """Row and head strides of [rows, heads, hd]; the stride of a dimension of one is free."""
+    rows, heads, hd = t.shape
+    row, head, one = t.stride()
+    if one != 1:
+        _fail(-3, f"{what}: the values of a head must be contiguous")
+    return row if rows > 1 else heads * hd, head if heads > 1 else hd
 
 
 def qk_norm_rope(ctx: ffi.Context, desc: ffi.AttnDesc, qkv, positions, q, k, v=None, *, q_gamma=None,
@@ -76,9 +91,11 @@ def qk_norm_rope(ctx: ffi.Context, desc: ffi.AttnDesc, qkv, positions, q, k, v=N
             if _type(g, name) != ffi.F32 or g.numel() != hd or not g.is_contiguous():
                 _fail(-3, f"{name}: a contiguous float32[{hd}] is needed")
             gammas[i] = _on(ctx, g, name)
-    ctx.check(ffi.lib().rrr_qk_norm_rope(
+    rc = ffi.lib().rrr_qk_norm_rope(
         ctx.h, byref(desc), _type(qkv, "qkv"), pin, sin, rows, _ints(ctx, positions, rows, "positions"),
-        gammas[0], gammas[1], eps, 1 if halves else 0, out, pq, sq, pk, sk, pv, sv, _stream(stream)))
+        gammas[0], gammas[1], eps, 1 if halves else 0, out, pq, sq, pk, sk, pv, sv, _stream(stream))
+    if rc:
+        ctx.check(rc)
 
 
 def attention_packed(ctx: ffi.Context, q, k, v, cu_q, cu_kv, out, *, causal: bool = True,
@@ -91,20 +108,16 @@ def attention_packed(ctx: ffi.Context, q, k, v, cu_q, cu_kv, out, *, causal: boo
     kind = _type(q, "q")
     if not (q.dtype == k.dtype == v.dtype == out.dtype):
         _fail(-2, "q, k, v and out must have one type")
-    d = ffi.PackedDesc(kind, q.shape[1], k.shape[1], q.shape[2], max(cu_q.shape[0] - 1, 0), 1 if causal else 0,
-                       scale, q.shape[0], k.shape[0])
-    ptr = []
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        row, head, one = t.stride()
-        if one != 1:
-            _fail(-3, f"{name}: the values of a head must be contiguous")
-        # the stride of a dimension of one is free
-        setattr(d, name + "_head", head if t.shape[1] > 1 else t.shape[2])
-        setattr(d, name + "_row", row if t.shape[0] > 1 else t.shape[1] * t.shape[2])
-        ptr.append(_on(ctx, t, name))
-    n = d.n_seqs + 1
-    ctx.check(ffi.lib().rrr_attention_packed(ctx.h, byref(d), ptr[0], ptr[1], ptr[2], _ints(ctx, cu_q, n, "cu_q"),
-                                             _ints(ctx, cu_kv, n, "cu_kv"), ptr[3], _stream(stream)))
+    qs, ks, vs, os = (_strides(t, name) for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
+    rows, heads, hd = q.shape
+    n = cu_q.shape[0]
+    d = ffi.PackedDesc(kind, heads, k.shape[1], hd, max(n - 1, 0), 1 if causal else 0, scale, rows, k.shape[0],
+                       *qs, *ks, *vs, *os)
+    rc = ffi.lib().rrr_attention_packed(ctx.h, byref(d), _on(ctx, q, "q"), _on(ctx, k, "k"), _on(ctx, v, "v"),
+                                        _ints(ctx, cu_q, n, "cu_q"), _ints(ctx, cu_kv, n, "cu_kv"),
+                                        _on(ctx, out, "out"), _stream(stream))
+    if rc:
+        ctx.check(rc)
     return out
 
 
@@ -126,6 +139,7 @@ class KV4Cache:
         stride = page_table.stride(0) if n_seqs > 1 else most
         self.desc = ffi.KV4Desc(_on(ctx, pages, "pages"), pages.shape[0], pages.shape[1], head_dim,
                                 _on(ctx, page_table, "page_table"), n_seqs, most, stride)
+        self._desc = byref(self.desc)
 
     @staticmethod
     def page_shape(n_pages: int, n_kv_heads: int, head_dim: int):
@@ -149,15 +163,17 @@ class KV4Cache:
     def store(self, k, v, cu_rows, kv_lens, stream=None) -> None:
         """rrr_kv4_store: packed rows [rows, n_kv, hd] become the last ones of their sequences,
         which have kv_lens rows then."""
-        self.ctx.check(ffi.lib().rrr_kv4_store(self.ctx.h, byref(self.desc), *self._rows(k, v, cu_rows, kv_lens),
-                                               _stream(stream)))
+        rc = ffi.lib().rrr_kv4_store(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens), _stream(stream))
+        if rc:
+            self.ctx.check(rc)
 
     def load(self, cu_rows, kv_lens, k=None, v=None, stream=None) -> None:
         """rrr_kv4_load: the last rows of every sequence, dequantised, into packed rows."""
         if k is None and v is None:
             _fail(-1, "load: k or v is needed")
-        self.ctx.check(ffi.lib().rrr_kv4_load(self.ctx.h, byref(self.desc), *self._rows(k, v, cu_rows, kv_lens),
-                                              _stream(stream)))
+        rc = ffi.lib().rrr_kv4_load(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens), _stream(stream))
+        if rc:
+            self.ctx.check(rc)
 
     def workspace(self, n_heads: int):
         """A workspace for `attention`; calls that can run at the same time need one each."""
@@ -175,8 +191,9 @@ class KV4Cache:
         heads = q.shape[1]
         pq, _, sq = _heads(self.ctx, q, heads, self.head_dim, "q", self.n_seqs)
         po, _, so = _heads(self.ctx, out, heads, self.head_dim, "out", self.n_seqs)
-        self.ctx.check(ffi.lib().rrr_attention_kv4(
-            self.ctx.h, byref(self.desc), heads, _type(q, "q"), pq, sq, _ints(self.ctx, kv_lens, self.n_seqs, "kv_lens"),
-            scale, po, so, _on(self.ctx, workspace, "workspace"), workspace.numel() * workspace.element_size(),
-            _stream(stream)))
+        rc = ffi.lib().rrr_attention_kv4(
+            self.ctx.h, self._desc, heads, _type(q, "q"), pq, sq, _ints(self.ctx, kv_lens, self.n_seqs, "kv_lens"),
+            scale, po, so, _on(self.ctx, workspace, "workspace"), workspace.nbytes, _stream(stream))
+        if rc:
+            self.ctx.check(rc)
         return out
