@@ -19,9 +19,11 @@
 // shared memory, rounded, every kFlush pages. The softmax runs online in base 2, with 32-bit maxima
 // and sums; scores, weights and sums keep f32 accuracy throughout.
 //
-// Work. A unit is one page (64 rows) of one (sequence, KV head). The CTAs share all units of the
+// Work. A unit is one page (64 rows) of one (sequence, KV head), and each of those has kStart units
+// more in front, which is what beginning and ending one costs. The CTAs share all U units of the
 // batch evenly, in order, whatever the lengths are (read on the device): CTA c of G takes the
-// units [c U / G, (c+1) U / G). One producer warp streams the pages' blocks, each one
+// pages in [c U / G, (c+1) U / G). (Without the units in front, the CTA with the most short
+// sequences took 137 us of the batch of 64, the middle one 103.) One producer warp streams the pages' blocks, each one
 // contiguous, with bulk copies into a ring of stages, the segment's query row with its first
 // page; four consumer warps take 16 rows of a page each and keep their own softmax state. At
 // the end of a (sequence, head) segment the warps' states are joined in order; a segment that
@@ -40,6 +42,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxStages = 16;
 constexpr int kMaxHpk = 8;
 constexpr float kLo = 1.f / 2048.f;
+constexpr int kStart = 2;   // units in front of a (sequence, head)'s pages
 constexpr int kFlush = 16;  // pages whose products one set of accumulators takes
 
 struct Kv4Params {
@@ -61,6 +64,7 @@ struct Kv4Params {
 struct Segment {  // beside each stage: this CTA's run of pages of one (sequence, head)
   long long base;  // unit of the (sequence, head)'s first page
   int seq, head, pages;
+  int more;        // whether another run follows
   int valid;       // rows of this page that count
   int first_page;  // of the run
   int first, left; // whether this page is the run's first; its pages from this one on
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   const int per = (p.n_seqs + kThreads - 1) / kThreads;
   const int my0 = min(p.n_seqs, (int)threadIdx.x * per), my1 = min(p.n_seqs, my0 + per);
   long long mine = 0;
-  for (int s = my0; s < my1; ++s) mine += (long long)pages_of(seq_len(s)) * p.nkv;
+  for (int s = my0; s < my1; ++s) mine += (long long)(pages_of(seq_len(s)) + kStart) * p.nkv;
   long long upto = mine;  // units of this warp's threads up to this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     int s = my0;
     long long base = before;
     for (;; ++s) {
-      const long long n = (long long)pages_of(seq_len(s)) * p.nkv;
+      const long long n = (long long)(pages_of(seq_len(s)) + kStart) * p.nkv;
       if (u0 < base + n || s + 1 >= my1) break;
       base += n;
     }
@@ -249,24 +253,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     first_base = base;
   }
   __syncthreads();
+  // the first page: its sequence, the sequence's first unit, its head and number
+  int s0 = first_seq;
+  const long long base0 = first_base;
+  int len0 = seq_len(s0), np0 = pages_of(len0);
+  const int head0 = (int)((u0 - base0) / (np0 + kStart));
+  const int page0 = max(0, (int)((u0 - base0) % (np0 + kStart)) - kStart);
+  if (base0 + (long long)head0 * (np0 + kStart) + kStart + page0 >= u1) return;  // units without a page
 
   if (warp == kConsumers) {
     // ---------------- producer
-    int s = first_seq;
-    long long base = first_base;
-    int len = seq_len(s), np = pages_of(len);
-    int head = (int)((u0 - base) / np), page = (int)((u0 - base) % np);
+    int s = s0, len = len0, np = np0, head = head0, page = page0;
+    long long base = base0;
     int first_page = page, ids_at = -1, id = 0;
     int it = 0, st = 0;
     uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
     bool ok = true;
     const uint32_t q_bytes = (uint32_t)(p.hpk * HD * sizeof(T));
-    for (long long u = u0; u < u1; ++u, ++it) {
+    for (;; ++it) {
       if (page >= np) {
         page = 0;
         if (++head >= p.nkv) {
           head = 0;
-          base += (long long)np * p.nkv;
+          base += (long long)(np + kStart) * p.nkv;
+          if (base + kStart >= u1) break;
           ++s;
           len = seq_len(s);
           np = pages_of(len);
@@ -274,6 +284,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         first_page = 0;
         ids_at = -1;
       }
+      const long long at = base + (long long)head * (np + kStart) + kStart;  // unit of page 0
+      if (at + page >= u1) break;
       if (ids_at < 0 || page >= ids_at + 32) {  // the numbers of the next 32 pages, one per lane
         ids_at = page;
         id = len > 0 && page + lane < np ? p.table[(int64_t)s * p.table_stride + page + lane] : 0;
@@ -288,9 +300,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)wait_asleep(&empty[st], phase, p.err, kDevErrEmptyTimeout) : 0, 0);
       if (!ok) break;
       if (lane == 0) {
-        const bool first = u == u0 || page == 0;
-        const int left = (int)(u1 - u < np - page ? u1 - u : np - page);
-        seg[st] = Segment{base + (long long)head * np, s, head, np, valid, first_page, first ? 1 : 0, left};
+        const bool first = it == 0 || page == 0;
+        const int left = (int)(u1 - (at + page) < np - page ? u1 - (at + page) : np - page);
+        seg[st] = Segment{at, s, head, np, at + np + kStart < u1, valid, first_page, first ? 1 : 0, left};
         uint8_t* dst = smem + (size_t)st * p.stage_bytes;
         mbar_arrive_expect_tx(&full[st], (valid ? (uint32_t)B::kBytes : 0u) + (first ? q_bytes : 0u));
         if (first)
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       phase ^= 1;
     }
   };
-  for (long long u = u0; u < u1; ++u) {
+  for (;;) {
     if (!landed()) return;
     const Segment sg = seg[st];
     const uint8_t* blk = smem + (size_t)st * p.stage_bytes;
@@ -643,6 +655,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         }
       }
     }
+    if (!sg.more) return;
     if (!sync()) return;  // the joined states are read: the next segment may write its own
   }
 }
@@ -734,7 +747,7 @@ cudaError_t launch(const LaunchEnv& env, Kv4Params p) {
   auto kern = kv4_attention_kernel<HD, NT, T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int64_t units = (int64_t)p.n_seqs * p.nkv * (p.max_pages > 0 ? p.max_pages : 1);
+  const int64_t units = (int64_t)p.n_seqs * p.nkv * ((p.max_pages > 0 ? p.max_pages : 1) + kStart);
   const int ctas = env.sm_count * kCtas;
   const int grid = (int)(units < ctas ? units : ctas);
   e = rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl, p);
