@@ -7,23 +7,31 @@
 // (f16 in, f32 accumulate): 16 rows of codes are the A operand, and the B operand's eight columns
 // are four query heads as (hi, lo) pairs: the f16 part of the (power-of-two scaled) query and
 // the remainder (q - hi) * 2^11, so a score carries 22 bits of the query. A code shifted into the
-// top of an f16's mantissa is 1 + code / 16 (a shift and an AND-OR for two operands); the
-// accumulators start at -sum q_j, the power of two leaves with the scales and d_j multiplies them
-// in f32. One more product takes the m_j. (The code in the low bits would be the subnormal code * 2^-24 for fewer
-// instructions, but the tensor core aligns a subnormal's products as if they were normal: they
-// lost 6 bits, an error of 1e-6 in the scores.) The second product is alike: A holds
-// V's codes, B the weights p_i d_ij of group j as (hi, lo), and the sums of p_i (m_ij + 7.5 d_ij)
-// run beside it in f32. V's codes are centred, code - 7.5: over a long context the weighted values
-// nearly cancel, and sums of the codes themselves would be hundreds of times the result (measured:
-// an error of 1.2e-3 at 131,000 rows). The tensor core truncates its sums, so they are moved to
-// shared memory, rounded, every kFlush pages. The softmax runs online in base 2, with 32-bit maxima
-// and sums; scores, weights and sums keep f32 accuracy throughout.
+// top of an f16's mantissa is 1 + code / 16 (a shift and an AND-OR for two operands); sum q_j is
+// taken off the products (as the accumulators' start it cost two moves per subtraction), the power
+// of two leaves with the scales and d_j multiplies them in f32. One more product takes the m_j.
+// (The code in the low bits would be the subnormal code * 2^-24 for fewer instructions, but the
+// tensor core aligns a subnormal's products as if they were normal: they lost 6 bits, an error of
+// 1e-6 in the scores.) The second product is alike: A holds V's codes, B the weights p_i d_ij of
+// group j as (hi, lo), and the sums of p_i (m_ij + 8 d_ij) run beside it in f32. V's codes are
+// centred, code - 8: over a long context the weighted values nearly cancel, and sums of the codes
+// themselves would be hundreds of times the result (measured: an error of 1.2e-3 at 131,000 rows).
+// (8 rather than 7.5 because both nibbles of a byte can then be centred where they stand.) The
+// tensor core truncates its sums, so they are moved to shared memory, rounded, every kFlush pages.
+// The softmax runs online in base 2, with 32-bit maxima and sums: a slice of rows without a new
+// maximum, which is nearly every one, skips the exchange of maxima and the rescaling. Scores,
+// weights and sums keep f32 accuracy throughout.
+//
+// Bound by instructions: about 520 per warp for 16 rows of 4 heads x 128, where the issue slots
+// are 61 % taken (131,072 rows of 8 heads: 66 us, 2.5 TB/s of codes; 64 sequences, 261,424 rows:
+// 111 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA per SM (96 registers,
+// a few spilt) was 8 % slower, so it is not latency that is missing.
 //
 // Work. A unit is one page (64 rows) of one (sequence, KV head), and each of those has kStart units
 // more in front, which is what beginning and ending one costs. The CTAs share all U units of the
 // batch evenly, in order, whatever the lengths are (read on the device): CTA c of G takes the
 // pages in [c U / G, (c+1) U / G). (Without the units in front, the CTA with the most short
-// sequences took 137 us of the batch of 64, the middle one 103.) One producer warp streams the pages' blocks, each one
+// sequences took 137 us of the batch of 64, the middle one 103; with them all take 118.) One producer warp streams the pages' blocks, each one
 // contiguous, with bulk copies into a ring of stages, the segment's query row with its first
 // page; four consumer warps take 16 rows of a page each and keep their own softmax state. At
 // the end of a (sequence, head) segment the warps' states are joined in order; a segment that
@@ -42,6 +50,7 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMaxStages = 16;
 constexpr int kMaxHpk = 8;
 constexpr float kLo = 1.f / 2048.f;
+constexpr float kNone = -3e38f;  // the maximum of no rows: finite, so that it may be subtracted from -inf
 constexpr int kStart = 2;   // units in front of a (sequence, head)'s pages
 constexpr int kFlush = 16;  // pages whose products one set of accumulators takes
 
@@ -113,7 +122,7 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {
 }
 
 // (w & mask) | bits in one instruction: `bits` comes in a register, an instruction has room for
-// one constant (with both as constants each pair of operands cost two: 16 % more time)
+// one constant (with both as constants each pair of operands cost two)
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t x;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "r"(mask), "r"(bits));
@@ -125,11 +134,17 @@ __device__ __forceinline__ uint32_t opaque(uint32_t v) {
 }
 // 1 + code / 16 of the four bits at 6..9 of both halves of w (one: 0x3C003C00)
 __device__ __forceinline__ uint32_t from_one(uint32_t w, uint32_t one) { return and_or(w, 0x03C003C0u, one); }
-// 16 (code - 7.5) of the four bits at 4..7 of both halves of w: 1024 + 16 code - 1144, exact
-// (big: 0x64006400)
+// 16 (code - 8) of the four bits at 4..7 and at 0..3 of both halves of w, exact: 1024 + 16 code
+// - 1152, and 16 (1024 + code) - 16512 (big: 0x64006400)
 __device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t big) {
   const uint32_t x = and_or(w, 0x00F000F0u, big);
-  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0xe478)));
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0xe480)));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ uint32_t centred_low(uint32_t w, uint32_t big) {
+  const uint32_t x = and_or(w, 0x000F000Fu, big);
+  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x4c00)),
+                            __half2half2(__ushort_as_half(0xf408)));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 // N words at p (N a power of two; p aligned to min(16, 4 N))
@@ -149,22 +164,6 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
       w[i + 1] = v.y;
       w[i + 2] = v.z;
       w[i + 3] = v.w;
-    }
-  }
-}
-
-// The producer's wait for a free stage, bounded: with several stages ahead it is in no hurry, and
-// a wait that polls takes issue slots from the consumers (measured: a third of all
-// instructions), so it sleeps between its polls.
-__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(err);
-  for (;;) {
-    __nanosleep(400);
-    if (mbar_try_wait(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > limit) {
-      if (err) atomicCAS(err, 0, code);
-      return false;
     }
   }
 }
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         if (lane == 0) flag_position(p.err);
         valid = 0;
       }
-      ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)wait_asleep(&empty[st], phase, p.err, kDevErrEmptyTimeout) : 0, 0);
+      ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)mbar_wait_bounded(&empty[st], phase, p.err, kDevErrEmptyTimeout) : 0, 0);
       if (!ok) break;
       if (lane == 0) {
         const bool first = it == 0 || page == 0;
@@ -335,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   const uint32_t one = opaque(0x3C003C00u), big = opaque(0x64006400u);
   ConsumerSync sync{&cons_bar, 0, p.err};
   uint32_t qb[NT][G][4], qm[NT];  // B: two k steps per group; the groups' sums of q
-  float qi[NT][G][2];             // head t: minus the sums of hi and lo
+  float qs[NT][G];                // head t: the groups' sums of q
   float kscale[NT], m[NT], l[NT], m_held[NT];  // head t; m_held: of what shared memory holds
   float o[NT][2 * G][4];          // values: [16 u + (g, g + 8)] of group j, head t
   float om[NT][G];                // middles of group j, head g / 2, this lane's rows
@@ -346,8 +345,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   auto flush = [&]() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m_use = m[n] == -INFINITY ? 0.f : m[n];
-      const float keep = ex2(m_held[n] - m_use);
+      const float keep = ex2(m_held[n] - m[n]);
       const int h = 4 * n + t;
       float* dst = wo + ((size_t)warp * p.hpk + h) * PITCH;
 #pragma unroll
@@ -405,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = 0.f;
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int P = 0; P < B::kPlanes; ++P) {
         uint32_t wa[J], wb[J];
@@ -420,18 +419,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           const float d0 = half_of(da[j / 2], j & 1), d1 = half_of(db[j / 2], j & 1);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float init[4] = {qi[n][j][0], qi[n][j][1], qi[n][j][0], qi[n][j][1]};
             float c[4];
-            mma_f16(c, a0, qb[n][j][0], qb[n][j][1], init);
+            mma_f16(c, a0, qb[n][j][0], qb[n][j][1], zero);
             mma_f16(c, a1, qb[n][j][2], qb[n][j][3]);
-            s[n][0] = fmaf(d0, fmaf(c[1], kLo, c[0]), s[n][0]);
-            s[n][1] = fmaf(d1, fmaf(c[3], kLo, c[2]), s[n][1]);
+            s[n][0] = fmaf(d0, fmaf(c[1], kLo, c[0] - qs[n][j]), s[n][0]);
+            s[n][1] = fmaf(d1, fmaf(c[3], kLo, c[2] - qs[n][j]), s[n][1]);
           }
         }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         float c[4];
         mma_f16(c, ma, qm[n], 0u, zero);
         s[n][0] = fmaf(s[n][0], 16.f, fmaf(c[1], kLo, c[0])) * kscale[n];
@@ -447,39 +444,39 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     }
     // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
     // rows 2t, 2t + 1 of the first (g even) or second eight rows
-    float pa[NT], pb[NT], alpha[NT];
+    float pa[NT], pb[NT];
     bool grow = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float top = fmaxf(s[n][0], s[n][1]);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      const float m_new = fmaxf(m[n], top), m_use = m_new == -INFINITY ? 0.f : m_new;
-      alpha[n] = ex2(m[n] - m_use);
-      grow |= m_new > m[n];
-      m[n] = m_new;
-      {
-        const float p0 = ex2(s[n][0] - m_use), p1 = ex2(s[n][1] - m_use);
-        l[n] = fmaf(l[n], alpha[n], p0 + p1);
-        const int from = 8 * t + (g >> 1);
-        const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
-        const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
-        pa[n] = odd ? a1 : a0;
-        pb[n] = odd ? b1 : b0;
-      }
-    }
-    if (__any_sync(0xffffffffu, grow)) {
+    for (int n = 0; n < NT; ++n) grow |= !(fmaxf(s[n][0], s[n][1]) <= m[n]);
+    if (__any_sync(0xffffffffu, grow)) {  // (rare after the first pages)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float top = fmaxf(s[n][0], s[n][1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        top = fmaxf(top, m[n]);
+        const float alpha = ex2(m[n] - top);
+        m[n] = top;
+        l[n] *= alpha;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha[n];
-        const float al = __shfl_sync(0xffffffffu, alpha[n], g >> 1);
+          for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha;
+        const float al = __shfl_sync(0xffffffffu, alpha, g >> 1);
 #pragma unroll
         for (int j = 0; j < G; ++j) om[n][j] *= al;
       }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float p0 = ex2(s[n][0] - m[n]), p1 = ex2(s[n][1] - m[n]);
+      l[n] += p0 + p1;
+      const int from = 8 * t + (g >> 1);
+      const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
+      const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
+      pa[n] = odd ? a1 : a0;
+      pb[n] = odd ? b1 : b0;
     }
     // ---- weighted rows
     {
@@ -504,12 +501,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
 #pragma unroll
         for (int i = 0; i < J; ++i) {
           const int j = P * J + i;
-          const uint32_t a0[4] = {centred(w0[i] << 4, big), centred(w0[i], big), centred(w1[i] << 4, big),
+          const uint32_t h0 = w0[i] >> 8, h1 = w1[i] >> 8;
+          const uint32_t a0[4] = {centred_low(w0[i], big), centred(w0[i], big), centred_low(w1[i], big),
                                   centred(w1[i], big)};
-          const uint32_t a1[4] = {centred(w0[i] >> 4, big), centred(w0[i] >> 8, big), centred(w1[i] >> 4, big),
-                                  centred(w1[i] >> 8, big)};
+          const uint32_t a1[4] = {centred_low(h0, big), centred(h0, big), centred_low(h1, big), centred(h1, big)};
           const float da = half_of(dw[j / 2], j & 1), db = half_of(dw[(G + j) / 2], j & 1);
-          const float ca = fmaf(7.5f, da, half_of(mw[j], 0)), cb = fmaf(7.5f, db, half_of(mw[j], 1));
+          const float ca = fmaf(8.f, da, half_of(mw[j], 0)), cb = fmaf(8.f, db, half_of(mw[j], 1));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             uint32_t b0, b1;
@@ -585,14 +582,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           const float sum = fmaf(sum_lo, kLo, sum_hi);
           if (j == 2 * t) s0 = sum;
           if (j == 2 * t + 1) s1 = sum;
-          qi[n][j][0] = -__shfl_sync(0xffffffffu, sum_hi, 8 * t);
-          qi[n][j][1] = -__shfl_sync(0xffffffffu, sum_lo, 8 * t);
+          qs[n][j] = __shfl_sync(0xffffffffu, sum, 8 * t);
           om[n][j] = 0.f;
         }
         uint32_t hi, lo;
         split2(s0, s1, hi, lo);
         qm[n] = odd ? lo : hi;
-        m[n] = m_held[n] = -INFINITY;
+        m[n] = m_held[n] = kNone;
         l[n] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
@@ -634,14 +630,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     T* out = static_cast<T*>(p.out) + sg.seq * p.out_stride + (int64_t)sg.head * p.hpk * HD;
     for (int i = threadIdx.x; i < p.hpk * HD; i += 32 * kConsumers) {
       const int h = i / HD;
-      float M = -INFINITY;
+      float M = kNone;
 #pragma unroll
       for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, wm[w][h]);
-      const float Mu = M == -INFINITY ? 0.f : M;
       float v = 0.f, L = 0.f;
 #pragma unroll
       for (int w = 0; w < kConsumers; ++w) {
-        const float e = ex2(wm[w][h] - Mu);
+        const float e = ex2(wm[w][h] - M);
         v = fmaf(e, wo[((size_t)w * p.hpk + h) * PITCH + i % HD], v);
         L = fmaf(e, wl[w][h], L);
       }
@@ -678,20 +673,19 @@ __global__ void __launch_bounds__(128 * kGroups) kv4_join_kernel(const __grid_co
   auto part_of = [&](int i) { return base + (size_t)(2 * i + (i == 0 ? 1 : 0)) * part_floats; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp < p.hpk) {
-    float M = -INFINITY, L = 0.f;
+    float M = kNone, L = 0.f;
     for (int i = lane; i < n; i += 32) {
       const float pm = __ldcg(part_of(i) + stat + warp), pl = __ldcg(part_of(i) + stat + p.hpk + warp);
-      const float Mn = fmaxf(M, pm), Mu = Mn == -INFINITY ? 0.f : Mn;
-      L = fmaf(L, ex2(M - Mu), pl * ex2(pm - Mu));
+      const float Mn = fmaxf(M, pm);
+      L = fmaf(L, ex2(M - Mn), pl * ex2(pm - Mn));
       M = Mn;
     }
     float top = M;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    const float Mu = top == -INFINITY ? 0.f : top;
-    L = warp_sum(L * ex2(M - Mu));
+    L = warp_sum(L * ex2(M - top));
     if (lane == 0) {
-      wm[warp] = Mu;
+      wm[warp] = top;
       wl[warp] = L;
     }
   }
@@ -703,11 +697,11 @@ __global__ void __launch_bounds__(128 * kGroups) kv4_join_kernel(const __grid_co
     const int e = e0 + 4 * col, h = e / hd;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (e < stat) {
-      const float Mu = wm[h];
+      const float M = wm[h];
 #pragma unroll 8
       for (int i = group; i < n; i += kGroups) {
         const float* q = part_of(i);
-        const float w = ex2(__ldcg(q + stat + h) - Mu);
+        const float w = ex2(__ldcg(q + stat + h) - M);
         const float2 x = __ldcg(reinterpret_cast<const float2*>(q + e)), y = __ldcg(reinterpret_cast<const float2*>(q + e + 2));
         v[0] = fmaf(w, x.x, v[0]);
         v[1] = fmaf(w, x.y, v[1]);
