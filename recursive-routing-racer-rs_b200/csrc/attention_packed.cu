@@ -115,30 +115,65 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], const void* p) {
                : "r"(smem_addr(p)));
 }
 
-// One query row by one warp in 32-bit arithmetic over the rows that it sees and no others. A
-// masked weight of zero times an infinite or NaN value is a NaN in a tile's product, so a row
-// that comes out not finite is computed again here: what a row does not see never reaches it.
+// Whether a row that came out not finite may owe that to what it does not see: a masked weight of
+// zero times an infinite or NaN value is a NaN in a tile's product. Where the weights' sum is not
+// a positive number the row's own scores made it so.
+__device__ __forceinline__ bool doubtful(bool bad, float sum) { return bad && sum > 0.f && sum <= 3.402823466e38f; }
+// One such query row by one warp: where the values that its tile took in beyond what it sees, up
+// to row `reach` of the sequence, are finite, it stands; else it is computed again in 32-bit
+// arithmetic over the rows that it sees and no others, so that the others never reach it.
 template <int HD, typename T>
-__device__ __noinline__ void slow_row(const PackedParams& p, const Tile& t, int row, int head) {
-  constexpr int D = HD / 32;
+__device__ __noinline__ void slow_row(const PackedParams& p, const Tile& t, int row, int head, int reach) {
+  constexpr int D = HD / 32, U = 4;  // rows at once
   const int lane = threadIdx.x & 31, kv = head / p.hpk, n = seen_by(p, t, row);
+  const T* kp = static_cast<const T*>(p.k) + t.k0 * p.k_row + kv * p.k_head + D * lane;
+  const T* vp = static_cast<const T*>(p.v) + t.k0 * p.v_row + kv * p.v_head + D * lane;
+  bool finite = true;
+  for (int j = n; j < reach; ++j) {
+    float x[D];
+    load_vec<T, D>(vp + j * p.v_row, x);
+#pragma unroll
+    for (int i = 0; i < D; ++i) finite &= fabsf(x[i]) <= 3.402823466e38f;
+  }
+  if (__all_sync(0xffffffffu, finite)) return;
   float q[D], o[D], m = -INFINITY, l = 0.f;
   load_vec<T, D>(static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head + D * lane, q);
 #pragma unroll
   for (int i = 0; i < D; ++i) o[i] = 0.f;
-  for (int j = 0; j < n; ++j) {
-    float x[D], dot = 0.f;
-    load_vec<T, D>(static_cast<const T*>(p.k) + (int64_t)(t.k0 + j) * p.k_row + kv * p.k_head + D * lane, x);
+  for (int j = 0; j < n; j += U) {
+    float x[U][D], s[U];
 #pragma unroll
-    for (int i = 0; i < D; ++i) dot = fmaf(q[i], x[i], dot);
-    const float s = warp_sum(dot) * p.scale;
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = ex2(m - mu), w = ex2(s - mu);
+    for (int u = 0; u < U; ++u) {
+      load_vec<T, D>(kp + min(j + u, n - 1) * p.k_row, x[u]);
+      s[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D; ++i) s[u] = fmaf(q[i], x[u][i], s[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_vec<T, D>(vp + min(j + u, n - 1) * p.v_row, x[u]);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], k);
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = j + u < n ? s[u] * p.scale : -INFINITY;
+      mn = fmaxf(mn, s[u]);
+    }
+    const float mu = mn == -INFINITY ? 0.f : mn, alpha = ex2(m - mu);
     m = mn;
-    l = fmaf(l, alpha, w);
-    load_vec<T, D>(static_cast<const T*>(p.v) + (int64_t)(t.k0 + j) * p.v_row + kv * p.v_head + D * lane, x);
+    l *= alpha;
 #pragma unroll
-    for (int i = 0; i < D; ++i) o[i] = fmaf(o[i], alpha, w * x[i]);
+    for (int i = 0; i < D; ++i) o[i] *= alpha;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j + u >= n) break;
+      const float w = ex2(s[u] - mu);
+      l += w;
+#pragma unroll
+      for (int i = 0; i < D; ++i) o[i] = fmaf(w, x[u][i], o[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < D; ++i) o[i] = n > 0 ? o[i] / l : 0.f;
@@ -271,11 +306,11 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const __grid_constant_
       bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
       if (r < rows) *reinterpret_cast<uint32_t*>(dst + 8 * n + 2 * c) = Mma<T>::pack(a, b);
     }
-    unsigned rows_bad = __ballot_sync(0xffffffffu, bad && r < rows);
+    unsigned rows_bad = __ballot_sync(0xffffffffu, doubtful(bad, l[i]) && r < rows);
     for (int rr = 0; rr < 8; ++rr)
       if (rows_bad & (0xfu << (4 * rr))) {
         __syncwarp();
-        slow_row<HD, T>(p, t, t.row0 + 16 * warp + 8 * i + rr, head);
+        slow_row<HD, T>(p, t, t.row0 + 16 * warp + 8 * i + rr, head, min(lk, (end + kKRows - 1) / kKRows * kKRows));
       }
   }
 }
@@ -756,12 +791,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        unsigned again = __ballot_sync(0xffffffffu, bad && mine);
+        unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
         while (again) {
           const int from = __ffs(again) - 1;
           again &= again - 1;
           __syncwarp();
-          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, head, from));
+          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, head, from),
+                          min(lk, (sees[i] + 15) & ~15));
         }
       }
       tc_fence_before();
@@ -812,8 +848,7 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
   auto kern = packed_tc_kernel<HD, T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int64_t slots = p.q_rows / (2 * tp.tokens) + p.n_seqs;
-  if (nkv * slots > INT32_MAX) return cudaErrorInvalidConfiguration;
+  const int64_t slots = p.q_rows / (2 * tp.tokens) + p.n_seqs;  // nkv times that fits the grid: the caller's check
   return rrr_launch_pdl(kern, dim3((unsigned)(nkv * slots)), dim3(kTcThreads), (size_t)smem, env.stream, env.pdl,
                         qmap, kmap, vmap, tp);
 }
@@ -845,7 +880,7 @@ extern "C" int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, cons
                                     void* stream) {
   const char* fn = "rrr_attention_packed";
   if (!ctx) return set_error(nullptr, RRR_ERR_INVALID_ARG, "null context");
-  if (!d || !cu_q || !cu_kv) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!d || (d->n_seqs > 0 && (!cu_q || !cu_kv))) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   if (d->type != RRR_F16 && d->type != RRR_BF16)
     return set_error(ctx, RRR_ERR_BAD_QTYPE, "%s: type must be 1 (F16) or 30 (BF16)", fn);
   const int hd = d->head_dim;
@@ -884,6 +919,9 @@ extern "C" int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, cons
   for (int i = 1; i < 4; ++i)
     if (!rows_disjoint(parts[0], parts[i]))
       return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: out overlaps an input", fn);
+  const int64_t per = nh / kvh < kTile ? 2 * (kTile / (nh / kvh)) : 2;  // query rows per CTA
+  if (kvh * (d->q_rows / per + d->n_seqs) > INT32_MAX)
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows, sequences and heads for one call", fn);
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
   if (d->q_rows == 0 || d->n_seqs == 0) return RRR_OK;

@@ -67,6 +67,7 @@ struct Kv4Params {
   int2* runs;    // [seq][head]: first CTA and CTAs of its pages
   float* parts;  // [CTA][2][hpk * (HD + 2)]: sums, maxima, weights' sums
   int stages, stage_bytes;
+  int ctas;      // of the first kernel
   int* err;
 };
 
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(128 * kGroups) kv4_join_kernel(const __grid_co
   pdl_wait();
   const int2 run = p.runs[blockIdx.x];
   const int n = run.y, stat = p.hpk * hd;
-  if (n < 2) return;
+  if (n < 2 || run.x < 0 || n > p.ctas - run.x) return;  // (nothing written where a wait gave up)
   const size_t part_floats = (size_t)p.hpk * (hd + 2);
   // the part that starts the (sequence, head) is its CTA's slot 1, the others slot 0
   const float* base = p.parts + (size_t)2 * run.x * part_floats;
@@ -744,6 +745,7 @@ cudaError_t launch(const LaunchEnv& env, Kv4Params p) {
   const int64_t units = (int64_t)p.n_seqs * p.nkv * ((p.max_pages > 0 ? p.max_pages : 1) + kStart);
   const int ctas = env.sm_count * kCtas;
   const int grid = (int)(units < ctas ? units : ctas);
+  p.ctas = grid;
   e = rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl, p);
   if (e != cudaSuccess || p.max_pages < 2) return e;  // a single page is one CTA's
   return rrr_launch_pdl(kv4_join_kernel<T>, dim3(p.n_seqs * p.nkv), dim3(128 * kGroups), 0, env.stream, env.pdl, p, HD);
@@ -796,7 +798,7 @@ int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int typ
   int rc = rrr_kv4_workspace(ctx, c, n_heads, &need);
   if (rc) return rc;
   if (!row_type(type)) return set_error(ctx, RRR_ERR_BAD_QTYPE, "%s: type must be 0 (F32), 1 (F16) or 30 (BF16)", fn);
-  if (!q || !kv_lens || !out || !workspace) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!workspace || (c->n_seqs > 0 && (!q || !kv_lens || !out))) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t width = (int64_t)n_heads * c->head_dim;
   if (q_stride < width || out_stride < width)
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: strides of at least n_heads * head_dim", fn);

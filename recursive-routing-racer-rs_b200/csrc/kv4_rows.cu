@@ -24,15 +24,17 @@
 namespace rrr {
 
 int check_kv4_cache(rrr_ctx* ctx, const rrr_kv4_cache* c, const char* fn) {
-  if (!c || !c->pages || !c->page_table) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!c) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   if ((c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) || c->n_kv_heads < 1 ||
-      c->n_kv_heads > 65535 || c->n_pages < 0 || c->n_seqs < 0 || c->max_pages < 0 ||
+      c->n_kv_heads > 65535 || c->n_pages < 0 || c->n_pages > INT32_MAX || c->n_seqs < 0 || c->max_pages < 0 ||
       c->max_pages > INT32_MAX / kPageRows || c->table_stride < c->max_pages ||
       (int64_t)c->n_seqs * c->n_kv_heads > INT32_MAX)
     return set_error(ctx, RRR_ERR_BAD_SHAPE,
                      "%s: need head_dim 64/128/256, 1 <= n_kv_heads <= 65535, counts >= 0, table_stride >= "
-                     "max_pages, at most 2^31 - 64 rows per sequence and 2^31 - 1 sequences times heads",
+                     "max_pages, at most 2^31 - 1 pages, 2^31 - 64 rows per sequence and 2^31 - 1 sequences times heads",
                      fn);
+  if ((c->n_pages > 0 && !c->pages) || (c->n_seqs > 0 && c->max_pages > 0 && !c->page_table))
+    return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   if (!aligned_to(c->pages, 16) || !aligned_to(c->page_table, 4))
     return set_error(ctx, RRR_ERR_MISALIGNED, "%s: pages must be 16-byte aligned", fn);
   return RRR_OK;
@@ -366,7 +368,7 @@ int kv4_rows(rrr_ctx* ctx, const char* fn, bool store, const rrr_kv4_cache* c, i
   int rc = check_kv4_cache(ctx, c, fn);
   if (rc) return rc;
   if (!row_type(type)) return set_error(ctx, RRR_ERR_BAD_QTYPE, "%s: type must be 0 (F32), 1 (F16) or 30 (BF16)", fn);
-  if ((store ? !k || !v : !k && !v) || !cu_rows || !kv_lens)
+  if ((rows > 0 && (store ? !k || !v : !k && !v)) || (c->n_seqs > 0 && (!cu_rows || !kv_lens)))
     return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
   if (rows < 0 || (k && k_stride < width) || (v && v_stride < width))

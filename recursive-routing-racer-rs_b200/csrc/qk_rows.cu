@@ -199,7 +199,7 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
   if (rc) return rc;
   if (!row_type(in_type) || !row_type(out_type))
     return set_error(ctx, RRR_ERR_BAD_QTYPE, "%s: types must be 0 (F32), 1 (F16) or 30 (BF16)", fn);
-  if (!qkv || !positions || !q || !k) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (rows > 0 && (!qkv || !positions || !q || !k)) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int hd = a->head_dim, nh = a->n_heads, nkv = a->n_kv_heads;
   if (rows < 0) return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows >= 0", fn);
   if (halves != 0 && halves != 1) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: halves is 0 or 1", fn);
@@ -261,7 +261,7 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
     p.turns[i] = pow((double)a->rope_theta, -2.0 * i / a->rope_dim) / 6.283185307179586476925;
   // all heads of a row in one warp once the rows alone fill the GPU's warps
   const int want = ctx->sm_count * 16;
-  int chunks = (want + rows - 1) / rows;
+  int chunks = (int)(((int64_t)want + rows - 1) / rows);
   const int most = (p.heads + kBatch - 1) / kBatch;
   chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
   p.chunk = (p.heads + chunks - 1) / chunks;

@@ -267,6 +267,34 @@ def test_attention_packed_refusals(rrr, host_ctx, over, code):
     assert L.rrr_attention_packed(None, ctypes.byref(d), 0, 0, 0, 0, 0, 0, None) == -1
 
 
+def test_empty_arrays_may_be_null_and_sizes_have_an_end(rrr, host_ctx):
+    """What has no element has no address in many frameworks; counts past what one launch or a page
+    number holds are refused before anything is launched."""
+    _no_gpu()
+    L, ref = rrr.ffi.lib(), ctypes.byref
+    none = dict(qkv=None, pos=None, q=None, k=None, v=None, rows=0)
+    assert L.rrr_qk_norm_rope(host_ctx, *_qk_args(rrr, **none)) == FINE
+    no_seqs = _cache(rrr, table=None, n_seqs=0)
+    no_pages = _cache(rrr, pages=None, n_pages=0, table=None, most=0, stride=0)
+    many = _cache(rrr, n_pages=1 << 31)
+    for f in (L.rrr_kv4_store, L.rrr_kv4_load):
+        assert f(host_ctx, ref(no_seqs), 30, None, 256, None, 256, 0, None, None, None) == FINE
+        assert f(host_ctx, ref(no_pages), 30, 1 << 20, 256, 2 << 20, 256, 5, 256, 512, None) == FINE
+        assert f(host_ctx, ref(many), 30, 1 << 20, 256, 2 << 20, 256, 5, 256, 512, None) == -3
+    need = ctypes.c_int64()
+    for c in (no_seqs, no_pages):
+        assert L.rrr_kv4_workspace(host_ctx, ref(c), 6, ref(need)) == 0
+        q = (None, 768, None) if c is no_seqs else (1 << 20, 768, 512)
+        assert L.rrr_attention_kv4(host_ctx, ref(c), 6, 0, *q, 0.0, None if c is no_seqs else 2 << 20, 768, 1 << 24,
+                                   need.value, None) == FINE
+    d = rrr.ffi.PackedDesc(30, 4, 2, 128, 0, 1, 0.0, 0, 0, *(512, 128, 256, 128, 256, 128, 512, 128))
+    assert L.rrr_attention_packed(host_ctx, ref(d), None, None, None, None, None, None, None) == FINE
+    # 65,535 heads times 2^24 / 256 tiles of rows
+    w = 65535 * 64
+    d = rrr.ffi.PackedDesc(30, 65535, 65535, 64, 1, 1, 0.0, 1 << 24, 1, w, 64, w, 64, w, 64, w, 64)
+    assert L.rrr_attention_packed(host_ctx, ref(d), 1 << 12, 1 << 60, 1 << 61, 256, 512, 1 << 62, None) == -3
+
+
 def test_python_host_refuses_what_the_kernels_cannot_take(rrr):
     class Ctx:  # refused before the library is asked
         h, device = None, 0
@@ -682,6 +710,38 @@ def test_attention_packed_masked_values_that_are_not_finite(rrr, ctx, hd):
     assert torch.equal(want.isnan(), out.isnan()) and torch.equal(want.isinf(), out.isinf())
     fine = torch.isfinite(want)
     assert float((out - plain)[fine].float().abs().max()) <= 4 * half_step(t) * float(v.nan_to_num(0, 0, 0).abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_packed_many_values_that_are_not_finite(rrr, ctx, hd):
+    """Values of every later row infinite in one place, before and behind what a row sees: the rows
+    that see none keep theirs, the others are infinite there and nowhere else. One infinite key, or
+    NaN queries of every row, leave NaN rows; none of these takes the time of a row by row pass."""
+    g, nh, nkv, n = gen(9), 4, 2, 1500
+    q, k, v = (normal(g, n, h, hd, dtype=torch.bfloat16) for h in (nh, nkv, nkv))
+    plain, out = torch.empty_like(q), torch.empty_like(q)
+    cu = ints([0, n])
+    rrr.attention_packed(ctx, q, k, v, cu, cu, plain)
+    vf = v.clone()
+    vf[700:, 1, 3] = math.inf
+    rrr.attention_packed(ctx, q, k, vf, cu, cu, out)
+    want = plain.clone()
+    want[700:, 2:, 3] = math.inf
+    assert torch.equal(torch.isinf(want), torch.isinf(out)) and not bool(out.isnan().any())
+    fine = torch.isfinite(want)
+    assert float((out - plain)[fine].float().abs().max()) <= 4 * half_step(torch.bfloat16) * float(v.abs().max())
+    for x in (k, q):
+        kept = x.clone()
+        x[100 if x is k else slice(None), 0, 1] = math.nan
+        rrr.attention_packed(ctx, q, k, v, cu, cu, out)
+        heads = slice(0, nh // nkv) if x is k else slice(0, 1)
+        first = 100 if x is k else 0
+        assert bool(out[first:, heads].isnan().all())
+        want = plain.clone()
+        want[first:, heads] = math.nan
+        assert torch.equal(want.isnan(), out.isnan())
+        x.copy_(kept)
 
 
 @pytest.mark.gpu
