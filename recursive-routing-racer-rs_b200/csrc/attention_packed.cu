@@ -180,7 +180,9 @@ __device__ __noinline__ void slow_row(const PackedParams& p, const Tile& t, int 
   store_vec<T, D>(static_cast<T*>(p.out) + row * p.out_row + head * p.out_head + D * lane, o);
 }
 
-// 64 query rows of one head per CTA, 16 per warp, against 64 KV rows at a time in shared memory.
+// 64 query rows of one head per CTA, 16 per warp, against 64 KV rows at a time in shared memory:
+// for more than 128 query heads per KV head, whose rows fit no tile of the kernels below, and for
+// batches without any KV row, which no tensor map describes.
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads) packed_kernel(const __grid_constant__ PackedParams p) {
   constexpr int PITCH = HD + 8;  // rows 16 bytes apart in the banks: conflict-free ldmatrix
@@ -335,8 +337,7 @@ constexpr int kTile = 128;   // MMA rows, and KV rows per block
 constexpr float kLazy = 8.f;
 
 // Stages of the ring of K and V tiles beside the two of Q: what fits. (Two stages of K and two of
-// V left the MMA thread waiting for copies half of the time: a copy had one block's time, and
-// 64 KB from the L2 take about that.)
+// V, freed apart, took 1756 us instead of 1720 for a prompt of 16,384 rows.)
 template <int HD>
 constexpr int tc_stages() { return HD == 128 ? 5 : 10; }
 
@@ -419,6 +420,172 @@ __device__ __forceinline__ void store_32(void* p, const uint32_t (&a)[4], const 
   } else {
     reinterpret_cast<uint4*>(p)[0] = make_uint4(a[0], a[1], a[2], a[3]);
     reinterpret_cast<uint4*>(p)[1] = make_uint4(b[0], b[1], b[2], b[3]);
+  }
+}
+
+// The softmax of one tile row, by one thread.
+template <typename T>
+struct RowSoftmax {
+  float scale;
+  float m;   // the maximum of the scaled scores, as of the last rescale
+  float2 l;  // the weights' sum, of even and odd columns
+  // the weights of 32 scores under the maximum m, stored over S as columns 32 part .. + 31; their
+  // sum to l
+  __device__ __forceinline__ void weights(uint32_t sc, const float* v, int part) {
+    const float neg = m == -INFINITY ? 0.f : -m;
+    const float2 neg2 = make_float2(neg, neg), scale2 = make_float2(scale, scale);
+    float2 sum = make_float2(0.f, 0.f);
+    uint32_t w[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const float2 e = __ffma2_rn(make_float2(v[2 * c], v[2 * c + 1]), scale2, neg2);
+      const float2 q = make_float2(ex2(e.x), ex2(e.y));
+      sum = __fadd2_rn(sum, q);
+      w[c] = Mma<T>::pack(q.x, q.y);
+    }
+    l = __fadd2_rn(l, sum);
+    tmem_st16(sc + 16 * part, w);
+  }
+  static __device__ __forceinline__ float top_of(const float* v) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+      top[0] = fmaxf(top[0], fmaxf(v[c], v[c + 1]));
+      top[1] = fmaxf(top[1], fmaxf(v[c + 2], v[c + 3]));
+    }
+    return fmaxf(top[0], top[1]);
+  }
+  // takes over a larger maximum where a row's has grown by more than kLazy; whether any has.
+  // scale_o(alpha) does that to the products so far.
+  template <class F>
+  __device__ __forceinline__ bool rescale(float m_new, F&& scale_o) {
+    if (!__any_sync(0xffffffffu, m_new > m + kLazy)) return false;
+    const bool grow = m_new > m;
+    const float next = grow ? m_new : m;
+    const float alpha = grow ? ex2(m - next) : 1.f;
+    m = next;
+    l.x *= alpha;
+    l.y *= alpha;
+    scale_o(alpha);
+    return true;
+  }
+  // Block j: the scores in sc become weights. open: columns that this row sees; every row of the
+  // warp sees all_see of them, none of its rows none_sees or more.
+  template <class F>
+  __device__ __forceinline__ void block(uint32_t sc, int j, int open, int all_see, int none_sees, F&& scale_o) {
+    if (j > 0 && (j + 1) * kTile <= all_see) {
+      // the weights under the old maximum; the new one is found meanwhile, and where it is too
+      // large for the old one they are computed again
+      uint32_t x[kTile];
+      const float* v = reinterpret_cast<const float*>(x);
+      tmem_ld32(sc, x);
+      tmem_wait_ld();
+      const float2 before = l;
+      float top = -INFINITY;
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+        if (part < 3) tmem_ld32(sc + 32 * (part + 1), x + 32 * (part + 1));
+        weights(sc, v + 32 * part, part);
+        top = fmaxf(top, top_of(v + 32 * part));
+        if (part < 3) tmem_wait_ld();
+      }
+      const float2 after = l;
+      l = before;
+      if (rescale(top * scale, scale_o)) {
+#pragma unroll
+        for (int part = 0; part < 4; ++part) weights(sc, v + 32 * part, part);
+      } else {
+        l = after;
+      }
+    } else {
+      // the first block, or one with masked columns: the maximum first. A part of 32 columns
+      // that no row of the warp sees has no weights, one that every row sees no mask.
+      auto load = [&](int part, uint32_t* x) {
+        const int at = j * kTile + 32 * part;
+        tmem_ld32(sc + 32 * part, x);
+        tmem_wait_ld();
+        if (at + 32 > all_see) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (c >= open - at) x[c] = 0xff800000u;
+        }
+      };
+      const int parts = min(4, (none_sees - j * kTile + 31) / 32);
+      float m_new = -INFINITY;
+#pragma unroll 1
+      for (int part = 0; part < parts; ++part) {
+        uint32_t x[32];
+        load(part, x);
+        m_new = fmaxf(m_new, top_of(reinterpret_cast<const float*>(x)));
+      }
+      rescale(m_new * scale, scale_o);
+#pragma unroll 1
+      for (int part = 0; part < 4; ++part) {
+        uint32_t x[32];
+        if (part < parts) {
+          load(part, x);
+          weights(sc, reinterpret_cast<const float*>(x), part);
+        } else {
+          const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+          tmem_st16(sc + 16 * part, zero);
+        }
+      }
+    }
+  }
+};
+// HD columns of this thread's row of O times alpha
+template <int HD>
+__device__ __forceinline__ void scale_row(uint32_t oc, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(oc + c, v);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+    tmem_st16(oc + c, v);
+  }
+}
+// This thread's row of out from O (`some`: whether there are products) over the weights' sum;
+// rows of the warp that need it are computed again.
+template <int HD, typename T>
+__device__ __forceinline__ void write_row(const PackedParams& p, const Tile& t, uint32_t oc, bool some, bool mine,
+                                          int row, int head, int seen, float sum, int reach) {
+  const float inv = seen > 0 ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head;
+  bool bad = false;
+  const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.out_row % 16 == 0 && p.out_head % 16 == 0;
+  for (int c = 0; c < HD; c += 32) {
+    uint32_t v[32];
+    if (some) {
+      tmem_ld32(oc + c, v);
+      tmem_wait_ld();
+    }
+    uint32_t pair[4];
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) {
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = seen > 0 ? __uint_as_float(v[k + 2 * e]) * inv : 0.f;
+        const float b = seen > 0 ? __uint_as_float(v[k + 2 * e + 1]) * inv : 0.f;
+        bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
+        o[e] = Mma<T>::pack(a, b);
+      }
+      if (k % 16 == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pair[e] = o[e];
+      } else if (mine) {
+        store_32(dst + c + k - 8, pair, o, wide);
+      }
+    }
+  }
+  unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
+  while (again) {
+    const int from = __ffs(again) - 1;
+    again &= again - 1;
+    __syncwarp();
+    slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, head, from), reach);
   }
 }
 
@@ -612,58 +779,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int end_block = (lk - 1) / kTile;
     const bool zeroes = lk % kTile != 0 && i == (blocks[0] > end_block ? 0 : 1);
     const bool frees = i == (blocks[1] > 0 ? 1 : 0);  // the tile whose products come last
-    float m = -INFINITY;             // scaled, as of the last rescale
-    float2 l = make_float2(0.f, 0.f);
+    RowSoftmax<T> rs{p.scale, -INFINITY, make_float2(0.f, 0.f)};
     bool ok = true;
-    const float2 scale2 = make_float2(p.scale, p.scale);
-    // the weights of 32 scores under the maximum m, stored over S as columns 32 part .. + 31; their
-    // sum to l
-    auto weights = [&](const float* v, int part) {
-      const float neg = m == -INFINITY ? 0.f : -m;
-      const float2 neg2 = make_float2(neg, neg);
-      float2 sum = make_float2(0.f, 0.f);
-      uint32_t w[16];
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float2 e = __ffma2_rn(make_float2(v[2 * c], v[2 * c + 1]), scale2, neg2);
-        const float2 q = make_float2(ex2(e.x), ex2(e.y));
-        sum = __fadd2_rn(sum, q);
-        w[c] = Mma<T>::pack(q.x, q.y);
-      }
-      l = __fadd2_rn(l, sum);
-      tmem_st16(sc + 16 * part, w);
-    };
-    auto top_of = [&](const float* v) {
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        top[0] = fmaxf(top[0], fmaxf(v[c], v[c + 1]));
-        top[1] = fmaxf(top[1], fmaxf(v[c + 2], v[c + 3]));
-      }
-      return fmaxf(top[0], top[1]);
-    };
-    // takes over a larger maximum where a row's has grown by more than kLazy; whether any has
-    auto rescale = [&](float m_new, bool has_o) {
-      if (!__any_sync(0xffffffffu, m_new > m + kLazy)) return false;
-      const bool grow = m_new > m;
-      const float next = grow ? m_new : m;
-      const float alpha = grow ? ex2(m - next) : 1.f;
-      m = next;
-      l.x *= alpha;
-      l.y *= alpha;
-      if (has_o) {
-#pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
-          uint32_t v[16];
-          tmem_ld16(oc + c, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
-          tmem_st16(oc + c, v);
-        }
-      }
-      return true;
-    };
     for (int j = 0; j < blocks[i]; ++j) {
       if (!warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
         abort_flag = 1;
@@ -690,64 +807,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
-      if (j > 0 && (j + 1) * kTile <= all_see) {
-        // the weights under the old maximum; the new one is found meanwhile, and where it is too
-        // large for the old one they are computed again
-        uint32_t x[kTile];
-        const float* v = reinterpret_cast<const float*>(x);
-        tmem_ld32(sc, x);
-        tmem_wait_ld();
-        const float2 before = l;
-        float top = -INFINITY;
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          if (part < 3) tmem_ld32(sc + 32 * (part + 1), x + 32 * (part + 1));
-          weights(v + 32 * part, part);
-          top = fmaxf(top, top_of(v + 32 * part));
-          if (part < 3) tmem_wait_ld();
-        }
-        const float2 after = l;
-        l = before;
-        if (rescale(top * p.scale, true)) {
-#pragma unroll
-          for (int part = 0; part < 4; ++part) weights(v + 32 * part, part);
-        } else {
-          l = after;
-        }
-      } else {
-        // the first block, or one with masked columns: the maximum first. A part of 32 columns
-        // that no row of the warp sees has no weights, one that every row sees no mask.
-        auto load = [&](int part, uint32_t* x) {
-          const int at = j * kTile + 32 * part;
-          tmem_ld32(sc + 32 * part, x);
-          tmem_wait_ld();
-          if (at + 32 > all_see) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c >= open - at) x[c] = 0xff800000u;
-          }
-        };
-        const int parts = min(4, (none_sees - j * kTile + 31) / 32);
-        float m_new = -INFINITY;
-#pragma unroll 1
-        for (int part = 0; part < parts; ++part) {
-          uint32_t x[32];
-          load(part, x);
-          m_new = fmaxf(m_new, top_of(reinterpret_cast<const float*>(x)));
-        }
-        rescale(m_new * p.scale, j > 0);
-#pragma unroll 1
-        for (int part = 0; part < 4; ++part) {
-          uint32_t x[32];
-          if (part < parts) {
-            load(part, x);
-            weights(reinterpret_cast<const float*>(x), part);
-          } else {
-            const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            tmem_st16(sc + 16 * part, zero);
-          }
-        }
-      }
+      rs.block(sc, j, open, all_see, none_sees, [&](float alpha) {
+        if (j > 0) scale_row<HD>(oc, alpha);
+      });
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -755,50 +817,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     // ---------------- out
     if (ok && i * tp.tokens < rows) {
-      const float sum = l.x + l.y;
-      const float inv = seen > 0 ? 1.f / sum : 0.f;
-      T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head;
-      bool bad = false;
-      const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0 && p.out_row % 16 == 0 && p.out_head % 16 == 0;
       if (blocks[i] > 0) {
         ok = warp_wait(&o_full[i], 0, p.err);
         if (!ok) abort_flag = 1;
       }
       if (ok) {
         tc_fence_after();
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t v[32];
-          if (blocks[i] > 0) {
-            tmem_ld32(oc + c, v);
-            tmem_wait_ld();
-          }
-          uint32_t pair[4];
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = seen > 0 ? __uint_as_float(v[k + 2 * e]) * inv : 0.f;
-              const float b = seen > 0 ? __uint_as_float(v[k + 2 * e + 1]) * inv : 0.f;
-              bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
-              o[e] = Mma<T>::pack(a, b);
-            }
-            if (k % 16 == 0) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) pair[e] = o[e];
-            } else if (mine) {
-              store_32(dst + c + k - 8, pair, o, wide);
-            }
-          }
-        }
-        unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
-        while (again) {
-          const int from = __ffs(again) - 1;
-          again &= again - 1;
-          __syncwarp();
-          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, head, from),
-                          min(lk, (sees[i] + 15) & ~15));
-        }
+        write_row<HD, T>(p, t, oc, blocks[i] > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees[i] + 15) & ~15));
       }
       tc_fence_before();
     }
@@ -807,6 +832,214 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
+    warp_wait(&fin, 0u, p.err);  // no product still runs when its TMEM is freed
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- head_dim 256: tcgen05, one tile per CTA -------------------------------------------------
+//
+// O of 128 rows takes half of TMEM here, so a CTA has one tile, and S two places: S of block j + 1
+// runs during the softmax of block j, S(0), S(1), PV(0), S(2), PV(1), ... A stage of the ring holds
+// half a tile, 128 KV rows x 128 values, which is half of S's depth or of O's columns. The copying
+// warp sees a stage free by the commit behind its products: s_full of K's, pv of V's.
+// Per block and CTA 128 KB come from the L2 for 2 x 1024 clocks of products, so it is that traffic
+// and not the tensor cores that bounds it.
+constexpr int kWideThreads = 192;  // warps 0-3 softmax, 4 products, 5 copies
+
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    packed_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcParams tp) {
+  constexpr int HD = 256, kChunks = HD / 64, kStages = 5;
+  constexpr uint32_t kPiece = kTile * 128, kStage = 2 * kPiece;
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint64_t q_full, full[kStages], s_full[2], p_full, pv, o_full, fin;  // pv: all but the last block's
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const PackedParams& p = tp.a;
+  uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
+  uint8_t* qs = smem;
+  uint8_t* ring = smem + kChunks * kPiece;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  pdl_wait();
+  Tile t;
+  const int nkv = p.nh / p.hpk;
+  if (!find_tile(p, tp.tokens, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
+  const int kv = blockIdx.x % nkv;
+  const int rows = min(tp.tokens, t.q1 - t.row0), lk = t.k1 - t.k0;
+  const int sees = seen_by(p, t, t.row0 + rows - 1);  // KV rows that the last row sees
+  const int n = (sees + kTile - 1) / kTile;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&pv, 1);
+    mbar_init(&o_full, 1);
+    mbar_init(&fin, 1);
+    abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 4) tmem_alloc(&tmem_slot, 512);
+  // tile rows past the last whole query row: zeros, so that their scores are
+  for (int k = tp.tokens * p.hpk * 8 + threadIdx.x; k < kTile * 8; k += kWideThreads)
+    for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(qs + c * kPiece + 16 * k) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, o_col = tmem + 2 * kTile;
+  auto wait = [&](uint64_t* bar, int use) {  // the use-th completion of a barrier
+    if (warp_wait(bar, (uint32_t)use & 1u, p.err)) return true;
+    abort_flag = 1;
+    return false;
+  };
+
+  if (warp == 5) {
+    // ---------------- copies. Halves come in pairs u: K(0), K(1), V(0), K(2), V(1), ..., V(n - 1)
+    auto is_v = [&](int u) { return u == 2 * n - 1 || (u > 0 && u % 2 == 0); };
+    auto block_of = [&](int u) { return is_v(u) ? (u == 2 * n - 1 ? n - 1 : u / 2 - 1) : (u + 1) / 2; };
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(&q_full, kChunks * (uint32_t)(tp.tokens * p.hpk) * 128u);
+      for (int c = 0; c < kChunks; ++c) tma_load_3d(qs + c * kPiece, &qmap, 64 * c, kv * p.hpk, t.row0, &q_full);
+    }
+    int issued = 0, s_seen = 0, v_seen = 0;  // blocks whose products are known to be done
+    for (; issued < 4 * n; ++issued) {
+      bool ok = !warp_aborted(&abort_flag);
+      if (ok && issued >= kStages) {  // what the stage held before
+        const int u = (issued - kStages) >> 1, j = block_of(u);
+        if (is_v(u)) {
+          if (j >= v_seen) ok = wait(&pv, j);
+          v_seen = j + 1;
+        } else {
+          if (j >= s_seen) ok = wait(&s_full[j & 1], j >> 1);
+          s_seen = j + 1;
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        const int u = issued >> 1, half = issued & 1, st = issued % kStages;
+        mbar_arrive_expect_tx(&full[st], kStage);
+        for (int c = 0; c < 2; ++c)
+          tma_load_3d(ring + (size_t)st * kStage + c * kPiece, is_v(u) ? &vmap : &kmap, 128 * half + 64 * c, kv,
+                      t.k0 + block_of(u) * kTile, &full[st]);
+      }
+      __syncwarp();
+    }
+    // copies in flight land before the CTA leaves
+    if (n > 0) warp_wait(&q_full, 0, p.err);
+    for (int i = 0; i < kStages; ++i) {
+      const int uses = issued > i ? (issued - i + kStages - 1) / kStages : 0;
+      if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
+    }
+  } else if (warp == 4) {
+    // ---------------- products
+    auto columns = [&](int j) { return min(kTile, (sees - j * kTile + 15) & ~15); };
+    int item = 0;
+    auto landed = [&]() {
+      const bool ok = wait(&full[item % kStages], item / kStages);
+      tc_fence_after();
+      return ok;
+    };
+    auto scores = [&](int j) {  // S(j) = Q K(j)^T
+      const uint32_t idesc = tp.idesc_s | ((uint32_t)(columns(j) >> 3) << 17);
+      for (int half = 0; half < 2; ++half, ++item) {
+        if (!landed()) return false;
+        const uint32_t qa = smem_addr(qs + half * kStage), ka = smem_addr(ring + (size_t)(item % kStages) * kStage);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4) * kPiece + 32u * (kk % 4);
+            umma_f16(tmem + kTile * (j & 1), sw128_desc(qa + off), sw128_desc(ka + off), idesc,
+                     half > 0 || kk > 0 ? 1u : 0u);
+          }
+          if (half == 1) umma_commit(&s_full[j & 1]);
+        }
+        __syncwarp();
+      }
+      return true;
+    };
+    bool ok = n == 0 || (wait(&q_full, 0) && scores(0));
+    for (int j = 0; j < n && ok; ++j) {
+      ok = (j + 1 >= n || scores(j + 1)) && wait(&p_full, j);
+      if (!ok) break;
+      const int steps = columns(j) / 16;
+      for (int half = 0; half < 2 && ok; ++half, ++item) {  // O's columns 128 half .. + 127
+        ok = landed();
+        if (!ok) break;
+        const uint32_t va = smem_addr(ring + (size_t)(item % kStages) * kStage);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            if (kk >= steps) break;
+            umma_f16_ta(o_col + 128 * half, tmem + kTile * (j & 1) + 8u * kk, sw128_desc_mn(va + 2048u * kk, kPiece),
+                        tp.idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+          }
+          if (half == 1) umma_commit(j + 1 < n ? &pv : &o_full);
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) umma_commit(&fin);
+    __syncwarp();
+  } else {
+    // ---------------- softmax: thread r = row r
+    const int r = threadIdx.x, token = r / p.hpk, head = kv * p.hpk + r % p.hpk, row = t.row0 + token;
+    const bool mine = token < tp.tokens && token < rows;
+    const int seen = mine ? seen_by(p, t, row) : 0;
+    const int open = mine ? seen : INT32_MAX;  // tile rows of no query mask nothing
+    const int all_see = (int)__reduce_min_sync(0xffffffffu, (unsigned)open);
+    const int none_sees = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);
+    const uint32_t sub = (uint32_t)(32 * warp) << 16;
+    const int end_block = (lk - 1) / kTile;
+    RowSoftmax<T> rs{p.scale, -INFINITY, make_float2(0.f, 0.f)};
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      ok = wait(&s_full[j & 1], j >> 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lk % kTile != 0 && j == end_block) {  // V rows behind the sequence; j is n - 1
+        const int from = lk - j * kTile;
+        for (int half = 0; half < 2 && ok; ++half) {
+          const int item = 4 * n - 2 + half;
+          ok = wait(&full[item % kStages], item / kStages);
+          uint8_t* v = ring + (size_t)(item % kStages) * kStage;
+          for (int c = 0; c < 2 && ok; ++c)
+            for (int k = r; k < (kTile - from) * 8; k += 128)
+              *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+        }
+        if (!ok) break;
+        fence_proxy_async_smem();
+      }
+      rs.block(tmem + kTile * (j & 1) + sub, j, open, all_see, none_sees, [&](float alpha) {
+        if (j == 0) return;
+        ok = wait(&pv, j - 1);  // the products so far (those before S(j) was issued are done)
+        tc_fence_after();
+        scale_row<HD>(o_col + sub, alpha);
+      });
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full);
+    }
+    if (ok) {
+      if (n > 0) ok = wait(&o_full, 0);
+      if (ok) {
+        tc_fence_after();
+        write_row<HD, T>(p, t, o_col + sub, n > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees + 15) & ~15));
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
     warp_wait(&fin, 0u, p.err);  // no product still runs when its TMEM is freed
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -827,17 +1060,18 @@ bool encode_heads(CUtensorMap* map, int type, const void* base, int hd, int64_t 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Query rows of a CTA of the tcgen05 kernels
+int rows_per_cta(int hd, int hpk) { return (hd == 256 ? 1 : 2) * (kTile / hpk); }
+
 template <int HD, typename T>
 cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
   TcParams tp{};
   tp.a = p;
   tp.tokens = kTile / p.hpk;
-  constexpr int kOperand = kTile * HD * 2;
-  const int smem = (2 + tc_stages<HD>()) * kOperand + 1024;
   const uint32_t fmt = type == RRR_F16 ? 0u : 1u;
   // f32 accumulator, A and B of the type, B of the second product N-contiguous, N / 8, M / 16
   tp.idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTile >> 4) << 24);  // N / 8: as wide as the block
-  tp.idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) |
+  tp.idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)((HD < 128 ? HD : 128) >> 3) << 17) |
                ((uint32_t)(kTile >> 4) << 24);
   CUtensorMap qmap, kmap, vmap;
   const int64_t nkv = p.nh / p.hpk;
@@ -845,12 +1079,21 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
       !encode_heads(&kmap, type, p.k, HD, nkv, p.kv_rows, p.k_head, p.k_row, 1, kTile) ||
       !encode_heads(&vmap, type, p.v, HD, nkv, p.kv_rows, p.v_head, p.v_row, 1, kTile))
     return cudaErrorInvalidValue;
-  auto kern = packed_tc_kernel<HD, T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  const int64_t slots = p.q_rows / (2 * tp.tokens) + p.n_seqs;  // nkv times that fits the grid: the caller's check
-  return rrr_launch_pdl(kern, dim3((unsigned)(nkv * slots)), dim3(kTcThreads), (size_t)smem, env.stream, env.pdl,
-                        qmap, kmap, vmap, tp);
+  // nkv times the slots fits the grid: the caller's check
+  const dim3 grid((unsigned)(nkv * (p.q_rows / rows_per_cta(HD, p.hpk) + p.n_seqs)));
+  if constexpr (HD == 256) {
+    const int smem = 7 * kTile * 128 * 2 + 1024;  // Q's two halves and five stages
+    auto kern = packed_wide_kernel<T>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return rrr_launch_pdl(kern, grid, dim3(kWideThreads), (size_t)smem, env.stream, env.pdl, qmap, kmap, vmap, tp);
+  } else {
+    const int smem = (2 + tc_stages<HD>()) * kTile * HD * 2 + 1024;
+    auto kern = packed_tc_kernel<HD, T>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return rrr_launch_pdl(kern, grid, dim3(kTcThreads), (size_t)smem, env.stream, env.pdl, qmap, kmap, vmap, tp);
+  }
 }
 
 template <int HD, typename T>
@@ -864,9 +1107,8 @@ cudaError_t launch(const LaunchEnv& env, const PackedParams& p) {
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, const PackedParams& p) {
-  if constexpr (HD < 256)
-    if (p.hpk <= kTile && p.kv_rows > 0)
-      return type == RRR_F16 ? launch_tc<HD, __half>(env, type, p) : launch_tc<HD, __nv_bfloat16>(env, type, p);
+  if (p.hpk <= kTile && p.kv_rows > 0)
+    return type == RRR_F16 ? launch_tc<HD, __half>(env, type, p) : launch_tc<HD, __nv_bfloat16>(env, type, p);
   return type == RRR_F16 ? launch<HD, __half>(env, p) : launch<HD, __nv_bfloat16>(env, p);
 }
 
@@ -919,7 +1161,7 @@ extern "C" int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, cons
   for (int i = 1; i < 4; ++i)
     if (!rows_disjoint(parts[0], parts[i]))
       return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: out overlaps an input", fn);
-  const int64_t per = nh / kvh < kTile ? 2 * (kTile / (nh / kvh)) : 2;  // query rows per CTA
+  const int64_t hpk = nh / kvh, per = hpk <= kTile ? rows_per_cta(hd, (int)hpk) : 1;
   if (kvh * (d->q_rows / per + d->n_seqs) > INT32_MAX)
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows, sequences and heads for one call", fn);
   DeviceGuard dev(ctx);

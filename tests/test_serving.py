@@ -671,6 +671,33 @@ def test_attention_packed(rrr, ctx, hd, nh, nkv, kind, lq, lk, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("nh", [43, 100, 128, 130])
+def test_attention_packed_many_query_heads_per_kv_head(rrr, ctx, hd, nh):
+    g, lq, lk, t = gen(nh), [3, 70, 1], [3, 200, 300], torch.bfloat16
+    q, k, v = (normal(g, sum(n), h, hd, dtype=t) for n, h in ((lq, nh), (lk, 1), (lk, 1)))
+    out = torch.full_like(q, 3.0)
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), out)
+    check_packed(out, q, k, v, lq, lk, True, 1 / math.sqrt(hd))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [128, 256])
+def test_attention_packed_many_blocks(rrr, ctx, hd):
+    """Long enough for every ring to go round several times, and for maxima that keep growing: the
+    sums of a row are rescaled in every block."""
+    g, n, t = gen(hd), 2300, torch.bfloat16
+    q, k, v = (normal(g, n, h, hd, dtype=t) for h in (2, 1, 1))
+    k *= torch.linspace(0.05, 6, n, device="cuda")[:, None, None].to(t)
+    out = torch.empty_like(q)
+    rrr.attention_packed(ctx, q, k, v, cu_of([n]), cu_of([n]), out)
+    check_packed(out, q, k, v, [n], [n], True, 1 / math.sqrt(hd))
+    again = torch.empty_like(q)
+    rrr.attention_packed(ctx, q, k, v, cu_of([n]), cu_of([n]), again)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["qkv rows", "heads of rows", "odd pitch"])
 def test_attention_packed_strides(rrr, ctx, layout):
     g, nh, nkv, hd, lens = gen(4), 4, 2, 128, [100, 257]
