@@ -12,6 +12,7 @@ DRAM figures of a capture are those of the bench's per-GEMV lines.
     python tests/profcases.py batched --m 64  # M-token decode step
     python tests/profcases.py timeline        # GEMV phase timeline (rrr_set_trace), no ncu
     python tests/profcases.py logits --m 64 --vocab 32768   # batched logits (tcgen05 3xTF32)
+    python tests/profcases.py serving --head-dim 128        # the packed-batch operators
 """
 import argparse
 import ctypes
@@ -208,8 +209,45 @@ def case_timeline(ctx, L, torch, args):
     L.rrr_batch_destroy(b)
 
 
+def case_serving(ctx, L, torch, args):
+    """One call of each packed-batch operator a round, 24 query heads on 8 KV heads of
+    --head-dim: 16,000 QKV rows normed and rotated, a causal prompt of 8,000 rows, its rows into
+    the 4-bit cache and back, and one query for each of 64 sequences over 4,000 cached rows."""
+    rrr = importlib.import_module(_PKG)
+    hd, nh, nkv, bf16 = args.head_dim, 24, 8, torch.bfloat16
+    g = torch.Generator("cuda").manual_seed(3)
+
+    def rows(n, h, dtype=bf16):
+        return torch.randn(n, h, hd, device="cuda", generator=g).to(dtype)
+
+    def ints(v):
+        return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    desc = rrr.ffi.AttnDesc(nh, nkv, hd, min(hd, 128), 1e4, 1.0, None, 0, 1 << 20)
+    qkv, pos = rows(16000, nh + 2 * nkv, torch.float32), torch.arange(16000, dtype=torch.int32, device="cuda")
+    q, k, v = rows(16000, nh), rows(16000, nkv), rows(16000, nkv)
+    gamma = torch.rand(hd, device="cuda", generator=g) + 0.5
+    n, seqs, held = 8000, 64, 4000
+    out, cu = torch.empty_like(q[:n]), ints([0, n])
+    per = -(-n // 64)
+    cache = rrr.KV4Cache(ctx, torch.empty(rrr.KV4Cache.page_shape(seqs * per, nkv, hd), dtype=torch.uint8, device="cuda"),
+                         torch.randperm(seqs * per, device="cuda", generator=g).int().view(seqs, per), hd)
+    one = rrr.KV4Cache(ctx, cache.pages, cache.page_table[:1], hd)
+    for s in range(seqs):
+        rrr.KV4Cache(ctx, cache.pages, cache.page_table[s:s + 1], hd).store(k[:n], v[:n], cu, ints([n]))
+    qs, lens, ws = rows(seqs, nh), ints([held] * seqs), cache.workspace(nh)
+    res, kk, vv, ln = torch.empty_like(qs), torch.empty_like(k[:n]), torch.empty_like(v[:n]), ints([n])
+    for _ in range(args.rounds):
+        rrr.qk_norm_rope(ctx, desc, qkv, pos, q, k, v, q_gamma=gamma, k_gamma=gamma, halves=True)
+        rrr.attention_packed(ctx, q[:n], k[:n], v[:n], cu, cu, out)
+        one.store(k[:n], v[:n], cu, ln)
+        one.load(cu, ln, kk, vv)
+        cache.attention(qs, lens, res, ws)
+
+
 CASES = {"gemv": case_gemv, "decode": case_decode, "gemm": case_gemm, "attn": case_attn,
-         "batched": case_batched, "timeline": case_timeline, "logits": case_logits}
+         "batched": case_batched, "timeline": case_timeline, "logits": case_logits,
+         "serving": case_serving}
 
 
 def main(argv=None):
@@ -222,6 +260,7 @@ def main(argv=None):
     ap.add_argument("--max-seq", type=int, default=0)
     ap.add_argument("--vocab", type=int, default=32768)
     ap.add_argument("--path", type=int, default=0)
+    ap.add_argument("--head-dim", type=int, default=128, choices=(64, 128, 256))
     args = ap.parse_args(argv)
     import torch
     rrr = importlib.import_module(_PKG)

@@ -547,6 +547,18 @@ def test_attention_kv4(rrr, ctx, hd, nh, nkv, kind, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hpk", [5, 6, 7, 8])
+def test_attention_kv4_query_heads_per_kv_head(rrr, ctx, hd, hpk):
+    lens, nkv = [130, 1, 0, 1000], 3
+    cache, kv = filled(rrr, ctx, nkv, hd, lens, hpk)
+    q = normal(gen(hpk), len(lens), nkv * hpk, hd)
+    out = torch.empty_like(q)
+    cache.c.attention(q, ints(lens), out, cache.c.workspace(nkv * hpk).fill_(0xff))
+    check_decode(out, q, kv, 1 / math.sqrt(hd), torch.float32)
+
+
+@pytest.mark.gpu
 def test_attention_kv4_long_context_and_offsets_over_32_bits(rrr, ctx):
     """One sequence of 70,001 rows on pages that lie past 4 GB."""
     first = 53000
