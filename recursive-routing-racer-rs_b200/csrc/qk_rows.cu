@@ -6,7 +6,7 @@
 // Mathematics. x' = (gamma x) / sqrt(mean(x^2) + eps); with c, s = af cos(2 pi t), af sin(2 pi
 // t) a pair (a, b) becomes (a c - b s, a s + b c). t = pos * f / factor / 2 pi turns is wanted
 // modulo 1 to 2^-24 at any position: f / factor / 2 pi is held modulo 1 as a 64-bit fraction F
-// (from 64-bit floats, so to 2^-53 of itself), and pos * F modulo 2^64 is exact in integers.
+// (from 64-bit floats, so to 2^-51 of itself), and pos * F modulo 2^64 is exact in integers.
 // sincospi of its top 32 bits, taken as a signed fraction, needs no range reduction.
 //
 // Bound by memory: each value is read once and written once. A warp owns a run of heads of one
@@ -257,8 +257,13 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
   p.max_pos = a->max_seq;
   p.eps = eps;
   p.attn_factor = a->rope_attn_factor;
-  for (int i = 0; i < p.half_dim; ++i)
-    p.turns[i] = pow((double)a->rope_theta, -2.0 * i / a->rope_dim) / 6.283185307179586476925;
+  // theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64, and three
+  // roundings, 2^-51 of itself
+  double fine[8], coarse[kMaxPairs / 8];
+  for (int i = 0; i < 8; ++i) fine[i] = pow((double)a->rope_theta, -2.0 * i / a->rope_dim);
+  for (int i = 0; 8 * i < p.half_dim; ++i)
+    coarse[i] = pow((double)a->rope_theta, -16.0 * i / a->rope_dim) / 6.283185307179586476925;
+  for (int i = 0; i < p.half_dim; ++i) p.turns[i] = coarse[i / 8] * fine[i % 8];
   // all heads of a row in one warp once the rows alone fill the GPU's warps
   const int want = ctx->sm_count * 16;
   int chunks = (int)(((int64_t)want + rows - 1) / rows);
