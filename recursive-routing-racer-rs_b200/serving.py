@@ -9,6 +9,7 @@ stream); a tensor made on another stream is the caller's to order."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import byref, c_int64
 
 from . import ffi
@@ -16,6 +17,9 @@ from .engine import _stream
 
 PAGE_ROWS = 64
 _TYPES: dict = {}  # torch dtype -> GGML type id
+_INTS: set = set()  # torch dtypes of 32-bit integers
+# The fields of a PackedDesc, packed: a third of the time of its constructor
+_packed = struct.Struct("@6if10q").pack
 
 
 def _type(t, what: str) -> int:
@@ -40,7 +44,11 @@ def _on(ctx: ffi.Context, t, what: str):
 
 
 def _ints(ctx: ffi.Context, t, n: int, what: str):
-    if t.shape != (n,) or t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous():
+    if t.dtype not in _INTS or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        if not _INTS:
+            import torch
+            _INTS.update({torch.int32, torch.uint32})
+            return _ints(ctx, t, n, what)
         _fail(-3, f"{what}: a contiguous int32[{n}] is needed, got {t.dtype}{list(t.shape)}")
     return _on(ctx, t, what)
 
@@ -50,23 +58,26 @@ def _heads(ctx: ffi.Context, t, heads: int, hd: int, what: str, rows: int | None
     (address, rows, row stride)."""
     shape = t.shape
     n = shape[0]
-    if t.is_contiguous():  # the usual case, told in fewer calls
-        row = heads * hd
-        fine = shape == (n, heads, hd) or shape == (n, row)
+    if len(shape) == 3:
+        fine = shape[1] == heads and shape[2] == hd
     else:
+        fine = len(shape) == 2 and shape[1] == heads * hd
+    row = heads * hd
+    if not t.is_contiguous():
         stride = t.stride()
-        fine = (shape == (n, heads, hd) and stride[2] == 1 and (heads == 1 or stride[1] == hd)) or \
-            (shape == (n, heads * hd) and stride[1] == 1)
-        row = stride[0] if n > 1 else heads * hd
+        fine = fine and stride[-1] == 1 and (len(shape) == 2 or heads == 1 or stride[1] == hd)
+        if n > 1:
+            row = stride[0]
     if not fine or (rows is not None and n != rows):
         _fail(-3, f"{what}: rows [{'rows' if rows is None else rows}, {heads}, {hd}] with their heads next to "
                   f"each other are needed, got {list(shape)} with strides {list(t.stride())}")
     return _on(ctx, t, what), n, row
 
 
-def _strides(t, what: str):
+def _strides(t, rows: int, heads: int, hd: int, what: str):
     """Row and head strides of [rows, heads, hd]; the stride of a dimension of one is free."""
-    rows, heads, hd = t.shape
+    if t.is_contiguous():
+        return heads * hd, hd
     row, head, one = t.stride()
     if one != 1:
         _fail(-3, f"{what}: the values of a head must be contiguous")
@@ -102,17 +113,19 @@ def attention_packed(ctx: ffi.Context, q, k, v, cu_q, cu_kv, out, *, causal: boo
                      scale: float = 0.0, stream=None):
     """rrr_attention_packed: q, out [q_rows, n_heads, hd], k, v [kv_rows, n_kv, hd] (any row
     and head strides) of one 16-bit type; causal rows are the last ones of their sequence."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or out.shape != q.shape or k.shape[2] != q.shape[2]:
-        _fail(-3, f"q and out [rows, heads, hd], k and v [rows, heads, hd] are needed, got {list(q.shape)}, "
-                  f"{list(out.shape)}, {list(k.shape)}, {list(v.shape)}")
+    qd, kd = q.shape, k.shape
+    if len(qd) != 3 or len(kd) != 3 or v.shape != kd or out.shape != qd or kd[2] != qd[2]:
+        _fail(-3, f"q and out [rows, heads, hd], k and v [rows, heads, hd] are needed, got {list(qd)}, "
+                  f"{list(out.shape)}, {list(kd)}, {list(v.shape)}")
     kind = _type(q, "q")
     if not (q.dtype == k.dtype == v.dtype == out.dtype):
         _fail(-2, "q, k, v and out must have one type")
-    qs, ks, vs, os = (_strides(t, name) for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
-    rows, heads, hd = q.shape
+    rows, heads, hd = qd
+    held, kvh, _ = kd
     n = cu_q.shape[0]
-    d = ffi.PackedDesc(kind, heads, k.shape[1], hd, max(n - 1, 0), 1 if causal else 0, scale, rows, k.shape[0],
-                       *qs, *ks, *vs, *os)
+    d = ffi.PackedDesc.from_buffer_copy(_packed(
+        kind, heads, kvh, hd, max(n - 1, 0), 1 if causal else 0, scale, rows, held, *_strides(q, rows, heads, hd, "q"),
+        *_strides(k, held, kvh, hd, "k"), *_strides(v, held, kvh, hd, "v"), *_strides(out, rows, heads, hd, "out")))
     rc = ffi.lib().rrr_attention_packed(ctx.h, byref(d), _on(ctx, q, "q"), _on(ctx, k, "k"), _on(ctx, v, "v"),
                                         _ints(ctx, cu_q, n, "cu_q"), _ints(ctx, cu_kv, n, "cu_kv"),
                                         _on(ctx, out, "out"), _stream(stream))
