@@ -23,7 +23,7 @@
 // weights and sums keep f32 accuracy throughout.
 //
 // Bound by instructions: about 520 per warp for 16 rows of 4 heads x 128, where the issue slots
-// are 61 % taken (131,072 rows of 8 heads: 66 us, 2.5 TB/s of codes; 64 sequences, 261,424 rows:
+// are 62 % taken (131,000 rows of 8 heads: 60 us, 2.8 TB/s of codes; 64 sequences, 261,424 rows:
 // 111 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA per SM (96 registers,
 // a few spilt) was 8 % slower, so it is not latency that is missing.
 //
