@@ -22,9 +22,9 @@
 // maximum, which is nearly every one, skips the exchange of maxima and the rescaling. Scores,
 // weights and sums keep f32 accuracy throughout.
 //
-// Bound by instructions: about 520 per warp for 16 rows of 4 heads x 128, where the issue slots
-// are 62 % taken (131,000 rows of 8 heads: 60 us, 2.8 TB/s of codes; 64 sequences, 261,424 rows:
-// 111 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA per SM (96 registers,
+// Bound by instructions: about 500 per warp for 16 rows of 4 heads x 128, where the issue slots
+// are 62 % taken (131,000 rows of 8 heads: 59 us, 2.8 TB/s of codes; 64 sequences, 261,424 rows:
+// 110 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA per SM (96 registers,
 // a few spilt) was 8 % slower, so it is not latency that is missing.
 //
 // Work. A unit is one page (64 rows) of one (sequence, KV head), and each of those has kStart units
@@ -115,7 +115,9 @@ __device__ __forceinline__ float from_half(__half h, float x) {  // h - x
 }
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
-  const __half2 l = __floats2half2_rn(from_half(__low2half(h), a) * -2048.f, from_half(__high2half(h), b) * -2048.f);
+  const float2 rest = __fmul2_rn(make_float2(from_half(__low2half(h), a), from_half(__high2half(h), b)),
+                                 make_float2(-2048.f, -2048.f));
+  const __half2 l = __floats2half2_rn(rest.x, rest.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   float qs[NT][G];                // head t: the groups' sums of q
   float kscale[NT], m[NT], l[NT], m_held[NT];  // head t; m_held: of what shared memory holds
   float o[NT][2 * G][4];          // values: [16 u + (g, g + 8)] of group j, head t
-  float om[NT][G];                // middles of group j, head g / 2, this lane's rows
+  float2 om[NT][G];               // middles of group j, head g / 2, this lane's even and odd rows
   bool held = false;
   int since = 0;
 
@@ -353,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       float* dst = wo + ((size_t)warp * p.hpk + h) * PITCH;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        float mid = om[n][j];
+        float mid = om[n][j].x + om[n][j].y;
         mid += __shfl_xor_sync(0xffffffffu, mid, 1);
         mid += __shfl_xor_sync(0xffffffffu, mid, 2);
         mid += __shfl_xor_sync(0xffffffffu, mid, 4);
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[n][2 * j][i] = o[n][2 * j + 1][i] = 0.f;
-        om[n][j] = 0.f;
+        om[n][j] = make_float2(0.f, 0.f);
       }
       m_held[n] = m[n];
     }
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     }
     // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
     // rows 2t, 2t + 1 of the first (g even) or second eight rows
-    float pa[NT], pb[NT];
+    float2 pw[NT];
     bool grow = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) grow |= !(fmaxf(s[n][0], s[n][1]) <= m[n]);
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           for (int k = 0; k < 4; ++k) o[n][i][k] *= alpha;
         const float al = __shfl_sync(0xffffffffu, alpha, g >> 1);
 #pragma unroll
-        for (int j = 0; j < G; ++j) om[n][j] *= al;
+        for (int j = 0; j < G; ++j) om[n][j] = __fmul2_rn(om[n][j], make_float2(al, al));
       }
     }
 #pragma unroll
@@ -478,8 +480,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       const int from = 8 * t + (g >> 1);
       const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
       const float b0 = __shfl_sync(0xffffffffu, p0, from + 4), b1 = __shfl_sync(0xffffffffu, p1, from + 4);
-      pa[n] = odd ? a1 : a0;
-      pb[n] = odd ? b1 : b0;
+      pw[n] = odd ? make_float2(a1, b1) : make_float2(a0, b0);
     }
     // ---- weighted rows
     {
@@ -508,15 +509,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           const uint32_t a0[4] = {centred_low(w0[i], big), centred(w0[i], big), centred_low(w1[i], big),
                                   centred(w1[i], big)};
           const uint32_t a1[4] = {centred_low(h0, big), centred(h0, big), centred_low(h1, big), centred(h1, big)};
-          const float da = half_of(dw[j / 2], j & 1), db = half_of(dw[(G + j) / 2], j & 1);
-          const float ca = fmaf(8.f, da, half_of(mw[j], 0)), cb = fmaf(8.f, db, half_of(mw[j], 1));
+          const float2 d = make_float2(half_of(dw[j / 2], j & 1), half_of(dw[(G + j) / 2], j & 1));
+          const float2 c = __ffma2_rn(make_float2(8.f, 8.f), d, make_float2(half_of(mw[j], 0), half_of(mw[j], 1)));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
+            const float2 w = __fmul2_rn(pw[n], d);
             uint32_t b0, b1;
-            columns(pa[n] * da, pb[n] * db, b0, b1);
+            columns(w.x, w.y, b0, b1);
             mma_f16(o[n][2 * j], a0, b0, b1);
             mma_f16(o[n][2 * j + 1], a1, b0, b1);
-            om[n][j] = fmaf(pa[n], ca, fmaf(pb[n], cb, om[n][j]));
+            om[n][j] = __ffma2_rn(pw[n], c, om[n][j]);
           }
         }
       }
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
           if (j == 2 * t) s0 = sum;
           if (j == 2 * t + 1) s1 = sum;
           qs[n][j] = __shfl_sync(0xffffffffu, sum, 8 * t);
-          om[n][j] = 0.f;
+          om[n][j] = make_float2(0.f, 0.f);
         }
         uint32_t hi, lo;
         split2(s0, s1, hi, lo);

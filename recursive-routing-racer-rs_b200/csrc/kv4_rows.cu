@@ -13,7 +13,8 @@
 // which are one word of codes. V: a lane takes the values 32i + 8n + g, + 1 (n = 0..3, g even) of
 // both rows of a pair, which are two words. A quotient is first taken by the reciprocal, and the
 // lane's quotients are divided out where one comes close to a rounding border, which the first
-// misses by less than 4e-6 of a code. (max - min) / 15 is rounded right by one correction of the
+// misses by less than 8e-6 of a code (the reciprocal by two units, its product with 1/15 and with
+// the value by half a one each, and the division itself: 2^-21 of 15). (max - min) / 15 is rounded right by one correction of the
 // product with 1/15 (Markstein's method), which the tests compare with the division.
 // 5,960 rows of 8 x 128 are stored and read back in 28 us, 10 us being their bytes; 8,000 in 31 + 14
 // us, cold: the stores are bound by some 29 instructions a value, the loads by the way to memory.
@@ -114,37 +115,44 @@ __device__ __noinline__ uint32_t divided(float a, float b, float c, float e, flo
   };
   return code(a) | code(b) << 4 | code(c) << 8 | code(e) << 12;
 }
+// The least and the largest of three, NaN where one is
+__device__ __forceinline__ float least(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Eight values of a group of 32, which four neighbouring lanes hold: their codes, value i at bit
 // 4i, and the group's d and m.
 __device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, __half& m16) {
   const float inf = __int_as_float(0x7f800000);
-  float lo = x[0], hi = x[0], zero = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    zero = fmaf(x[i], 0.f, zero);
-  }
-  if (zero != 0.f) hi = inf;  // an infinity or a NaN among them
+  float lo = least(least(x[0], x[1], x[2]), least(x[3], x[4], x[5]), least(x[6], x[7], x[7]));
+  float hi = largest(largest(x[0], x[1], x[2]), largest(x[3], x[4], x[5]), largest(x[6], x[7], x[7]));
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = least(lo, l, l);
+    hi = largest(hi, h, h);
   }
+  const bool finite = fabsf(lo) < inf && fabsf(hi) < inf;
   // (hi - lo) / 15 by the product with 1/15 and its remainder
   const float range = __fsub_rn(hi, lo), first = __fmul_rn(range, 1.f / 15.f);
   const float step = fmaf(fmaf(-15.f, first, range), 1.f / 15.f, first);
   m16 = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  d16 = hi == inf ? __ushort_as_half(0x7fff) : __float2half_rn(fminf(range > 1e6f ? 65504.f : step, 65504.f));
+  d16 = finite ? __float2half_rn(fminf(range > 1e6f ? 65504.f : step, 65504.f)) : __ushort_as_half(0x7fff);
   const float d = __half2float(d16), m = __half2float(m16);
-  const float inv = d > 0.f ? __fdividef(1.f, d) : 0.f;
+  const float inv = d > 0.f ? __fdividef(1.f / 15.f, d) : 0.f;
   uint32_t w = 0;
   bool near = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = __fsub_rn(x[i], m) * inv;
-    const float t = fminf(fmaxf(q, 0.f), 15.f) + 12582912.f;  // the nearest integer in the low bits
-    near |= fabsf(q - (t - 12582912.f)) > 0.49999f;
+    const float q = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv));  // in units of 15, within 0..15
+    const float t = fmaf(q, 15.f, 12582912.f);                      // the nearest integer in the low bits
+    near |= fabsf(fmaf(q, 15.f, 12582912.f - t)) > 0.49999f;
     w += __float_as_uint(t) << (4 * i);
   }
   // what 12582912's own bits added

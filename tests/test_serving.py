@@ -474,6 +474,32 @@ def test_kv4_store_and_load(rrr, ctx, hd, nkv, kind, new, held):
 
 
 @pytest.mark.gpu
+def test_kv4_store_at_the_borders_between_codes(rrr, ctx):
+    """Values half way between two codes and the next ones above and below, for steps of all sizes
+    and minima far from zero: the division of the formula decides, bit by bit."""
+    pick, hd, rows = np.random.default_rng(5), 128, 960
+    x = np.empty((rows, hd // 32, 32), np.float32)
+    for r in range(rows):
+        for j in range(hd // 32):
+            d = np.float32(np.float16(2.0 ** pick.uniform(-20, 10)))
+            m = np.float32(np.float16(d * pick.choice([0, 1, -7.3, 100.0, -3000.0])))
+            half = (m + d * (pick.integers(0, 15, 30) + 0.5).astype(np.float32)).astype(np.float32)
+            step = pick.integers(-2, 3, 30)
+            for _ in range(2):
+                half = np.where(step > 0, np.nextafter(half, np.float32(np.inf)), np.where(step < 0, np.nextafter(half, np.float32(-np.inf)), half))
+                step -= np.sign(step)
+            x[r, j] = pick.permutation(np.concatenate([[m, m + 15 * d], half]).astype(np.float32))
+    x = x.reshape(rows, 1, hd)
+    t = torch.from_numpy(x).cuda()
+    cache = Cache(rrr, ctx, 1, hd, [rows], 2)
+    back = [torch.empty_like(t) for _ in range(2)]
+    cache.c.store(t, t, ints([0, rows]), ints([rows]))
+    cache.c.load(ints([0, rows]), ints([rows]), *back)
+    for b in back:
+        assert np.array_equal(b.cpu().numpy(), np_values(x), equal_nan=True)  # (some minima overflow f16)
+
+
+@pytest.mark.gpu
 def test_kv4_rows_that_are_not_finite_and_places_that_do_not_exist(rrr, ctx):
     cache = Cache(rrr, ctx, 1, 64, [70, 70], 1)
     x = normal(gen(1), 4, 64)
