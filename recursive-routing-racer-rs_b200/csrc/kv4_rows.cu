@@ -8,17 +8,20 @@
 // rounding.
 //
 // Bound by memory (2 bytes of a 16-bit row in and 5/8 out per value, or the reverse), and not far
-// from it by instructions. One warp takes the rows of one block of 16 (aligned in the page, where
-// V's codes of 16 rows lie together) of K or V of one head. K: a lane takes 8 consecutive values,
-// which are one word of codes. V: a lane takes the values 32i + 8n + g, + 1 (n = 0..3, g even) of
-// both rows of a pair, which are two words. A quotient is first taken by the reciprocal, and the
-// lane's quotients are divided out where one comes close to a rounding border, which the first
-// misses by less than 8e-6 of a code (the reciprocal by two units, its product with 1/15 and with
-// the value by half a one each, and the division itself: 2^-21 of 15). (max - min) / 15 is rounded right by one correction of the
-// product with 1/15 (Markstein's method), which the tests compare with the division.
-// 5,960 rows of 8 x 128 are stored and read back in 28 us, 10 us being their bytes; 8,000 in 31 + 14
-// us, cold: the stores are bound by some 29 instructions a value, the loads by the way to memory.
-// (First version: a warp per row with codes shuffled together and a division per value, 58 us.)
+// from it by instructions. One warp takes the rows of one block of 8 or 16 (aligned in the page, so
+// that the two rows of a pair, whose V codes share words, are one warp's) of K or V of one head. K:
+// a lane takes 8 consecutive values, which are one word of codes. V: a lane takes the values 32i +
+// 8n + g, + 1 (n = 0..3, g even) of both rows of a pair, which are two words. A quotient is first
+// taken by the reciprocal, and the lane's quotients are divided out where one comes close to a
+// rounding border, which the first misses by less than 8e-6 of a code (the reciprocal by two units,
+// its product with 1/15 and with the value by half a one each, and the division itself: 2^-21 of
+// 15). (max - min) / 15 is rounded right by one correction of the product with 1/15 (Markstein's
+// method), which the tests compare with the division.
+//
+// 5,960 rows of 8 x 128 are stored and read back in 27.6 us, 10 us being their bytes: the stores are
+// bound by some 25 instructions a value, the loads by the way to memory. (29.0 with 64-bit divisions
+// to find a warp's rows; first version, a warp per row with codes shuffled together and a division
+// per value: 58.)
 #include <math.h>
 
 #include "kv4.cuh"
@@ -45,14 +48,13 @@ int check_kv4_cache(rrr_ctx* ctx, const rrr_kv4_cache* c, const char* fn) {
 namespace {
 
 constexpr int kRowWarps = 8;
-constexpr int kBlockRows = 16;
 
 struct Kv4RowParams {
   uint8_t* pages;
   int64_t n_pages, table_stride;
   const int* table;
   int n_seqs, max_pages, nkv, rows;
-  int slots;  // blocks of 16 rows, with room for the sequences' ends
+  int slots;  // blocks of rows, with room for the sequences' ends
   void* k;
   void* v;
   int64_t k_stride, v_stride;
@@ -61,51 +63,57 @@ struct Kv4RowParams {
   int* err;
 };
 
-// The rows of a warp: packed rows [row0, row0 + n) are the rows first .. first + n - 1 (first < 16)
-// of 16-row block `block` of a page.
+// The rows of a warp: packed rows [row0, row0 + n) are the rows first .. first + n - 1 (first < R)
+// of a block of R rows of a page, from row in_page of it on.
 struct RowBlock {
   uint8_t* blk;
   int64_t row0;
-  int block, first, n;
+  int in_page, first, n;
 };
 
-// Slot x belongs to the last sequence s with cu[s] / 16 + 2 s <= x (sequences get disjoint runs
+// Slot x belongs to the last sequence s with cu[s] / R + 2 s <= x (sequences get disjoint runs
 // of slots that are long enough), searched by the warp 32 sequences at a time.
-template <int HD>
+template <int HD, int R>
 __device__ __forceinline__ bool find_rows(const Kv4RowParams& p, int x, int h, RowBlock& b) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.n_seqs;  // the sequence lies in [lo, hi)
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, s = lo + lane * step;
-    const bool at = s < hi && p.cu[s] / kBlockRows + 2 * s <= x;
+    const bool at = s < hi && p.cu[s] / R + 2 * s <= x;
     const unsigned below = __ballot_sync(0xffffffffu, at);
     lo += below ? (31 - __clz(below)) * step : 0;
     hi = min(hi, lo + step);
   }
-  const int r0 = p.cu[lo], r1 = p.cu[lo + 1], len = p.lens[lo];
+  const int r0 = p.cu[lo], r1 = p.cu[lo + 1], len = p.lens[lo], most = p.max_pages * kPageRows;
   if (r0 < 0 || r1 < r0 || r1 > p.rows) {
     if (lane == 0) flag_position(p.err);
     return false;
   }
-  const int64_t pos0 = (int64_t)len - (r1 - r0);  // position of the sequence's first packed row
-  if (r1 > r0 && (pos0 < 0 || len > (int64_t)p.max_pages * kPageRows) && lane == 0) flag_position(p.err);
+  const int rows = r1 - r0, k = x - (r0 / R + 2 * lo);  // k: the block among the sequence's
+  if (rows > 0 && (len < rows || len > most) && lane == 0) flag_position(p.err);
   // (rows at positions that do not exist are left out)
-  int64_t at = pos0 >= 0 ? pos0 : 0;
-  const int64_t end = min((int64_t)len, (int64_t)p.max_pages * kPageRows);
-  const int64_t q = at / kBlockRows + (x - (r0 / kBlockRows + 2 * lo));  // 16-row block of the sequence
-  const int64_t from = max(at, q * kBlockRows), to = min(end, (q + 1) * kBlockRows);
-  if (q < 0 || from >= to) return false;
-  const int page = p.table[(int64_t)lo * p.table_stride + from / kPageRows];
+  if (k < 0 || len <= 0) return false;
+  const int pos0 = len - rows;  // position of the sequence's first packed row
+  const int at = max(pos0, 0), end = min(len, most);
+  const int64_t start = (int64_t)(at / R + (int64_t)k) * R;
+  if (start >= end) return false;
+  const int from = max(at, (int)start), to = min(end, (int)start + R);  // (end <= 2^31 - 64)
+  if (from >= to) return false;
+  const int page = p.table[(int64_t)lo * p.table_stride + (unsigned)from / kPageRows];
   if (page < 0 || page >= p.n_pages) {
     if (lane == 0) flag_position(p.err);
     return false;
   }
   b.blk = p.pages + ((int64_t)page * p.nkv + h) * Kv4Block<HD>::kBytes;
   b.row0 = r0 + (from - pos0);
-  b.block = (int)(from % kPageRows) / kBlockRows;
-  b.first = (int)(from % kBlockRows);
-  b.n = (int)(to - from);
+  b.in_page = from % kPageRows;
+  b.first = from % R;
+  b.n = to - from;
   return true;
+}
+// CTAs: a head of K (z even) or V each, kRowWarps slots in y and z
+__device__ __forceinline__ int slot_of() {
+  return (int)(((blockIdx.z >> 1) * gridDim.y + blockIdx.y) * kRowWarps + (threadIdx.x >> 5));
 }
 
 // Codes of four values by the division itself (out of line: rarely called)
@@ -168,30 +176,29 @@ __device__ __forceinline__ void dequantise(uint32_t w, float d, float m, float (
     x[i] = fmaf(__uint_as_float(((w >> (4 * i)) & 15u) | 0x4b000000u) - 8388608.f, d, m);
 }
 
-template <int HD>
-struct Lanes {  // of a warp: groups at once, and rows (K) or pairs of rows (V) at once
+template <int HD, int R>
+struct Lanes {  // of a warp of R rows: groups at once, and rows (K) or pairs of rows (V) at once
   static constexpr int kGroups = Kv4Block<HD>::kGroups;
   static constexpr int kRows = 32 / (4 * kGroups);
-  static constexpr int kAhead = kBlockRows / kRows < 4 ? kBlockRows / kRows : 4;  // rows in flight
+  static constexpr int kAhead = R / kRows < 4 ? (R / kRows < 1 ? 1 : R / kRows) : 4;  // rows in flight
   static constexpr int kPairsAhead = kRows >= 4 ? 1 : 2;
 };
 
-template <int HD, typename T>
+template <int HD, int R, typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_store_kernel(const __grid_constant__ Kv4RowParams p) {
   using B = Kv4Block<HD>;
-  using L = Lanes<HD>;
+  using L = Lanes<HD, R>;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  const int x = (int)(item / (2 * p.nkv));
+  const int x = slot_of(), h = blockIdx.x;
+  const bool is_v = blockIdx.z & 1;
   if (x >= p.slots) return;
-  const int hv = (int)(item - (int64_t)x * 2 * p.nkv), h = hv % p.nkv;
   RowBlock b;
-  if (!find_rows<HD>(p, x, h, b)) return;
-  const int in_page = kBlockRows * b.block + b.first;
+  if (!find_rows<HD, R>(p, x, h, b)) return;
+  const int in_page = b.in_page;
   const int j = lane / 4 % L::kGroups, t = lane % 4, set = lane / (4 * L::kGroups);
-  if (hv < p.nkv) {
+  if (!is_v) {
     const T* src = static_cast<const T*>(p.k) + (int64_t)h * HD + 32 * j + 8 * t;
 #pragma unroll 1
     for (int r0 = set; r0 < b.n + set; r0 += L::kAhead * L::kRows) {
@@ -279,23 +286,22 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_store_kernel(const __grid_
   }
 }
 
-template <int HD, typename T>
+template <int HD, int R, typename T>
 __global__ void __launch_bounds__(32 * kRowWarps) kv4_load_kernel(const __grid_constant__ Kv4RowParams p) {
   using B = Kv4Block<HD>;
-  using L = Lanes<HD>;
+  using L = Lanes<HD, R>;
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  const int x = (int)(item / (2 * p.nkv));
+  const int x = slot_of(), h = blockIdx.x;
+  const bool is_v = blockIdx.z & 1;
   if (x >= p.slots) return;
-  const int hv = (int)(item - (int64_t)x * 2 * p.nkv), h = hv % p.nkv;
-  if (!(hv < p.nkv ? p.k : p.v)) return;
+  if (!(is_v ? p.v : p.k)) return;
   RowBlock b;
-  if (!find_rows<HD>(p, x, h, b)) return;
-  const int in_page = kBlockRows * b.block + b.first;
+  if (!find_rows<HD, R>(p, x, h, b)) return;
+  const int in_page = b.in_page;
   const int j = lane / 4 % L::kGroups, t = lane % 4, set = lane / (4 * L::kGroups);
-  if (hv < p.nkv) {
+  if (!is_v) {
     T* dst = static_cast<T*>(p.k) + (int64_t)h * HD + 32 * j + 8 * t;
 #pragma unroll 1
     for (int r0 = set; r0 < b.n; r0 += L::kAhead * L::kRows) {
@@ -355,11 +361,23 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv4_load_kernel(const __grid_c
   }
 }
 
+template <int HD, int R, typename T>
+cudaError_t launch_rows(const LaunchEnv& env, bool store, Kv4RowParams p) {
+  p.slots = p.rows / R + 2 * p.n_seqs;
+  const int64_t across = ((int64_t)p.slots + kRowWarps - 1) / kRowWarps, y = across < 65535 ? across : 65535;
+  const dim3 grid(p.nkv, (unsigned)y, (unsigned)(2 * ((across + y - 1) / y))), block(32 * kRowWarps);
+  return store ? rrr_launch_pdl(kv4_store_kernel<HD, R, T>, grid, block, 0, env.stream, env.pdl, p)
+               : rrr_launch_pdl(kv4_load_kernel<HD, R, T>, grid, block, 0, env.stream, env.pdl, p);
+}
 template <int HD, typename T>
 cudaError_t launch(const LaunchEnv& env, bool store, const Kv4RowParams& p) {
-  const dim3 grid((unsigned)((2 * (int64_t)p.slots * p.nkv + kRowWarps - 1) / kRowWarps)), block(32 * kRowWarps);
-  return store ? rrr_launch_pdl(kv4_store_kernel<HD, T>, grid, block, 0, env.stream, env.pdl, p)
-               : rrr_launch_pdl(kv4_load_kernel<HD, T>, grid, block, 0, env.stream, env.pdl, p);
+  // Blocks of 8 rows where those of 16 would not fill the SMs once or twice, and for long rows:
+  // 12,000 rows of 2 x 128 stored and read back 15.7 us (16 rows: 18.5), of 8 x 128 47.5 (46.0), of
+  // 1 x 256 18.1 (25.3), of 8 x 256 77.5 (78.2).
+  if constexpr (HD < 256)
+    if (2 * ((int64_t)p.rows / 16 + p.n_seqs) * p.nkv >= 32 * (int64_t)env.sm_count)
+      return launch_rows<HD, 16, T>(env, store, p);
+  return launch_rows<HD, 8, T>(env, store, p);
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, bool store, const Kv4RowParams& p) {
@@ -394,11 +412,11 @@ int kv4_rows(rrr_ctx* ctx, const char* fn, bool store, const rrr_kv4_cache* c, i
   DeviceGuard dev(ctx);
   if (dev.rc) return dev.rc;
   if (rows == 0 || c->n_seqs == 0) return RRR_OK;
-  if (c->n_seqs > INT32_MAX / 4 || ((int64_t)rows / kBlockRows + 2 * (int64_t)c->n_seqs) * c->n_kv_heads > INT32_MAX)
+  if (c->n_seqs > INT32_MAX / 4 || rows > INT32_MAX / 4)
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows and sequences for one call", fn);
   const LaunchEnv env = make_env(ctx, stream);
   const Kv4RowParams p{static_cast<uint8_t*>(c->pages), c->n_pages, c->table_stride, c->page_table, c->n_seqs,
-                       c->max_pages, c->n_kv_heads, rows, rows / kBlockRows + 2 * c->n_seqs, k, v, k_stride, v_stride, cu_rows, kv_lens, env.d_err};
+                       c->max_pages, c->n_kv_heads, rows, 0, k, v, k_stride, v_stride, cu_rows, kv_lens, env.d_err};
   cudaError_t e;
   switch (c->head_dim) {
     case 64: e = launch_type<64>(env, type, store, p); break;

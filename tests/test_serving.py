@@ -474,6 +474,7 @@ def test_kv4_store_and_load(rrr, ctx, hd, nkv, kind, new, held):
 
 
 @pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:overflow")  # some minima are beyond f16
 def test_kv4_store_at_the_borders_between_codes(rrr, ctx):
     """Values half way between two codes and the next ones above and below, for steps of all sizes
     and minima far from zero: the division of the formula decides, bit by bit."""
@@ -496,7 +497,7 @@ def test_kv4_store_at_the_borders_between_codes(rrr, ctx):
     cache.c.store(t, t, ints([0, rows]), ints([rows]))
     cache.c.load(ints([0, rows]), ints([rows]), *back)
     for b in back:
-        assert np.array_equal(b.cpu().numpy(), np_values(x), equal_nan=True)  # (some minima overflow f16)
+        assert np.array_equal(b.cpu().numpy(), np_values(x), equal_nan=True)
 
 
 @pytest.mark.gpu
