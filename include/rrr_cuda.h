@@ -445,7 +445,8 @@ int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_
 /* Attention of one query row per sequence over its kv_lens[s] cached rows: out[s][h] = sum_p
  * softmax_p(scale * q[s][h] . k[p][g]) v[p][g], g = h / (n_heads / n_kv_heads), at most 8
  * query heads per KV head; scale 0 = 1/sqrt(head_dim). q, out: rows of n_heads*head_dim values
- * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros. Scores and sums
+ * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros, and so does one whose
+ * kv_lens is out of range; rows on pages that do not exist are left out. Scores and sums
  * carry 32-bit accuracy whatever the type. workspace: rrr_kv4_workspace bytes of device
  * memory, whatever they hold; calls that can run at the same time, replays of captured
  * graphs among them, need one each. */

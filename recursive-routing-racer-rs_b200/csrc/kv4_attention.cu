@@ -835,8 +835,8 @@ int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int typ
   if (!row_type(type)) return set_error(ctx, RRR_ERR_BAD_QTYPE, "%s: type must be 0 (F32), 1 (F16) or 30 (BF16)", fn);
   if (!workspace || (c->n_seqs > 0 && (!q || !kv_lens || !out))) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t width = (int64_t)n_heads * c->head_dim;
-  if (q_stride < width || out_stride < width)
-    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: strides of at least n_heads * head_dim", fn);
+  if (!stride_fits(q_stride, width) || !stride_fits(out_stride, width))
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: strides of n_heads * head_dim to 2^38", fn);
   if (!(scale >= 0.f) || scale > 3.4e38f) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: scale must be finite, not negative", fn);
   if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % 8 || out_stride % 8 || !aligned_to(kv_lens, 4) ||
       !aligned_to(workspace, 16))

@@ -398,8 +398,8 @@ int kv4_rows(rrr_ctx* ctx, const char* fn, bool store, const rrr_kv4_cache* c, i
   if ((rows > 0 && (store ? !k || !v : !k && !v)) || (c->n_seqs > 0 && (!cu_rows || !kv_lens)))
     return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
-  if (rows < 0 || (k && k_stride < width) || (v && v_stride < width))
-    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows >= 0 and strides of at least n_kv_heads * head_dim", fn);
+  if (rows < 0 || (k && !stride_fits(k_stride, width)) || (v && !stride_fits(v_stride, width)))
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows >= 0 and strides of n_kv_heads * head_dim to 2^38", fn);
   if (!aligned_to(k, 16) || !aligned_to(v, 16) || (k && k_stride % 8) || (v && v_stride % 8) ||
       !aligned_to(cu_rows, 4) || !aligned_to(kv_lens, 4))
     return set_error(ctx, RRR_ERR_MISALIGNED, "%s: rows must be 16-byte aligned, strides multiples of 8 elements", fn);

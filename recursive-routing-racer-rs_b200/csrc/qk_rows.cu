@@ -223,9 +223,9 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rope_dim must be a multiple of head_dim / 16 with halves", fn);
   if (!(a->rope_theta > 0.f)) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: rope_theta must be positive", fn);
   if (!(eps >= 0.f)) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: eps must not be negative", fn);
-  if (row_stride < (int64_t)(nh + 2 * nkv) * hd || q_stride < (int64_t)nh * hd ||
-      k_stride < (int64_t)nkv * hd || (v && v_stride < (int64_t)nkv * hd))
-    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: a row stride is shorter than its row", fn);
+  if (!stride_fits(row_stride, (int64_t)(nh + 2 * nkv) * hd) || !stride_fits(q_stride, (int64_t)nh * hd) ||
+      !stride_fits(k_stride, (int64_t)nkv * hd) || (v && !stride_fits(v_stride, (int64_t)nkv * hd)))
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: a row stride is shorter than its row, or over 2^38", fn);
   if (!aligned_to(qkv, 16) || !aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) ||
       row_stride % 8 || q_stride % 8 || k_stride % 8 || (v && v_stride % 8) || !aligned_to(positions, 4) ||
       !aligned_to(q_gamma, 4) || !aligned_to(k_gamma, 4))

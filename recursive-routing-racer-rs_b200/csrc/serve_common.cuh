@@ -83,6 +83,9 @@ inline int elem_bytes(int type) { return type == RRR_F32 ? 4 : 2; }
 inline bool row_type(int type) { return type == RRR_F32 || type == RRR_F16 || type == RRR_BF16; }
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// A row stride in elements that rows of `width` fit and whose products stay in 64 bits
+inline bool stride_fits(int64_t stride, int64_t width) { return stride >= width && stride <= (int64_t)1 << 38; }
+
 // Rows of `width` bytes at a pitch of `stride` bytes.
 struct RowSet {
   const void* p;
@@ -92,8 +95,9 @@ struct RowSet {
 inline bool rows_disjoint(const RowSet& a, const RowSet& b) {
   if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return true;
   const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
-  const uintptr_t ea = pa + (a.rows - 1) * a.stride + a.width, eb = pb + (b.rows - 1) * b.stride + b.width;
-  if (ea <= pb || eb <= pa) return true;
+  const __int128 ea = (__int128)pa + (__int128)(a.rows - 1) * a.stride + a.width;
+  const __int128 eb = (__int128)pb + (__int128)(b.rows - 1) * b.stride + b.width;
+  if (ea <= (__int128)pb || eb <= (__int128)pa) return true;
   if (a.stride != b.stride || a.stride < 1) return false;
   const int64_t d = (int64_t)(pb - pa) % a.stride, off = d < 0 ? d + a.stride : d;
   return off >= a.width && off + b.width <= a.stride;

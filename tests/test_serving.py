@@ -281,6 +281,11 @@ def test_empty_arrays_may_be_null_and_sizes_have_an_end(rrr, host_ctx):
         assert f(host_ctx, ref(no_seqs), 30, None, 256, None, 256, 0, None, None, None) == FINE
         assert f(host_ctx, ref(no_pages), 30, 1 << 20, 256, 2 << 20, 256, 5, 256, 512, None) == FINE
         assert f(host_ctx, ref(many), 30, 1 << 20, 256, 2 << 20, 256, 5, 256, 512, None) == -3
+    far = 1 << 40
+    assert L.rrr_qk_norm_rope(host_ctx, *_qk_args(rrr, stride=far)) == -3
+    assert L.rrr_kv4_store(host_ctx, ref(_cache(rrr)), 30, 1 << 20, far, 2 << 20, 256, 5, 256, 512, None) == -3
+    assert L.rrr_attention_kv4(host_ctx, ref(_cache(rrr)), 6, 0, 1 << 20, far, 512, 0.0, 2 << 20, 768, 1 << 24, 1 << 40,
+                               None) == -3
     need = ctypes.c_int64()
     for c in (no_seqs, no_pages):
         assert L.rrr_kv4_workspace(host_ctx, ref(c), 6, ref(need)) == 0
@@ -911,6 +916,39 @@ def test_a_batch_from_its_prompts_to_its_tokens(rrr, ctx, hd, rd, halves, norm):
         check_decode(out, q, [(kk[a:b].double(), vv[a:b].double()) for a, b in zip(c, c[1:])], 1 / math.sqrt(hd), t)
         new = [x[h - 1] for x, h in ((kk[a:b], b - a) for a, b in zip(c, c[1:]))]
         assert torch.equal(torch.stack(new).cpu(), torch.from_numpy(np_values(k.float().cpu().numpy())))
+    assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_captured_calls_replay_with_other_lengths(rrr, ctx, hd):
+    """One graph of prompt attention and one of a decode step over batches of other shapes: lengths
+    and row starts are the device's, so nothing of the capture's batch may remain."""
+    g, nh, nkv, t = gen(hd), 6, 2, torch.bfloat16
+    batches = [([40, 300, 7], [40, 300, 7]), ([1, 1, 1], [500, 0, 130]), ([0, 600, 0], [0, 600, 0]), ([129, 200, 30], [140, 333, 30])]
+    q, k, v = (normal(g, 700, h, hd, dtype=t) for h in (nh, nkv, nkv))
+    cq, ck, out = ints([0] * 4), ints([0] * 4), torch.empty_like(q)
+    lens = [[5, 0, 64], [3000, 1, 700], [0, 0, 0], [64, 2999, 65]]
+    cache, kv = filled(rrr, ctx, nkv, hd, [3000] * 3, hd)
+    dq, dlens = normal(g, 3, nh, hd), ints([0] * 3)
+    dout, ws = torch.empty_like(dq), cache.c.workspace(nh).fill_(0xff)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        stream = torch.cuda.current_stream()
+        rrr.attention_packed(ctx, q, k, v, cq, ck, out, stream=stream)
+        cache.c.attention(dq, dlens, dout, ws, stream=stream)
+    for (lq, lk), n in zip(batches, lens):
+        out.fill_(2.0)
+        before = out.clone()
+        cq.copy_(cu_of(lq))
+        ck.copy_(cu_of(lk))
+        dlens.copy_(ints(n))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_packed(out, q, k, v, lq, lk, True, 1 / math.sqrt(hd), before)
+        check_decode(dout, dq, [(a[:m], b[:m]) for (a, b), m in zip(kv, n)], 1 / math.sqrt(hd), torch.float32)
     assert ctx.device_error() == 0
 
 
