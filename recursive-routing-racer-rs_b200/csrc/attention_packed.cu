@@ -10,7 +10,7 @@
 //
 // Where a tile begins. Tile x of the grid belongs to the last sequence s with floor(cu[s] /
 // rows) + s <= x and starts at its row cu[s] + rows * (x - floor(cu[s] / rows) - s): sequences
-// get disjoint runs of x that are long enough, found by a binary search on the device.
+// get disjoint runs of x that are long enough; a warp searches 32 sequences at a time.
 #include <math.h>
 
 #include "serve_common.cuh"
@@ -41,13 +41,13 @@ struct Tile {
   int k0, k1;             // its KV rows
 };
 __device__ __forceinline__ bool find_tile(const PackedParams& p, int rows, int x, Tile& t) {
-  int lo = 0, hi = p.n_seqs - 1;  // the last s with cu[s] / rows + s <= x
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] / rows + mid <= x)
-      lo = mid;
-    else
-      hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.n_seqs;  // the last s with cu[s] / rows + s <= x lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, s < hi && p.cu_q[s] / rows + s <= x);
+    lo += below ? (31 - __clz(below)) * step : 0;
+    hi = min(hi, lo + step);
   }
   t.seq = lo;
   t.q0 = p.cu_q[lo];
@@ -400,6 +400,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
       : "r"(taddr)
       : "memory");
 }
+// Brings a tensor map on its way before the first copy wants it (a prompt of 77 rows 8.03 -> 7.89 us)
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -615,22 +619,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
-  pdl_wait();
-  Tile t;
-  const int both = 2 * tp.tokens, nkv = p.nh / p.hpk;
-  if (!find_tile(p, both, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
-  const int kv = blockIdx.x % nkv;
-  const int rows = min(both, t.q1 - t.row0);
-  // KV rows that each tile's last row sees, and the blocks of 128 of them
-  int sees[2], blocks[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int last = min(rows, (i + 1) * tp.tokens) - 1;
-    sees[i] = last >= i * tp.tokens ? seen_by(p, t, t.row0 + last) : 0;
-    blocks[i] = (sees[i] + kTile - 1) / kTile;
-  }
-  const int n = max(blocks[0], blocks[1]);
-
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < kStages; ++s) {
@@ -646,7 +634,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     abort_flag = 0;
     fence_mbarrier_init();
   }
+  if (warp == 9 && lane < 3) prefetch_map(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
+  pdl_wait();
+  Tile t;
+  const int both = 2 * tp.tokens, nkv = p.nh / p.hpk;
+  if (!find_tile(p, both, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
   if (warp == 8) tmem_alloc(&tmem_slot, 512);
+  const int kv = blockIdx.x % nkv;
+  const int rows = min(both, t.q1 - t.row0);
+  // KV rows that each tile's last row sees, and the blocks of 128 of them
+  int sees[2], blocks[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min(rows, (i + 1) * tp.tokens) - 1;
+    sees[i] = last >= i * tp.tokens ? seen_by(p, t, t.row0 + last) : 0;
+    blocks[i] = (sees[i] + kTile - 1) / kTile;
+  }
+  const int n = max(blocks[0], blocks[1]);
+
   // tile rows past the last whole query row: zeros, so that their scores are
   for (int k = tp.tokens * p.hpk * 8 + threadIdx.x; k < kTile * 8; k += kTcThreads)
     for (int c = 0; c < 2 * kChunks; ++c) *reinterpret_cast<uint4*>(qs + c * kPiece + 16 * k) = make_uint4(0, 0, 0, 0);
@@ -873,15 +878,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
-  pdl_wait();
-  Tile t;
-  const int nkv = p.nh / p.hpk;
-  if (!find_tile(p, tp.tokens, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
-  const int kv = blockIdx.x % nkv;
-  const int rows = min(tp.tokens, t.q1 - t.row0), lk = t.k1 - t.k0;
-  const int sees = seen_by(p, t, t.row0 + rows - 1);  // KV rows that the last row sees
-  const int n = (sees + kTile - 1) / kTile;
-
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
@@ -893,7 +889,17 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     abort_flag = 0;
     fence_mbarrier_init();
   }
+  if (warp == 5 && lane < 3) prefetch_map(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
+  pdl_wait();
+  Tile t;
+  const int nkv = p.nh / p.hpk;
+  if (!find_tile(p, tp.tokens, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
   if (warp == 4) tmem_alloc(&tmem_slot, 512);
+  const int kv = blockIdx.x % nkv;
+  const int rows = min(tp.tokens, t.q1 - t.row0), lk = t.k1 - t.k0;
+  const int sees = seen_by(p, t, t.row0 + rows - 1);  // KV rows that the last row sees
+  const int n = (sees + kTile - 1) / kTile;
+
   // tile rows past the last whole query row: zeros, so that their scores are
   for (int k = tp.tokens * p.hpk * 8 + threadIdx.x; k < kTile * 8; k += kWideThreads)
     for (int c = 0; c < kChunks; ++c) *reinterpret_cast<uint4*>(qs + c * kPiece + 16 * k) = make_uint4(0, 0, 0, 0);
