@@ -350,6 +350,7 @@ constexpr int tc_stages() { return HD == 128 ? 5 : 10; }
 struct TcParams {
   PackedParams a;
   int tokens;  // query rows per tile
+  int splits;  // CTAs of a cluster, each with a part of the KV rows (1, 2, 4 or 8)
   uint32_t idesc_s, idesc_o;
 };
 
@@ -599,7 +600,28 @@ __device__ __forceinline__ void write_row(const PackedParams& p, const Tile& t, 
   }
 }
 
-template <int HD, typename T>
+// Where the tiles are too few for the SMs, a cluster of CTAs takes one item, each CTA an equal part
+// of its blocks of KV rows, as if the sequence's rows began and ended there. Then every CTA sends
+// its rows' maxima and sums to all, and of O's columns each CTA's share to it, over the cluster's
+// shared memory; a CTA adds up its columns in the order of the parts and writes them.
+__device__ __forceinline__ uint32_t in_cta(const void* local, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(local)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void send2(uint32_t at, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(a), "f"(b) : "memory");
+}
+__device__ __forceinline__ void send4(uint32_t at, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
+template <int HD, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcParams tp) {
@@ -638,16 +660,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   pdl_wait();
   Tile t;
   const int both = 2 * tp.tokens, nkv = p.nh / p.hpk;
-  if (!find_tile(p, both, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
+  const int splits = SPLIT ? tp.splits : 1, rank = SPLIT ? blockIdx.x % splits : 0;
+  const int item = blockIdx.x / splits, items = gridDim.x / splits;
+  if (!find_tile(p, both, (items - 1 - item) / nkv, t)) return;
   if (warp == 8) tmem_alloc(&tmem_slot, 512);
-  const int kv = blockIdx.x % nkv;
+  const int kv = item % nkv;
   const int rows = min(both, t.q1 - t.row0);
-  // KV rows that each tile's last row sees, and the blocks of 128 of them
-  int sees[2], blocks[2];
+  // KV rows that each tile's last row sees, of those that this CTA takes: from row `from` of the
+  // sequence on, `most` at the most; and the blocks of 128 of them
+  int all_sees[2], sees[2], blocks[2], from = 0, most = INT32_MAX;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int last = min(rows, (i + 1) * tp.tokens) - 1;
-    sees[i] = last >= i * tp.tokens ? seen_by(p, t, t.row0 + last) : 0;
+    all_sees[i] = last >= i * tp.tokens ? seen_by(p, t, t.row0 + last) : 0;
+  }
+  if constexpr (SPLIT) {
+    const int all = (max(all_sees[0], all_sees[1]) + kTile - 1) / kTile;
+    from = all * rank / splits * kTile;
+    most = all * (rank + 1) / splits * kTile - from;
+  }
+  auto part = [&](int seen) { return SPLIT ? max(0, min(seen - from, most)) : seen; };
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    sees[i] = part(all_sees[i]);
     blocks[i] = (sees[i] + kTile - 1) / kTile;
   }
   const int n = max(blocks[0], blocks[1]);
@@ -660,6 +695,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  if constexpr (SPLIT) cluster_barrier();  // every CTA has begun
   const uint32_t s_col[2] = {tmem, tmem + kTile}, o_col[2] = {tmem + 2 * kTile, tmem + 2 * kTile + HD};
 
   // registers: 384 x 168 at launch = 256 x 232 + 128 x 40
@@ -685,7 +721,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_arrive_expect_tx(&full[s], kOperand);
         for (int c = 0; c < kChunks; ++c)
           tma_load_3d(ring + (size_t)s * kOperand + c * kPiece, issued & 1 ? &vmap : &kmap, 64 * c, kv,
-                      t.k0 + (issued >> 1) * kTile, &full[s]);
+                      t.k0 + from + (issued >> 1) * kTile, &full[s]);
       }
       __syncwarp();
       if (++s == kStages) {
@@ -780,11 +816,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int token = r / p.hpk, head = kv * p.hpk + r % p.hpk;
     const int row = t.row0 + i * tp.tokens + token;  // query row
     const bool mine = token < tp.tokens && i * tp.tokens + token < rows;
-    const int seen = mine ? seen_by(p, t, row) : 0;
+    const int all_seen = mine ? seen_by(p, t, row) : 0, seen = part(all_seen);
     const int open = mine ? seen : INT32_MAX;  // tile rows of no query mask nothing
     const int all_see = (int)__reduce_min_sync(0xffffffffu, (unsigned)open);    // every row of the warp,
     const int none_sees = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);  // and none from here on
-    const int lk = t.k1 - t.k0;
+    const int lk = t.k1 - t.k0 - from;  // rows of the sequence from this CTA's first on
     const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sc = s_col[i] + sub, oc = o_col[i] + sub;
     const int end_block = (lk - 1) / kTile;
@@ -812,10 +848,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           break;
         }
         uint8_t* v = ring + (size_t)(item % kStages) * kOperand;
-        const int from = lk - j * kTile;
+        const int left = lk - j * kTile;
         for (int c = 0; c < kChunks; ++c)
-          for (int k = (threadIdx.x & 127); k < (kTile - from) * 8; k += 128)
-            *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+          for (int k = (threadIdx.x & 127); k < (kTile - left) * 8; k += 128)
+            *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)left * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
       }
       rs.block(sc, j, open, all_see, none_sees, [&](float alpha) {
@@ -827,18 +863,86 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive(&p_full[i]);
     }
     // ---------------- out
-    if (ok && i * tp.tokens < rows) {
-      if (blocks[i] > 0) {
-        ok = warp_wait(&o_full[i], 0, p.err);
-        if (!ok) abort_flag = 1;
-      }
-      if (ok) {
-        tc_fence_after();
-        write_row<HD, T>(p, t, oc, blocks[i] > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees[i] + 15) & ~15));
-      }
-      tc_fence_before();
+    if (ok && blocks[i] > 0) {
+      ok = warp_wait(&o_full[i], 0, p.err);
+      if (!ok) abort_flag = 1;
     }
+    tc_fence_after();
+    if constexpr (!SPLIT) {
+      if (ok && i * tp.tokens < rows)
+        write_row<HD, T>(p, t, oc, blocks[i] > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees[i] + 15) & ~15));
+    } else {
+      // in every CTA, once the products of all are done: maxima and sums [part][row] and, of the first,
+      // what came out not finite [part][row] in Q's place; [part][4 columns][row] in the ring's
+      const int at = threadIdx.x, width = HD / splits;
+      float2* stats = reinterpret_cast<float2*>(qs);
+      int* bad_rows = reinterpret_cast<int*>(qs + 8 * 256 * sizeof(float2));
+      cluster_barrier();
+      const bool some = ok && blocks[i] > 0, sends = some && mine;
+      for (int c = 0; c < splits; ++c)
+        send2(in_cta(stats + rank * 256 + at, c), sends ? rs.m : -INFINITY, sends ? rs.l.x + rs.l.y : 0.f);
+      if (some)
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(oc + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) {
+            const int to = (c + k) / width, four = (c + k) % width / 4;
+            if (sends) send4(in_cta(ring + ((size_t)(rank * (width / 4) + four) * 256 + at) * 16, to), v + k);
+          }
+        }
+      cluster_barrier();
+      float top = -INFINITY, sum = 0.f;
+      for (int c = 0; c < splits; ++c) top = fmaxf(top, stats[c * 256 + at].x);
+      const float use = top == -INFINITY ? 0.f : top;
+      for (int c = 0; c < splits; ++c) sum = fmaf(ex2(stats[c * 256 + at].x - use), stats[c * 256 + at].y, sum);
+      const float inv = all_seen > 0 ? 1.f / sum : 0.f;
+      T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head + rank * width;
+      bool bad = false;
+      for (int e = 0; e < width; e += 8) {
+        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < splits; ++c) {
+          const float m = stats[c * 256 + at].x;
+          if (m == -INFINITY) continue;  // (nothing was sent, or nothing but zeros)
+          const float w = ex2(m - use);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(ring + ((size_t)(c * (width / 4) + e / 4 + k) * 256 + at) * 16);
+            o[4 * k] = fmaf(w, x.x, o[4 * k]);
+            o[4 * k + 1] = fmaf(w, x.y, o[4 * k + 1]);
+            o[4 * k + 2] = fmaf(w, x.z, o[4 * k + 2]);
+            o[4 * k + 3] = fmaf(w, x.w, o[4 * k + 3]);
+          }
+        }
+        uint32_t packed[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = all_seen > 0 ? o[2 * k] * inv : 0.f, b = all_seen > 0 ? o[2 * k + 1] * inv : 0.f;
+          bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
+          packed[k] = Mma<T>::pack(a, b);
+        }
+        if (mine) *reinterpret_cast<uint4*>(dst + e) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      }
+      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(in_cta(bad_rows + rank * 256 + at, 0)), "r"((int)bad) : "memory");
+      cluster_barrier();
+      if (rank == 0) {
+        for (int c = 0; c < splits; ++c) bad |= bad_rows[c * 256 + at] != 0;
+        unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
+        while (again) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          __syncwarp();
+          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, head, who),
+                          min(t.k1 - t.k0, (all_sees[i] + 15) & ~15));
+        }
+      }
+    }
+    tc_fence_before();
   }
+  if constexpr (SPLIT)
+    if (warp >= 8)
+      for (int k = 0; k < 3; ++k) cluster_barrier();
 
   tc_fence_before();
   __syncthreads();
@@ -1103,10 +1207,33 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
     return rrr_launch_pdl(kern, grid, dim3(kWideThreads), (size_t)smem, env.stream, env.pdl, qmap, kmap, vmap, tp);
   } else {
     const int smem = (2 + tc_stages<HD>()) * kTile * HD * 2 + 1024;
-    auto kern = packed_tc_kernel<HD, T>;
+    // Few tiles with many blocks of KV rows (of the mean sequence) go to clusters. Joining costs 3 to 5
+    // us, and no more than some 9 clusters of 8 such CTAs run at once: 1 row of 24 heads on 9,000 rows
+    // 123 us alone, 75, 44 and 28 by 2, 4 and 8 CTAs; 100 rows on 2,000 36.5, 32, 24 and, in two rounds,
+    // 36; 1,000 on 1,000 with 8 heads on 2 23, 24.5 and 20.6; 500 rows on 500 16 and 20.
+    const int64_t deep = (p.kv_rows / p.n_seqs + kTile - 1) / kTile;
+    tp.splits = 1;
+    for (const int by : {8, 4, 2}) {
+      if ((int64_t)grid.x * by > (by == 8 ? env.sm_count / 2 : env.sm_count) || deep < (by == 2 ? 12 : 2 * by)) continue;
+      tp.splits = by;
+      break;
+    }
+    auto kern = tp.splits > 1 ? packed_tc_kernel<HD, T, true> : packed_tc_kernel<HD, T, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    return rrr_launch_pdl(kern, grid, dim3(kTcThreads), (size_t)smem, env.stream, env.pdl, qmap, kmap, vmap, tp);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = env.pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)tp.splits, 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid.x * tp.splits);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = env.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = tp.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, qmap, kmap, vmap, tp);
   }
 }
 

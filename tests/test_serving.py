@@ -816,6 +816,33 @@ def test_attention_packed_many_values_that_are_not_finite(rrr, ctx, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(128, 24, 8), (64, 24, 8), (128, 4, 1), (64, 5, 5), (256, 4, 2)])
+@pytest.mark.parametrize("lq,lk", [([1], [3000]), ([37], [2111]), ([100], [2048]), ([3, 0, 50], [2500, 900, 2600]), ([700], [1600])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_packed_few_rows_on_many(rrr, ctx, hd, nh, nkv, lq, lk, causal):
+    """Few tiles: the KV rows of one are shared by several CTAs, some of which see none of them."""
+    g, t = gen(sum(lq) + hd), torch.bfloat16
+    q, k, v = (normal(g, sum(n) + 2, h, hd, dtype=t) for n, h in ((lq, nh), (lk, nkv), (lk, nkv)))
+    k[sum(lk):], v[sum(lk):] = math.nan, math.inf
+    out = torch.full_like(q, 3.0)
+    before = out.clone()
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), out, causal=causal)
+    check_packed(out, q, k, v, lq, lk, causal, 1 / math.sqrt(hd), before)
+    again = before.clone()
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), again, causal=causal)
+    assert torch.equal(out, again) and ctx.device_error() == 0
+    # an infinite value that the last row alone sees, in one head
+    if causal and len(lq) == 1 and lq[0] > 1:
+        v[lk[0] - 1, 0, 7] = math.inf
+        rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), again)
+        want = out.clone()
+        want[lq[0] - 1, :nh // nkv, 7] = math.inf
+        assert torch.equal(want.isinf(), again.isinf()) and not bool(again[:lq[0]].isnan().any())
+        fine = torch.isfinite(want)
+        assert float((again - out)[fine].float().abs().max()) <= 4 * half_step(t) * float(v[:lk[0]].nan_to_num(0, 0, 0).abs().max())
+
+
+@pytest.mark.gpu
 def test_attention_packed_bad_row_starts(rrr, ctx):
     q = normal(gen(1), 64, 2, 64, dtype=torch.float16)
     out = torch.full_like(q, 2.0)
