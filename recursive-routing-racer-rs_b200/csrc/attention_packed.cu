@@ -621,6 +621,80 @@ __device__ __forceinline__ void send4(uint32_t at, const uint32_t* v) {
                : "memory");
 }
 
+// The end of an item that a cluster shares, for one tile row (of ROWS in the CTA): m_own, l_own and
+// the row of O at oc are of this CTA's part (`some`: whether it has products). All threads of the
+// cluster pass three barriers.
+template <int HD, typename T, int ROWS>
+__device__ __forceinline__ void join_rows(const PackedParams& p, const Tile& t, uint8_t* qs, uint8_t* ring, int splits,
+                                          int rank, int at, bool some, bool mine, int row, int head, int all_seen,
+                                          float m_own, float l_own, uint32_t oc, int reach) {
+  // in every CTA, once the products of all are done: maxima and sums [part][row] and, of the first,
+  // what came out not finite [part][row] in Q's place; [part][4 columns][row] in the ring's
+  const int width = HD / splits;
+  float2* stats = reinterpret_cast<float2*>(qs);
+  int* bad_rows = reinterpret_cast<int*>(qs + 8 * ROWS * sizeof(float2));
+  cluster_barrier();
+  const bool sends = some && mine;
+  for (int c = 0; c < splits; ++c)
+    send2(in_cta(stats + rank * ROWS + at, c), sends ? m_own : -INFINITY, sends ? l_own : 0.f);
+  if (some)
+    for (int c = 0; c < HD; c += 16) {
+      uint32_t v[16];
+      tmem_ld16(oc + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const int to = (c + k) / width, four = (c + k) % width / 4;
+        if (sends) send4(in_cta(ring + ((size_t)(rank * (width / 4) + four) * ROWS + at) * 16, to), v + k);
+      }
+    }
+  cluster_barrier();
+  float top = -INFINITY, sum = 0.f;
+  for (int c = 0; c < splits; ++c) top = fmaxf(top, stats[c * ROWS + at].x);
+  const float use = top == -INFINITY ? 0.f : top;
+  for (int c = 0; c < splits; ++c) sum = fmaf(ex2(stats[c * ROWS + at].x - use), stats[c * ROWS + at].y, sum);
+  const float inv = all_seen > 0 ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head + rank * width;
+  bool bad = false;
+  for (int e = 0; e < width; e += 8) {
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < splits; ++c) {
+      const float m = stats[c * ROWS + at].x;
+      if (m == -INFINITY) continue;  // (nothing was sent, or nothing but zeros)
+      const float w = ex2(m - use);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(ring + ((size_t)(c * (width / 4) + e / 4 + k) * ROWS + at) * 16);
+        o[4 * k] = fmaf(w, x.x, o[4 * k]);
+        o[4 * k + 1] = fmaf(w, x.y, o[4 * k + 1]);
+        o[4 * k + 2] = fmaf(w, x.z, o[4 * k + 2]);
+        o[4 * k + 3] = fmaf(w, x.w, o[4 * k + 3]);
+      }
+    }
+    uint32_t packed[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = all_seen > 0 ? o[2 * k] * inv : 0.f, b = all_seen > 0 ? o[2 * k + 1] * inv : 0.f;
+      bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
+      packed[k] = Mma<T>::pack(a, b);
+    }
+    if (mine) *reinterpret_cast<uint4*>(dst + e) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  }
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(in_cta(bad_rows + rank * ROWS + at, 0)), "r"((int)bad) : "memory");
+  cluster_barrier();
+  if (rank == 0) {
+    for (int c = 0; c < splits; ++c) bad |= bad_rows[c * ROWS + at] != 0;
+    unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
+    while (again) {
+      const int who = __ffs(again) - 1;
+      again &= again - 1;
+      __syncwarp();
+      slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, head, who),
+                      reach);
+    }
+  }
+}
+
 template <int HD, typename T, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -872,71 +946,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (ok && i * tp.tokens < rows)
         write_row<HD, T>(p, t, oc, blocks[i] > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees[i] + 15) & ~15));
     } else {
-      // in every CTA, once the products of all are done: maxima and sums [part][row] and, of the first,
-      // what came out not finite [part][row] in Q's place; [part][4 columns][row] in the ring's
-      const int at = threadIdx.x, width = HD / splits;
-      float2* stats = reinterpret_cast<float2*>(qs);
-      int* bad_rows = reinterpret_cast<int*>(qs + 8 * 256 * sizeof(float2));
-      cluster_barrier();
-      const bool some = ok && blocks[i] > 0, sends = some && mine;
-      for (int c = 0; c < splits; ++c)
-        send2(in_cta(stats + rank * 256 + at, c), sends ? rs.m : -INFINITY, sends ? rs.l.x + rs.l.y : 0.f);
-      if (some)
-        for (int c = 0; c < HD; c += 16) {
-          uint32_t v[16];
-          tmem_ld16(oc + c, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 16; k += 4) {
-            const int to = (c + k) / width, four = (c + k) % width / 4;
-            if (sends) send4(in_cta(ring + ((size_t)(rank * (width / 4) + four) * 256 + at) * 16, to), v + k);
-          }
-        }
-      cluster_barrier();
-      float top = -INFINITY, sum = 0.f;
-      for (int c = 0; c < splits; ++c) top = fmaxf(top, stats[c * 256 + at].x);
-      const float use = top == -INFINITY ? 0.f : top;
-      for (int c = 0; c < splits; ++c) sum = fmaf(ex2(stats[c * 256 + at].x - use), stats[c * 256 + at].y, sum);
-      const float inv = all_seen > 0 ? 1.f / sum : 0.f;
-      T* dst = static_cast<T*>(p.out) + row * p.out_row + (int64_t)head * p.out_head + rank * width;
-      bool bad = false;
-      for (int e = 0; e < width; e += 8) {
-        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int c = 0; c < splits; ++c) {
-          const float m = stats[c * 256 + at].x;
-          if (m == -INFINITY) continue;  // (nothing was sent, or nothing but zeros)
-          const float w = ex2(m - use);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(ring + ((size_t)(c * (width / 4) + e / 4 + k) * 256 + at) * 16);
-            o[4 * k] = fmaf(w, x.x, o[4 * k]);
-            o[4 * k + 1] = fmaf(w, x.y, o[4 * k + 1]);
-            o[4 * k + 2] = fmaf(w, x.z, o[4 * k + 2]);
-            o[4 * k + 3] = fmaf(w, x.w, o[4 * k + 3]);
-          }
-        }
-        uint32_t packed[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = all_seen > 0 ? o[2 * k] * inv : 0.f, b = all_seen > 0 ? o[2 * k + 1] * inv : 0.f;
-          bad |= !(fabsf(a) <= 3.402823466e38f) || !(fabsf(b) <= 3.402823466e38f);
-          packed[k] = Mma<T>::pack(a, b);
-        }
-        if (mine) *reinterpret_cast<uint4*>(dst + e) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      }
-      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(in_cta(bad_rows + rank * 256 + at, 0)), "r"((int)bad) : "memory");
-      cluster_barrier();
-      if (rank == 0) {
-        for (int c = 0; c < splits; ++c) bad |= bad_rows[c * 256 + at] != 0;
-        unsigned again = __ballot_sync(0xffffffffu, doubtful(bad, sum) && mine);
-        while (again) {
-          const int who = __ffs(again) - 1;
-          again &= again - 1;
-          __syncwarp();
-          slow_row<HD, T>(p, t, __shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, head, who),
-                          min(t.k1 - t.k0, (all_sees[i] + 15) & ~15));
-        }
-      }
+      join_rows<HD, T, 256>(p, t, qs, ring, splits, rank, threadIdx.x, ok && blocks[i] > 0, mine, row, head, all_seen,
+                            rs.m, rs.l.x + rs.l.y, oc, min(t.k1 - t.k0, (all_sees[i] + 15) & ~15));
     }
     tc_fence_before();
   }
@@ -965,7 +976,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // mma.sync kernel above took 2622 us.
 constexpr int kWideThreads = 192;  // warps 0-3 softmax, 4 products, 5 copies
 
-template <typename T>
+template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1)
     packed_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcParams tp) {
@@ -997,11 +1008,21 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   pdl_wait();
   Tile t;
   const int nkv = p.nh / p.hpk;
-  if (!find_tile(p, tp.tokens, (int)((gridDim.x - 1 - blockIdx.x) / nkv), t)) return;
+  const int splits = SPLIT ? tp.splits : 1, rank = SPLIT ? blockIdx.x % splits : 0;
+  const int tile = blockIdx.x / splits, tiles = gridDim.x / splits;
+  if (!find_tile(p, tp.tokens, (tiles - 1 - tile) / nkv, t)) return;
   if (warp == 4) tmem_alloc(&tmem_slot, 512);
-  const int kv = blockIdx.x % nkv;
-  const int rows = min(tp.tokens, t.q1 - t.row0), lk = t.k1 - t.k0;
-  const int sees = seen_by(p, t, t.row0 + rows - 1);  // KV rows that the last row sees
+  const int kv = tile % nkv;
+  const int rows = min(tp.tokens, t.q1 - t.row0);
+  const int all_sees = seen_by(p, t, t.row0 + rows - 1);  // KV rows that the last row sees
+  int from = 0, most = INT32_MAX;                         // those that this CTA takes
+  if constexpr (SPLIT) {
+    const int all = (all_sees + kTile - 1) / kTile;
+    from = all * rank / splits * kTile;
+    most = all * (rank + 1) / splits * kTile - from;
+  }
+  auto part = [&](int seen) { return SPLIT ? max(0, min(seen - from, most)) : seen; };
+  const int sees = part(all_sees), lk = t.k1 - t.k0 - from;  // lk: rows of the sequence from there on
   const int n = (sees + kTile - 1) / kTile;
 
   // tile rows past the last whole query row: zeros, so that their scores are
@@ -1011,6 +1032,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if constexpr (SPLIT) cluster_barrier();  // every CTA has begun
   const uint32_t tmem = tmem_slot, o_col = tmem + 2 * kTile;
   auto wait = [&](uint64_t* bar, int use) {  // the use-th completion of a barrier
     if (warp_wait(bar, (uint32_t)use & 1u, p.err)) return true;
@@ -1045,7 +1067,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         mbar_arrive_expect_tx(&full[st], kStage);
         for (int c = 0; c < 2; ++c)
           tma_load_3d(ring + (size_t)st * kStage + c * kPiece, is_v(u) ? &vmap : &kmap, 128 * half + 64 * c, kv,
-                      t.k0 + block_of(u) * kTile, &full[st]);
+                      t.k0 + from + block_of(u) * kTile, &full[st]);
       }
       __syncwarp();
     }
@@ -1109,7 +1131,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     // ---------------- softmax: thread r = row r
     const int r = threadIdx.x, token = r / p.hpk, head = kv * p.hpk + r % p.hpk, row = t.row0 + token;
     const bool mine = token < tp.tokens && token < rows;
-    const int seen = mine ? seen_by(p, t, row) : 0;
+    const int all_seen = mine ? seen_by(p, t, row) : 0, seen = part(all_seen);
     const int open = mine ? seen : INT32_MAX;  // tile rows of no query mask nothing
     const int all_see = (int)__reduce_min_sync(0xffffffffu, (unsigned)open);
     const int none_sees = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);
@@ -1122,14 +1144,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       if (!ok) break;
       tc_fence_after();
       if (lk % kTile != 0 && j == end_block) {  // V rows behind the sequence; j is n - 1
-        const int from = lk - j * kTile;
+        const int left = lk - j * kTile;
         for (int half = 0; half < 2 && ok; ++half) {
           const int item = 4 * n - 2 + half;
           ok = wait(&full[item % kStages], item / kStages);
           uint8_t* v = ring + (size_t)(item % kStages) * kStage;
           for (int c = 0; c < 2 && ok; ++c)
-            for (int k = r; k < (kTile - from) * 8; k += 128)
-              *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)from * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+            for (int k = r; k < (kTile - left) * 8; k += 128)
+              *reinterpret_cast<uint4*>(v + c * kPiece + (size_t)left * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
         }
         if (!ok) break;
         fence_proxy_async_smem();
@@ -1145,15 +1167,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full);
     }
-    if (ok) {
-      if (n > 0) ok = wait(&o_full, 0);
-      if (ok) {
-        tc_fence_after();
-        write_row<HD, T>(p, t, o_col + sub, n > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees + 15) & ~15));
-      }
-      tc_fence_before();
+    if (ok && n > 0) ok = wait(&o_full, 0);
+    tc_fence_after();
+    if constexpr (SPLIT) {
+      join_rows<HD, T, 128>(p, t, qs, ring, splits, rank, r, ok && n > 0, mine, row, head, all_seen, rs.m,
+                            rs.l.x + rs.l.y, o_col + sub, min(t.k1 - t.k0, (all_sees + 15) & ~15));
+    } else if (ok) {
+      write_row<HD, T>(p, t, o_col + sub, n > 0, mine, row, head, seen, rs.l.x + rs.l.y, min(lk, (sees + 15) & ~15));
     }
+    tc_fence_before();
   }
+  if constexpr (SPLIT)
+    if (warp >= 4)
+      for (int k = 0; k < 3; ++k) cluster_barrier();
 
   tc_fence_before();
   __syncthreads();
@@ -1181,6 +1207,14 @@ bool encode_heads(CUtensorMap* map, int type, const void* base, int hd, int64_t 
 // Query rows of a CTA of the tcgen05 kernels
 int rows_per_cta(int hd, int hpk) { return (hd == 256 ? 1 : 2) * (kTile / hpk); }
 
+template <int HD, typename T, bool SPLIT>
+auto tc_kernel() {
+  if constexpr (HD == 256)
+    return &packed_wide_kernel<T, SPLIT>;
+  else
+    return &packed_tc_kernel<HD, T, SPLIT>;
+}
+
 template <int HD, typename T>
 cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
   TcParams tp{};
@@ -1199,42 +1233,35 @@ cudaError_t launch_tc(const LaunchEnv& env, int type, const PackedParams& p) {
     return cudaErrorInvalidValue;
   // nkv times the slots fits the grid: the caller's check
   const dim3 grid((unsigned)(nkv * (p.q_rows / rows_per_cta(HD, p.hpk) + p.n_seqs)));
-  if constexpr (HD == 256) {
-    const int smem = 7 * kTile * 128 * 2 + 1024;  // Q's two halves and five stages
-    auto kern = packed_wide_kernel<T>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    return rrr_launch_pdl(kern, grid, dim3(kWideThreads), (size_t)smem, env.stream, env.pdl, qmap, kmap, vmap, tp);
-  } else {
-    const int smem = (2 + tc_stages<HD>()) * kTile * HD * 2 + 1024;
-    // Few tiles with many blocks of KV rows (of the mean sequence) go to clusters. Joining costs 3 to 5
-    // us, and no more than some 9 clusters of 8 such CTAs run at once: 1 row of 24 heads on 9,000 rows
-    // 123 us alone, 75, 44 and 28 by 2, 4 and 8 CTAs; 100 rows on 2,000 36.5, 32, 24 and, in two rounds,
-    // 36; 1,000 on 1,000 with 8 heads on 2 23, 24.5 and 20.6; 500 rows on 500 16 and 20.
-    const int64_t deep = (p.kv_rows / p.n_seqs + kTile - 1) / kTile;
-    tp.splits = 1;
-    for (const int by : {8, 4, 2}) {
-      if ((int64_t)grid.x * by > (by == 8 ? env.sm_count / 2 : env.sm_count) || deep < (by == 2 ? 12 : 2 * by)) continue;
-      tp.splits = by;
-      break;
-    }
-    auto kern = tp.splits > 1 ? packed_tc_kernel<HD, T, true> : packed_tc_kernel<HD, T, false>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = env.pdl ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim = {(unsigned)tp.splits, 1, 1};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid.x * tp.splits);
-    cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = env.stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = tp.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, qmap, kmap, vmap, tp);
+  // Few tiles with many blocks of KV rows (of the mean sequence) go to clusters. Joining costs 3 to 5
+  // us, and no more than some 9 clusters of 8 such CTAs run at once: 1 row of 24 heads on 9,000 rows
+  // 123 us alone, 75, 44 and 28 by 2, 4 and 8 CTAs; 100 rows on 2,000 36.5, 32, 24 and, in two rounds,
+  // 36; 1,000 on 1,000 with 8 heads on 2 23, 24.5 and 20.6; 500 rows on 500 16 and 20 (128 values;
+  // with 256 1 row on 9,000 126 and 34).
+  const int64_t deep = (p.kv_rows / p.n_seqs + kTile - 1) / kTile;
+  tp.splits = 1;
+  for (const int by : {8, 4, 2}) {
+    if ((int64_t)grid.x * by > (by == 8 ? env.sm_count / 2 : env.sm_count) || deep < (by == 2 ? 12 : 2 * by)) continue;
+    tp.splits = by;
+    break;
   }
+  const int smem = (HD == 256 ? 7 * kTile * 128 : (2 + tc_stages<HD>()) * kTile * HD) * 2 + 1024;
+  auto kern = tp.splits > 1 ? tc_kernel<HD, T, true>() : tc_kernel<HD, T, false>();
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = env.pdl ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)tp.splits, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid.x * tp.splits);
+  cfg.blockDim = dim3(HD == 256 ? kWideThreads : kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = env.stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = tp.splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, qmap, kmap, vmap, tp);
 }
 
 template <int HD, typename T>
