@@ -11,6 +11,10 @@
 // Where a tile begins. Tile x of the grid belongs to the last sequence s with floor(cu[s] /
 // rows) + s <= x and starts at its row cu[s] + rows * (x - floor(cu[s] / rows) - s): sequences
 // get disjoint runs of x that are long enough; a warp searches 32 sequences at a time.
+//
+// Which kernel. packed_tc_kernel: head_dim 64 and 128, two tiles of 128 (row, head) pairs per CTA.
+// packed_wide_kernel: head_dim 256, one tile. Both share the KV rows of an item among the CTAs of a
+// cluster where there are few items. packed_kernel (mma.sync): what neither can describe.
 #include <math.h>
 
 #include "serve_common.cuh"

@@ -1,7 +1,7 @@
 // kv4.cuh — the page layout of the 4-bit KV cache (rrr_kv4_cache) shared by the kernels that
 // write it, read it back and attend over it. Offsets in bytes inside the block of one (page,
 // KV head); the order of the codes is the order in which lane (g, t) = (lane / 4, lane % 4)
-// of a warp feeds them to mma.m16n8k16 as B operands (kv4_attention.cu).
+// of a warp feeds them to mma.m16n8k16 as A operands (kv4_attention.cu).
 #pragma once
 #include "serve_common.cuh"
 

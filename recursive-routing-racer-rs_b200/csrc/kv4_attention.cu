@@ -31,13 +31,14 @@
 // more in front, which is what beginning and ending one costs. The CTAs share all U units of the
 // batch evenly, in order, whatever the lengths are (read on the device): CTA c of G takes the
 // pages in [c U / G, (c+1) U / G). (Without the units in front, the CTA with the most short
-// sequences took 137 us of the batch of 64, the middle one 103; with them all take 118.) One producer warp streams the pages' blocks, each one
-// contiguous, with bulk copies into a ring of stages, the segment's query row with its first
-// page; four consumer warps take 16 rows of a page each and keep their own softmax state. At
-// the end of a (sequence, head) segment the warps' states are joined in order; a segment that
-// other CTAs share goes to the workspace, and a second small kernel joins the parts in order. (The
-// CTA that finishes last did that first, found by a counter: 6 of 14 us at one short sequence,
-// most of it instructions that no SM had executed before, by one CTA per head.)
+// sequences took 137 us of the batch of 64, the middle one 103; with them all took 118.) One
+// producer warp streams the pages' blocks, each one contiguous, with bulk copies into a ring of
+// stages, the segment's query row with its first page; four consumer warps take 16 rows of a page
+// each and keep their own softmax state. At the end of a (sequence, head) segment the warps' states
+// are joined in order; a segment that other CTAs share goes to the workspace, and a second small
+// kernel joins the parts in order. (The CTA that finishes last did that first, found by a counter:
+// 6 of 14 us at one short sequence, most of it instructions that no SM had executed before, by one
+// CTA per head.)
 #include <math.h>
 
 #include "kv4.cuh"

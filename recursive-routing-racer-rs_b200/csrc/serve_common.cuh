@@ -1,7 +1,7 @@
 // serve_common.cuh — pieces shared by the packed-batch operators (qk_rows.cu, kv4_rows.cu,
 // kv4_attention.cu, attention_packed.cu): element types, vector loads and stores of a lane's
-// values, the sequence of a packed row, the argument rules that they share, and the current
-// device's guard of their entry points.
+// values, the argument rules that they share, and the current device's guard of their entry
+// points.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -59,20 +59,6 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) u.v[i] = from_f32<T>(x[i]);
   *reinterpret_cast<Words<N * (int)sizeof(T)>*>(p) = u.raw;
-}
-
-// The sequence s with cu[s] <= row < cu[s + 1] of n, -1 when there is none. cu ascends; what
-// it holds otherwise, the search stays inside it.
-__device__ __forceinline__ int seq_of_row(const int* __restrict__ cu, int n, int row) {
-  int lo = 0, hi = n;  // the first index whose cu is above the row lies in (lo, hi]
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid + 1] > row)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo < n && cu[lo] <= row ? lo : -1;
 }
 
 __device__ __forceinline__ void flag_position(int* err) {
