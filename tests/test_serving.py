@@ -854,6 +854,27 @@ def test_attention_packed_bad_row_starts(rrr, ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_packed_shared_items_on_two_streams_and_with_bad_row_starts(rrr, ctx, hd):
+    g, t = gen(hd), torch.float16
+    q, k, v = (normal(g, n, 2, hd, dtype=t) for n in (50, 3000, 3000))
+    out = torch.full_like(q, 2.0)
+    for cu_q, cu_kv in (([0, 51], [0, 3000]), ([0, 50], [0, 3001]), ([5, 3], [0, 3000]), ([-1, 50], [0, 3000]), ([0, 50], [9, 3])):
+        rrr.attention_packed(ctx, q, k, v, ints(cu_q), ints(cu_kv), out)
+        assert ctx.device_error() == 6 and bool((out == 2).all())
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], [torch.empty_like(q) for _ in range(3)]
+    cq, ck = ints([0, 50]), ints([0, 3000])
+    rrr.attention_packed(ctx, q, k, v, cq, ck, out)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, o in zip(streams, outs):
+            rrr.attention_packed(ctx, q, k, v, cq, ck, o, stream=s)
+    torch.cuda.synchronize()
+    check_packed(out, q, k, v, [50], [3000], True, 1 / math.sqrt(hd))
+    assert all(torch.equal(o, out) for o in outs) and ctx.device_error() == 0
+
+
+@pytest.mark.gpu
 def test_attention_packed_large_scores(rrr, ctx):
     """Scores in the thousands: the running maximum keeps every weight at or below one."""
     g, lens = gen(2), [300]
