@@ -763,7 +763,9 @@ cudaError_t launch(const LaunchEnv& env, Kv4Params p) {
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = p.stages * p.stage_bytes + join;
   auto kern = kv4_attention_kernel<HD, NT, T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // The attribute is the function's on the device, whatever context or thread calls: one value for
+  // every number of query heads, so that no call takes back what another is about to launch with
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
   if (e != cudaSuccess) return e;
   const int64_t units = (int64_t)p.n_seqs * p.nkv * ((p.max_pages > 0 ? p.max_pages : 1) + kStart);
   const int ctas = env.sm_count * kCtas;
