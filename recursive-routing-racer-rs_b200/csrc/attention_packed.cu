@@ -1318,20 +1318,23 @@ extern "C" int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, cons
   if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16) ||
       !aligned_to(cu_q, 4) || !aligned_to(cu_kv, 4))
     return set_error(ctx, RRR_ERR_MISALIGNED, "%s: q, k, v and out must be 16-byte aligned", fn);
-  // out: rows of heads or heads of rows, without two elements in one place, apart from the inputs
-  const int64_t nh = d->n_heads;
-  if (!(d->out_row >= (nh - 1) * d->out_head + hd || d->out_head >= (d->q_rows - 1) * d->out_row + hd))
+  // out: rows of heads or heads of rows, without two elements in one place, apart from the inputs.
+  // (2^30 rows of 2^38 elements: extents take more than 64 bits)
+  using Wide = __int128;
+  const int64_t nh = d->n_heads, kvh = d->n_kv_heads;
+  if (!(d->out_row >= (nh - 1) * d->out_head + hd || d->out_head >= (Wide)(d->q_rows - 1) * d->out_row + hd))
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows and heads of out overlap", fn);
-  auto extent = [&](int64_t rows, int64_t row, int64_t heads, int64_t head) {
-    return rows < 1 ? (int64_t)0 : 2 * ((rows - 1) * row + (heads - 1) * head + hd);
+  struct Range {
+    Wide from, end;
   };
-  const int64_t kvh = d->n_kv_heads;
-  const RowSet parts[4] = {{out, 0, extent(d->q_rows, d->out_row, nh, d->out_head), 1},
-                           {q, 0, extent(d->q_rows, d->q_row, nh, d->q_head), 1},
-                           {k, 0, extent(d->kv_rows, d->k_row, kvh, d->k_head), 1},
-                           {v, 0, extent(d->kv_rows, d->v_row, kvh, d->v_head), 1}};
-  for (int i = 1; i < 4; ++i)
-    if (!rows_disjoint(parts[0], parts[i]))
+  auto range = [&](const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head) {
+    const Wide at = reinterpret_cast<uintptr_t>(p);
+    return Range{at, rows < 1 ? at : at + 2 * ((Wide)(rows - 1) * row + (heads - 1) * head + hd)};
+  };
+  const Range mine = range(out, d->q_rows, d->out_row, nh, d->out_head);
+  for (const Range& in : {range(q, d->q_rows, d->q_row, nh, d->q_head), range(k, d->kv_rows, d->k_row, kvh, d->k_head),
+                          range(v, d->kv_rows, d->v_row, kvh, d->v_head)})
+    if (std::max(mine.from, in.from) < std::min(mine.end, in.end))
       return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: out overlaps an input", fn);
   const int64_t hpk = nh / kvh, per = hpk <= kTile ? rows_per_cta(hd, (int)hpk) : 1;
   if (kvh * (d->q_rows / per + d->n_seqs) > INT32_MAX)

@@ -1,5 +1,5 @@
-"""The packed-batch operators where a plain comparison of random values sees little: calls of two
-host threads. Formulas and helpers are test_serving.py's."""
+"""The packed-batch operators where a plain comparison of random values sees little: arrays that
+share a buffer, calls of two host threads. Formulas and helpers are test_serving.py's."""
 import ctypes
 import os
 import subprocess
@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from test_serving import ROOT, filled, gen, ints, normal
+from test_serving import FINE, ROOT, _no_gpu, filled, gen, host_ctx, ints, normal  # noqa: F401
 
 
 class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
@@ -17,6 +17,36 @@ class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
                 ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)]
 
 
+# ------------------------------------------------------------------ CPU
+def packed_call(rrr, host_ctx, over):
+    """rrr_attention_packed of 9 rows of 4 heads on 11 of 2 heads of 128, with made-up addresses."""
+    a = dict(type=30, nh=4, nkv=2, hd=128, n_seqs=2, causal=1, scale=0.0, q_rows=9, kv_rows=11, q_row=512, q_head=128,
+             k_row=256, k_head=128, v_row=256, v_head=128, out_row=512, out_head=128, q=1 << 20, k=2 << 20, v=4 << 20,
+             out=8 << 20)
+    a.update(over)
+    d = rrr.ffi.PackedDesc(*(a[f] for f in ("type", "nh", "nkv", "hd", "n_seqs", "causal", "scale", "q_rows", "kv_rows",
+                                            "q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
+                                            "out_head")))
+    return rrr.ffi.lib().rrr_attention_packed(host_ctx, ctypes.byref(d), a["q"], a["k"], a["v"], 256, 512, a["out"], None)
+
+
+FAR = 1 << 38  # the longest stride
+
+
+@pytest.mark.parametrize("over,code", [
+    # 2^29 rows of 2^38 elements end at 2^68 bytes: out begins at one of q's rows, or between them
+    (dict(q_rows=(1 << 29) + 1, q_row=FAR, out_row=FAR, out=(1 << 20) + 10 * FAR), -1),
+    (dict(kv_rows=(1 << 29) + 1, k_row=FAR, out=(2 << 20) + 6 * FAR), -1),
+    (dict(kv_rows=(1 << 29) + 1, v_row=FAR, out=(4 << 20) + 6 * FAR), -1),
+    # rows of out that reach its next head after 2^64 elements
+    (dict(q_rows=(1 << 28) + 1, out_row=FAR // 4, out_head=FAR), -3),
+])
+def test_attention_packed_extents_past_64_bits(rrr, host_ctx, over, code):
+    _no_gpu()
+    assert packed_call(rrr, host_ctx, over) == code
+
+
+# ------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_attention_kv4_two_threads_with_a_context_each(rrr, ctx, hd, tmp_path):
