@@ -1208,6 +1208,33 @@ bool encode_heads(CUtensorMap* map, int type, const void* base, int hd, int64_t 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of heads of hd 16-bit values; strides in elements.
+struct HeadRows {
+  const void* p;
+  int64_t rows, row, heads, head, hd;
+};
+// Whether two such arrays share no byte, for certain: their extents do not meet, or all of their
+// places lie apart modulo a stride (both in one buffer whose rows or heads hold a part of each).
+bool apart(const HeadRows& a, const HeadRows& b) {
+  using Wide = __int128;
+  if (a.rows < 1 || b.rows < 1) return true;
+  auto from = [](const HeadRows& x) { return (Wide) reinterpret_cast<uintptr_t>(x.p); };
+  // bytes from the first place to the end of the last, where multiples of m elements do not count
+  auto width = [](const HeadRows& x, int64_t m) {
+    Wide w = x.hd;
+    if (m == 0 || x.row % m) w += (Wide)(x.rows - 1) * x.row;
+    if (m == 0 || x.head % m) w += (Wide)(x.heads - 1) * x.head;
+    return 2 * w;
+  };
+  const Wide between = from(b) - from(a);
+  if (between >= width(a, 0) || -between >= width(b, 0)) return true;
+  for (const int64_t m : {a.row, a.head, b.row, b.head}) {
+    const Wide period = 2 * (Wide)m, off = (between % period + period) % period;
+    if (off >= width(a, m) && off + width(b, m) <= period) return true;
+  }
+  return false;
+}
+
 // Query rows of a CTA of the tcgen05 kernels
 int rows_per_cta(int hd, int hpk) { return (hd == 256 ? 1 : 2) * (kTile / hpk); }
 
@@ -1324,18 +1351,11 @@ extern "C" int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, cons
   const int64_t nh = d->n_heads, kvh = d->n_kv_heads;
   if (!(d->out_row >= (nh - 1) * d->out_head + hd || d->out_head >= (Wide)(d->q_rows - 1) * d->out_row + hd))
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: rows and heads of out overlap", fn);
-  struct Range {
-    Wide from, end;
-  };
-  auto range = [&](const void* p, int64_t rows, int64_t row, int64_t heads, int64_t head) {
-    const Wide at = reinterpret_cast<uintptr_t>(p);
-    return Range{at, rows < 1 ? at : at + 2 * ((Wide)(rows - 1) * row + (heads - 1) * head + hd)};
-  };
-  const Range mine = range(out, d->q_rows, d->out_row, nh, d->out_head);
-  for (const Range& in : {range(q, d->q_rows, d->q_row, nh, d->q_head), range(k, d->kv_rows, d->k_row, kvh, d->k_head),
-                          range(v, d->kv_rows, d->v_row, kvh, d->v_head)})
-    if (std::max(mine.from, in.from) < std::min(mine.end, in.end))
-      return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: out overlaps an input", fn);
+  const HeadRows mine{out, d->q_rows, d->out_row, nh, d->out_head, hd};
+  for (const HeadRows& in : {HeadRows{q, d->q_rows, d->q_row, nh, d->q_head, hd},
+                             HeadRows{k, d->kv_rows, d->k_row, kvh, d->k_head, hd},
+                             HeadRows{v, d->kv_rows, d->v_row, kvh, d->v_head, hd}})
+    if (!apart(mine, in)) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: out overlaps an input", fn);
   const int64_t hpk = nh / kvh, per = hpk <= kTile ? rows_per_cta(hd, (int)hpk) : 1;
   if (kvh * (d->q_rows / per + d->n_seqs) > INT32_MAX)
     return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many rows, sequences and heads for one call", fn);

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 import torch
 
-from test_serving import FINE, ROOT, _no_gpu, filled, gen, host_ctx, ints, normal  # noqa: F401
+from test_serving import FINE, ROOT, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal  # noqa: F401
 
 
 class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
@@ -46,7 +46,58 @@ def test_attention_packed_extents_past_64_bits(rrr, host_ctx, over, code):
     assert packed_call(rrr, host_ctx, over) == code
 
 
+Q = 1 << 20
+
+
+@pytest.mark.parametrize("over,code", [
+    # rows of [q | out]; heads of [q | out]; the same where heads are the outer dimension
+    (dict(q_row=1024, out_row=1024, out=Q + 2 * 512), FINE),
+    (dict(q_row=1024, out_row=1024, out=Q + 2 * 520), -1),
+    (dict(q_row=1024, out_row=1024, out=Q + 2 * 504), -1),
+    (dict(q_row=1024, q_head=256, out_row=1024, out_head=256, out=Q + 2 * 128), FINE),
+    (dict(q_row=1024, q_head=256, out_row=1024, out_head=256, out=Q + 2 * 120), -1),
+    (dict(q_row=256, q_head=9 * 256, out_row=256, out_head=9 * 256, out=Q + 2 * 128), FINE),
+    (dict(q_row=256, q_head=9 * 256, out_row=256, out_head=9 * 256, out=Q + 2 * 136), -1),
+    # out's first row lies beside a later one of q, or across two of them
+    (dict(q_row=1024, out_row=1024, out=Q + 2 * (3 * 1024 + 512)), FINE),
+    (dict(q_row=1024, out_row=1024, out=Q + 2 * (3 * 1024 + 768)), -1),
+    (dict(q_row=1024, out_row=1024, out=Q - 2 * (3 * 1024 - 512)), FINE),
+    # one buffer of [q | k | v | out] rows
+    (dict(q_row=1536, k_row=1536, v_row=1536, out_row=1536, k=Q + 1024, v=Q + 1536, out=Q + 2048), FINE),
+    (dict(q_row=1536, k_row=1536, v_row=1536, out_row=1536, k=Q + 1024, v=Q + 1536, out=Q + 2032), -1),
+    # pitches that are multiples of each other, or not; one row, whose pitch is free
+    (dict(q_row=2048, out_row=1024, out=Q + 2 * 512), FINE),
+    (dict(q_row=1024, out_row=2048, out=Q + 2 * 512), FINE),
+    (dict(q_row=1024, out_row=1032, out=Q + 2 * 512), -1),
+    (dict(q_rows=1, q_row=1032, out_row=1024, out=Q + 2 * 512), FINE),
+    # what has no element overlaps nothing
+    (dict(q_rows=0, out=Q), FINE),
+    (dict(kv_rows=0, k=(8 << 20) + 256, v=(8 << 20) + 512), FINE),
+])
+def test_attention_packed_arrays_that_interleave(rrr, host_ctx, over, code):
+    _no_gpu()
+    assert packed_call(rrr, host_ctx, over) == code, rrr.ffi.last_error(host_ctx)
+
+
 # ------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["rows", "heads"])
+def test_attention_packed_rows_of_inputs_and_output(rrr, ctx, order):
+    """One buffer of [q | k | v | out] rows, or of heads of such rows: the bits of separate arrays, and
+    nothing else written."""
+    nh, nkv, hd, lens, t = 4, 2, 128, [100, 257], torch.bfloat16
+    rows, heads = sum(lens), 2 * nh + 2 * nkv
+    x = normal(gen(5), *((rows, heads, hd) if order == "rows" else (heads, rows, hd)), dtype=t)
+    whole = x if order == "rows" else x.transpose(0, 1)
+    q, k, v, out = whole.split([nh, nkv, nkv, nh], 1)
+    cu, apart, before = cu_of(lens), torch.empty(rows, nh, hd, dtype=t, device="cuda"), x.clone()
+    rrr.attention_packed(ctx, *(y.contiguous() for y in (q, k, v)), cu, cu, apart)
+    rrr.attention_packed(ctx, q, k, v, cu, cu, out)
+    assert torch.equal(out, apart) and ctx.device_error() == 0
+    out.copy_((before if order == "rows" else before.transpose(0, 1))[:, -nh:])
+    assert torch.equal(x, before)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_attention_kv4_two_threads_with_a_context_each(rrr, ctx, hd, tmp_path):
