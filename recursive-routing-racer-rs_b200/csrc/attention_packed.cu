@@ -442,6 +442,8 @@ __device__ __forceinline__ void store_32(void* p, const uint32_t (&a)[4], const 
 template <typename T>
 struct RowSoftmax {
   float scale;
+  bool mine;  // whether it is a query row of the tile's sequence: the others, of the next sequence or
+              // of none, hold anything and have no vote (nor are their weights anyone's concern)
   float m;   // the maximum of the scaled scores, as of the last rescale
   float2 l;  // the weights' sum, of even and odd columns
   // the weights of 32 scores under the maximum m, stored over S as columns 32 part .. + 31; their
@@ -474,8 +476,8 @@ struct RowSoftmax {
   // scale_o(alpha) does that to the products so far.
   template <class F>
   __device__ __forceinline__ bool rescale(float m_new, F&& scale_o) {
-    if (!__any_sync(0xffffffffu, m_new > m + kLazy)) return false;
-    const bool grow = m_new > m;
+    if (!__any_sync(0xffffffffu, mine && m_new > m + kLazy)) return false;
+    const bool grow = mine && m_new > m;
     const float next = grow ? m_new : m;
     const float alpha = grow ? ex2(m - next) : 1.f;
     m = next;
@@ -904,7 +906,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int end_block = (lk - 1) / kTile;
     const bool zeroes = lk % kTile != 0 && i == (blocks[0] > end_block ? 0 : 1);
     const bool frees = i == (blocks[1] > 0 ? 1 : 0);  // the tile whose products come last
-    RowSoftmax<T> rs{p.scale, -INFINITY, make_float2(0.f, 0.f)};
+    RowSoftmax<T> rs{p.scale, mine, -INFINITY, make_float2(0.f, 0.f)};
     bool ok = true;
     for (int j = 0; j < blocks[i]; ++j) {
       if (!warp_wait(&s_full[i], (uint32_t)j & 1u, p.err)) {
@@ -1141,7 +1143,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const int none_sees = (int)__reduce_max_sync(0xffffffffu, (unsigned)seen);
     const uint32_t sub = (uint32_t)(32 * warp) << 16;
     const int end_block = (lk - 1) / kTile;
-    RowSoftmax<T> rs{p.scale, -INFINITY, make_float2(0.f, 0.f)};
+    RowSoftmax<T> rs{p.scale, mine, -INFINITY, make_float2(0.f, 0.f)};
     bool ok = true;
     for (int j = 0; j < n && ok; ++j) {
       ok = wait(&s_full[j & 1], j >> 1);

@@ -1,13 +1,14 @@
 """The packed-batch operators where a plain comparison of random values sees little: arrays that
 share a buffer, calls of two host threads. Formulas and helpers are test_serving.py's."""
 import ctypes
+import math
 import os
 import subprocess
 
 import pytest
 import torch
 
-from test_serving import FINE, ROOT, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal  # noqa: F401
+from test_serving import DT, FINE, ROOT, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal  # noqa: F401
 
 
 class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
@@ -96,6 +97,32 @@ def test_attention_packed_rows_of_inputs_and_output(rrr, ctx, order):
     assert torch.equal(out, apart) and ctx.device_error() == 0
     out.copy_((before if order == "rows" else before.transpose(0, 1))[:, -nh:])
     assert torch.equal(x, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("held,seqs", [(1100, 40), (2600, 1)])  # items of their own, and shared by clusters
+def test_attention_packed_bits_do_not_depend_on_the_rows_behind(rrr, ctx, hd, kind, held, seqs):
+    """A tile's last rows are the next sequence's queries, or rows of none: whatever those hold, and
+    however their scores grow, the sequence before keeps every bit."""
+    nh, nkv, t, lq = 6, 2, DT[kind], 23
+    g, rows = gen(hd), lq * seqs + 40
+    q, k, v = normal(g, rows, nh, hd, dtype=t), normal(g, held * seqs, nkv, hd, dtype=t), normal(g, held * seqs, nkv, hd, dtype=t)
+    # keys that grow, so that larger queries' scores do too
+    k *= torch.linspace(0.1, 1.5, held, device="cuda").repeat(seqs)[:, None, None].to(t)
+    cu_q, cu_kv = ints([lq * i for i in range(seqs + 1)]), ints([held * i for i in range(seqs + 1)])
+    outs = []
+    for fill in (0.0, 25.0, math.inf, math.nan):
+        x, out = q.clone(), torch.full_like(q, 3.0)
+        x[lq * seqs:] = x[lq * seqs:] * fill if math.isfinite(fill) else fill
+        for s in range(1, seqs, 2):  # every second sequence's queries
+            x[lq * s:lq * (s + 1)] = x[lq * s:lq * (s + 1)] * fill if math.isfinite(fill) else fill
+        rrr.attention_packed(ctx, x, k, v, cu_q, cu_kv, out)
+        assert bool((out[lq * seqs:] == 3).all())
+        outs.append(torch.stack([out[lq * s:lq * (s + 1)] for s in range(0, seqs, 2)]))
+    assert bool(torch.isfinite(outs[0]).all())
+    assert all(torch.equal(o, outs[0]) for o in outs[1:]) and ctx.device_error() == 0
 
 
 @pytest.mark.gpu
