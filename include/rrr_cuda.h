@@ -447,7 +447,8 @@ int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_
  * query heads per KV head; scale 0 = 1/sqrt(head_dim). q, out: rows of n_heads*head_dim values
  * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros, and so does one whose
  * kv_lens is out of range; rows on pages that do not exist are left out. Scores and sums
- * carry 32-bit accuracy whatever the type. workspace: rrr_kv4_workspace bytes of device
+ * carry 32-bit accuracy whatever the type and the values' size; a weight times a group's d
+ * counts to 2^-22 of itself or 2^-35 of the largest weight times the largest d. workspace: rrr_kv4_workspace bytes of device
  * memory, whatever they hold; calls that can run at the same time, replays of captured
  * graphs among them, need one each. */
 int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t* bytes);

@@ -16,7 +16,11 @@
 // group j as (hi, lo), and the sums of p_i (m_ij + 8 d_ij) run beside it in f32. V's codes are
 // centred, code - 8: over a long context the weighted values nearly cancel, and sums of the codes
 // themselves would be hundreds of times the result (measured: an error of 1.2e-3 at 131,000 rows).
-// (8 rather than 7.5 because both nibbles of a byte can then be centred where they stand.) The
+// (8 rather than 7.5 because both nibbles of a byte can then be centred where they stand.) A weight
+// is 2^(s - ref) with ref below the running maximum by as much as brings the largest weight times the
+// largest step so far to 2^-1 (for larger steps ref is the maximum): a p d keeps 22 bits down to 2^-13
+// of that, and 2^-35 of it below, where f16 has no normal numbers. (Relative to the maximum, values of
+// 1e-4 behind a first row that draws the weight, as texts have, came out with 8 bits.) The
 // tensor core truncates its sums, so they are moved to shared memory, rounded, every kFlush pages.
 // The softmax runs online in base 2, with 32-bit maxima and sums: a slice of rows without a new
 // maximum, which is nearly every one, skips the exchange of maxima and the rescaling. Scores,
@@ -54,6 +58,7 @@ constexpr float kLo = 1.f / 2048.f;
 constexpr float kNone = -3e38f;  // the maximum of no rows: finite, so that it may be subtracted from -inf
 constexpr int kStart = 2;   // units in front of a (sequence, head)'s pages
 constexpr int kFlush = 16;  // pages whose products one set of accumulators takes
+constexpr int kWeightBits = -1;  // weights times V's steps stay below 2^kWeightBits, if the steps do
 
 struct Kv4Params {
   const uint8_t* pages;
@@ -341,7 +346,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   ConsumerSync sync{&cons_bar, 0, p.err};
   uint32_t qb[NT][G][4], qm[NT];  // B: two k steps per group; the groups' sums of q
   float qs[NT][G];                // head t: the groups' sums of q
-  float kscale[NT], m[NT], l[NT], m_held[NT];  // head t; m_held: of what shared memory holds
+  // head t: what weights are relative to (2^(s - ref), at most 2^lift), their sum, and the reference
+  // of what shared memory holds
+  float kscale[NT], ref[NT], l[NT], ref_held[NT];
+  uint32_t cap;  // the power of two that V's steps d stay below, as a pair of f16, each with bit 15 set
+  float lift;    // how far below the maximum a reference lies
   float o[NT][2 * G][4];          // values: [16 u + (g, g + 8)] of group j, head t
   float2 om[NT][G];               // middles of group j, head g / 2, this lane's even and odd rows
   bool held = false;
@@ -351,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   auto flush = [&]() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float keep = ex2(m_held[n] - m[n]);
+      const float keep = ex2(ref_held[n] - ref[n]);
       const int h = 4 * n + t;
       float* dst = wo + ((size_t)warp * p.hpk + h) * PITCH;
 #pragma unroll
@@ -376,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         for (int i = 0; i < 4; ++i) o[n][2 * j][i] = o[n][2 * j + 1][i] = 0.f;
         om[n][j] = make_float2(0.f, 0.f);
       }
-      m_held[n] = m[n];
+      ref_held[n] = ref[n];
     }
     held = true;
     since = 0;
@@ -395,6 +404,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
   // slower: the loop outgrows the instruction cache)
   auto rows = [&](const uint8_t* blk, int valid) {
     const int r0 = 16 * warp;
+    const uint8_t* vb = blk + B::kHalf;
+    // ---- V's steps, of a row (64 values) or half a row to each lane
+    constexpr int W = G / 4 < 1 ? 1 : G / 4, kLanes = 8 * G / W;
+    uint32_t steps[W];
+    lds_words<W>(vb + B::kCodes + 2 * B::scale(r0, 0) + 4 * W * (lane % kLanes), steps);
     // ---- scores of rows r0 + g, r0 + 8 + g for head t of every tile
     float s[NT][2];
     {
@@ -446,24 +460,57 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (r0 + 8 * i + g >= valid) s[n][i] = -INFINITY;
+        if (r0 + lane % kLanes * 16 / kLanes >= valid)
+#pragma unroll
+          for (int i = 0; i < W; ++i) steps[i] = 0u;
       }
     }
     // ---- online softmax; then the weights in B's order: lane (g, t) takes of head g / 2 the
     // rows 2t, 2t + 1 of the first (g even) or second eight rows
     float2 pw[NT];
-    bool grow = false;
+    float x[NT][2];
+    bool above = false;  // a step above cap (a borrow from bit 15; steps are not negative)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) grow |= !(fmaxf(s[n][0], s[n][1]) <= m[n]);
+    for (int i = 0; i < W; ++i) above |= (~(cap - steps[i]) & 0x80008000u) != 0u;
+    bool grow = above;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      x[n][0] = s[n][0] - ref[n];
+      x[n][1] = s[n][1] - ref[n];
+      grow |= !(fmaxf(x[n][0], x[n][1]) <= lift);
+    }
     if (__any_sync(0xffffffffu, grow)) {  // (rare after the first pages)
+      const float lift_before = lift;
+      if (__any_sync(0xffffffffu, above)) {
+        uint32_t top_step = 0u;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int k = 0; k < 32; k += 16) {
+            const uint32_t d = steps[i] >> k & 0xffffu;
+            if (d < 0x7c00u) top_step = max(top_step, d);  // (the NaN of a group that is not finite has no size)
+          }
+        top_step = __reduce_max_sync(0xffffffffu, top_step);
+        if (top_step > (cap & 0x7fffu)) {  // steps are below 2^e now
+          const int e = ((int)__float_as_uint(__half2float(__ushort_as_half((unsigned short)top_step))) >> 23) - 126;
+          const __half to = __float2half_rn(fminf(__uint_as_float((uint32_t)(e + 127) << 23), 65504.f));
+          cap = 0x80008000u | __half_as_ushort(to) * 0x10001u;
+          lift = fmaxf((float)(kWeightBits - e), 0.f);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float top = fmaxf(s[n][0], s[n][1]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        top = fmaxf(top, m[n]);
-        const float alpha = ex2(m[n] - top);
-        m[n] = top;
+        // (from 2^24 on a difference is rounded, to or fro between two neighbours at the worst; the
+        // lift of up to 22 becomes 32 at the most, and of over 2^29 nothing)
+        top = fmaxf(top, ref[n] + lift_before) - lift;
+        const float alpha = ex2(ref[n] - top);
+        ref[n] = top;
+        x[n][0] = s[n][0] - top;
+        x[n][1] = s[n][1] - top;
         l[n] *= alpha;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
@@ -476,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float p0 = ex2(s[n][0] - m[n]), p1 = ex2(s[n][1] - m[n]);
+      const float p0 = ex2(x[n][0]), p1 = ex2(x[n][1]);
       l[n] += p0 + p1;
       const int from = 8 * t + (g >> 1);
       const float a0 = __shfl_sync(0xffffffffu, p0, from), a1 = __shfl_sync(0xffffffffu, p1, from);
@@ -485,7 +532,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
     }
     // ---- weighted rows
     {
-      const uint8_t* vb = blk + B::kHalf;
       const int rw = r0 + 2 * t + (odd ? 8 : 0);  // rows of pa, pb
       uint32_t dw[G], mw[G];                      // f16 d [row][group]; m [group][row]
       lds_words<G>(vb + B::kCodes + 2 * B::scale(rw, 0), dw);
@@ -594,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
         uint32_t hi, lo;
         split2(s0, s1, hi, lo);
         qm[n] = odd ? lo : hi;
-        m[n] = m_held[n] = kNone;
+        ref[n] = ref_held[n] = kNone;
         l[n] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * G; ++i)
@@ -603,28 +649,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
       }
       held = false;
       since = 0;
+      cap = 0x80008000u;
+      lift = 0.f;
     }
     if (16 * warp < sg.valid) rows(blk, sg.valid);
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[st]);
     next();
-    if (sg.left > 1) {
-      if (++since == kFlush) flush();
-      continue;
-    }
-
-    // ---------------- end of the segment: join the warps in order
+    const bool last = sg.left <= 1;
+    if (last) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
-      if (g == 0 && 4 * n + t < p.hpk) {
-        wm[warp][4 * n + t] = m[n];
-        wl[warp][4 * n + t] = l[n];
+      for (int n = 0; n < NT; ++n) {
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+        if (g == 0 && 4 * n + t < p.hpk) {
+          wm[warp][4 * n + t] = ref[n];
+          wl[warp][4 * n + t] = l[n];
+        }
       }
     }
-    flush();
+    if (last || ++since == kFlush) flush();  // (in one place: with two the loop was 2 to 5 % slower)
+    if (!last) continue;
+
+    // ---------------- end of the segment: join the warps in order
     if (!sync()) return;
     // the CTAs of this (sequence, head)
     const long long last_unit = sg.base + sg.pages - 1;

@@ -5,10 +5,12 @@ import math
 import os
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
-from test_serving import DT, FINE, ROOT, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal  # noqa: F401
+from test_serving import (DT, FINE, ROOT, U, Cache, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal,  # noqa: F401
+                          np_quantise, np_values, within)
 
 
 class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
@@ -123,6 +125,108 @@ def test_attention_packed_bits_do_not_depend_on_the_rows_behind(rrr, ctx, hd, ki
         outs.append(torch.stack([out[lq * s:lq * (s + 1)] for s in range(0, seqs, 2)]))
     assert bool(torch.isfinite(outs[0]).all())
     assert all(torch.equal(o, outs[0]) for o in outs[1:]) and ctx.device_error() == 0
+
+
+def check_decode_of_small_values(got, q, k, v, scale):
+    """got, q [heads, hd] of one sequence with rows k, v [rows, n_kv, hd] (f32, as they are stored),
+    within a bound that knows how little a row weighs: a weight is off by w = 2 (48 A + 8) u of
+    itself (48 A of a score and of the maximum, the exponential and the split 8), which moves the
+    result by w sum p |v - out|; a product is of d |code - 8| and m + 8 d, each rounded once or its
+    sum, in (rows / 64 + 64) u of sum p (8 d + |m + 8 d|); and the rows compared with carry the
+    rounding of d code + m."""
+    n, n_kv, hd = v.shape
+    _, d, m, _ = np_quantise(v.cpu().numpy())
+    d, m = (torch.from_numpy(x.astype(np.float64)).cuda().repeat_interleave(32, -1) for x in (d, m))
+    held = torch.from_numpy(np_values(v.cpu().numpy())).cuda().double()
+    per = q.shape[0] // n_kv
+    for h in range(q.shape[0]):
+        keys = torch.from_numpy(np_values(k[:, h // per].cpu().numpy())).cuda().double()
+        x = q[h].double()
+        p = torch.softmax(keys @ x * scale, 0)[:, None]
+        A = float((keys.abs() @ x.abs()).max()) * scale
+        vv, dd, mm = held[:, h // per], d[:, h // per], m[:, h // per]
+        ref = (p * vv).sum(0)
+        bound = U * (2 * (48 * A + 8) * (p * (vv - ref).abs()).sum(0)
+                     + (n / 64 + 64) * (p * (8 * dd + (mm + 8 * dd).abs())).sum(0) + (p * vv.abs()).sum(0))
+        within(got[h], ref, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 4, 2), (64, 7, 1), (128, 6, 2), (128, 5, 1), (128, 8, 1), (256, 3, 1), (256, 7, 1)])
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-2, 1e-4, 1e-6])
+def test_attention_kv4_small_values_behind_a_row_that_takes_the_weight(rrr, ctx, hd, nh, nkv, size):
+    """A first row of no value draws nearly all weight, as the first token of a text does: what is
+    left is a sum of small weights times values of any size, and no less exact."""
+    rows, g = [23, 70, 1500], gen(hd + nh)
+    cache = Cache(rrr, ctx, nkv, hd, rows, 4)
+    k = 0.1 * normal(g, sum(rows), nkv, hd)
+    v = size * (normal(g, sum(rows), nkv, hd) + 0.3)
+    q = normal(g, 3, nh, hd).sign()
+    starts = [0, *np.cumsum(rows)[:-1]]
+    for s, a in enumerate(starts):
+        v[a] = 0
+        k[a] = q[s].unflatten(0, (nkv, -1)).mean(1) * 14 / math.sqrt(hd)
+    q = q + 0.05 * normal(g, 3, nh, hd)
+    cache.c.store(k, v, cu_of(rows), ints(rows))
+    out = torch.empty_like(q)
+    cache.c.attention(q, ints(rows), out, cache.c.workspace(nh))
+    for s, a in enumerate(starts):
+        check_decode_of_small_values(out[s], q[s], k[a:a + rows[s]], v[a:a + rows[s]], 1 / math.sqrt(hd))
+    assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 8, 1), (128, 3, 1), (128, 5, 1), (256, 4, 2)])
+@pytest.mark.parametrize("first,last", [(1e-6, 1e4), (1e3, 1e-5), (0.0, 1e-3), (3e-3, 0.0)])
+@pytest.mark.parametrize("rising", [True, False])
+def test_attention_kv4_values_that_grow_or_shrink_along_a_sequence(rrr, ctx, hd, nh, nkv, first, last, rising):
+    """Values from one size to another over the rows (the largest step so far sets the weights' scale),
+    under scores that rise or fall along with them."""
+    n, g = 5000, gen(hd)
+    cache = Cache(rrr, ctx, nkv, hd, [n], 4)
+    ramp = torch.linspace(0, 1, n, device="cuda")[:, None, None]
+    size = (max(first, 1e-8) ** (1 - ramp)) * (max(last, 1e-8) ** ramp)
+    if first == 0.0:
+        size = torch.where(ramp < 0.4, 0.0, last)
+    if last == 0.0:
+        size = torch.where(ramp > 0.7, 0.0, first)
+    v = size * normal(g, n, nkv, hd)
+    k = 0.1 * normal(g, n, nkv, hd) + 1.5 * (ramp if rising else 1 - ramp) / math.sqrt(hd)
+    q = 0.3 * normal(g, 1, nh, hd) + 1
+    cache.c.store(k, v, ints([0, n]), ints([n]))
+    out = torch.empty_like(q)
+    cache.c.attention(q, ints([n]), out, cache.c.workspace(nh))
+    check_decode_of_small_values(out[0], q[0], k, v, 1 / math.sqrt(hd))
+    assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh", [(64, 3), (64, 8), (128, 4), (128, 5), (256, 2), (256, 7)])
+@pytest.mark.parametrize("size", [1.0, 1e-5])
+@pytest.mark.parametrize("top", [2.0 ** 18, 2.0 ** 20, 2.0 ** 23, 2.0 ** 27, 2.0 ** 31, -2.0 ** 20, -2.0 ** 26])
+def test_attention_kv4_scores_whose_steps_are_coarse(rrr, ctx, hd, nh, size, top):
+    """Scores of 2^18 to 2^31 that rise along the sequence in one head, beside heads of ordinary ones:
+    the largest takes all, whatever the others' maxima and the values' sizes do meanwhile."""
+    n, g = 3000, gen(hd)
+    cache = Cache(rrr, ctx, 1, hd, [n], 4)
+    k, v = normal(g, n, 1, hd), size * (normal(g, n, 1, hd) + 0.2)
+    k[:, 0, 32:64] = torch.linspace(0.5, 1, n, device="cuda").flip(0 if top < 0 else ())[:, None]
+    q = normal(g, 1, nh, hd)
+    q[0, 0] = 0
+    q[0, 0, 40] = top * math.log(2) * math.sqrt(hd)  # that head's scores, in base 2, are this times k[:, 0, 40]
+    cache.c.store(k, v, ints([0, n]), ints([n]))
+    out = torch.empty_like(q)
+    cache.c.attention(q, ints([n]), out, cache.c.workspace(nh))
+    held = torch.from_numpy(np_values(v.cpu().numpy())).cuda()[:, 0]
+    keys = torch.from_numpy(np_values(k.cpu().numpy())).cuda()[:, 0, 40]
+    best = (keys * top).argmax()
+    # every row of a group of 32 equal keys is held exactly to f16, and 2^18 steps of 2^-11 part them
+    alike = keys == keys[best]
+    want = held[alike].double().mean(0)
+    mag = float(held.abs().max())
+    within(out[0, 0], want, torch.full_like(want, 64 * U * mag * (1 if int(alike.sum()) == 1 else 8)))
+    assert bool(torch.isfinite(out).all()) and ctx.device_error() == 0
+    check_decode_of_small_values(out[0, 1:], q[0, 1:], k, v, 1 / math.sqrt(hd))
 
 
 @pytest.mark.gpu
