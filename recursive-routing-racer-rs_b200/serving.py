@@ -4,8 +4,8 @@ with its decode attention. The rows of the sequences of a batch lie one after an
 an int32 tensor of n_seqs + 1 ascending row starts.
 
 Tensors are checked for device, type, shape and contiguity of their last dimension; the C ABI
-checks strides, alignment and overlap. `stream`: a torch stream, an int, or None (the default
-stream); a tensor made on another stream is the caller's to order."""
+checks strides, alignment and overlap. `stream`: a torch stream, an int, or None (torch's current
+stream of the context's GPU); a tensor made on another stream is the caller's to order."""
 from __future__ import annotations
 
 import ctypes
@@ -13,11 +13,12 @@ import struct
 from ctypes import byref, c_int64
 
 from . import ffi
-from .engine import _stream
+from .engine import _stream as _handle
 
 PAGE_ROWS = 64
 _TYPES: dict = {}  # torch dtype -> GGML type id
 _INTS: set = set()  # torch dtypes of 32-bit integers
+_torch = None
 # The fields of a PackedDesc, packed: a third of the time of its constructor
 _packed = struct.Struct("@6if10q").pack
 
@@ -34,6 +35,15 @@ def _type(t, what: str) -> int:
 
 def _fail(code: int, message: str):
     raise ffi.RRRError(code, message)
+
+
+def _stream(ctx: ffi.Context, stream):
+    global _torch
+    if stream is not None:
+        return _handle(stream)
+    if _torch is None:
+        import torch as _torch
+    return _torch._C._cuda_getCurrentRawStream(ctx.device)  # current_stream() without its object
 
 
 def _on(ctx: ffi.Context, t, what: str):
@@ -104,7 +114,7 @@ def qk_norm_rope(ctx: ffi.Context, desc: ffi.AttnDesc, qkv, positions, q, k, v=N
             gammas[i] = _on(ctx, g, name)
     rc = ffi.lib().rrr_qk_norm_rope(
         ctx.h, byref(desc), _type(qkv, "qkv"), pin, sin, rows, _ints(ctx, positions, rows, "positions"),
-        gammas[0], gammas[1], eps, 1 if halves else 0, out, pq, sq, pk, sk, pv, sv, _stream(stream))
+        gammas[0], gammas[1], eps, 1 if halves else 0, out, pq, sq, pk, sk, pv, sv, _stream(ctx, stream))
     if rc:
         ctx.check(rc)
 
@@ -128,7 +138,7 @@ def attention_packed(ctx: ffi.Context, q, k, v, cu_q, cu_kv, out, *, causal: boo
         *_strides(k, held, kvh, hd, "k"), *_strides(v, held, kvh, hd, "v"), *_strides(out, rows, heads, hd, "out")))
     rc = ffi.lib().rrr_attention_packed(ctx.h, byref(d), _on(ctx, q, "q"), _on(ctx, k, "k"), _on(ctx, v, "v"),
                                         _ints(ctx, cu_q, n, "cu_q"), _ints(ctx, cu_kv, n, "cu_kv"),
-                                        _on(ctx, out, "out"), _stream(stream))
+                                        _on(ctx, out, "out"), _stream(ctx, stream))
     if rc:
         ctx.check(rc)
     return out
@@ -176,7 +186,8 @@ class KV4Cache:
     def store(self, k, v, cu_rows, kv_lens, stream=None) -> None:
         """rrr_kv4_store: packed rows [rows, n_kv, hd] become the last ones of their sequences,
         which have kv_lens rows then."""
-        rc = ffi.lib().rrr_kv4_store(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens), _stream(stream))
+        rc = ffi.lib().rrr_kv4_store(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens),
+                                     _stream(self.ctx, stream))
         if rc:
             self.ctx.check(rc)
 
@@ -184,7 +195,8 @@ class KV4Cache:
         """rrr_kv4_load: the last rows of every sequence, dequantised, into packed rows."""
         if k is None and v is None:
             _fail(-1, "load: k or v is needed")
-        rc = ffi.lib().rrr_kv4_load(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens), _stream(stream))
+        rc = ffi.lib().rrr_kv4_load(self.ctx.h, self._desc, *self._rows(k, v, cu_rows, kv_lens),
+                                    _stream(self.ctx, stream))
         if rc:
             self.ctx.check(rc)
 
@@ -206,7 +218,7 @@ class KV4Cache:
         po, _, so = _heads(self.ctx, out, heads, self.head_dim, "out", self.n_seqs)
         rc = ffi.lib().rrr_attention_kv4(
             self.ctx.h, self._desc, heads, _type(q, "q"), pq, sq, _ints(self.ctx, kv_lens, self.n_seqs, "kv_lens"),
-            scale, po, so, _on(self.ctx, workspace, "workspace"), workspace.nbytes, _stream(stream))
+            scale, po, so, _on(self.ctx, workspace, "workspace"), workspace.nbytes, _stream(self.ctx, stream))
         if rc:
             self.ctx.check(rc)
         return out

@@ -1,9 +1,10 @@
 """The packed-batch operators where a plain comparison of random values sees little: arrays that
-share a buffer, calls of two host threads. Formulas and helpers are test_serving.py's."""
+share a buffer, streams, small values, rows of other sequences, calls of two host threads. Formulas and helpers are test_serving.py's."""
 import ctypes
 import math
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -82,7 +83,84 @@ def test_attention_packed_arrays_that_interleave(rrr, host_ctx, over, code):
     assert packed_call(rrr, host_ctx, over) == code, rrr.ffi.last_error(host_ctx)
 
 
+def test_python_host_runs_on_the_current_stream(rrr, monkeypatch):
+    """Without `stream`, the calls go to torch's current stream of the context's GPU, where the
+    tensors' other work is; `stream` overrides it. (CPU tensors and a library that notes its calls.)"""
+    serving, seen = sys.modules[rrr.qk_norm_rope.__module__], []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: seen.append((name, args[-1])) or 0
+
+    class Ctx:
+        h, device = None, -1  # CPU tensors' device number
+
+    monkeypatch.setattr(serving.ffi, "lib", Library)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0x5000 + device, raising=False)
+    zeros, pos = torch.zeros, torch.zeros(3, dtype=torch.int32)
+    q, kv, out = zeros(3, 4, 128).half(), zeros(3, 2, 128).half(), zeros(3, 4, 128).half()
+    cache = rrr.KV4Cache(Ctx, zeros(4, 2, 80 * 128, dtype=torch.uint8), zeros(2, 4, dtype=torch.int32), 128)
+    desc, cu, n = rrr.ffi.AttnDesc(4, 2, 128, 96, 1e4, 1.0, None, 0, 16), pos, pos[:2]
+
+    def calls(**stream):
+        rrr.qk_norm_rope(Ctx, desc, zeros(3, 8, 128), pos, q, kv, **stream)
+        rrr.attention_packed(Ctx, q, kv, kv, cu, cu, out, **stream)
+        cache.store(kv, kv, cu, n, **stream)
+        cache.load(cu, n, kv, **stream)
+        cache.attention(q[:2], n, out[:2], zeros(64, dtype=torch.uint8), **stream)
+
+    def number(s):
+        return s if isinstance(s, int) else getattr(s, "value", None)
+
+    calls()
+    assert [number(s) for _, s in seen] == [0x4fff] * 5, seen
+    seen.clear()
+    calls(stream=77)
+    assert [number(s) for _, s in seen] == [77] * 5
+
+
 # ------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+def test_calls_follow_the_current_stream(rrr, ctx):
+    """Inputs that the current stream is still writing, and a capture of it, without `stream`."""
+    nh, nkv, hd, lens, t = 4, 2, 128, [70, 300], torch.bfloat16
+    g, rows, cu, n = gen(1), sum(lens), cu_of(lens), ints(lens)
+    x, pos = normal(g, rows, nh + 2 * nkv, hd, dtype=t), ints([i for m in lens for i in range(m)])
+    desc = rrr.ffi.AttnDesc(nh, nkv, hd, 128, 1e4, 1.0, None, 0, 4096)
+    cache = Cache(rrr, ctx, nkv, hd, lens, 1)
+    ws = cache.c.workspace(nh)
+
+    def step(qkv, q, k, v, out, kk, token):
+        rrr.qk_norm_rope(ctx, desc, qkv, pos, q, k, v)
+        rrr.attention_packed(ctx, q, k, v, cu, cu, out)
+        cache.c.store(k, v, cu, n)
+        cache.c.load(cu, n, kk)
+        cache.c.attention(q[:2], n, token, ws)
+
+    def arrays():
+        return [torch.zeros_like(x)] + [torch.zeros(r, h, hd, dtype=t, device="cuda")
+                                        for r, h in ((rows, nh), (rows, nkv), (rows, nkv), (rows, nh), (rows, nkv), (2, nh))]
+
+    want, late, graphed = arrays(), arrays(), arrays()
+    want[0].copy_(x)
+    step(*want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # some 10 ms
+        late[0].copy_(x)
+        step(*late)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, late))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*graphed)
+    graphed[0].copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, graphed)) and ctx.device_error() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("order", ["rows", "heads"])
 def test_attention_packed_rows_of_inputs_and_output(rrr, ctx, order):
