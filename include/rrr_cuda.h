@@ -438,7 +438,8 @@ int rrr_kv4_store(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, const void* k,
                   const void* v, int64_t v_stride, int rows, const int32_t* cu_rows,
                   const int32_t* kv_lens, void* stream);
 /* The reverse: the last rows of every sequence, as the values they stand for, into packed
- * rows (the prefix of a continued prompt for rrr_attention_packed). k or v may be NULL. */
+ * rows, without room between the sequences (for rrr_attention_packed of continued prompts, whose
+ * new rows are stored first and loaded with their prefix). k or v may be NULL. */
 int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_t k_stride, void* v,
                  int64_t v_stride, int rows, const int32_t* cu_rows, const int32_t* kv_lens,
                  void* stream);
@@ -448,9 +449,9 @@ int rrr_kv4_load(rrr_ctx* ctx, const rrr_kv4_cache* c, int type, void* k, int64_
  * of `type`, q 16-byte aligned rows. A sequence without rows gives zeros, and so does one whose
  * kv_lens is out of range; rows on pages that do not exist are left out. Scores and sums
  * carry 32-bit accuracy whatever the type and the values' size; a weight times a group's d
- * counts to 2^-22 of itself or 2^-35 of the largest weight times the largest d. workspace: rrr_kv4_workspace bytes of device
- * memory, whatever they hold; calls that can run at the same time, replays of captured
- * graphs among them, need one each. */
+ * counts to 2^-22 of itself or 2^-35 of the largest weight times the largest d. workspace:
+ * rrr_kv4_workspace bytes of device memory, whatever they hold; calls that can run at the
+ * same time, replays of captured graphs among them, need one each. */
 int rrr_kv4_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int64_t* bytes);
 int rrr_attention_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int type, const void* q,
                       int64_t q_stride, const int32_t* kv_lens, float scale, void* out,

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_serving import (DT, FINE, ROOT, U, Cache, _no_gpu, cu_of, filled, gen, host_ctx, ints, normal,  # noqa: F401
+from test_serving import (DT, FINE, ROOT, U, Cache, _no_gpu, check_packed, cu_of, filled, gen, host_ctx, ints, normal,  # noqa: F401
                           np_quantise, np_values, within)
 
 
@@ -120,6 +120,41 @@ def test_python_host_runs_on_the_current_stream(rrr, monkeypatch):
 
 
 # ------------------------------------------------------------------ GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_continued_prompts_of_a_batch(rrr, ctx, hd):
+    """New rows of several sequences over their prefixes in the cache: stored, loaded with their
+    prefixes, attended as the cache holds them, and with the unrounded rows copied over theirs."""
+    nh, nkv, t, g = 6, 2, torch.bfloat16, gen(hd)
+    old, new = [90, 0, 200, 64, 1], [40, 17, 0, 65, 300]
+    held = [a + b for a, b in zip(old, new)]
+    cache = Cache(rrr, ctx, nkv, hd, held, 3)
+    k, v = (normal(g, sum(old), nkv, hd, dtype=t) for _ in range(2))
+    cache.c.store(k, v, cu_of(old), ints(old))
+    prefix = [torch.empty_like(k) for _ in range(2)]
+    cache.c.load(cu_of(old), ints(old), *prefix)
+    q = normal(g, sum(new), nh, hd, dtype=t)
+    rows = [normal(g, sum(new), nkv, hd, dtype=t) for _ in range(2)]
+    cu_q, cu_kv, lens = cu_of(new), cu_of(held), ints(held)
+    cache.c.store(*rows, cu_q, lens)
+    both = [torch.empty(sum(held), nkv, hd, dtype=t, device="cuda") for _ in range(2)]
+    cache.c.load(cu_kv, lens, *both)
+    ends = np.cumsum(held)
+    old_at = torch.tensor([e - h + i for e, h, n in zip(ends, held, old) for i in range(n)], device="cuda")
+    new_at = torch.tensor([e - n + i for e, n in zip(ends, new) for i in range(n)], device="cuda")
+    for whole, a, b in zip(both, prefix, rows):
+        assert torch.equal(whole[old_at], a)
+        assert torch.equal(whole[new_at].float().cpu(), torch.from_numpy(np_values(b.float().cpu().numpy())).to(t).float())
+    out = torch.empty_like(q)
+    rrr.attention_packed(ctx, q, *both, cu_q, cu_kv, out)
+    check_packed(out, q, *both, new, held, True, 1 / math.sqrt(hd))
+    for whole, b in zip(both, rows):
+        whole[new_at] = b
+    rrr.attention_packed(ctx, q, *both, cu_q, cu_kv, out)
+    check_packed(out, q, *both, new, held, True, 1 / math.sqrt(hd))
+    assert ctx.device_error() == 0
+
+
 @pytest.mark.gpu
 def test_calls_follow_the_current_stream(rrr, ctx):
     """Inputs that the current stream is still writing, and a capture of it, without `stream`."""
