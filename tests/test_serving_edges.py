@@ -10,8 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_serving import (DT, FINE, ROOT, U, Cache, _no_gpu, check_packed, cu_of, filled, gen, host_ctx, ints, normal,  # noqa: F401
-                          np_quantise, np_values, within)
+from test_serving import (DT, FINE, ROOT, U, Cache, _no_gpu, check_packed, cu_of, filled, gen, half_step, host_ctx,  # noqa: F401
+                          ints, normal, np_quantise, np_values, within)
 
 
 class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
@@ -19,6 +19,25 @@ class KV4Call(ctypes.Structure):  # tests/cpp/two_threads.cpp
                 ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("kv_lens", ctypes.c_void_p),
                 ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p),
                 ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)]
+
+
+# Rows told apart. `spread`: q is zero, so that rows weigh the same, and row j has one value, in place
+# j % hd: a result is (rows seen with that place) / (rows seen), of whole numbers that are summed
+# exactly. `paired`: row j's key answers the queries of class j % hd alone (a score of 40, 2^-57 of the
+# weight to the others), its value stands in place j / hd % hd: a key or value that is lost, read
+# twice, or of another row shows in full, as one row in some (rows seen) / hd.
+def told_apart(pattern, rows, n_kv, hd, t, device="cuda"):
+    """Keys and values of one sequence, shifted by one row per KV head."""
+    j = torch.arange(rows, device=device)[:, None] + torch.arange(n_kv, device=device)
+    one = torch.eye(hd, device=device, dtype=t)
+    return (one[j % hd], one[j % hd]) if pattern == "spread" else (one[j % hd], one[j // hd % hd])
+
+
+def asking(pattern, rows, heads, hd, t, device="cuda"):
+    if pattern == "spread":
+        return torch.zeros(rows, heads, hd, device=device, dtype=t)
+    i = 7 * torch.arange(rows, device=device)[:, None] + 5 * torch.arange(heads, device=device)
+    return 40 * torch.eye(hd, device=device, dtype=t)[i % hd]
 
 
 # ------------------------------------------------------------------ CPU
@@ -48,6 +67,23 @@ FAR = 1 << 38  # the longest stride
 def test_attention_packed_extents_past_64_bits(rrr, host_ctx, over, code):
     _no_gpu()
     assert packed_call(rrr, host_ctx, over) == code
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [700, 3000, 9001])
+def test_rows_told_apart_show_a_lost_and_a_doubled_one(hd, n):
+    """The patterns against their tests' widest tolerance (bf16), with the mistake in the formula."""
+    w = torch.float64
+    k, v = (x[:, 0] for x in told_apart("paired", n, 1, hd, w, "cpu"))
+    q = asking("paired", 1, hd, hd, w, "cpu")[0]
+    s = q @ k.T
+    ref, count = torch.softmax(s, -1) @ v, torch.zeros(n, dtype=w)
+    for row in (0, 1, 63, 64, 127, 128, 511, 512, n // 2, n - 2, n - 1):
+        for times in (0, 2):
+            count.fill_(1)[row] = times
+            e = s.exp() * count
+            wrong = e / e.sum(-1, keepdim=True) @ v
+            assert float(((wrong - ref).abs() / (ref * half_step(torch.bfloat16) * 1.01 + n * 2.0 ** -57)).max()) > 4
 
 
 Q = 1 << 20
@@ -238,6 +274,96 @@ def test_attention_packed_bits_do_not_depend_on_the_rows_behind(rrr, ctx, hd, ki
         outs.append(torch.stack([out[lq * s:lq * (s + 1)] for s in range(0, seqs, 2)]))
     assert bool(torch.isfinite(outs[0]).all())
     assert all(torch.equal(o, outs[0]) for o in outs[1:]) and ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 24, 8), (64, 5, 5), (128, 24, 8), (128, 4, 1), (256, 4, 2), (128, 130, 1), (64, 129, 1)])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("lq,lk", [
+    ([1], [3000]), ([5], [9001]), ([37], [2111]), ([100], [2048]), ([3, 0, 50], [2500, 900, 2600]), ([700], [1600]),
+    ([513], [513]), ([127, 1, 0, 130, 64], [127, 1, 0, 130, 64]), ([1500], [1500]), ([21] * 40, [21 + 37 * i for i in range(40)])])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("pattern", ["spread", "paired"])
+def test_attention_packed_every_row_counts_once(rrr, ctx, hd, nh, nkv, kind, lq, lk, causal, pattern):
+    """The weights are 1 (or too small to count) and the sums whole numbers below 2^24, so all that is
+    rounded is the inverse, its product and the output: half a step and 2 u, and 2^-57 times the rows
+    for the others' weights."""
+    t = DT[kind]
+    k, v = (torch.cat(x) for x in zip(*(told_apart(pattern, n, nkv, hd, t) for n in lk)))
+    q = torch.cat([asking(pattern, n, nh, hd, t) for n in lq])
+    out = torch.full_like(q, 3.0)
+    rrr.attention_packed(ctx, q, k, v, cu_of(lq), cu_of(lk), out, causal=causal, scale=1.0)
+    a = b = 0
+    for n, m in zip(lq, lk):
+        seen = torch.ones(n, m, dtype=torch.bool, device="cuda")
+        if causal:
+            seen = seen.tril(m - n)
+        kk, vv = (x[b:b + m].double().repeat_interleave(nh // nkv, 1).transpose(0, 1) for x in (k, v))
+        s = (q[a:a + n].double().transpose(0, 1) @ kk.transpose(1, 2)).masked_fill(~seen, -math.inf)
+        ref = (torch.softmax(s, -1).nan_to_num(0) @ vv).transpose(0, 1)
+        within(out[a:a + n], ref, ref * (half_step(t) + 2 * U) * 1.01 + m * 2.0 ** -57 + (2.0 ** -25 if t == torch.float16 else 0))
+        a, b = a + n, b + m
+    assert ctx.device_error() == 0
+
+
+def check_packed_by_weights(out, q, k, v, scale):
+    """One causal sequence within a bound that knows what a row weighs: a weight is off by
+    2 ((hd + 16) A + 8) u of itself and half a step of the type (below 2^-14 of the reference f16 has
+    no normal numbers: 2^-25, and the sum is at least one), the sums by (rows / 16 + 64) u."""
+    t, (n, nh, hd), rows = q.dtype, q.shape, k.shape[0]
+    seen = torch.ones(n, rows, dtype=torch.bool, device="cuda").tril(rows - n)
+    for h in range(nh):
+        x, y, z = q[:, h].double(), k[:, h * k.shape[1] // nh].double(), v[:, h * k.shape[1] // nh].double()
+        A = (x.abs() @ y.abs().T * scale * seen).amax(-1, keepdim=True)
+        p = torch.softmax((x @ y.T * scale).masked_fill(~seen, -math.inf), -1)
+        ref, mag = p @ z, p @ z.abs()
+        bound = U * (2 * ((hd + 16) * A + 8) * (mag + ref.abs()) + (rows / 16 + 64) * mag) \
+            + half_step(t) * 1.01 * (mag + ref.abs())
+        if t == torch.float16:
+            bound = bound + 2.0 ** -25 * (1 + seen.sum(-1, keepdim=True) * float(z.abs().max()))
+        within(out[:, h], ref, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("n,rows", [(300, 1300), (2, 3000)])
+@pytest.mark.parametrize("step", [0.0, 1.0, 7.9, 8.1, 40.0, -7.9])
+def test_attention_packed_maxima_that_grow_from_block_to_block(rrr, ctx, hd, kind, n, rows, step):
+    """The largest score of every 128 rows is `step` above the last ones', in powers of two: a maximum is
+    taken over only when it has grown by more than 8, and weights are up to 2^8 until then."""
+    t, g = DT[kind], gen(hd + n)
+    q, k, v = normal(g, n, 2, hd), 0.1 * normal(g, rows, 1, hd), normal(g, rows, 1, hd, dtype=t)
+    q[:, :, 0] = 1
+    k[:, 0, 0] = (torch.arange(rows, device="cuda") // 128 - 5) * step * math.log(2) - 3
+    k[::128, 0, 0] += 3
+    q, k = q.to(t), k.to(t)
+    out = torch.empty_like(q)
+    rrr.attention_packed(ctx, q, k, v, cu_of([n]), cu_of([rows]), out, scale=1.0)
+    check_packed_by_weights(out, q, k, v, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 8, 1), (64, 4, 2), (64, 5, 1), (128, 6, 2), (128, 8, 1), (128, 7, 1), (256, 4, 2), (256, 8, 1), (256, 5, 1)])
+@pytest.mark.parametrize("lens", [[1, 17, 64, 0, 65, 128, 1023], [3000, 1, 130, 700], [30001], [150] * 90])
+@pytest.mark.parametrize("pattern", ["spread", "paired"])
+def test_attention_kv4_every_row_counts_once(rrr, ctx, hd, nh, nkv, lens, pattern):
+    """As of prompts; one is held as 15 f16(1/15), and the sums of centred codes and middles may be
+    off by (rows that count / 64 + 64) u of 16 d and 8 u more for weights, inverse and product."""
+    cache = Cache(rrr, ctx, nkv, hd, lens, 7)
+    k, v = (torch.cat(x) for x in zip(*(told_apart(pattern, n, nkv, hd, torch.float32) for n in lens)))
+    cache.c.store(k, v, cu_of(lens), ints(lens))
+    q = asking(pattern, len(lens), nh, hd, torch.float32)
+    out = torch.empty_like(q)
+    cache.c.attention(q, ints(lens), out, cache.c.workspace(nh), scale=1.0)
+    one, a = 15 * float(np.float16(1 / 15)), 0
+    for s, n in enumerate(lens):
+        kk, vv = (x[a:a + n].double().repeat_interleave(nh // nkv, 1).transpose(0, 1) * one for x in (k, v))
+        ref = (torch.softmax((kk @ q[s].double()[:, :, None])[..., 0], -1)[:, None] @ vv)[:, 0] if n else torch.zeros_like(q[s])
+        count = n if pattern == "spread" else n / hd + 1
+        within(out[s], ref, torch.full_like(ref, U * (count / 64 + 64 + 8) * 16 / 15 + n * 2.0 ** -57))
+        a += n
+    assert ctx.device_error() == 0
 
 
 def check_decode_of_small_values(got, q, k, v, scale):
