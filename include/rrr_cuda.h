@@ -400,10 +400,11 @@ enum { RRR_F32 = 0, RRR_F16 = 1, RRR_BF16 = 30 };
  * normed) and its first a->rope_dim values are rotated for the row's position (device
  * int32[rows], 0 <= position < a->max_seq; a row outside is left as it was), in one pass,
  * rounded once. Frequencies as in apply_rope_cfg (phi4.rs:238-256), but the angle is not
- * rounded to 32 bits before its sine (exact to 2^-24 turns at any position). halves = 0
- * rotates the pairs (2i, 2i+1) as rrr_rope_kv_store does, 1 the pairs (i, i + rope_dim/2)
- * (rope_dim then a multiple of head_dim/16). V is copied; v = NULL leaves it out. q, k, v
- * may lie in their own place in qkv (same type and stride), and overlap nothing else. */
+ * rounded to 32 bits before its sine (with theta and factors of at least one, exact to 2^-24
+ * turns below position 2^27 and to position * 2^-51 turns beyond). halves = 0 rotates the
+ * pairs (2i, 2i+1) as rrr_rope_kv_store does, 1 the pairs (i, i + rope_dim/2) (rope_dim then a
+ * multiple of head_dim/16). V is copied; v = NULL leaves it out. q, k, v may lie in their own
+ * place in qkv (same type and stride), and overlap nothing else. */
 int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_type, const void* qkv,
                      int64_t row_stride, int rows, const int32_t* positions, const float* q_gamma,
                      const float* k_gamma, float eps, int halves, int out_type, void* q,

@@ -5,9 +5,11 @@
 //
 // Mathematics. x' = (gamma x) / sqrt(mean(x^2) + eps); with c, s = af cos(2 pi t), af sin(2 pi
 // t) a pair (a, b) becomes (a c - b s, a s + b c). t = pos * f / factor / 2 pi turns is wanted
-// modulo 1 to 2^-24 at any position: f / factor / 2 pi is held modulo 1 as a 64-bit fraction F
-// (from 64-bit floats, so to 2^-51 of itself), and pos * F modulo 2^64 is exact in integers.
-// sincospi of its top 32 bits, taken as a signed fraction, needs no range reduction.
+// modulo 1 to 2^-24: f / factor / 2 pi is held modulo 1 as a 64-bit fraction F, and pos * F modulo
+// 2^64 is exact in integers. sincospi of its top 32 bits, taken as a signed fraction, needs no range
+// reduction; as a float it is off by 2^-25 turns at most. F comes from 64-bit floats: where f and 1 /
+// factor are at most one it is off by less than 2^-52.5 turns (nine roundings of at most 2^-53 / 2 pi,
+// those of the exponents included), which reaches the rest of 2^-24 at position 2^27.
 //
 // Bound by memory: each value is read once and written once. A warp owns a run of heads of one
 // row, lane l the values D*l .. D*l + D - 1 (D = head_dim / 32) of each, so that a row's sines
@@ -273,8 +275,7 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
   p.max_pos = a->max_seq;
   p.eps = eps;
   p.attn_factor = a->rope_attn_factor;
-  // theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64, and three
-  // roundings, 2^-51 of itself
+  // theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64
   double fine[8], coarse[kMaxPairs / 8];
   for (int i = 0; i < 8; ++i) fine[i] = pow((double)a->rope_theta, -2.0 * i / a->rope_dim);
   for (int i = 0; 8 * i < p.half_dim; ++i)

@@ -233,6 +233,38 @@ def test_calls_follow_the_current_stream(rrr, ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("theta,factors", [(10000.0, False), (500000.0, True), (1.0, False)])
+@pytest.mark.parametrize("halves", [False, True])
+def test_qk_norm_rope_far_positions(rrr, ctx, theta, factors, halves):
+    """Angles of positions up to the last, against 80-bit floats: 2^-24 turns below 2^27 and position *
+    2^-51 turns beyond, 2 u for the sine and 3 u for the rotation's own roundings. (The formula's
+    frequency is theta's as a 32-bit float; its angle in 80 bits is off by position * 2^-62.)"""
+    nh, nkv, hd, rd, g = 2, 1, 128, 96, gen(7)
+    at = [0, 1, 2 ** 20 + 7] + [2 ** e + d for e in (24, 26, 27, 28, 30) for d in (-1, 0, 12345)] + [2 ** 31 - 2 - i for i in range(9)]
+    x = normal(g, len(at), nh + 2 * nkv, hd)
+    f = torch.rand(rd // 2, device="cuda", generator=g) * 3 + 1 if factors else None
+    desc = rrr.ffi.AttnDesc(nh, nkv, hd, rd, theta, 1.0, None if f is None else f.data_ptr(), 0 if f is None else f.numel(), 2 ** 31 - 1)
+    outs = [torch.empty(len(at), n, hd, device="cuda") for n in (nh, nkv, nkv)]
+    rrr.qk_norm_rope(ctx, desc, x.flatten(1), ints(at), *outs, halves=halves)
+    wide = np.longdouble
+    freq = np.power(wide(np.float32(theta)), -2 * np.arange(rd // 2, dtype=wide) / wide(rd))
+    if factors:
+        freq = freq / f.cpu().numpy().astype(wide)
+    angle = np.array(at, wide)[:, None] * freq
+    c, s = (torch.from_numpy(y.astype(np.float64)).cuda()[:, None] for y in (np.cos(angle), np.sin(angle)))
+    far = torch.tensor([max(2.0 ** -24, p * 2.0 ** -51) for p in at], device="cuda", dtype=torch.float64)[:, None, None]
+    e = torch.arange(rd // 2, device="cuda")
+    a, b = (e, e + rd // 2) if halves else (2 * e, 2 * e + 1)
+    for got, y in ((outs[0], x[:, :nh]), (outs[1], x[:, nh:nh + nkv])):
+        y, want = y.double(), y.double().clone()
+        want[..., a], want[..., b] = y[..., a] * c - y[..., b] * s, y[..., a] * s + y[..., b] * c
+        bound = torch.zeros_like(y)
+        bound[..., a] = bound[..., b] = (y[..., a].abs() + y[..., b].abs()) * (2 * math.pi * far + 5 * U)
+        within(got, want, bound)
+    assert torch.equal(outs[2], x[:, nh + nkv:]) and ctx.device_error() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("order", ["rows", "heads"])
 def test_attention_packed_rows_of_inputs_and_output(rrr, ctx, order):
     """One buffer of [q | k | v | out] rows, or of heads of such rows: the bits of separate arrays, and
