@@ -38,10 +38,14 @@ int rrr::cuda_error(rrr_ctx* ctx, cudaError_t e, const char* what) {
 }
 
 int rrr::bind_device(rrr_ctx* ctx) {
+  // A thread that has made no CUDA call has device 0 but no context, which the driver's tensor-map
+  // encoder needs (a launch would make it, too late): the first call of a thread sets the device
+  static thread_local int set = -1;
   int cur = -1;
-  if (cudaGetDevice(&cur) != cudaSuccess || cur != ctx->device) {
+  if (set != ctx->device || cudaGetDevice(&cur) != cudaSuccess || cur != ctx->device) {
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return cuda_error(ctx, e, "cudaSetDevice");
+    set = ctx->device;
   }
   return RRR_OK;
 }

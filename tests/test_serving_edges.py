@@ -5,6 +5,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -156,6 +157,50 @@ def test_python_host_runs_on_the_current_stream(rrr, monkeypatch):
 
 
 # ------------------------------------------------------------------ GPU
+def in_a_new_thread(call):
+    """call() in a thread that has made no CUDA call before; its exception here."""
+    raised = []
+
+    def run():
+        try:
+            call()
+        except Exception as e:
+            raised.append(e)
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    if raised:
+        raise raised[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("name", ["qk_norm_rope", "attention_packed", "store", "load", "attention"])
+def test_first_call_of_a_thread(rrr, ctx, hd, name):
+    """A thread that has made no CUDA call yet (a worker of a server) gives the bits of the main one."""
+    nh, nkv, n, t, g = 4, 2, 150, torch.bfloat16, gen(hd)
+    q, k, v = (normal(g, n, h, hd, dtype=t) for h in (nh, nkv, nkv))
+    cu, lens, cache = ints([0, n]), ints([n]), Cache(rrr, ctx, nkv, hd, [n], 1)
+    cache.c.store(k, v, cu, lens)
+    desc, ws = rrr.ffi.AttnDesc(nh, nkv, hd, 64, 1e4, 1.0, None, 0, 4096), cache.c.workspace(nh)
+    x, pos = normal(g, n, (nh + 2 * nkv) * hd), torch.arange(n, dtype=torch.int32, device="cuda")
+    got = []
+    for where in (lambda call: call(), in_a_new_thread):
+        out = [torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)]
+        if name == "store":
+            cache.pages.zero_()
+        torch.cuda.synchronize()
+        where({"qk_norm_rope": lambda: rrr.qk_norm_rope(ctx, desc, x, pos, *out),
+               "attention_packed": lambda: rrr.attention_packed(ctx, q, k, v, cu, cu, out[0]),
+               "store": lambda: cache.c.store(k, v, cu, lens),
+               "load": lambda: cache.c.load(cu, lens, *out[1:]),
+               "attention": lambda: cache.c.attention(q[:1], lens, out[0][:1], ws)}[name])
+        torch.cuda.synchronize()
+        got.append([cache.pages.clone(), *out])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and ctx.device_error() == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_continued_prompts_of_a_batch(rrr, ctx, hd):
