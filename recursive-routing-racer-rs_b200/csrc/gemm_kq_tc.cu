@@ -542,7 +542,8 @@ cudaError_t launch_t(const LaunchEnv& env, const TcPlan& pl, const void* w, cons
   p.err = env.d_err;
 
   auto kern = gemm_kq_tc_kernel<QT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem);
+  // (the function's on the device, whatever context or thread calls: one value for every plan)
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.n_tiles, pl.m_tiles, pl.splits);

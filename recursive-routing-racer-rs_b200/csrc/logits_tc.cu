@@ -350,7 +350,8 @@ cudaError_t launch_logits_tc(const LaunchEnv& env, const float* W, const float* 
     return cudaErrorInvalidValue;
 
   auto kern = logits_tc_kernel;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // (the function's on the device, whatever context or thread calls: one value for every batch)
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget);
   if (e != cudaSuccess) return e;
   const int grid = std::max(1, std::min(p.v_tiles * p.m_tiles, env.sm_count));
   return rrr_launch_pdl(kern, dim3(grid), dim3(kThreads), (size_t)smem, env.stream, env.pdl,

@@ -568,7 +568,7 @@ def test_attention_kv4_two_threads_with_a_context_each(rrr, ctx, hd, tmp_path):
     torch.cuda.synchronize()
     code = repeat(ctypes.cast(rrr.ffi.lib().rrr_attention_kv4, ctypes.c_void_p), calls, 30000)
     torch.cuda.synchronize()
+    assert code == 0, [rrr.ffi.last_error(x[4].h) for x in keep]
     for _, out, first, _, own, _ in keep:
-        assert code == 0, rrr.ffi.last_error(own.h)
         assert torch.equal(out, first) and own.device_error() == 0
         own.close()
