@@ -989,7 +989,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   constexpr int HD = 256, kChunks = HD / 64, kStages = 5;
   constexpr uint32_t kPiece = kTile * 128, kStage = 2 * kPiece;
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ uint64_t q_full, full[kStages], s_full[2], p_full, pv, o_full, fin;  // pv: all but the last block's
+  // p_full: one per place, as a warp may be through a block whose S came early while others are at the
+  // one before; pv: the products of all but the last block
+  __shared__ uint64_t q_full, full[kStages], s_full[2], p_full[2], pv, o_full, fin;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const PackedParams& p = tp.a;
@@ -1002,8 +1004,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
-    mbar_init(&p_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
     mbar_init(&pv, 1);
     mbar_init(&o_full, 1);
     mbar_init(&fin, 1);
@@ -1112,7 +1116,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     };
     bool ok = n == 0 || (wait(&q_full, 0) && scores(0));
     for (int j = 0; j < n && ok; ++j) {
-      ok = (j + 1 >= n || scores(j + 1)) && wait(&p_full, j);
+      ok = (j + 1 >= n || scores(j + 1)) && wait(&p_full[j & 1], j >> 1);
       if (!ok) break;
       const int steps = columns(j) / 16;
       for (int half = 0; half < 2 && ok; ++half, ++item) {  // O's columns 128 half .. + 127
@@ -1171,7 +1175,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
     if (ok && n > 0) ok = wait(&o_full, 0);
     tc_fence_after();

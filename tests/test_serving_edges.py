@@ -421,6 +421,27 @@ def test_attention_packed_maxima_that_grow_from_block_to_block(rrr, ctx, hd, kin
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("lq,lk,nh,nkv", [([257], [779], 8, 8), ([1121], [1121], 21, 3), ([30], [3000], 8, 8), ([90, 200, 7], [900, 1200, 2000], 5, 5)])
+@pytest.mark.parametrize("scale", [0.3, 1.0, 3.0])
+def test_attention_packed_warps_that_rescale_at_different_blocks(rrr, ctx, hd, kind, lq, lk, nh, nkv, scale):
+    """Scores of a size at which some warps of a tile rescale their sums, and wait for the products so
+    far, while others go on to the next block: no product takes weights that are not there yet."""
+    t = DT[kind]
+    for seed in range(3):
+        g = gen(seed + hd)
+        q, k, v = (normal(g, sum(n), h, hd, dtype=t) for n, h in ((lq, nh), (lk, nkv), (lk, nkv)))
+        out, again, cu_q, cu_kv = torch.empty_like(q), torch.empty_like(q), cu_of(lq), cu_of(lk)
+        rrr.attention_packed(ctx, q, k, v, cu_q, cu_kv, out, scale=scale)
+        check_packed(out, q, k, v, lq, lk, True, scale)
+        for _ in range(5):
+            rrr.attention_packed(ctx, q, k, v, cu_q, cu_kv, again, scale=scale)
+            assert torch.equal(out, again)
+    assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd,nh,nkv", [(64, 8, 1), (64, 4, 2), (64, 5, 1), (128, 6, 2), (128, 8, 1), (128, 7, 1), (256, 4, 2), (256, 8, 1), (256, 5, 1)])
 @pytest.mark.parametrize("lens", [[1, 17, 64, 0, 65, 128, 1023], [3000, 1, 130, 700], [30001], [150] * 90])
 @pytest.mark.parametrize("pattern", ["spread", "paired"])
