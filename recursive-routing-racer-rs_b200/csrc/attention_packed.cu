@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(kThreads) packed_kernel(const __grid_constant_
 // V rows behind the sequence are zeroed in shared memory before their product: other
 // sequences' values, or none, may be anything.
 //
-// Measured (head_dim 128): a prompt of 16,384 rows of 24 heads 1340 us at full clocks and 1500-1580
-// at the power limit (1.1 PFLOP/s), two tiles' block in some 3600 clocks, of which the products need
+// Measured (head_dim 128): a prompt of 16,384 rows of 24 heads 1575 us in a row of calls, at the power
+// limit (1.05 PFLOP/s), and 1340 once at full clocks, two tiles' block in some 3600 clocks, of which the products need
 // 2100 and the exponentials (16 a clock) 2050; short items pay 4 to 5 us for a CTA's start and end.
 // Tried without gain: exponentials by a polynomial, weights handed over by halves, two threads per
 // row, persistent CTAs with the longest items first.
@@ -976,7 +976,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // runs during the softmax of block j, S(0), S(1), PV(0), S(2), PV(1), ... A stage of the ring holds
 // half a tile, 128 KV rows x 128 values, which is half of S's depth or of O's columns. The copying
 // warp sees a stage free by the commit behind its products: s_full of K's, pv of V's.
-// Measured: 8,000 rows of 8 heads 227 us, 1150 TFLOP/s, the tensor cores 60 % busy, the L2 36 %.
+// Measured: 8,000 rows of 8 heads 223 us, 1175 TFLOP/s, the tensor cores 60 % busy, the L2 36 %.
 // Without the softmax it took 203 us, without the copies 211 (each product takes some 70 clocks of
 // 64, each commit holds up the next by 120, and a CTA's start and end are not overlapped). The
 // mma.sync kernel above took 2622 us.

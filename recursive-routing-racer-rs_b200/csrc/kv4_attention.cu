@@ -26,10 +26,10 @@
 // maximum, which is nearly every one, skips the exchange of maxima and the rescaling. Scores,
 // weights and sums keep f32 accuracy throughout.
 //
-// Bound by instructions: about 500 per warp for 16 rows of 4 heads x 128, where the issue slots
-// are 62 % taken (131,000 rows of 8 heads: 59 us, 2.8 TB/s of codes; 64 sequences, 261,424 rows:
-// 110 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA per SM (96 registers,
-// a few spilt) was 8 % slower, so it is not latency that is missing.
+// Bound by instructions and their latency: about 500 per warp for 16 rows of 4 heads x 128, where
+// the issue slots are 60 % taken by 12 warps (131,000 rows of 8 heads: 59 us, 2.8 TB/s of codes; 64
+// sequences, 261,424 rows: 110 us, 3.0 TB/s; the memory alone would take 26 and 51 us). A fourth CTA
+// per SM leaves 96 registers, some of which spilt: 8 % slower.
 //
 // Work. A unit is one page (64 rows) of one (sequence, KV head), and each of those has kStart units
 // more in front, which is what beginning and ending one costs. The CTAs share all U units of the
@@ -830,7 +830,7 @@ template <int HD, typename T>
 cudaError_t launch_tiles(const LaunchEnv& env, Kv4Params p) {
   // Six and eight queries per KV head of 128 or 256 values are taken as two heads of half as many,
   // which read the pages twice but keep more warps on an SM. (Eight queries on 4 KV heads, 10 x
-  // 20,000 rows and 1 x 2,000: 209 -> 165 us and 29.5 -> 19.7 us with 256 values, 82 -> 84 and 18.1
+  // 20,000 rows and 1 x 2,000: 209 -> 166 us and 29.5 -> 19.7 us with 256 values, 82 -> 84 and 18.1
   // -> 13.5 with 128. With 64 values the second tile of columns costs less than the unpacking that
   // it saves: 45 us against 59.)
   if (HD >= 128 && p.hpk > 4 && p.hpk % 2 == 0 && (int64_t)p.n_seqs * p.nkv <= INT32_MAX / 2) {

@@ -16,7 +16,7 @@
 // are computed once for all its heads and a partner of a pair (i, i + rope_dim/2) sits in
 // another lane at the same place (rope_dim a multiple of 2D). Four heads are in flight per warp,
 // and their sums of squares are reduced together: 16,000 rows of 48 heads of 128 values, f32 to
-// bf16, take 95 us, 6.2 TB/s (124 us head by head, with the norm and the rotation decided per
+// bf16, take 100 us, 5.9 TB/s (124 us head by head, with the norm and the rotation decided per
 // head). One row is 3 us of launch; it is spread over as many warps as it has fours of heads.
 #include <math.h>
 
