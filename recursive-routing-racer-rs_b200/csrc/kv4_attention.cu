@@ -23,7 +23,7 @@
 // 1e-4 behind a first row that draws the weight, as texts have, came out with 8 bits.) The
 // tensor core truncates its sums, so they are moved to shared memory, rounded, every kFlush pages.
 // The softmax runs online in base 2, with 32-bit maxima and sums: a slice of rows without a new
-// maximum, which is nearly every one, skips the exchange of maxima and the rescaling. Scores,
+// maximum, as most of a long run are, skips the exchange of maxima and the rescaling. Scores,
 // weights and sums keep f32 accuracy throughout.
 //
 // Bound by instructions and their latency: about 500 per warp for 16 rows of 4 heads x 128, where
@@ -73,7 +73,7 @@ struct Kv4Params {
   const int* lens;
   float scale;  // with log2(e)
   int2* runs;    // [seq][head]: first CTA and CTAs of its pages
-  float* parts;  // [CTA][2][hpk * (HD + 2)]: sums, maxima, weights' sums
+  float* parts;  // [CTA][2][hpk * (HD + 2)]: sums, references, weights' sums
   int stages, stage_bytes;
   int ctas;      // of the first kernel
   int* err;
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<HD, NT>())
 // lane, and the rest are groups that take every `groups`-th part each, kAtOnce of them in flight;
 // the groups' sums are added in order. Few heads: one warp across, and CTAs for the other columns,
 // as each has many parts; many heads: four across, as most have one or two. Every thread takes its
-// head's maxima and weights' sums along with the values. (A pass for them first, by one warp per
+// head's references and weights' sums along with the values. (A pass for them first, by one warp per
 // query head, and four across always: one sequence of 1,023 rows 11.6 us instead of 10.4, of
 // 131,000 66.7 instead of 59.4. One across always: 64 sequences 116 us instead of 111.)
 constexpr int kJoinWarps = 16, kAtOnce = 4;
