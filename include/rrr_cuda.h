@@ -476,6 +476,76 @@ int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, const void* q, 
                          const void* v, const int32_t* cu_q, const int32_t* cu_kv, void* out,
                          void* stream);
 
+/* ---- a step of speculative decoding over the 4-bit cache -----------------------------
+ * A cheaper source drafts tokens behind the last one of every sequence and the model checks them
+ * in one step. A sequence's packed rows are a tree: row 0 its last token, whose K and V are not
+ * cached yet, each other row a drafted token whose parent, parents[cu[s] + i] < i (a row of the
+ * sequence, -1 at row 0), is the token before it; parents NULL: chains, parent i - 1. The step:
+ * QKV rows (rrr_qk_norm_rope for each row's own position, kv_lens[s] + depth), per layer
+ * rrr_attention_tree_kv4; from the logits rrr_verify_drafts says which rows stand; per layer
+ * rrr_kv4_append of those. Lengths, trees and results stay on the device. */
+
+/* Appends QKV rows [Q heads | K heads | V heads] to the cache, in one pass: K heads normed and
+ * rotated as by rrr_qk_norm_rope (its a, gammas, eps and halves) and quantised from 32 bits, V heads
+ * quantised, as rrr_kv4_store holds them. Sequence s has kv_lens[s] rows afterwards, and its packed
+ * rows are its last ones. q not NULL: its rows get the query heads, normed and rotated, in out_type.
+ * path and counts not NULL (then q is NULL): of sequence s the counts[s] rows path[cu[s]],
+ * path[cu[s] + 1], .. (rows of the sequence) are appended in this order, no others: the accepted
+ * rows of rrr_verify_drafts. A row is rotated for positions[row], or, with positions NULL, for its
+ * place in the cache; 0 <= position < a->max_seq, and a row outside is left out. */
+int rrr_kv4_append(rrr_ctx* ctx, const rrr_attn_desc* a, const rrr_kv4_cache* c, int in_type,
+                   const void* qkv, int64_t row_stride, int rows, const int32_t* cu_rows,
+                   const int32_t* kv_lens, const int32_t* path, const int32_t* counts,
+                   const int32_t* positions, const float* q_gamma, const float* k_gamma, float eps,
+                   int halves, int out_type, void* q, int64_t q_stride, void* stream);
+
+/* Attention of a tree's rows: row i of sequence s over its kv_lens[s] cached rows and, among the
+ * sequence's packed rows, over i and its ancestors: out_i = sum_j softmax_j(scale * q_i . k_j) v_j,
+ * at most 8 query heads per KV head. q, k and v are the rows' own, normed and rotated; 16-bit
+ * types; scale 0 = 1/sqrt(head_dim). At most 128 rows of a sequence: one with more is left as it was
+ * (and recorded). A kv_lens out of range counts as 0, rows on pages that do not exist are left out, and
+ * a parent that does not lie before its row is none. Scores and softmax statistics in 32 bits.
+ * Pointers 16-byte aligned, strides multiples of 8 elements; out overlaps no input. workspace:
+ * rrr_tree_workspace bytes for this cache and rows (or more of either), whatever they hold; calls that can
+ * run at the same time, replays of captured graphs among them, need one each. */
+typedef struct rrr_tree_desc {
+  int type;     /* RRR_F16 or RRR_BF16: q, k, v and out */
+  int n_heads;
+  int rows;     /* of q, k, v and out */
+  float scale;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head; /* strides */
+} rrr_tree_desc;
+int rrr_tree_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int rows, int64_t* bytes);
+int rrr_attention_tree_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, const rrr_tree_desc* d,
+                           const void* q, const void* k, const void* v, const int32_t* cu_rows,
+                           const int32_t* parents, const int32_t* kv_lens, void* out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* Which drafted rows stand, and the token that follows them. logits: row r is the target's behind
+ * row r's token; temperature f32[n_seqs] (NULL: 1); p = softmax(logits / temperature). uniforms
+ * f32[rows][2] in [0, 1): an acceptance and a draw for every row. A token is drawn from p as the first
+ * i with p_0 + .. + p_i > u; at temperature 0 it is the largest logit's, the first of equals. NaN
+ * counts as -inf and +inf as the largest finite value; a row without any value draws -1.
+ * draft NULL: from row 0 on, a token is drawn at the row; where a child carries it (the first such
+ * child) the walk goes on there, else it ends.
+ * draft not NULL: its row r is the draft's logits that token r was drawn from (row 0 of a
+ * sequence is not read), at the same temperature, q = softmax(draft / temperature); chains only
+ * (parents NULL). Token x of row r stands if u q(x) < p(x), u = uniforms[r][0], p of row r - 1; at
+ * the first that does not the next token is drawn from max(p - q, 0) normalised (p, where that is
+ * zero), behind the last row of all from p, by uniforms[.][1] of the last row that stands. At
+ * temperature 0 a draft stands if it is the largest logit's.
+ * path int32[rows]: of each sequence the rows that stand in their order, row 0 first, then -1;
+ * counts int32[n_seqs]: how many stand (0 without rows); next_tokens int32[n_seqs]: the token drawn
+ * last (-1 without rows). A token outside 0 .. vocab - 1 does not stand. Exponentials and sums are
+ * held in 64 bits. A temperature that is negative, infinite or NaN counts as 0. logits and draft: rows of `type`, aligned to
+ * their elements. workspace: rrr_verify_workspace bytes, 16-byte aligned, as for rrr_attention_tree_kv4. */
+int rrr_verify_workspace(rrr_ctx* ctx, int rows, int vocab, int n_seqs, int with_draft, int64_t* bytes);
+int rrr_verify_drafts(rrr_ctx* ctx, int type, const void* logits, int64_t logits_stride,
+                      const void* draft, int64_t draft_stride, int rows, int vocab, int n_seqs,
+                      const int32_t* cu_rows, const int32_t* tokens, const int32_t* parents,
+                      const float* uniforms, const float* temperature, int32_t* path, int32_t* counts,
+                      int32_t* next_tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Phi-4-mini-shape decode step (replaces forward_gpu, phi4.rs:1099-1196) --------
  * max_seq == 0: one token at position 0 (attention output = V, see RRR_X_GQA_V): per layer
  *   h += Wo . expand(V(Wqkv . rms(h)*g_attn)); h += Wdown . (silu(g) * u),

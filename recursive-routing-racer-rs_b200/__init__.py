@@ -12,7 +12,7 @@ from .engine import ComputeEngine, GpuBuffer, QType, gpu_matmul_f32, gpu_matmul_
 from .ffi import Context, RRRError  # noqa: F401
 from .gguf import GGUFModel, TensorInfo  # noqa: F401
 from .phi4 import ModelConfig, Phi4Decoder, SyntheticPhi4  # noqa: F401
-from .serving import KV4Cache, attention_packed, qk_norm_rope  # noqa: F401
+from .serving import KV4Cache, attention_packed, qk_norm_rope, verify_drafts, verify_workspace  # noqa: F401
 
 
 def build(verbose: bool = False) -> str:

@@ -1214,33 +1214,6 @@ bool encode_heads(CUtensorMap* map, int type, const void* base, int hd, int64_t 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows of heads of hd 16-bit values; strides in elements.
-struct HeadRows {
-  const void* p;
-  int64_t rows, row, heads, head, hd;
-};
-// Whether two such arrays share no byte, for certain: their extents do not meet, or all of their
-// places lie apart modulo a stride (both in one buffer whose rows or heads hold a part of each).
-bool apart(const HeadRows& a, const HeadRows& b) {
-  using Wide = __int128;
-  if (a.rows < 1 || b.rows < 1) return true;
-  auto from = [](const HeadRows& x) { return (Wide) reinterpret_cast<uintptr_t>(x.p); };
-  // bytes from the first place to the end of the last, where multiples of m elements do not count
-  auto width = [](const HeadRows& x, int64_t m) {
-    Wide w = x.hd;
-    if (m == 0 || x.row % m) w += (Wide)(x.rows - 1) * x.row;
-    if (m == 0 || x.head % m) w += (Wide)(x.heads - 1) * x.head;
-    return 2 * w;
-  };
-  const Wide between = from(b) - from(a);
-  if (between >= width(a, 0) || -between >= width(b, 0)) return true;
-  for (const int64_t m : {a.row, a.head, b.row, b.head}) {
-    const Wide period = 2 * (Wide)m, off = (between % period + period) % period;
-    if (off >= width(a, m) && off + width(b, m) <= period) return true;
-  }
-  return false;
-}
-
 // Query rows of a CTA of the tcgen05 kernels
 int rows_per_cta(int hd, int hpk) { return (hd == 256 ? 1 : 2) * (kTile / hpk); }
 

@@ -116,59 +116,6 @@ __device__ __forceinline__ int slot_of() {
   return (int)(((blockIdx.z >> 1) * gridDim.y + blockIdx.y) * kRowWarps + (threadIdx.x >> 5));
 }
 
-// Codes of four values by the division itself (out of line: rarely called)
-__device__ __noinline__ uint32_t divided(float a, float b, float c, float e, float m, float d) {
-  auto code = [&](float x) {
-    return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, m), d)), 0.f), 15.f);
-  };
-  return code(a) | code(b) << 4 | code(c) << 8 | code(e) << 12;
-}
-// The least and the largest of three, NaN where one is
-__device__ __forceinline__ float least(float a, float b, float c) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ float largest(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-// Eight values of a group of 32, which four neighbouring lanes hold: their codes, value i at bit
-// 4i, and the group's d and m.
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, __half& m16) {
-  const float inf = __int_as_float(0x7f800000);
-  float lo = least(least(x[0], x[1], x[2]), least(x[3], x[4], x[5]), least(x[6], x[7], x[7]));
-  float hi = largest(largest(x[0], x[1], x[2]), largest(x[3], x[4], x[5]), largest(x[6], x[7], x[7]));
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
-    lo = least(lo, l, l);
-    hi = largest(hi, h, h);
-  }
-  const bool finite = fabsf(lo) < inf && fabsf(hi) < inf;
-  // (hi - lo) / 15 by the product with 1/15 and its remainder
-  const float range = __fsub_rn(hi, lo), first = __fmul_rn(range, 1.f / 15.f);
-  const float step = fmaf(fmaf(-15.f, first, range), 1.f / 15.f, first);
-  m16 = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-  d16 = finite ? __float2half_rn(fminf(range > 1e6f ? 65504.f : step, 65504.f)) : __ushort_as_half(0x7fff);
-  const float d = __half2float(d16), m = __half2float(m16);
-  const float inv = d > 0.f ? __fdividef(1.f / 15.f, d) : 0.f;
-  uint32_t w = 0;
-  bool near = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv));  // in units of 15, within 0..15
-    const float t = fmaf(q, 15.f, 12582912.f);                      // the nearest integer in the low bits
-    near |= fabsf(fmaf(q, 15.f, 12582912.f - t)) > 0.49999f;
-    w += __float_as_uint(t) << (4 * i);
-  }
-  // what 12582912's own bits added
-  w -= 0x4b400000u + 0xb4000000u + 0x40000000u;
-  if (near && d > 0.f)
-    w = divided(x[0], x[1], x[2], x[3], m, d) | divided(x[4], x[5], x[6], x[7], m, d) << 16;
-  return w;
-}
 // The same eight values back
 __device__ __forceinline__ void dequantise(uint32_t w, float d, float m, float (&x)[8]) {
 #pragma unroll

@@ -27,7 +27,6 @@
 namespace rrr {
 namespace {
 
-constexpr int kMaxPairs = 64;
 constexpr int kQkWarps = 4;
 constexpr int kFew = 4;  // heads in flight per warp
 // ... and of 128 values in 16 bits, where there are as many: 6,000 rows of 24 + 8 + 8 heads in bf16
@@ -84,14 +83,7 @@ __global__ void __launch_bounds__(32 * kQkWarps) qk_rows_kernel(const __grid_con
       const int i = HALVES ? (e < p.half_dim ? e : e - p.half_dim) : e >> 1;
       double t = p.turns[i];
       if (i < p.n_factors) t /= (double)p.factors[i];
-      t -= floor(t);
-      const unsigned long long F = __double2ull_rd(t * 18446744073709551616.0);
-      const unsigned long long a = F * (unsigned long long)(unsigned)pos;
-      const float frac = (float)(int)(unsigned)(a >> 32) * 4.656612873077393e-10f;  // 2 x turns, in [-1, 1)
-      float s, c;
-      sincospif(frac, &s, &c);
-      cs[d] = c * p.attn_factor;
-      sn[d] = s * p.attn_factor;
+      rope_turn(t, pos, p.attn_factor, cs[d], sn[d]);
       // the first of a pair subtracts its partner's product, the second adds it
       if (HALVES && e < p.half_dim) sn[d] = -sn[d];
     }
@@ -275,12 +267,7 @@ extern "C" int rrr_qk_norm_rope(rrr_ctx* ctx, const rrr_attn_desc* a, int in_typ
   p.max_pos = a->max_seq;
   p.eps = eps;
   p.attn_factor = a->rope_attn_factor;
-  // theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64
-  double fine[8], coarse[kMaxPairs / 8];
-  for (int i = 0; i < 8; ++i) fine[i] = pow((double)a->rope_theta, -2.0 * i / a->rope_dim);
-  for (int i = 0; 8 * i < p.half_dim; ++i)
-    coarse[i] = pow((double)a->rope_theta, -16.0 * i / a->rope_dim) / 6.283185307179586476925;
-  for (int i = 0; i < p.half_dim; ++i) p.turns[i] = coarse[i / 8] * fine[i % 8];
+  rope_turns(p.turns, a->rope_theta, a->rope_dim);
   // all heads of a row in one warp once the rows alone fill the GPU's warps
   const int want = ctx->sm_count * 16;
   int chunks = (int)(((int64_t)want + rows - 1) / rows);

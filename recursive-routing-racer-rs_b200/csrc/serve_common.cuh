@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "capi_internal.h"
@@ -61,6 +62,26 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   *reinterpret_cast<Words<N * (int)sizeof(T)>*>(p) = u.raw;
 }
 
+// cos and sin (times af) of a rotation by pos * t turns, t = f / factor / 2 pi (qk_rows.cu has the
+// mathematics and the error).
+__device__ __forceinline__ void rope_turn(double t, int pos, float af, float& c, float& s) {
+  t -= floor(t);
+  const unsigned long long F = __double2ull_rd(t * 18446744073709551616.0);
+  const unsigned long long a = F * (unsigned long long)(unsigned)pos;
+  const float frac = (float)(int)(unsigned)(a >> 32) * 4.656612873077393e-10f;  // 2 x turns, in [-1, 1)
+  sincospif(frac, &s, &c);
+  c *= af;
+  s *= af;
+}
+constexpr int kMaxPairs = 64;  // rope_dim / 2
+// turns[i] = theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64
+inline void rope_turns(double (&turns)[kMaxPairs], float theta, int rope_dim) {
+  double fine[8], coarse[kMaxPairs / 8];
+  for (int i = 0; i < 8; ++i) fine[i] = pow((double)theta, -2.0 * i / rope_dim);
+  for (int i = 0; 16 * i < rope_dim; ++i) coarse[i] = pow((double)theta, -16.0 * i / rope_dim) / 6.283185307179586476925;
+  for (int i = 0; 2 * i < rope_dim; ++i) turns[i] = coarse[i / 8] * fine[i % 8];
+}
+
 __device__ __forceinline__ void flag_position(int* err) {
   if (err) atomicCAS(err, 0, (int)kDevErrPosition);
 }
@@ -87,6 +108,33 @@ inline bool rows_disjoint(const RowSet& a, const RowSet& b) {
   if (a.stride != b.stride || a.stride < 1) return false;
   const int64_t d = (int64_t)(pb - pa) % a.stride, off = d < 0 ? d + a.stride : d;
   return off >= a.width && off + b.width <= a.stride;
+}
+
+// Rows of heads of hd 16-bit values; strides in elements.
+struct HeadRows {
+  const void* p;
+  int64_t rows, row, heads, head, hd;
+};
+// Whether two such arrays share no byte, for certain: their extents do not meet, or all of their
+// places lie apart modulo a stride (both in one buffer whose rows or heads hold a part of each).
+inline bool apart(const HeadRows& a, const HeadRows& b) {
+  using Wide = __int128;
+  if (a.rows < 1 || b.rows < 1) return true;
+  auto from = [](const HeadRows& x) { return (Wide) reinterpret_cast<uintptr_t>(x.p); };
+  // bytes from the first place to the end of the last, where multiples of m elements do not count
+  auto width = [](const HeadRows& x, int64_t m) {
+    Wide w = x.hd;
+    if (m == 0 || x.row % m) w += (Wide)(x.rows - 1) * x.row;
+    if (m == 0 || x.head % m) w += (Wide)(x.heads - 1) * x.head;
+    return 2 * w;
+  };
+  const Wide between = from(b) - from(a);
+  if (between >= width(a, 0) || -between >= width(b, 0)) return true;
+  for (const int64_t m : {a.row, a.head, b.row, b.head}) {
+    const Wide period = 2 * (Wide)m, off = (between % period + period) % period;
+    if (off >= width(a, m) && off + width(b, m) <= period) return true;
+  }
+  return false;
 }
 
 // Makes the context's device current for one call and puts the caller's back.

@@ -88,6 +88,13 @@ class KV4Desc(ctypes.Structure):
                 ("page_table", c_void_p), ("n_seqs", c_int), ("max_pages", c_int), ("table_stride", c_int64)]
 
 
+class TreeDesc(ctypes.Structure):
+    """rrr_tree_desc: attention of drafted trees."""
+    _fields_ = [("type", c_int), ("n_heads", c_int), ("rows", c_int), ("scale", c_float), ("q_row", c_int64),
+                ("q_head", c_int64), ("k_row", c_int64), ("k_head", c_int64), ("v_row", c_int64),
+                ("v_head", c_int64), ("out_row", c_int64), ("out_head", c_int64)]
+
+
 vp = c_void_p
 PROTOS = {
     "rrr_abi_version": (c_int, []),
@@ -179,6 +186,14 @@ PROTOS = {
     "rrr_attention_kv4": (c_int, [vp, POINTER(KV4Desc), c_int, c_int, vp, c_int64, vp, c_float, vp, c_int64,
                                   vp, c_int64, vp]),
     "rrr_attention_packed": (c_int, [vp, POINTER(PackedDesc), vp, vp, vp, vp, vp, vp, vp]),
+    "rrr_kv4_append": (c_int, [vp, POINTER(AttnDesc), POINTER(KV4Desc), c_int, vp, c_int64, c_int, vp, vp, vp, vp, vp,
+                               vp, vp, c_float, c_int, c_int, vp, c_int64, vp]),
+    "rrr_tree_workspace": (c_int, [vp, POINTER(KV4Desc), c_int, c_int, POINTER(c_int64)]),
+    "rrr_attention_tree_kv4": (c_int, [vp, POINTER(KV4Desc), POINTER(TreeDesc), vp, vp, vp, vp, vp, vp, vp, vp, c_int64,
+                                       vp]),
+    "rrr_verify_workspace": (c_int, [vp, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
+    "rrr_verify_drafts": (c_int, [vp, c_int, vp, c_int64, vp, c_int64, c_int, c_int, c_int, vp, vp, vp, vp, vp, vp, vp,
+                                  vp, vp, c_int64, vp]),
     "rrr_embed_rows": (c_int, [vp, c_int, vp, c_int64, c_int, vp, c_int, vp, vp]),
     "rrr_fill_kquant_random": (c_int, [vp, c_int, vp, c_int64, c_uint64, vp]),
     "rrr_fill_f32_normal": (c_int, [vp, vp, c_int64, c_float, c_float, c_uint64, vp]),
