@@ -101,8 +101,8 @@ def random_tree(rng, n, kind):
     if kind == "chain":
         return [i - 1 for i in range(n)]
     if kind == "star":
-        return [-1] + [0] * (n - 1)
-    return [-1] + [int(rng.integers(max(0, i - 6), i)) for i in range(1, n)]
+        return ([-1] + [0] * (n - 1))[:n]
+    return ([-1] + [int(rng.integers(max(0, i - 6), i)) for i in range(1, n)])[:n]
 
 
 # ------------------------------------------------------------------ CPU
