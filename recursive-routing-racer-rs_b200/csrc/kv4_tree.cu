@@ -37,11 +37,13 @@ struct TreeParams {
   float scale;   // with log2(e)
   int* err;
   // workspace
-  int4* runs;     // [seq][KV head][tile]: first CTA, CTAs, whether to compute again
-  float2* stats;  // [slot][column]: maximum, sum
-  int* again;     // [slot]
-  float* parts;   // [slot][column][value]
-  int most_tiles, ctas;
+  struct Opened* opened;  // [CTA]: the segment that it opened and shares
+  float2* stats;          // [slot][column]: maximum, sum
+  int* again;             // [slot]
+  float* parts;           // [slot][column][value]
+};
+struct Opened {
+  int run, seq, kv, r0, len, c0, cols, pad;  // run: CTAs that share it, 0 for none
 };
 
 // ---- what the sequences are
@@ -69,17 +71,25 @@ __device__ __forceinline__ Shape shape_of(const TreeParams& p, int seq) {
   s.blocks = s.nodes ? (s.len + kRows - 1) / kRows + 1 : 0;
   return s;
 }
-__device__ __forceinline__ long long units_of(const TreeParams& p, const Shape& s) {
-  return s.nodes ? (long long)s.tiles * p.nkv * (s.blocks + kStart) : 0;
+__device__ __forceinline__ int units_of(const TreeParams& p, const Shape& s) {
+  return s.nodes ? s.tiles * p.nkv * (s.blocks + kStart) : 0;
 }
+// The units of a CTA: U / G each, one more for the first U % G
+struct Share {
+  int each, more;
+  __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ int cta_of(int unit) const {
+    const int wide = more * (each + 1);
+    return unit < wide ? unit / (each + 1) : more + (unit - wide) / each;
+  }
+};
 
 enum { kDraft = 1, kFirst = 2, kLast = 4, kAlone = 8, kStop = 16, kOpens = 32 };
 struct Info {  // of a block
-  int flags, seq, kv, seg;    // seg: index in runs
+  int flags, seq, kv, len;
   int r0, nodes, c0, cols, n; // the tile's columns c0 .. c0 + cols - 1 of the sequence's (row, head) pairs; n: with the padding
   int valid[2];               // rows of each page that count
-  int slot, count, run;       // where a shared segment's part goes, the segment's number in this CTA, its CTAs
-  int first_cta;
+  int count, run;             // the segment's number in this CTA, its CTAs
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -102,10 +112,9 @@ __device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, int* 
   return warp_wait(bar, parity, err);
 }
 
-// Bounded barrier of four warps; `any`: which also tells whether one of their lanes says yes.
+// Bounded barrier of four warps.
 struct Quartet {
   uint64_t* bar;
-  volatile int* votes;  // [2][4]
   uint32_t phase;
   int* err;
   __device__ __forceinline__ bool operator()() {
@@ -115,14 +124,19 @@ struct Quartet {
     phase ^= 1;
     return ok;
   }
-  __device__ __forceinline__ bool any(bool yes, bool& ok) {
-    volatile int* v = votes + 4 * phase;
-    yes = __any_sync(0xffffffffu, yes);
-    if ((threadIdx.x & 31) == 0) v[(threadIdx.x >> 5) & 3] = yes;
-    ok = (*this)();
-    return (v[0] | v[1] | v[2] | v[3]) != 0;
-  }
 };
+// A barrier of 128 threads that tells whether one of them says yes. (All of them pass as many of these, also where a
+// wait gave up.)
+__device__ __forceinline__ bool any_of_128(int id, bool yes) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)yes), "r"(id)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
@@ -167,10 +181,10 @@ __device__ __forceinline__ float to_one(uint32_t top, bool& fine) {
   return !fine || top == 0 ? 1.f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
 }
 constexpr uint32_t kHalfMax = 0x477fe000u;  // 65504
-// What drafted values of at most `top` are multiplied by, 2^-e, so that f16 holds them with all their bits
-__device__ __forceinline__ float lift_of(uint32_t top) {
-  return top >= 0x3b000000u /* 2^-9 */ ? 1.f : top >= 0x37000000u /* 2^-17 */ ? 256.f : 65536.f;
-}
+// Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, so that f16 holds them with all their bits (and
+// their rows' weights are divided by it, which have bits to spare)
+__device__ __forceinline__ int lift_of(uint32_t top) { return top >= 0x3b000000u /* 2^-9 */ ? 0 : top >= 0x37000000u /* 2^-17 */ ? 1 : 2; }
+__device__ __forceinline__ float lifted_by(int lift) { return lift == 0 ? 1.f : lift == 1 ? 256.f : 32768.f; }
 // Eight 16-bit values times s as f16, in the order (0,4) (1,5) (2,6) (3,7) in which a word of K's codes comes apart
 template <typename T>
 __device__ __forceinline__ void scaled_pairs(const uint4& w, float s, uint32_t (&x)[4]) {
@@ -183,29 +197,6 @@ __device__ __forceinline__ void scaled_pairs(const uint4& w, float s, uint32_t (
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = as_u32(__floats2half2_rn(v[i], v[i + 4]));
-}
-
-// The sum over the warp's lanes of each of N values; lane l gets that of column_of<N>(l).
-template <int N>
-__device__ __forceinline__ int column_of(int lane) { return N >= 32 ? lane : lane % N; }
-template <int N>
-__device__ __forceinline__ float transposed_sum(float (&v)[N]) {
-  static_assert(N == 32 || N == 16, "");
-  const int lane = threadIdx.x & 31;
-  int n = N;
-#pragma unroll
-  for (int o = N / 2; o > 0; o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int k = 0; k < N / 2; ++k)
-      if (k < o) {
-        const float give = up ? v[k] : v[k + o], keep = up ? v[k + o] : v[k];
-        v[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
-  }
-  (void)n;
-  if constexpr (N == 16) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
-  return v[0];
 }
 
 template <int HD, int NT>
@@ -224,31 +215,90 @@ struct Sizes {
   static constexpr int kFit = (227 * 1024 - kStatic - 1024 - kFixed) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kFixed + kStages * kStage + 1024;
-  static constexpr int kSCol = 2 * kKCols, kOCol = kSCol + 2 * NT;
-  static_assert(kStages >= 2 && kOCol + kHalves * NT <= 512, "");
+  // TMEM: keys, scores, sums of the weights, O, and ones times 2^0, 2^8 and 2^15
+  static constexpr int kKs = 2 * kKCols + (3 + kHalves) * NT + 24 <= 512 ? 2 : 1;  // places for K
+  static constexpr int kSCol = kKs * kKCols, kLCol = kSCol + 2 * NT, kOCol = kLCol + NT, kOnes = kOCol + kHalves * NT;
+  static_assert(kStages >= 2 && kOnes + 24 <= 512, "");
 };
+
+// One row of one query head by one warp in 32-bit arithmetic, over the rows that it sees and no others:
+// for what f16 does not hold (values that are not finite, or of 65,520 and more). Lane l has the values D l .. D l + D - 1.
+template <int HD, typename T>
+__device__ __noinline__ void plain_row(const TreeParams& p, int seq, int r0, int len, int row, int kv, int head) {
+  using B = Kv4Block<HD>;
+  constexpr int D = HD / 32;
+  const int e0 = D * (threadIdx.x & 31);
+  float q[D], o[D], m = kNone, l = 0.f;
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] = 0.f;
+  load_vec<T, D>(static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head + e0, q);
+  auto take = [&](const float (&k)[D], const float (&v)[D]) {
+    float s = 0.f;
+#pragma unroll
+    for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
+    s = warp_sum(s) * p.scale;
+    const float top = fmaxf(m, s), keep = ex2(m - top), w = ex2(s - top);
+    m = top;
+    l = fmaf(l, keep, w);
+#pragma unroll
+    for (int d = 0; d < D; ++d) o[d] = fmaf(o[d], keep, w * v[d]);
+  };
+#pragma unroll 1
+  for (int at = 0; at < len; ++at) {
+    const int page = p.table[(int64_t)seq * p.table_stride + at / kPageRows], r = at % kPageRows;
+    if (page < 0 || page >= p.n_pages) continue;
+    const uint8_t* blk = p.pages + ((int64_t)page * p.nkv + kv) * B::kBytes;
+    const uint8_t* vb = blk + B::kHalf;
+    const int j = e0 / 32;
+    const __half* ks = reinterpret_cast<const __half*>(blk + B::kCodes);
+    const __half* vs = reinterpret_cast<const __half*>(vb + B::kCodes);
+    const uint32_t word = reinterpret_cast<const uint32_t*>(blk)[B::k_word(r, j, e0 % 32 / 8)];
+    const float kd = __half2float(ks[B::scale(r, j)]), km = __half2float(ks[HD * 2 + B::scale(r, j)]);
+    const float vd = __half2float(vs[B::scale(r, j)]), vm = __half2float(vs[HD * 2 + B::v_min(r, j)]);
+    float k[D], v[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int e = e0 + d;
+      k[d] = fmaf((float)((word >> (4 * (e % 8))) & 15u), kd, km);
+      const uint32_t c = reinterpret_cast<const uint16_t*>(vb)[B::v_half(r, j, e % 8)];
+      v[d] = fmaf((float)((c >> (4 * (e % 32 / 8))) & 15u), vd, vm);
+    }
+    take(k, v);
+  }
+  // the row and its ancestors; a parent that does not lie before its child is none
+#pragma unroll 1
+  for (int node = row - r0; node >= 0;) {
+    float k[D], v[D];
+    load_vec<T, D>(static_cast<const T*>(p.k) + (r0 + node) * p.k_row + kv * p.k_head + e0, k);
+    load_vec<T, D>(static_cast<const T*>(p.v) + (r0 + node) * p.v_row + kv * p.v_head + e0, v);
+    take(k, v);
+    const int above = p.parents ? p.parents[r0 + node] : node - 1;
+    node = above < node ? above : -1;
+  }
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] = o[d] / l;
+  store_vec<T, D>(static_cast<T*>(p.out) + row * p.out_row + head * p.out_head + e0, o);
+}
 
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ TreeParams p) {
   using S = Sizes<HD, NT>;
   constexpr int G = HD / 32, J = G < 4 ? G : 4, PL = G / J;  // groups, groups per plane, planes
-  constexpr int kHalfCols = NT / 2;
   extern __shared__ uint8_t smem_dyn[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages], k_full[2], s_full[2], v_full[S::kVs], p_full[2], p_empty[2], o_empty, fin;
+  __shared__ uint64_t teams[2];                   // of K's and V's warps
   __shared__ Info infos[kInfos];
   __shared__ uint4 seen[4][kMaxNodes];            // of a tree's row: the rows that it sees, as bits
   __shared__ int up[kMaxNodes];
-  __shared__ float q_scale[4][NT], k_scale[4][kRows], v_lift[4];
+  __shared__ float k_scale[4][kRows];
+  __shared__ int v_lift[4];
   __shared__ int k_again[4], v_again[4];
-  __shared__ uint32_t k_tops[4], v_tops[4];
-  __shared__ __align__(16) float2 line[NT];       // of a column: s = score * x, argument = s + y
-  __shared__ float quad[2][4][kHalfCols], change[2][kHalfCols];
-  __shared__ long long warp_units[kThreads / 32], first_base;
-  __shared__ int first_seq;
+  __shared__ uint32_t v_tops[4];
+  __shared__ __align__(16) float2 lines[4][NT];   // of a column: the argument of a weight's exponential is score * x + y
+  __shared__ float quad[2][4][NT / 2], change[2][NT / 2];
+  __shared__ int warp_units[kThreads / 32], first_base, first_seq, dead[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ uint64_t teams[4];   // of the softmax's halves, K's and V's warps
-  __shared__ int votes[2][2][4];
   uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
   uint8_t* const qs = smem;
   uint8_t* const vs = qs + S::kQ;
@@ -265,217 +315,216 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 8);
       mbar_init(&p_empty[i], 1);
+      mbar_init(&teams[i], 4);
+      dead[i] = 0;
     }
     for (int i = 0; i < S::kVs; ++i) mbar_init(&v_full[i], 4);
     mbar_init(&o_empty, 8);
     mbar_init(&fin, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&teams[i], 4);
     fence_mbarrier_init();
     prefetch_map(&map);
   }
+  if (warp == 16) tmem_alloc(&tmem_slot, 512);
   pdl_launch_dependents();
   pdl_wait();
 
   // ---- this CTA's units [u0, u1) of all U
   const int per = (p.n_seqs + kThreads - 1) / kThreads;
   const int my0 = min(p.n_seqs, (int)threadIdx.x * per), my1 = min(p.n_seqs, my0 + per);
-  long long mine = 0;
+  int mine = 0;
   for (int s = my0; s < my1; ++s) mine += units_of(p, shape_of<NT>(p, s));
-  long long upto = mine;
+  int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
   if (lane == 31) warp_units[warp] = upto;
+  if (threadIdx.x == 0) p.opened[blockIdx.x].run = 0;
+  tc_fence_before();
   __syncthreads();
-  long long before = upto - mine, U = 0;
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  int before = upto - mine, U = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += warp_units[w];
     U += warp_units[w];
   }
-  const long long grid = U < (long long)gridDim.x ? U : (long long)gridDim.x;
-  if ((long long)blockIdx.x >= grid) return;
-  const long long u0 = blockIdx.x * U / grid, u1 = (blockIdx.x + 1) * U / grid;
+  const Share share{U / (int)gridDim.x, U % (int)gridDim.x};
+  const int u0 = share.first(blockIdx.x), u1 = share.first(blockIdx.x + 1);
   if (u0 >= before && u0 < before + mine) {
-    int s = my0;
-    long long base = before;
+    int s = my0, base = before;
     for (;; ++s) {
-      const long long n = units_of(p, shape_of<NT>(p, s));
+      const int n = units_of(p, shape_of<NT>(p, s));
       if (u0 < base + n || s + 1 >= my1) break;
       base += n;
     }
     first_seq = s;
     first_base = base;
   }
-  if (warp == 16) tmem_alloc(&tmem_slot, 512);
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_slot;
   // Every wait is bounded; a role that gave up leaves, and so do those that wait for it.
   auto wait = [&](uint64_t* bar, uint32_t parity) { return quick_wait(bar, parity, p.err); };
 
-  // registers: 640 x 96 at launch = 256 x 128 + 256 x 96 + 128 x 32
-  if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    if (warp == 17) {
-      // ---------------- the blocks in order, and the copies of their pages
-      int s = first_seq, seg = -1, count = -1, it = 0, st = 0;
-      long long base = first_base;
-      Shape sh = shape_of<NT>(p, s);
-      long long each = sh.blocks + kStart;
-      int g = (int)((u0 - base) / each), blk = max(0, (int)((u0 - base) % each) - kStart);
-      bool begin = true, stop = false;
-      uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
-      for (;; ++it) {
-        if (blk >= sh.blocks) {
-          blk = 0;
-          begin = true;
-          if (++g >= sh.tiles * p.nkv) {
-            g = 0;
-            base += units_of(p, sh);
-            do {
-              ++s;
-              if (s >= p.n_seqs) break;
-              sh = shape_of<NT>(p, s);
-            } while (sh.nodes == 0);
-            each = sh.blocks + kStart;
-          }
-        }
-        const long long seg0 = base + (long long)g * each + kStart;  // unit of the segment's block 0
-        stop = s >= p.n_seqs || seg0 + blk >= u1;
-        int page = 0, valid = 0;
-        const bool draft = blk + 1 == sh.blocks;
-        if (!stop && !draft && lane < 2) {
-          const int at = 2 * blk + lane;
-          valid = min(kPageRows, sh.len - at * kPageRows);
-          if (valid > 0) page = p.table[(int64_t)s * p.table_stride + at];
-          if (valid < 0) valid = 0;
-          if (page < 0 || page >= p.n_pages) {
-            flag_position(p.err);
-            valid = 0;
-          }
-        }
-        if (begin) {
-          ++count;
-          seg = ((s * p.nkv) + g / max(sh.tiles, 1)) * p.most_tiles + g % max(sh.tiles, 1);
-        }
-        if (!wait(&empty[st], phase)) break;
-        const int v0 = __shfl_sync(0xffffffffu, valid, 0), v1 = __shfl_sync(0xffffffffu, valid, 1);
-        const int p0 = __shfl_sync(0xffffffffu, page, 0), p1 = __shfl_sync(0xffffffffu, page, 1);
-        if (lane == 0) {
-          Info f;
-          if (stop) {
-            f.flags = kStop;
-          } else {
-            const int kv = g / sh.tiles, tile = g % sh.tiles;
-            const long long end = seg0 + sh.blocks - 1;
-            const int c0 = (int)(((seg0 + 1) * grid - 1) / U), c1 = (int)(((end + 1) * grid - 1) / U);
-            f.flags = (draft ? kDraft : 0) | (begin ? kFirst : 0) | (draft || seg0 + blk + 1 >= u1 ? kLast : 0) |
-                      (c0 == c1 ? kAlone : 0) | (c0 == (int)blockIdx.x ? kOpens : 0);
-            f.seq = s;
-            f.kv = kv;
-            f.seg = seg;
-            f.r0 = sh.r0;
-            f.nodes = sh.nodes;
-            f.c0 = tile * sh.per;
-            f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
-            f.n = sh.per;
-            f.valid[0] = draft ? min(sh.nodes, 64) : v0;
-            f.valid[1] = draft ? max(sh.nodes - 64, 0) : v1;
-            f.slot = 2 * blockIdx.x + (f.flags & kOpens ? 1 : 0);
-            f.count = count;
-            f.run = c1 - c0 + 1;
-            f.first_cta = c0;
-          }
-          infos[it % kInfos] = f;
-          uint8_t* dst = ring + (size_t)st * S::kStage;
-          if (stop || draft) {
-            mbar_arrive(&full[st]);
-          } else {
-            mbar_arrive_expect_tx(&full[st], (uint32_t)((v0 > 0) + (v1 > 0)) * S::kPage);
-            if (v0 > 0) tma_load_2d(dst, &map, 0, (int)(((int64_t)p0 * p.nkv + f.kv) * (S::kPage / 128)), &full[st]);
-            if (v1 > 0)
-              tma_load_2d(dst + S::kPage, &map, 0, (int)(((int64_t)p1 * p.nkv + f.kv) * (S::kPage / 128)), &full[st]);
-          }
-        }
-        __syncwarp();
-        begin = false;
-        if (++st == S::kStages) {
-          st = 0;
-          phase ^= 1;
-        }
-        if (stop) {
-          ++it;
-          break;
-        }
-        ++blk;
-      }
-      // copies in flight land before the CTA leaves
-      for (int i = 0; i < S::kStages; ++i) {
-        const int uses = it > i ? (it - i + S::kStages - 1) / S::kStages : 0;
-        if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
-      }
-    } else if (warp == 16) {
-      // ---------------- products: S(0), S(1), PV(0), S(2), PV(1), ...
-      const uint32_t fmt = 1u << 4;  // f16 operands, f32 sums; M = 128
-      auto weighed = [&](int i) {    // O^T += V^T P^T of block i
-        const Info& f = infos[i % kInfos];
-        if (!wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u) || !wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u))
-          return false;
-        if ((f.flags & kFirst) && f.count > 0 && !wait(&o_empty, (uint32_t)(f.count - 1) & 1u)) return false;
-        tc_fence_after();
-        const uint32_t idesc = fmt | (1u << 16) | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-        const uint32_t va = smem_addr(vs + (i % S::kVs) * S::kV), pa = smem_addr(ps + (i & 1) * S::kP);
-        const bool first = f.flags & kFirst;
-        if (elect_one()) {
-#pragma unroll
-          for (int h = 0; h < S::kHalves; ++h)
-#pragma unroll
-            for (int kk = 0; kk < kRows / 16; ++kk)
-              umma_f16(tmem + S::kOCol + h * NT,
-                       sw128_desc(va + (uint32_t)(h * 2 + kk / 4) * S::kERows * 128 + 32u * (kk % 4)),
-                       sw128_desc_mn(pa + 2048u * kk, kRows * 128), idesc, first && kk == 0 ? 0u : 1u);
-          umma_commit(&p_empty[i & 1]);
-        }
-        __syncwarp();
-        return true;
-      };
-      int i = 0;
-      for (;; ++i) {
-        if (!wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
-        tc_fence_after();
-        const Info& f = infos[i % kInfos];
-        const bool stop = f.flags & kStop;
-        if (!stop) {
-          const uint32_t idesc = fmt | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-          const uint32_t qa = smem_addr(qs);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              umma_f16_ta(tmem + S::kSCol + (i & 1) * NT, tmem + (i & 1) * S::kKCols + 8u * kk,
-                          sw128_desc(qa + (uint32_t)(kk / 4) * NT * 128 + 32u * (kk % 4)), idesc, kk > 0 ? 1u : 0u);
-            umma_commit(&s_full[i & 1]);
-          }
-          __syncwarp();
-        }
-        if (i > 0 && !weighed(i - 1)) break;
-        if (stop) {
-          if (lane == 0) mbar_arrive(&s_full[i & 1]);
-          break;
-        }
-      }
+  if (u0 >= u1) {
+    // nothing to do
+    if (warp == 16) {
       if (elect_one()) umma_commit(&fin);
       __syncwarp();
     }
+  } else if (warp == 17) {
+    // ---------------- the blocks in order, and the copies of their pages
+    int s = first_seq, count = -1, it = 0, st = 0, base = first_base;
+    Shape sh = shape_of<NT>(p, s);
+    int each = sh.blocks + kStart;
+    int g = (u0 - base) / each, blk = max(0, (u0 - base) % each - kStart);
+    bool begin = true, stop = false;
+    uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
+    for (;; ++it) {
+      if (blk >= sh.blocks) {
+        blk = 0;
+        begin = true;
+        if (++g >= sh.tiles * p.nkv) {
+          g = 0;
+          base += units_of(p, sh);
+          do {
+            ++s;
+            if (s >= p.n_seqs) break;
+            sh = shape_of<NT>(p, s);
+          } while (sh.nodes == 0);
+          each = sh.blocks + kStart;
+        }
+      }
+      const int seg0 = base + g * each + kStart;  // unit of the segment's block 0
+      stop = s >= p.n_seqs || seg0 + blk >= u1;
+      int page = 0, valid = 0;
+      const bool draft = blk + 1 == sh.blocks;
+      if (!stop && !draft && lane < 2) {
+        const int at = 2 * blk + lane;
+        valid = min(kPageRows, sh.len - at * kPageRows);
+        if (valid > 0) page = p.table[(int64_t)s * p.table_stride + at];
+        if (valid < 0) valid = 0;
+        if (page < 0 || page >= p.n_pages) {
+          flag_position(p.err);
+          valid = 0;
+        }
+      }
+      if (begin) ++count;
+      if (!wait(&empty[st], phase)) break;
+      const int v0 = __shfl_sync(0xffffffffu, valid, 0), v1 = __shfl_sync(0xffffffffu, valid, 1);
+      const int p0 = __shfl_sync(0xffffffffu, page, 0), p1 = __shfl_sync(0xffffffffu, page, 1);
+      if (lane == 0) {
+        const int kv = stop ? 0 : g / sh.tiles;
+        uint8_t* dst = ring + (size_t)st * S::kStage;
+        if (v0 > 0 || v1 > 0) {
+          if (v0 > 0) tma_load_2d(dst, &map, 0, (int)(((int64_t)p0 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
+          if (v1 > 0)
+            tma_load_2d(dst + S::kPage, &map, 0, (int)(((int64_t)p1 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
+        }
+        Info& f = infos[it % kInfos];
+        if (stop) {
+          f.flags = kStop;
+        } else {
+          const int tile = g - kv * sh.tiles, c0 = share.cta_of(seg0), c1 = share.cta_of(seg0 + sh.blocks - 1);
+          f.flags = (draft ? kDraft : 0) | (begin ? kFirst : 0) | (draft || seg0 + blk + 1 >= u1 ? kLast : 0) |
+                    (c0 == c1 ? kAlone : 0) | (c0 == (int)blockIdx.x ? kOpens : 0);
+          f.seq = s;
+          f.kv = kv;
+          f.len = sh.len;
+          f.r0 = sh.r0;
+          f.nodes = sh.nodes;
+          f.c0 = tile * sh.per;
+          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.n = sh.per;
+          f.valid[0] = v0;
+          f.valid[1] = v1;
+          f.count = count;
+          f.run = c1 - c0 + 1;
+        }
+        mbar_arrive_expect_tx(&full[st], (uint32_t)((v0 > 0) + (v1 > 0)) * S::kPage);
+      }
+      __syncwarp();
+      begin = false;
+      if (++st == S::kStages) {
+        st = 0;
+        phase ^= 1;
+      }
+      if (stop) {
+        ++it;
+        break;
+      }
+      ++blk;
+    }
+    // copies in flight land before the CTA leaves
+    for (int i = 0; i < S::kStages; ++i) {
+      const int uses = it > i ? (it - i + S::kStages - 1) / S::kStages : 0;
+      if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
+    }
+  } else if (warp == 16) {
+    // ---------------- products: S(0), S(1), PV(0), S(2), PV(1), ...
+    const uint32_t fmt = 1u << 4;  // f16 operands, f32 sums; M = 128
+    auto weighed = [&](int i) {    // O^T += V^T P^T of block i, and the sums of the weights
+      const Info& f = infos[i % kInfos];
+      if (!wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u) || !wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u))
+        return false;
+      if ((f.flags & kFirst) && f.count > 0 && !wait(&o_empty, (uint32_t)(f.count - 1) & 1u)) return false;
+      tc_fence_after();
+      const uint32_t idesc = fmt | (1u << 16) | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint32_t va = smem_addr(vs + (i % S::kVs) * S::kV), pa = smem_addr(ps + (i & 1) * S::kP);
+      const uint32_t more = f.flags & kFirst ? 0u : 1u;
+      const uint32_t ones = tmem + S::kOnes + (f.flags & kDraft ? 8u * v_lift[f.count & 3] : 0u);
+      if (elect_one()) {
+#pragma unroll 1
+        for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+          for (int kk = 0; kk < kRows / 16; ++kk)
+            umma_f16(tmem + S::kOCol + h * NT, sw128_desc(va + (uint32_t)(h * 2 + kk / 4) * S::kERows * 128 + 32u * (kk % 4)),
+                     sw128_desc_mn(pa + 2048u * kk, kRows * 128), idesc, kk > 0 ? 1u : more);
+#pragma unroll
+        for (int kk = 0; kk < kRows / 16; ++kk)
+          umma_f16_ta(tmem + S::kLCol, ones, sw128_desc_mn(pa + 2048u * kk, kRows * 128), idesc, kk > 0 ? 1u : more);
+        umma_commit(&p_empty[i & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    int i = 0;
+#pragma unroll 1
+    for (;; ++i) {
+      if (!wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+      tc_fence_after();
+      const Info& f = infos[i % kInfos];
+      const bool stop = f.flags & kStop;
+      if (!stop) {
+        const uint32_t idesc = fmt | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+        const uint32_t qa = smem_addr(qs);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            umma_f16_ta(tmem + S::kSCol + (i & 1) * NT, tmem + (i % S::kKs) * S::kKCols + 8u * kk,
+                        sw128_desc(qa + (uint32_t)(kk / 4) * NT * 128 + 32u * (kk % 4)), idesc, kk > 0 ? 1u : 0u);
+          umma_commit(&s_full[i & 1]);
+        }
+        __syncwarp();
+      }
+      if (i > 0 && !weighed(i - 1)) break;
+      if (stop) {
+        if (lane == 0) mbar_arrive(&s_full[i & 1]);
+        break;
+      }
+    }
+    if (elect_one()) umma_commit(&fin);
+    __syncwarp();
+  } else if (warp >= 18) {
+    // (no role)
   } else if (warp >= 12) {
-    // ---------------- V: two rows' pairs of values, transposed to rows of values
+    // ---------------- V: pairs of rows, transposed to rows of values
     const int tid = threadIdx.x - 12 * 32;
-    Quartet team{&teams[3], nullptr, 0, p.err};
+    Quartet team{&teams[1], 0, p.err};
     int st = 0;
     uint32_t phase = 0;
+#pragma unroll 1
     for (int i = 0;; ++i) {
       if (!wait(&full[st], phase)) break;
       const Info& f = infos[i % kInfos];
@@ -485,15 +534,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (tid == 0) v_again[par] = 0;
         if (!team()) break;
       }
-      // the place is free once PV(i - kVs) is done
-      if (i >= S::kVs && !wait(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u)) break;
+      uint8_t* const stage = ring + (size_t)st * S::kStage;
       uint8_t* const dst = vs + (i % S::kVs) * S::kV;
+      // the place is free once PV(i - kVs) is done
+      auto free_place = [&]() {
+        return i < S::kVs || wait(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u);
+      };
       if (!(f.flags & kDraft)) {
+        if (f.valid[0] < kPageRows || f.valid[1] < kPageRows) {
+          // rows that do not count: d = m = 0
+          const int half = tid >> 6, row = tid & 63;
+          if (row >= f.valid[half])
+            for (int j = 0; j < G; ++j) {
+              *reinterpret_cast<uint16_t*>(stage + half * S::kPage + swizzled(72 * HD + 2 * (row * G + j))) = 0;
+              *reinterpret_cast<uint16_t*>(stage + half * S::kPage + swizzled(76 * HD + 4 * ((row >> 1) * G + j) + 2 * (row & 1))) = 0;
+            }
+          if (!team()) break;
+        }
         const int o = tid >> 3, g = tid & 7;  // rows 8 o .. + 7 of the block, values 32 i + 8 n + g
-        const uint8_t* const page = ring + (size_t)st * S::kStage + (o >> 3) * S::kPage;
-        const int r = (o & 7) * 8, valid = f.valid[o >> 3];
+        const uint8_t* const page = stage + (o >> 3) * S::kPage;
+        const int r = (o & 7) * 8;
+        // (whether f16 holds what the groups stand for: a share of them each)
         __half2 most = as_half2(0u);
 #pragma unroll
+        for (int k = 0; k < G / 2; ++k) {
+          const int row = r + 2 * (g & 3), j = (g >> 2) * (G / 2) + k;
+          const __half2 dd = __halves2half2(*reinterpret_cast<const __half*>(page + swizzled(72 * HD + 2 * (row * G + j))),
+                                            *reinterpret_cast<const __half*>(page + swizzled(72 * HD + 2 * ((row + 1) * G + j))));
+          const uint32_t mm = *reinterpret_cast<const uint32_t*>(page + swizzled(76 * HD + 4 * ((row >> 1) * G + j)));
+          most = __hmax2(most, __hfma2(dd, as_half2(0x4b804b80u), __habs2(as_half2(mm))));
+        }
+        if (__hisinf(__low2half(most)) || __hisinf(__high2half(most))) v_again[par] = 1;
+        if (!free_place()) break;
+#pragma unroll 1
         for (int P = 0; P < PL; ++P) {
           uint32_t w[4 * J];  // [t][i]
 #pragma unroll
@@ -508,59 +581,54 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int row = r + 2 * t;
-            const bool even = row < valid, odd = row + 1 < valid;
-#pragma unroll
-            for (int k = 0; k < J; k += 2) {
-              const int j = P * J + k;
-              const uint32_t a = *reinterpret_cast<const uint32_t*>(page + swizzled(72 * HD + 2 * (row * G + j)));
-              const uint32_t b = *reinterpret_cast<const uint32_t*>(page + swizzled(72 * HD + 2 * ((row + 1) * G + j)));
-              const uint2 c = *reinterpret_cast<const uint2*>(page + swizzled(76 * HD + 4 * ((row >> 1) * G + j)));
-              const uint32_t mask = (even ? 0x0000ffffu : 0u) | (odd ? 0xffff0000u : 0u);
-              d[t][k] = as_half2(__byte_perm(a, b, 0x5410) & mask);
-              d[t][k + 1] = as_half2(__byte_perm(a, b, 0x7632) & mask);
-              m[t][k] = as_half2(c.x & mask);
-              m[t][k + 1] = as_half2(c.y & mask);
-              most = __hmax2(most, __hfma2(d[t][k], as_half2(0x4b804b80u), __habs2(m[t][k])));
-              most = __hmax2(most, __hfma2(d[t][k + 1], as_half2(0x4b804b80u), __habs2(m[t][k + 1])));
+            const uint8_t* const da = page + swizzled(72 * HD + 2 * (row * G + P * J));
+            const uint8_t* const db = page + swizzled(72 * HD + 2 * ((row + 1) * G + P * J));
+            const uint8_t* const ma = page + swizzled(76 * HD + 4 * ((row >> 1) * G + P * J));
+            if constexpr (J == 4) {
+              const uint2 a = *reinterpret_cast<const uint2*>(da), b = *reinterpret_cast<const uint2*>(db);
+              const uint4 c = *reinterpret_cast<const uint4*>(ma);
+              d[t][0] = as_half2(__byte_perm(a.x, b.x, 0x5410));
+              d[t][1] = as_half2(__byte_perm(a.x, b.x, 0x7632));
+              d[t][2] = as_half2(__byte_perm(a.y, b.y, 0x5410));
+              d[t][3] = as_half2(__byte_perm(a.y, b.y, 0x7632));
+              m[t][0] = as_half2(c.x);
+              m[t][1] = as_half2(c.y);
+              m[t][2] = as_half2(c.z);
+              m[t][3] = as_half2(c.w);
+            } else {
+              const uint32_t a = *reinterpret_cast<const uint32_t*>(da), b = *reinterpret_cast<const uint32_t*>(db);
+              const uint2 c = *reinterpret_cast<const uint2*>(ma);
+              d[t][0] = as_half2(__byte_perm(a, b, 0x5410));
+              d[t][1] = as_half2(__byte_perm(a, b, 0x7632));
+              m[t][0] = as_half2(c.x);
+              m[t][1] = as_half2(c.y);
             }
           }
+          uint8_t* const to = dst + (P * 2 + (o >> 3)) * S::kERows * 128 + g * 128 + (((o & 7) ^ g) << 4);
 #pragma unroll
           for (int k = 0; k < J; ++k) {
-            uint32_t x[4][4];  // [t][n]
+            uint32_t x[4][4];  // [t][n]: nibble n of the halves, the even row's and the odd row's
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              // (nibble n of the halves: the even row's and the odd row's)
-              const uint32_t big = 0x64006400u, word = w[t * J + k], v = word >> 8;
-              const __half2 less = as_half2(0xe400e400u), sixteenth = as_half2(0x2c002c00u), less64 = as_half2(0xd400d400u);
-              x[t][0] = as_u32(__hfma2(__hadd2(as_half2(and_or(word, 0x000f000fu, big)), less), d[t][k], m[t][k]));
-              x[t][1] = as_u32(__hfma2(__hfma2(as_half2(and_or(word, 0x00f000f0u, big)), sixteenth, less64), d[t][k], m[t][k]));
-              x[t][2] = as_u32(__hfma2(__hadd2(as_half2(and_or(v, 0x000f000fu, big)), less), d[t][k], m[t][k]));
-              x[t][3] = as_u32(__hfma2(__hfma2(as_half2(and_or(v, 0x00f000f0u, big)), sixteenth, less64), d[t][k], m[t][k]));
-            }
+            for (int t = 0; t < 4; ++t) values_of(w[t * J + k], d[t][k], m[t][k], x[t]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const int e = 32 * k + 8 * n + g;
-              *reinterpret_cast<uint4*>(dst + (P * 2 + (o >> 3)) * S::kERows * 128 + e * 128 + (((o & 7) ^ g) << 4)) =
-                  make_uint4(x[0][n], x[1][n], x[2][n], x[3][n]);
-            }
+            for (int n = 0; n < 4; ++n)
+              *reinterpret_cast<uint4*>(to + (32 * k + 8 * n) * 128) = make_uint4(x[0][n], x[1][n], x[2][n], x[3][n]);
           }
         }
-        if (__hisinf(__low2half(most)) || __hisinf(__high2half(most))) v_again[par] = 1;
       } else {
+        constexpr int C = HD / 64;
         const int o = tid & 15, x = tid >> 4;  // rows 8 o .. + 7, values 8 (x + 8 c) .. + 7
         const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head;
-        auto load = [&](int c, uint4 (&w)[8]) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            w[r] = 8 * o + r < f.nodes
-                       ? *reinterpret_cast<const uint4*>(src + (int64_t)(f.r0 + 8 * o + r) * p.v_row + 8 * (x + 8 * c))
-                       : make_uint4(0, 0, 0, 0);
-        };
+        const int rows = min(max(f.nodes - 8 * o, 0), 8);
         uint32_t top = 0;
 #pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
+        for (int c = 0; c < C; ++c) {
           uint4 w[8];
-          load(c, w);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + (int64_t)(f.r0 + 8 * o + r) * p.v_row + 8 * (x + 8 * c));
+          }
 #pragma unroll
           for (int r = 0; r < 8; ++r) top = max(top, top_bits<T>(w[r]));
         }
@@ -568,11 +636,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) v_tops[warp & 3] = top;
         if (!team()) break;
         top = max(max(v_tops[0], v_tops[1]), max(v_tops[2], v_tops[3]));
-        const float lift = lift_of(top);
+        const float lift = lifted_by(lift_of(top));
+        if (tid == 0) {
+          v_lift[par] = lift_of(top);
+          if (top > kHalfMax) v_again[par] = 1;
+        }
+        if (!free_place()) break;
 #pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
+        for (int c = 0; c < C; ++c) {
           uint4 w[8];
-          load(c, w);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + (int64_t)(f.r0 + 8 * o + r) * p.v_row + 8 * (x + 8 * c));
+          }
           const int e0 = 8 * (x + 8 * c);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -603,9 +680,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 8) {
     // ---------------- K: a row of keys per thread, into TMEM; and the tile's queries
     const int r = threadIdx.x - 8 * 32;
-    Quartet team{&teams[2], nullptr, 0, p.err};
+    const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
+    Quartet team{&teams[0], 0, p.err};
     int st = 0;
     uint32_t phase = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint32_t ones[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ones[e] = k == 0 ? 0x3c003c00u : k == 1 ? 0x5c005c00u : 0x78007800u;
+      tmem_st8(tmem + S::kOnes + 8 * k + sub, ones);
+    }
+#pragma unroll 1
     for (int i = 0;; ++i) {
       if (!wait(&full[st], phase)) break;
       const Info& f = infos[i % kInfos];
@@ -617,103 +703,101 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       if (flags & kFirst) {
-        // S of the segment before has read its queries
-        if (i > 0 && !wait(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
         if (r == 0) k_again[par] = 0;
         if (!team()) break;
-        if (r < f.n) {
-          const int c = f.c0 + r, head = f.kv * p.hpk + c % p.hpk;
-          const T* src = static_cast<const T*>(p.q) + (int64_t)(f.r0 + c / p.hpk) * p.q_row + head * p.q_head;
-          const bool some = r < f.cols;
-          uint32_t top = 0;
-          if (some)
-#pragma unroll 8
-            for (int x = 0; x < HD / 8; ++x) top = max(top, top_bits<T>(reinterpret_cast<const uint4*>(src)[x]));
+        // S of the segment before has read its queries
+        if (i > 0 && !wait(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
+        // kLanes lanes per row, 8 values each; a row is brought to [1, 2) by a power of two
+        constexpr int kLanes = HD / 8 < 32 ? HD / 8 : 32, kAcross = 128 / kLanes;
+        const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // the place among the words of a row of codes
+#pragma unroll 2
+        for (int c = r / kLanes; c < f.n; c += kAcross) {
+          const int column = f.c0 + c, token = column / p.hpk, head = f.kv * p.hpk + column - token * p.hpk;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (c < f.cols)
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(f.r0 + token) * p.q_row + head * p.q_head + 8 * x);
+          uint32_t top = top_bits<T>(v);
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           bool fine;
           const float s = to_one(top, fine);
           if (!fine) k_again[par] = 1;
-#pragma unroll 4
-          for (int x = 0; x < HD / 8; ++x) {
-            uint32_t y[4] = {0, 0, 0, 0};
-            if (some) scaled_pairs<T>(reinterpret_cast<const uint4*>(src)[x], s, y);
-            const int j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // its place among the words of a row of codes
-            *reinterpret_cast<uint4*>(qs + (w / 8) * NT * 128 + sw128_off(r, w % 8)) = make_uint4(y[0], y[1], y[2], y[3]);
-          }
-          q_scale[par][r] = some ? p.scale / s : 0.f;
+          uint32_t y[4];
+          scaled_pairs<T>(v, s, y);
+          *reinterpret_cast<uint4*>(qs + (w / 8) * NT * 128 + sw128_off(c, w % 8)) = make_uint4(y[0], y[1], y[2], y[3]);
+          if (x == 0) lines[par][c] = make_float2(c < f.cols ? p.scale / s : 0.f, kBias);
         }
         fence_proxy_async_smem();
       }
-      // the place is free once S(i - 2) is done
-      if (i >= 2 && !wait(&s_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
-      tc_fence_after();
-      const uint32_t dst = tmem + (i & 1) * S::kKCols + ((uint32_t)(32 * (warp & 3)) << 16);
+      const uint32_t dst = tmem + (i % S::kKs) * S::kKCols + sub;
+      // the place is free once S(i - kKs) is done
+      auto free_place = [&]() {
+        const bool ok = i < S::kKs || wait(&s_full[(i - S::kKs) & 1], (uint32_t)((i - S::kKs) >> 1) & 1u);
+        tc_fence_after();
+        return ok;
+      };
       if (!(flags & kDraft)) {
         const int half = r >> 6, row = r & 63;
         const uint8_t* const page = ring + (size_t)st * S::kStage + half * S::kPage;
-        uint32_t d[G / 2], m[G / 2];
+        __half2 d[G / 2], m[G / 2], most = as_half2(0u);
 #pragma unroll
         for (int k = 0; k < G / 2; ++k) {
-          d[k] = *reinterpret_cast<const uint32_t*>(page + swizzled(32 * HD + 2 * (row * G + 2 * k)));
-          m[k] = *reinterpret_cast<const uint32_t*>(page + swizzled(36 * HD + 2 * (row * G + 2 * k)));
+          d[k] = *reinterpret_cast<const __half2*>(page + swizzled(32 * HD + 2 * (row * G + 2 * k)));
+          m[k] = *reinterpret_cast<const __half2*>(page + swizzled(36 * HD + 2 * (row * G + 2 * k)));
+          most = __hmax2(most, __hfma2(d[k], as_half2(0x4b804b80u), __habs2(m[k])));
         }
-        __half2 most = as_half2(0u);
-#pragma unroll
-        for (int k = 0; k < G / 2; ++k) most = __hmax2(most, __hfma2(as_half2(d[k]), as_half2(0x4b804b80u), __habs2(as_half2(m[k]))));
         if (row < f.valid[half] && (__hisinf(__low2half(most)) || __hisinf(__high2half(most)))) k_again[par] = 1;
+        if (!free_place()) break;
 #pragma unroll
-        for (int P = 0; P < PL; ++P)
+        for (int P = 0; P < PL; ++P) {
+          __half2 dd[J], mm[J];
 #pragma unroll
-          for (int q = 0; q < J; q += 2) {  // eight words, 32 columns
-            uint32_t y[32];
+          for (int k = 0; k < J; ++k) {
+            const int j = P * J + k;
+            dd[k] = j & 1 ? __high2half2(d[j / 2]) : __low2half2(d[j / 2]);
+            mm[k] = j & 1 ? __high2half2(m[j / 2]) : __low2half2(m[j / 2]);
+          }
+#pragma unroll 1
+          for (int u = 0; u < J; ++u) {  // four words, 16 columns
+            const uint4 x = *reinterpret_cast<const uint4*>(page + swizzled(P * 1024 * J + row * 16 * J + 16 * u));
+            uint32_t y[16];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint4 x = *reinterpret_cast<const uint4*>(page + swizzled(P * 1024 * J + row * 16 * J + 16 * (q + u)));
+            for (int k = 0; k < 4; ++k) {
+              uint32_t z[4];
+              values_of((&x.x)[k], dd[k % J], mm[k % J], z);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int j = P * J + (4 * (q + u) + k) % J;
-                const __half2 dd = j & 1 ? __high2half2(as_half2(d[j / 2])) : __low2half2(as_half2(d[j / 2]));
-                const __half2 mm = j & 1 ? __high2half2(as_half2(m[j / 2])) : __low2half2(as_half2(m[j / 2]));
-                uint32_t z[4];
-                values_of((&x.x)[k], dd, mm, z);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[16 * u + 4 * k + e] = z[e];
-              }
+              for (int e = 0; e < 4; ++e) y[4 * k + e] = z[e];
             }
             __syncwarp();
-            tmem_st32(dst + P * 16 * J + q * 16, y);
+            tmem_st16(dst + P * 16 * J + 16 * u, y);
           }
+        }
       } else {
-        // drafted rows: to [1, 2) by a power of two each; what their V is lifted by; who sees whom
+        // drafted rows: to [1, 2) by a power of two each; who sees whom
         const bool some = r < f.nodes;
         const T* src = static_cast<const T*>(p.k) + (int64_t)(f.r0 + r) * p.k_row + f.kv * p.k_head;
-        const T* vsrc = static_cast<const T*>(p.v) + (int64_t)(f.r0 + r) * p.v_row + f.kv * p.v_head;
-        uint32_t top = 0, vtop = 0;
-        if (some)
-#pragma unroll 4
-          for (int x = 0; x < HD / 8; ++x) {
-            top = max(top, top_bits<T>(reinterpret_cast<const uint4*>(src)[x]));
-            vtop = max(vtop, top_bits<T>(reinterpret_cast<const uint4*>(vsrc)[x]));
-          }
-        bool fine;
-        const float s = to_one(top, fine);
-        if (!fine || vtop > kHalfMax) k_again[par] = 1;
-        k_scale[par][r] = 1.f / s;
-        vtop = __reduce_max_sync(0xffffffffu, vtop);
-        if (lane == 0) k_tops[warp & 3] = vtop;
-        uint4 bits = make_uint4(0, 0, 0, 0);
         int parent = -1;
         if (some) {
-          (&bits.x)[r >> 5] = 1u << (r & 31);
           parent = p.parents ? p.parents[f.r0 + r] : r - 1;
           if (parent < -1 || parent >= r) {
             flag_position(p.err);
             parent = -1;
           }
         }
+        uint32_t top = 0;
+        if (some)
+#pragma unroll 8
+          for (int x = 0; x < HD / 8; ++x) top = max(top, top_bits<T>(reinterpret_cast<const uint4*>(src)[x]));
+        bool fine;
+        const float s = to_one(top, fine);
+        if (!fine) k_again[par] = 1;
+        k_scale[par][r] = 1.f / s;
+        uint4 bits = make_uint4(0, 0, 0, 0);
+        if (some) (&bits.x)[r >> 5] = 1u << (r & 31);
         seen[par][r] = bits;
         up[r] = parent;
         bool ok = team();
-        if (r == 0) v_lift[par] = 1.f / lift_of(max(max(k_tops[0], k_tops[1]), max(k_tops[2], k_tops[3])));
+#pragma unroll 1
         for (int n = 1; ok && n < f.nodes; n <<= 1) {  // ancestors up to 2 n rows above
           uint4 more = make_uint4(0, 0, 0, 0);
           int next = -1;
@@ -731,12 +815,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           up[r] = parent;
           ok = ok && team();
         }
-        if (!ok) break;
+        if (!ok || !free_place()) break;
+#pragma unroll 1
+        for (int w0 = 0; w0 < HD / 8; w0 += 4) {  // four words, 16 columns
+          uint32_t y[16];
 #pragma unroll
-        for (int w0 = 0; w0 < HD / 8; w0 += 8) {  // eight words, 32 columns
-          uint32_t y[32];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 4; ++k) {
             const int w = w0 + k, P = w / (4 * J), t = w % (4 * J) / J, j = P * J + w % J;
             uint32_t z[4] = {0, 0, 0, 0};
             if (some) scaled_pairs<T>(reinterpret_cast<const uint4*>(src)[4 * j + t], s, z);
@@ -744,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 4; ++e) y[4 * k + e] = z[e];
           }
           __syncwarp();
-          tmem_st32(dst + 4 * w0, y);
+          tmem_st16(dst + 4 * w0, y);
         }
       }
       tmem_wait_st();
@@ -760,100 +844,126 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     // ---------------- softmax: a KV row per thread, half of the columns
-    const int h = warp >> 2, qd = warp & 3, r = threadIdx.x & 127;
-    Quartet team{&teams[h], &votes[h][0][0], 0, p.err};
+    const int h = warp >> 2, qd = warp & 3, r = threadIdx.x & 127, bar = 1 + h;
     const uint32_t sub = (uint32_t)(32 * qd) << 16;
-    float l[kHalfCols];
+#pragma unroll 1
     for (int i = 0;; ++i) {
-      if (!wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+      bool ok = wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u);
       const Info& f = infos[i % kInfos];
-      const int flags = f.flags;
-      if (flags & kStop) break;
-      tc_fence_after();
+      const int flags = ok ? f.flags : kStop;
       const int par = f.count & 3, cols = f.n >> 1, x0 = h * cols;  // this half: columns x0 .. x0 + cols - 1 of the tile
       const bool first = flags & kFirst;
-      if (first) {
-        if (!team()) break;  // the segment before no longer reads its lines
-        if (r < cols) line[x0 + r] = make_float2(q_scale[par][x0 + r], kBias);
-#pragma unroll
-        for (int x = 0; x < kHalfCols; ++x) l[x] = 0.f;
-        if (!team()) break;
-      }
-      // the arguments of the weights' exponentials
-      float a[kHalfCols];
       const uint32_t sc = tmem + S::kSCol + (i & 1) * NT + x0 + sub;
-      __syncwarp();
-#pragma unroll
-      for (int x = 0; x < kHalfCols; x += 8)
-        if (x < cols) tmem_ld8_async(sc + x, reinterpret_cast<uint32_t*>(a) + x);
-      tmem_wait_ld();
-      const bool here = (r & 63) < f.valid[r >> 6];
-      float top = -INFINITY;
+      uint8_t* const dst = ps + (i & 1) * S::kP + (r >> 3) * 1024 + (r & 7) * 128;
+      float2* const line = lines[par] + x0;
+      tc_fence_after();
+      // P's place is free once PV(i - 2) is done
+      if (!(flags & kStop) && i >= 2) ok = wait(&p_empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u);
+      const bool plain = !(flags & kDraft) && (r & ~31 & 63) + 32 <= f.valid[r >> 6];  // every row of the warp counts, for all columns
+      float ks = 1.f, low = 1.f;
       if (flags & kDraft) {
-        const float ks = k_scale[par][r];
-        int token = (f.c0 + x0) / p.hpk, sub_head = (f.c0 + x0) % p.hpk;
-        const uint32_t* bits = reinterpret_cast<const uint32_t*>(seen[par]) + qd;
+        ok = ok && wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u);  // (v_lift)
+        ks = k_scale[par][r];
+        low = 1.f / lifted_by(v_lift[par]);
+      }
+      // eight arguments from column x on; those that this row does not have are -inf
+      auto arguments = [&](int x, float (&a)[8]) {
+        __syncwarp();
+        tmem_ld8(sc + x, reinterpret_cast<uint32_t(&)[8]>(a));
 #pragma unroll
-        for (int x = 0; x < kHalfCols; ++x)
-          if (x < cols) {
-            const bool sees = x0 + x < f.cols && ((bits[4 * min(token, kMaxNodes - 1)] >> lane) & 1u);
-            const float2 ln = line[x0 + x];
-            a[x] = sees ? fmaf(a[x] * ks, ln.x, ln.y) : -INFINITY;
-            top = fmaxf(top, a[x]);
+        for (int e = 0; e < 8; e += 2) {
+          const float4 ln = *reinterpret_cast<const float4*>(line + x + e);
+          a[e] = fmaf(a[e] * ks, ln.x, ln.y);
+          a[e + 1] = fmaf(a[e + 1] * ks, ln.z, ln.w);
+        }
+        if (flags & kDraft) {
+          int token = (f.c0 + x0 + x) / p.hpk, sub_head = (f.c0 + x0 + x) - token * p.hpk;
+          const uint32_t* bits = reinterpret_cast<const uint32_t*>(seen[par]) + qd;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (x0 + x + e >= f.cols || !((bits[4 * min(token, kMaxNodes - 1)] >> lane) & 1u)) a[e] = -INFINITY;
             if (++sub_head == p.hpk) {
               sub_head = 0;
               ++token;
             }
           }
-      } else {
+        } else if ((r & 63) >= f.valid[r >> 6]) {
 #pragma unroll
-        for (int x = 0; x < kHalfCols; x += 2)
-          if (x < cols) {
-            const float4 ln = *reinterpret_cast<const float4*>(&line[x0 + x]);
-            a[x] = fmaf(a[x], ln.x, ln.y);
-            a[x + 1] = fmaf(a[x + 1], ln.z, ln.w);
-            top = fmaxf(top, fmaxf(a[x], a[x + 1]));
-          }
-        if (!__all_sync(0xffffffffu, here)) {
-          top = here ? top : -INFINITY;
-#pragma unroll
-          for (int x = 0; x < kHalfCols; ++x) a[x] = here ? a[x] : -INFINITY;
+          for (int e = 0; e < 8; ++e) a[e] = -INFINITY;
         }
-      }
-      // a new maximum, where a weight would be larger than the lazy ones may be
-      bool ok;
-      const bool grown = team.any(first || top > kBias + kLazy, ok);
-      if (!ok) break;
-      if (grown) {
+      };
+      // the weights of all columns into P; the largest argument
+      auto weights = [&]() {
+        float top = -INFINITY;
+        if (plain) {
+#pragma unroll 1
+          for (int x = 0; x < cols; x += 8) {
+            uint32_t s[8], w[4];
+            tmem_ld8(sc + x, s);
+            const float4* ln = reinterpret_cast<const float4*>(line + x);
 #pragma unroll
-        for (int x = 0; x < kHalfCols; ++x)
-          if (x < cols) {
-            const float m = redux_max(a[x]);
-            if (lane == 0) quad[h][qd][x] = m;
+            for (int e = 0; e < 4; ++e) {
+              const float4 l = ln[e];
+              const float u = fmaf(__uint_as_float(s[2 * e]), l.x, l.y), v = fmaf(__uint_as_float(s[2 * e + 1]), l.z, l.w);
+              top = fmaxf(top, fmaxf(u, v));
+              w[e] = as_u32(__floats2half2_rn(ex2(u), ex2(v)));
+            }
+            const int c = x0 + x;
+            *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
-        if (!team()) break;
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < cols; x += 8) {
+            float a[8];
+            arguments(x, a);
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              top = fmaxf(top, fmaxf(a[2 * e], a[2 * e + 1]));
+              w[e] = as_u32(__floats2half2_rn(ex2(a[2 * e]) * low, ex2(a[2 * e + 1]) * low));
+            }
+            const int c = x0 + x;
+            *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        return top;
+      };
+      float top = -INFINITY;
+      if (ok && !(flags & kStop) && !first) top = weights();
+      // a new maximum, where a weight would be larger than the lazy ones may be
+      if (!ok) dead[h] = 1;
+      const bool grown = any_of_128(bar, first || top > kBias + kLazy);
+      if ((flags & kStop) || *reinterpret_cast<volatile int*>(&dead[h])) break;
+      if (grown) {
+#pragma unroll 1
+        for (int x = 0; x < cols; x += 8) {
+          float a[8];
+          arguments(x, a);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float m = redux_max(a[e]);
+            if (lane == 0) quad[h][qd][x + e] = m;
+          }
+        }
+        any_of_128(bar, false);
         if (r < cols) {
           float m = fmaxf(fmaxf(quad[h][0][r], quad[h][1][r]), fmaxf(quad[h][2][r], quad[h][3][r])) - kBias;
           if (!first) m = fmaxf(m, 0.f);
           if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
-          change[h][r] = m;
-          line[x0 + r].y -= m;
+          change[h][r] = ex2(-m);
+          line[r].y -= m;
         }
-        if (!team()) break;
         // (O of the blocks before is complete)
-        if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
+        if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) dead[h] = 1;
+        any_of_128(bar, false);
+        if (*reinterpret_cast<volatile int*>(&dead[h])) break;
         tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < kHalfCols; ++x)
-          if (x < cols) {
-            a[x] -= change[h][x];
-            if (!first) l[x] *= ex2(-change[h][x]);
-          }
         if (!first) {
 #pragma unroll 1
-          for (int k = 0; k < S::kHalves; ++k)
+          for (int k = -1; k < S::kHalves; ++k)  // the sums of the weights, and O
 #pragma unroll 1
             for (int x = 0; x < cols; x += 8) {
               const uint32_t oc = tmem + S::kOCol + k * NT + x0 + x + sub;
@@ -861,32 +971,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               tmem_ld8(oc, o);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ex2(-change[h][x + e]));
+              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * change[h][x + e]);
               tmem_st8(oc, o);
             }
           tmem_wait_st();
-          tc_fence_before();
         }
-        if (!team()) break;  // `change` and `quad` are read
+        weights();
       }
-      // the weights, in P's place once PV(i - 2) is done
-      if (i >= 2 && !wait(&p_empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
-      uint8_t* const dst = ps + (i & 1) * S::kP;
-      const float low = flags & kDraft ? v_lift[par] : 1.f;
-#pragma unroll
-      for (int x = 0; x < kHalfCols; x += 8)
-        if (x < cols) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u = ex2(a[x + 2 * e]), v = ex2(a[x + 2 * e + 1]);
-            l[x + 2 * e] += u;
-            l[x + 2 * e + 1] += v;
-            w[e] = flags & kDraft ? as_u32(__floats2half2_rn(u * low, v * low)) : as_u32(__floats2half2_rn(u, v));
-          }
-          const int c = x0 + x;
-          *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + sw128_off(r, (c & 63) >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
@@ -894,61 +985,60 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(flags & kLast)) continue;
 
       // ---------------- the end of the segment, in this CTA
-#pragma unroll
-      for (int x = 0; x < kHalfCols; x += 32) {
-        if (x >= cols) break;
-        if constexpr (kHalfCols >= 32) {
-          if (x + 32 <= kHalfCols) {
-            float v[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = x + k < kHalfCols ? l[(x + k) % kHalfCols] : 0.f;
-            quad[h][qd][x + lane] = transposed_sum(v);
-          } else {
-            float v[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = l[(x + k) % kHalfCols];
-            const float s = transposed_sum(v);
-            if (lane < 16) quad[h][qd][x + lane] = s;
-          }
-        }
+      if (!wait(&p_empty[i & 1], (uint32_t)(i >> 1) & 1u)) {
+        dead[h] = 1;  // (the others of this half see it at the next barrier)
+        continue;
       }
-      if (!wait(&p_empty[i & 1], (uint32_t)(i >> 1) & 1u)) break;
       tc_fence_after();
-      if (!team()) break;
-      const bool alone = flags & kAlone;
-      if (r < cols) {
-        const float s = (quad[h][0][r] + quad[h][1][r]) + (quad[h][2][r] + quad[h][3][r]);
-        change[h][r] = alone ? 1.f / s : s;
-        if (!alone) p.stats[(size_t)f.slot * NT + x0 + r] = make_float2(kBias - line[x0 + r].y, s);
+      const bool alone = flags & kAlone, again = (k_again[par] | v_again[par]) != 0;
+      const int slot = 2 * blockIdx.x + (flags & kOpens ? 1 : 0);
+      const int used = min(cols, f.cols - x0);  // (columns past them are padding)
+      if (!alone) {
+        if (threadIdx.x == 0) {
+          p.again[slot] = again;
+          if (flags & kOpens) p.opened[blockIdx.x] = Opened{f.run, f.seq, f.kv, f.r0, f.len, f.c0, f.cols, 0};
+        }
+        if (qd == 0)
+#pragma unroll 1
+          for (int x = 0; x < cols; x += 8) {
+            uint32_t l[8];
+            __syncwarp();
+            tmem_ld8(tmem + S::kLCol + x0 + x + sub, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (lane == e) p.stats[(size_t)slot * NT + x0 + x + e] = make_float2(kBias - line[x + e].y, __uint_as_float(l[e]));
+          }
       }
-      if (!team()) break;
-      if (threadIdx.x == 0) {
-        const int again = k_again[par] | v_again[par];
-        if (alone || (flags & kOpens)) p.runs[f.seg] = make_int4(f.first_cta, f.run, alone ? again : 0, 0);
-        if (!alone) p.again[f.slot] = again;
-      }
-      if (qd * 32 < S::kERows) {
-        const int used = min(cols, f.cols - x0);  // (columns past them are padding)
+      if (alone && again) {
+        for (int x = qd; x < used; x += 4) {
+          const int token = (f.c0 + x0 + x) / p.hpk;
+          plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + x0 + x) - token * p.hpk);
+        }
+      } else if (qd * 32 < S::kERows) {
 #pragma unroll 1
         for (int k = 0; k < S::kHalves; ++k) {
           const int e = 128 * k + 32 * qd + lane;
-          int token = (f.c0 + x0) / p.hpk, sub_head = (f.c0 + x0) % p.hpk;
+          int token = (f.c0 + x0) / p.hpk, sub_head = (f.c0 + x0) - token * p.hpk;
+          T* out = static_cast<T*>(p.out) + (f.r0 + token) * p.out_row + (int64_t)(f.kv * p.hpk + sub_head) * p.out_head + e;
+          float* part = p.parts + ((size_t)slot * NT + x0) * HD + e;
 #pragma unroll 1
           for (int x = 0; x < used; x += 8) {
-            uint32_t o[8];
+            uint32_t o[8], l[8];
             __syncwarp();
+            tmem_ld8_async(tmem + S::kLCol + x0 + x + sub, l);
             tmem_ld8(tmem + S::kOCol + k * NT + x0 + x + sub, o);
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               if (x + c >= used) break;
-              if (alone)
-                static_cast<T*>(p.out)[(f.r0 + token) * p.out_row + (int64_t)(f.kv * p.hpk + sub_head) * p.out_head + e] =
-                    from_f32<T>(__uint_as_float(o[c]) * change[h][x + c]);
-              else
-                p.parts[((size_t)f.slot * NT + x0 + x + c) * HD + e] = __uint_as_float(o[c]);
-              if (++sub_head == p.hpk) {
-                sub_head = 0;
-                ++token;
+              if (alone) {
+                *out = from_f32<T>(__fdividef(__uint_as_float(o[c]), __uint_as_float(l[c])));
+                out += p.out_head;
+                if (++sub_head == p.hpk) {
+                  sub_head = 0;
+                  out += p.out_row - p.hpk * p.out_head;
+                }
+              } else {
+                part[(size_t)(x + c) * HD] = __uint_as_float(o[c]);
               }
             }
           }
@@ -968,149 +1058,70 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// One row and KV head by four warps in 32-bit arithmetic, over the rows that it sees and no others; the
-// query heads first .. end - 1 of the KV head's are written. Each warp takes every fourth row, lane l the
-// values D l .. D l + D - 1 of a head.
-template <int HD, typename T>
-__device__ __noinline__ void plain_row(const TreeParams& p, int seq, int r0, int len, int row, int kv, int first, int end) {
-  using B = Kv4Block<HD>;
-  constexpr int D = HD / 32;
-  __shared__ float joined[4][kMaxHpk][HD];
-  __shared__ float tops[4][kMaxHpk], sums[4][kMaxHpk];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e0 = D * lane;
-  float q[kMaxHpk][D], o[kMaxHpk][D], m[kMaxHpk], l[kMaxHpk];
-#pragma unroll
-  for (int h = 0; h < kMaxHpk; ++h) {
-    m[h] = kNone;
-    l[h] = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) q[h][d] = o[h][d] = 0.f;
-    if (h < p.hpk)
-      load_vec<T, D>(static_cast<const T*>(p.q) + row * p.q_row + (int64_t)(kv * p.hpk + h) * p.q_head + e0, q[h]);
-  }
-  auto take = [&](const float (&k)[D], const float (&v)[D]) {
-#pragma unroll
-    for (int h = 0; h < kMaxHpk; ++h) {
-      if (h >= p.hpk) break;
-      float s = 0.f;
-#pragma unroll
-      for (int d = 0; d < D; ++d) s = fmaf(q[h][d], k[d], s);
-      s = warp_sum(s) * p.scale;
-      const float top = fmaxf(m[h], s), keep = ex2(m[h] - top), w = ex2(s - top);
-      m[h] = top;
-      l[h] = fmaf(l[h], keep, w);
-#pragma unroll
-      for (int d = 0; d < D; ++d) o[h][d] = fmaf(o[h][d], keep, w * v[d]);
-    }
-  };
-  for (int at = warp; at < len; at += 4) {
-    const int page = p.table[(int64_t)seq * p.table_stride + at / kPageRows], r = at % kPageRows;
-    if (page < 0 || page >= p.n_pages) continue;
-    const uint8_t* blk = p.pages + ((int64_t)page * p.nkv + kv) * B::kBytes;
-    const uint8_t* vb = blk + B::kHalf;
-    const int j = e0 / 32;
-    const __half* ks = reinterpret_cast<const __half*>(blk + B::kCodes);
-    const __half* vs = reinterpret_cast<const __half*>(vb + B::kCodes);
-    const uint32_t word = reinterpret_cast<const uint32_t*>(blk)[B::k_word(r, j, e0 % 32 / 8)];
-    const float kd = __half2float(ks[B::scale(r, j)]), km = __half2float(ks[HD * 2 + B::scale(r, j)]);
-    const float vd = __half2float(vs[B::scale(r, j)]), vm = __half2float(vs[HD * 2 + B::v_min(r, j)]);
-    float k[D], v[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int e = e0 + d;
-      k[d] = fmaf((float)((word >> (4 * (e % 8))) & 15u), kd, km);
-      const uint32_t c = reinterpret_cast<const uint16_t*>(vb)[B::v_half(r, j, e % 8)];
-      v[d] = fmaf((float)((c >> (4 * (e % 32 / 8))) & 15u), vd, vm);
-    }
-    take(k, v);
-  }
-  // the row and its ancestors; a parent that does not lie before its child is none
-  int node = row - r0;
-  for (int step = 0; node >= 0; ++step) {
-    if (step % 4 == warp) {
-      float k[D], v[D];
-      load_vec<T, D>(static_cast<const T*>(p.k) + (r0 + node) * p.k_row + kv * p.k_head + e0, k);
-      load_vec<T, D>(static_cast<const T*>(p.v) + (r0 + node) * p.v_row + kv * p.v_head + e0, v);
-      take(k, v);
-    }
-    const int above = p.parents ? p.parents[r0 + node] : node - 1;
-    node = above < node ? above : -1;
-  }
-#pragma unroll
-  for (int h = 0; h < kMaxHpk; ++h) {
-    if (h >= p.hpk) break;
-#pragma unroll
-    for (int d = 0; d < D; ++d) joined[warp][h][e0 + d] = o[h][d];
-    if (lane == 0) {
-      tops[warp][h] = m[h];
-      sums[warp][h] = l[h];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x + first * HD; i < end * HD; i += 128) {
-    const int h = i / HD, e = i % HD;
-    float top = kNone;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w][h]);
-    float s = 0.f, x = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = ex2(tops[w][h] - top);
-      s = fmaf(a, sums[w][h], s);
-      x = fmaf(a, joined[w][h][e], x);
-    }
-    static_cast<T*>(p.out)[row * p.out_row + (int64_t)(kv * p.hpk + h) * p.out_head + e] = from_f32<T>(x / s);
-  }
-  __syncthreads();
-}
-
-// Joins the parts of the tiles of one (sequence, KV head) in the order of the CTAs; a tile whose values f16
-// does not hold is computed again in 32 bits.
+// Joins the parts of the segment that a CTA opened and others share, in the order of the CTAs; where f16 did not hold
+// its values it is computed again in 32 bits.
+constexpr int kJoinThreads = 256;
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p, int ctas) {
+  constexpr int kAtOnce = 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.x / p.nkv, kv = blockIdx.x % p.nkv;
-  const Shape sh = shape_of<NT>(p, seq);
-  for (int tile = 0; tile < sh.tiles; ++tile) {
-    const int4 run = p.runs[(int64_t)blockIdx.x * p.most_tiles + tile];
-    const int first_cta = run.x, n = run.y, c0 = tile * sh.per, cols = min(sh.per, sh.nodes * p.hpk - c0);
-    if (n < 1 || first_cta < 0 || n > p.ctas - first_cta) continue;  // (nothing written where a wait gave up)
-    bool again = run.z != 0;
-    if (n > 1) {
-      // the part that starts the segment is its CTA's slot 1, the others slot 0
-      auto slot = [&](int i) { return (size_t)2 * (first_cta + i) + (i == 0 ? 1 : 0); };
-      for (int i = 0; i < n; ++i) again |= p.again[slot(i)] != 0;
-      if (!again)
-        for (int x = blockIdx.y * 128 + threadIdx.x; x < cols * HD / 4; x += 128 * gridDim.y) {
-          const int c = x / (HD / 4), e = 4 * (x % (HD / 4));
-          float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int i = 0; i < n; ++i) top = fmaxf(top, __ldcg(&p.stats[slot(i) * NT + c]).x);
-          for (int i = 0; i < n; ++i) {
-            const float2 st = __ldcg(&p.stats[slot(i) * NT + c]);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.parts + (slot(i) * NT + c) * HD + e));
-            const float w = ex2(st.x - top);
-            sum = fmaf(w, st.y, sum);
-            v[0] = fmaf(w, o.x, v[0]);
-            v[1] = fmaf(w, o.y, v[1]);
-            v[2] = fmaf(w, o.z, v[2]);
-            v[3] = fmaf(w, o.w, v[3]);
-          }
-          const float inv = 1.f / sum;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= inv;
-          store_vec<T, 4>(static_cast<T*>(p.out) + (sh.r0 + (c0 + c) / p.hpk) * p.out_row +
-                              (int64_t)(kv * p.hpk + (c0 + c) % p.hpk) * p.out_head + e, v);
-        }
+  const Opened f = p.opened[blockIdx.x];
+  if (f.run < 2 || f.run > ctas - (int)blockIdx.x) return;
+  // the part that starts the segment is its CTA's slot 1, the others slot 0
+  auto slot = [&](int i) { return (size_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
+  int again = 0;
+  for (int i = threadIdx.x & 31; i < f.run; i += 32) again |= p.again[slot(i)];
+  if (__any_sync(0xffffffffu, again != 0)) {
+    for (int c = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); c < f.cols; c += gridDim.y * (kJoinThreads / 32)) {
+      const int token = (f.c0 + c) / p.hpk;
+      plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + c) - token * p.hpk);
     }
-    if (again)
-      for (int token = c0 / p.hpk + blockIdx.y; token * p.hpk < c0 + cols; token += gridDim.y)
-        plain_row<HD, T>(p, seq, sh.r0, sh.len, sh.r0 + token, kv, max(0, c0 - token * p.hpk), min(p.hpk, c0 + cols - token * p.hpk));
+    return;
+  }
+  for (int x = blockIdx.y * kJoinThreads + threadIdx.x; x < f.cols * HD / 4; x += kJoinThreads * gridDim.y) {
+    const int c = x / (HD / 4), e = 4 * (x % (HD / 4));
+    float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < f.run; i0 += kAtOnce) {
+      float2 st[kAtOnce];
+      float4 o[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        st[k] = make_float2(kNone, 0.f);
+        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + k < f.run) {
+          st[k] = __ldcg(&p.stats[slot(i0 + k) * NT + c]);
+          o[k] = __ldcg(reinterpret_cast<const float4*>(p.parts + (slot(i0 + k) * NT + c) * HD + e));
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
+      const float keep = ex2(top - next);
+      top = next;
+      sum *= keep;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= keep;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float w = ex2(st[k].x - top);
+        sum = fmaf(w, st[k].y, sum);
+        v[0] = fmaf(w, o[k].x, v[0]);
+        v[1] = fmaf(w, o[k].y, v[1]);
+        v[2] = fmaf(w, o[k].z, v[2]);
+        v[3] = fmaf(w, o[k].w, v[3]);
+      }
+    }
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= inv;
+    const int token = (f.c0 + c) / p.hpk, head = f.kv * p.hpk + (f.c0 + c) - token * p.hpk;
+    store_vec<T, 4>(static_cast<T*>(p.out) + (f.r0 + token) * p.out_row + head * p.out_head + e, v);
   }
 }
 
 template <int HD, int NT, typename T>
-cudaError_t launch(const LaunchEnv& env, TreeParams p) {
+cudaError_t launch(const LaunchEnv& env, const TreeParams& p) {
   using S = Sizes<HD, NT>;
   CUtensorMap map{};
   if (p.n_pages > 0 && !encode_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.pages, 128, (uint64_t)p.n_pages * p.nkv * (S::kPage / 128),
@@ -1119,15 +1130,10 @@ cudaError_t launch(const LaunchEnv& env, TreeParams p) {
   auto kern = tree_kernel<HD, NT, T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  p.ctas = env.sm_count;
-  p.most_tiles = (kMaxNodes * p.hpk + NT - 1) / NT;
   e = rrr_launch_pdl(kern, dim3(env.sm_count), dim3(kThreads), (size_t)S::kSmem, env.stream, env.pdl, map, p);
   if (e != cudaSuccess) return e;
-  // few heads: their columns are shared by several CTAs
-  const int64_t heads = (int64_t)p.n_seqs * p.nkv;
-  int64_t across = (4 * (int64_t)env.sm_count + heads - 1) / heads;
-  if (across > 64) across = 64;
-  return rrr_launch_pdl(tree_join_kernel<HD, NT, T>, dim3((unsigned)heads, (unsigned)across), dim3(128), 0, env.stream, env.pdl, p);
+  return rrr_launch_pdl(tree_join_kernel<HD, NT, T>, dim3(env.sm_count, 6), dim3(kJoinThreads), 0, env.stream, env.pdl, p,
+                        env.sm_count);
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, const TreeParams& p) {
@@ -1137,14 +1143,14 @@ cudaError_t launch_type(const LaunchEnv& env, int type, const TreeParams& p) {
   return type == RRR_F16 ? launch<HD, 64, __half>(env, p) : launch<HD, 64, __nv_bfloat16>(env, p);
 }
 
-// The workspace: runs, statistics, flags, parts; for the widest tiles
+// The workspace: segments opened, statistics, flags, parts; for the widest tiles
 struct Layout {
   int64_t stats, again, parts, bytes;
 };
-Layout layout_of(const rrr_kv4_cache* c, int n_heads, int sms) {
-  const int64_t hpk = n_heads / c->n_kv_heads, tiles = (kMaxNodes * hpk + 63) / 64, slots = 2 * (int64_t)sms;
+Layout layout_of(const rrr_kv4_cache* c, int sms) {
+  const int64_t slots = 2 * (int64_t)sms;
   Layout l;
-  l.stats = ((int64_t)c->n_seqs * c->n_kv_heads * tiles * 16 + 255) / 256 * 256;
+  l.stats = ((int64_t)sms * (int64_t)sizeof(Opened) + 255) / 256 * 256;
   l.again = l.stats + slots * 96 * 8;
   l.parts = l.again + (slots * 4 + 255) / 256 * 256;
   l.bytes = l.parts + slots * 96 * c->head_dim * 4;
@@ -1159,9 +1165,11 @@ int check_tree(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int rows, cons
     return set_error(ctx, RRR_ERR_BAD_SHAPE,
                      "%s: n_heads must be a multiple of n_kv_heads, at most 8 query heads per KV head", fn);
   if (rows < 0 || rows > 1 << 24) return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: need 0 <= rows <= 2^24", fn);
-  // (a page is addressed by its line of 128 bytes, and one launch has 2^31 CTAs)
-  if (c->n_pages * c->n_kv_heads > INT32_MAX / (80 * c->head_dim / 128) || (int64_t)c->n_seqs * c->n_kv_heads > INT32_MAX / 16)
-    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: at most 2^38 bytes of pages and 2^27 sequences times heads", fn);
+  // (a page is addressed by its line of 128 bytes, the work counted in 32 bits)
+  const int64_t tiles = (kMaxNodes * (int64_t)(n_heads / c->n_kv_heads) + 63) / 64;
+  if (c->n_pages * c->n_kv_heads > INT32_MAX / (80 * c->head_dim / 128) ||
+      (__int128)c->n_seqs * c->n_kv_heads * tiles * (c->max_pages / 2 + 2 + kStart) > INT32_MAX)
+    return set_error(ctx, RRR_ERR_BAD_SHAPE, "%s: too many pages, or sequences times heads times pages of a sequence", fn);
   return RRR_OK;
 }
 
@@ -1178,7 +1186,7 @@ int rrr_tree_workspace(rrr_ctx* ctx, const rrr_kv4_cache* c, int n_heads, int ro
   if (rc) return rc;
   if (!bytes) return set_error(ctx, RRR_ERR_INVALID_ARG, "%s: null pointer", fn);
   (void)rows;
-  *bytes = layout_of(c, n_heads, ctx->sm_count).bytes;
+  *bytes = layout_of(c, ctx->sm_count).bytes;
   return RRR_OK;
 }
 
@@ -1252,9 +1260,9 @@ int rrr_attention_tree_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, const rrr_tree_
   p.rows = d->rows;
   p.scale = (d->scale == 0.f ? 1.f / sqrtf((float)hd) : d->scale) * 1.4426950408889634f;
   p.err = env.d_err;
-  const Layout l = layout_of(c, nh, ctx->sm_count);
+  const Layout l = layout_of(c, ctx->sm_count);
   char* w = static_cast<char*>(workspace);
-  p.runs = reinterpret_cast<int4*>(w);
+  p.opened = reinterpret_cast<Opened*>(w);
   p.stats = reinterpret_cast<float2*>(w + l.stats);
   p.again = reinterpret_cast<int*>(w + l.again);
   p.parts = reinterpret_cast<float*>(w + l.parts);
