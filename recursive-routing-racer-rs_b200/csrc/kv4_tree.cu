@@ -39,7 +39,7 @@ struct TreeParams {
   // workspace
   struct Opened* opened;  // [CTA]: the segment that it opened and shares
   float2* stats;          // [slot][column]: maximum, sum
-  int* again;             // [slot]
+  int* again;             // [slot][half of the columns]
   float* parts;           // [slot][column][value]
 };
 struct Opened {
@@ -51,7 +51,7 @@ struct Shape {
   int r0, nodes, len, blocks, tiles, per;  // per: columns of a tile
 };
 template <int NT>
-__device__ __forceinline__ Shape shape_of(const TreeParams& p, int seq) {
+__device__ __noinline__ Shape shape_of(const TreeParams& p, int seq) {
   Shape s;
   s.r0 = p.cu[seq];
   const int r1 = p.cu[seq + 1];
@@ -85,11 +85,12 @@ struct Share {
 };
 
 enum { kDraft = 1, kFirst = 2, kLast = 4, kAlone = 8, kStop = 16, kOpens = 32 };
-struct Info {  // of a block
-  int flags, seq, kv, len;
-  int r0, nodes, c0, cols, n; // the tile's columns c0 .. c0 + cols - 1 of the sequence's (row, head) pairs; n: with the padding
-  int valid[2];               // rows of each page that count
-  int count, run;             // the segment's number in this CTA, its CTAs
+struct __align__(16) Info {  // of a block
+  int flags;                // and the segment's number modulo 4 from bit 8 on
+  int n, valid[2];          // columns with the padding; rows of each page that count
+  int c0, cols, kv, count;  // the tile's columns c0 .. c0 + cols - 1 of the sequence's (row, head) pairs; the segment's number in this CTA
+  int r0, nodes, seq, len;
+  int run;                  // CTAs that share the segment
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -103,13 +104,27 @@ __device__ __forceinline__ float redux_max(float x) {
   return y;
 }
 // Bounded wait of a warp. The limit lies in memory: it is looked up only where a few tries of some microseconds each were
-// in vain.
-__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, int* err) {
+// in vain. (Out of line, with what else is not in the blocks' loops: with all of it in place the kernel was 165 KB of
+// instructions, and half of the warps' time went into fetching them.)
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* err) {
   bool ok = false;
 #pragma unroll 1
   for (int k = 0; k < 32 && !ok; ++k) ok = mbar_try_wait(bar, parity);
-  if (__all_sync(0xffffffffu, ok)) return true;
-  return warp_wait(bar, parity, err);
+  return __all_sync(0xffffffffu, ok) || warp_wait(bar, parity, err);
+}
+__device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, err);
+}
+
+// Whether a phase is complete, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // Bounded barrier of four warps.
@@ -174,13 +189,11 @@ __device__ __forceinline__ uint32_t top_bits(const uint4& w) {
   }
   return t;
 }
-// The power of two that brings values of at most `top` (finite, not zero) into [1, 2)
-__device__ __forceinline__ float to_one(uint32_t top, bool& fine) {
-  fine = top < 0x7f800000u;
+// The power of two that brings values of at most `top` into [1, 2) (1 where they are not finite)
+__device__ __forceinline__ float to_one(uint32_t top) {
   const int e = (int)(top >> 23);  // (a subnormal top counts as 2^-126)
-  return !fine || top == 0 ? 1.f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
+  return e == 255 || top == 0 ? 1.f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
 }
-constexpr uint32_t kHalfMax = 0x477fe000u;  // 65504
 // Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, so that f16 holds them with all their bits (and
 // their rows' weights are divided by it, which have bits to spare)
 __device__ __forceinline__ int lift_of(uint32_t top) { return top >= 0x3b000000u /* 2^-9 */ ? 0 : top >= 0x37000000u /* 2^-17 */ ? 1 : 2; }
@@ -280,6 +293,123 @@ __device__ __noinline__ void plain_row(const TreeParams& p, int seq, int r0, int
   store_vec<T, D>(static_cast<T*>(p.out) + row * p.out_row + head * p.out_head + e0, o);
 }
 
+// The tile's queries into shared memory, in the order of K's words: HD / 8 lanes per row, 8 values each; a row is
+// brought to [1, 2) by a power of two, which its line takes back.
+template <int HD, int NT, typename T>
+__device__ __noinline__ void queries(const TreeParams& p, const Info& f, int r, uint8_t* qs, float* line) {
+  constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes;
+  const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // the place among the words of a row of codes
+  constexpr int kBatch = 4;
+#pragma unroll 1
+  for (int c0 = r / kLanes; c0 < f.n; c0 += kBatch * kAcross) {
+    uint4 v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = c0 + k * kAcross, column = f.c0 + c, token = column / p.hpk, head = f.kv * p.hpk + column - token * p.hpk;
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (c < f.cols)
+        v[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(f.r0 + token) * p.q_row + head * p.q_head + 8 * x);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = c0 + k * kAcross;
+      uint32_t top = top_bits<T>(v[k]);
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (c >= f.n) break;
+      const float s = to_one(top);
+      uint32_t y[4];
+      scaled_pairs<T>(v[k], s, y);
+      *reinterpret_cast<uint4*>(qs + (w / 8) * NT * 128 + sw128_off(c, w % 8)) = make_uint4(y[0], y[1], y[2], y[3]);
+      if (x == 0) {
+        line[c] = c < f.cols ? p.scale / s : 0.f;
+        line[NT + c] = kBias;
+      }
+    }
+  }
+}
+// Up to 64 drafted keys from row `first` on: HD / 8 lanes per row, 8 values each; a row is brought to [1, 2) by a power of two.
+// They go to shared memory, from where their threads take them to TMEM.
+template <int HD, typename T>
+__device__ __noinline__ void drafted_keys(const TreeParams& p, const Info& f, int r, int first, uint8_t* to, float* scales) {
+  constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes, kBatch = 4;
+  const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J, rows = min(f.nodes - first, 64);
+  const T* src = static_cast<const T*>(p.k) + (int64_t)(f.r0 + first) * p.k_row + f.kv * p.k_head + 8 * x;
+#pragma unroll 1
+  for (int c0 = r / kLanes; c0 < 64; c0 += kBatch * kAcross) {
+    if (c0 - r / kLanes >= rows) break;
+    uint4 v[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (c0 + k * kAcross < rows) v[k] = *reinterpret_cast<const uint4*>(src + (c0 + k * kAcross) * p.k_row);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = c0 + k * kAcross;
+      uint32_t top = top_bits<T>(v[k]);
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float s = to_one(top);
+      uint32_t y[4];
+      scaled_pairs<T>(v[k], s, y);
+      *reinterpret_cast<uint4*>(to + c * (2 * HD) + ((w ^ (c & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      if (x == 0) scales[first + c] = 1.f / s;
+    }
+  }
+}
+// Drafted values: rows 8 o .. + 7 (o = tid % 16), values 8 (tid / 16 + 8 c) .. + 7 of them; the largest of their bits, and the
+// values, lifted, into shared memory
+template <int HD, typename T>
+__device__ __forceinline__ void drafted_eight(const TreeParams& p, const Info& f, int tid, int c, uint4 (&w)[8]) {
+  const int o = tid & 15, rows = min(max(f.nodes - 8 * o, 0), 8);
+  const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head + (int64_t)(f.r0 + 8 * o) * p.v_row + 8 * ((tid >> 4) + 8 * c);
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    w[r] = make_uint4(0, 0, 0, 0);
+    if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + r * p.v_row);
+  }
+}
+template <int HD, typename T>
+__device__ __noinline__ uint32_t drafted_top(const TreeParams& p, const Info& f, int tid) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < HD / 64; c += 2) {
+    uint4 w[2][8];
+    drafted_eight<HD, T>(p, f, tid, c, w[0]);
+    if (HD > 64) drafted_eight<HD, T>(p, f, tid, c + 1, w[1]);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      top = max(top, top_bits<T>(w[0][r]));
+      if (HD > 64) top = max(top, top_bits<T>(w[1][r]));
+    }
+  }
+  return __reduce_max_sync(0xffffffffu, top);
+}
+template <int HD, typename T>
+__device__ __noinline__ void drafted_values(const TreeParams& p, const Info& f, int tid, float lift, uint8_t* dst) {
+  constexpr int kERows = HD < 128 ? HD : 128;
+  const int o = tid & 15;
+#pragma unroll 1
+  for (int c = 0; c < HD / 64; ++c) {
+    uint4 w[8];
+    drafted_eight<HD, T>(p, f, tid, c, w);
+    const int e0 = 8 * ((tid >> 4) + 8 * c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float2 a = pair_of<T>((&w[2 * r].x)[k / 2]), b = pair_of<T>((&w[2 * r + 1].x)[k / 2]);
+        y[r] = as_u32(__floats2half2_rn((k & 1 ? a.y : a.x) * lift, (k & 1 ? b.y : b.x) * lift));
+      }
+      const int e = e0 + k;
+      *reinterpret_cast<uint4*>(dst + ((e >> 7) * 2 + (o >> 3)) * kERows * 128 + (e & 127) * 128 + (((o & 7) ^ (e & 7)) << 4)) =
+          make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
+
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ TreeParams p) {
@@ -287,15 +417,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int G = HD / 32, J = G < 4 ? G : 4, PL = G / J;  // groups, groups per plane, planes
   extern __shared__ uint8_t smem_dyn[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages], k_full[2], s_full[2], v_full[S::kVs], p_full[2], p_empty[2], o_empty, fin;
+  __shared__ uint64_t told[kInfos];                // that the info of a segment's first block is there, or that there is none
+  __shared__ uint64_t lifted[4];                  // v_lift is there, by the segment's number (every segment but the last has drafted rows here)
   __shared__ uint64_t teams[2];                   // of K's and V's warps
   __shared__ Info infos[kInfos];
   __shared__ uint4 seen[4][kMaxNodes];            // of a tree's row: the rows that it sees, as bits
   __shared__ int up[kMaxNodes];
   __shared__ float k_scale[4][kRows];
   __shared__ int v_lift[4];
-  __shared__ int k_again[4], v_again[4];
+  __shared__ int k_again[4];
   __shared__ uint32_t v_tops[4];
-  __shared__ __align__(16) float2 lines[4][NT];   // of a column: the argument of a weight's exponential is score * x + y
+  __shared__ __align__(16) float lines[4][2 * NT];  // of a column c: the argument of a weight's exponential is score * [c] + [NT + c]
   __shared__ float quad[2][4][NT / 2], change[2][NT / 2];
   __shared__ int warp_units[kThreads / 32], first_base, first_seq, dead[2];
   __shared__ uint32_t tmem_slot;
@@ -320,6 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < S::kVs; ++i) mbar_init(&v_full[i], 4);
     mbar_init(&o_empty, 8);
+    for (int i = 0; i < kInfos; ++i) mbar_init(&told[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&lifted[i], 1);
     mbar_init(&fin, 1);
     fence_mbarrier_init();
     prefetch_map(&map);
@@ -379,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Shape sh = shape_of<NT>(p, s);
     int each = sh.blocks + kStart;
     int g = (u0 - base) / each, blk = max(0, (u0 - base) % each - kStart);
+    int the = 0, run = 0;  // (of lane 0) the segment's flags, its CTAs
     bool begin = true, stop = false;
     uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
     for (;; ++it) {
@@ -398,8 +533,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int seg0 = base + g * each + kStart;  // unit of the segment's block 0
       stop = s >= p.n_seqs || seg0 + blk >= u1;
-      int page = 0, valid = 0;
       const bool draft = blk + 1 == sh.blocks;
+      Info& f = infos[it % kInfos];
+      const int kv = stop ? 0 : g / sh.tiles, tile = g - kv * sh.tiles;
+      if (begin || stop) {
+        // what the segment is, before its first block is there; its rows on their way to L2
+        if (lane == 0) {
+          const int c0 = share.cta_of(seg0), c1 = share.cta_of(seg0 + sh.blocks - 1);
+          ++count;
+          the = (c0 == c1 ? kAlone : 0) | (c0 == (int)blockIdx.x ? kOpens : 0) | (count & 3) << 8;
+          run = c1 - c0 + 1;
+          f.flags = stop ? kStop : the | kFirst;
+          f.n = sh.per;
+          f.c0 = tile * sh.per;
+          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.kv = kv;
+          f.r0 = sh.r0;
+          mbar_arrive(&told[it % kInfos]);
+        }
+        if (!stop) {
+          constexpr int kLines = HD / 64;
+          const int c0 = tile * sh.per, cols = min(sh.per, sh.nodes * p.hpk - c0);
+          for (int x = lane; x < (cols + 2 * sh.nodes) * kLines; x += 32) {
+            const int c = x / kLines, part = x % kLines * 64;
+            const T* a;
+            if (c < cols) {
+              const int token = (c0 + c) / p.hpk;
+              a = static_cast<const T*>(p.q) + (int64_t)(sh.r0 + token) * p.q_row + (kv * p.hpk + (c0 + c) - token * p.hpk) * p.q_head;
+            } else if (c < cols + sh.nodes) {
+              a = static_cast<const T*>(p.k) + (int64_t)(sh.r0 + c - cols) * p.k_row + kv * p.k_head;
+            } else {
+              a = static_cast<const T*>(p.v) + (int64_t)(sh.r0 + c - cols - sh.nodes) * p.v_row + kv * p.v_head;
+            }
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a + part));
+          }
+        }
+      }
+      int page = 0, valid = 0;
       if (!stop && !draft && lane < 2) {
         const int at = 2 * blk + lane;
         valid = min(kPageRows, sh.len - at * kPageRows);
@@ -410,37 +580,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           valid = 0;
         }
       }
-      if (begin) ++count;
       if (!wait(&empty[st], phase)) break;
       const int v0 = __shfl_sync(0xffffffffu, valid, 0), v1 = __shfl_sync(0xffffffffu, valid, 1);
       const int p0 = __shfl_sync(0xffffffffu, page, 0), p1 = __shfl_sync(0xffffffffu, page, 1);
       if (lane == 0) {
-        const int kv = stop ? 0 : g / sh.tiles;
         uint8_t* dst = ring + (size_t)st * S::kStage;
-        if (v0 > 0 || v1 > 0) {
-          if (v0 > 0) tma_load_2d(dst, &map, 0, (int)(((int64_t)p0 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
-          if (v1 > 0)
-            tma_load_2d(dst + S::kPage, &map, 0, (int)(((int64_t)p1 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
-        }
-        Info& f = infos[it % kInfos];
+        if (v0 > 0) tma_load_2d(dst, &map, 0, (int)(((int64_t)p0 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
+        if (v1 > 0) tma_load_2d(dst + S::kPage, &map, 0, (int)(((int64_t)p1 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
         if (stop) {
           f.flags = kStop;
         } else {
-          const int tile = g - kv * sh.tiles, c0 = share.cta_of(seg0), c1 = share.cta_of(seg0 + sh.blocks - 1);
-          f.flags = (draft ? kDraft : 0) | (begin ? kFirst : 0) | (draft || seg0 + blk + 1 >= u1 ? kLast : 0) |
-                    (c0 == c1 ? kAlone : 0) | (c0 == (int)blockIdx.x ? kOpens : 0);
-          f.seq = s;
-          f.kv = kv;
-          f.len = sh.len;
-          f.r0 = sh.r0;
-          f.nodes = sh.nodes;
-          f.c0 = tile * sh.per;
-          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.flags = the | (draft ? kDraft : 0) | (begin ? kFirst : 0) | (draft || seg0 + blk + 1 >= u1 ? kLast : 0);
           f.n = sh.per;
           f.valid[0] = v0;
           f.valid[1] = v1;
+          f.c0 = tile * sh.per;
+          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.kv = kv;
           f.count = count;
-          f.run = c1 - c0 + 1;
+          f.r0 = sh.r0;
+          f.nodes = sh.nodes;
+          f.seq = s;
+          f.len = sh.len;
+          f.run = run;
         }
         mbar_arrive_expect_tx(&full[st], (uint32_t)((v0 > 0) + (v1 > 0)) * S::kPage);
       }
@@ -464,56 +626,71 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 16) {
     // ---------------- products: S(0), S(1), PV(0), S(2), PV(1), ...
     const uint32_t fmt = 1u << 4;  // f16 operands, f32 sums; M = 128
-    auto weighed = [&](int i) {    // O^T += V^T P^T of block i, and the sums of the weights
-      const Info& f = infos[i % kInfos];
-      if (!wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u) || !wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u))
-        return false;
-      if ((f.flags & kFirst) && f.count > 0 && !wait(&o_empty, (uint32_t)(f.count - 1) & 1u)) return false;
-      tc_fence_after();
-      const uint32_t idesc = fmt | (1u << 16) | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      const uint32_t va = smem_addr(vs + (i % S::kVs) * S::kV), pa = smem_addr(ps + (i & 1) * S::kP);
-      const uint32_t more = f.flags & kFirst ? 0u : 1u;
-      const uint32_t ones = tmem + S::kOnes + (f.flags & kDraft ? 8u * v_lift[f.count & 3] : 0u);
+    const uint64_t q_desc = sw128_desc(smem_addr(qs)), v_desc = sw128_desc(smem_addr(vs)), p_desc = sw128_desc_mn(smem_addr(ps), kRows * 128);
+    auto scores = [&](int i) {   // S = K Q^T of block i
+      const uint32_t idesc = fmt | ((uint32_t)(infos[i % kInfos].n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint32_t to = tmem + S::kSCol + (i & 1) * NT, k = tmem + (i % S::kKs) * S::kKCols;
       if (elect_one()) {
-#pragma unroll 1
-        for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-          for (int kk = 0; kk < kRows / 16; ++kk)
-            umma_f16(tmem + S::kOCol + h * NT, sw128_desc(va + (uint32_t)(h * 2 + kk / 4) * S::kERows * 128 + 32u * (kk % 4)),
-                     sw128_desc_mn(pa + 2048u * kk, kRows * 128), idesc, kk > 0 ? 1u : more);
+        for (int kk = 0; kk < HD / 16; ++kk)
+          umma_f16_ta(to, k + 8u * kk, q_desc + (((kk / 4) * NT * 128 + 32 * (kk % 4)) >> 4), idesc, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[i & 1]);
+      }
+      __syncwarp();
+    };
+    auto weighed = [&](int i) {  // O^T += V^T P^T of block i, and the sums of the weights
+      const Info& f = infos[i % kInfos];
+      const int flags = f.flags;
+      const uint32_t idesc = fmt | (1u << 16) | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint64_t v = v_desc + (uint32_t)((i % S::kVs) * (S::kV >> 4)), w = p_desc + (uint32_t)((i & 1) * (S::kP >> 4));
+      const uint32_t more = flags & kFirst ? 0u : 1u;
+      const uint32_t ones = tmem + S::kOnes + (flags & kDraft ? 8u * v_lift[(flags >> 8) & 3] : 0u);
+      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk)
-          umma_f16_ta(tmem + S::kLCol, ones, sw128_desc_mn(pa + 2048u * kk, kRows * 128), idesc, kk > 0 ? 1u : more);
+        for (int kk = 0; kk < kRows / 16; ++kk) {
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h)
+            umma_f16(tmem + S::kOCol + h * NT, v + (((h * 2 + kk / 4) * S::kERows * 128 + 32 * (kk % 4)) >> 4), w + (2048 * kk >> 4), idesc,
+                     kk > 0 ? 1u : more);
+          umma_f16_ta(tmem + S::kLCol, ones, w + (2048 * kk >> 4), idesc, kk > 0 ? 1u : more);
+        }
         umma_commit(&p_empty[i & 1]);
       }
       __syncwarp();
-      return true;
     };
-    int i = 0;
-#pragma unroll 1
-    for (;; ++i) {
-      if (!wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+    // S(0), S(1), then in turn, once P(i) is there: S(i + 2), whose place that frees, and PV(i); S later, if its keys are
+    auto have_keys = [&](int i) {
+      const bool ok = wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u);
       tc_fence_after();
-      const Info& f = infos[i % kInfos];
-      const bool stop = f.flags & kStop;
-      if (!stop) {
-        const uint32_t idesc = fmt | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-        const uint32_t qa = smem_addr(qs);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            umma_f16_ta(tmem + S::kSCol + (i & 1) * NT, tmem + (i % S::kKs) * S::kKCols + 8u * kk,
-                        sw128_desc(qa + (uint32_t)(kk / 4) * NT * 128 + 32u * (kk % 4)), idesc, kk > 0 ? 1u : 0u);
-          umma_commit(&s_full[i & 1]);
-        }
-        __syncwarp();
-      }
-      if (i > 0 && !weighed(i - 1)) break;
-      if (stop) {
-        if (lane == 0) mbar_arrive(&s_full[i & 1]);
-        break;
-      }
+      return ok;
+    };
+    bool ok = have_keys(0), stop = ok && (infos[0].flags & kStop);
+    int next = 0;  // the block whose scores come next, or the one that says stop
+    if (ok && !stop) scores(next++);
+    if (ok && !stop) {
+      ok = have_keys(1);
+      stop = ok && (infos[1].flags & kStop);
+      if (ok && !stop) scores(next++);
     }
+#pragma unroll 1
+    for (int i = 0; ok && i < next; ++i) {
+      ok = wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u);
+      auto ahead = [&]() {
+        ok = have_keys(next);
+        stop = ok && (infos[next % kInfos].flags & kStop);
+        if (ok && !stop) scores(next++);
+      };
+      const bool early = ok && !stop && __all_sync(0xffffffffu, mbar_test(&k_full[next & 1], (uint32_t)(next >> 1) & 1u));
+      if (early) ahead();
+      ok = ok && wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u);
+      const int flags = infos[i % kInfos].flags, count = infos[i % kInfos].count;
+      ok = ok && (!(flags & kFirst) || count == 0 || wait(&o_empty, (uint32_t)(count - 1) & 1u));
+      if (!ok) break;
+      tc_fence_after();
+      weighed(i);
+      if (!early && !stop) ahead();
+    }
+    if (stop && lane == 0) mbar_arrive(&s_full[next & 1]);
     if (elect_one()) umma_commit(&fin);
     __syncwarp();
   } else if (warp >= 18) {
@@ -528,19 +705,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0;; ++i) {
       if (!wait(&full[st], phase)) break;
       const Info& f = infos[i % kInfos];
-      if (f.flags & kStop) break;
-      const int par = f.count & 3;
-      if (f.flags & kFirst) {
-        if (tid == 0) v_again[par] = 0;
-        if (!team()) break;
-      }
+      const int flags = f.flags;
+      if (flags & kStop) break;
       uint8_t* const stage = ring + (size_t)st * S::kStage;
       uint8_t* const dst = vs + (i % S::kVs) * S::kV;
       // the place is free once PV(i - kVs) is done
       auto free_place = [&]() {
         return i < S::kVs || wait(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u);
       };
-      if (!(f.flags & kDraft)) {
+      if (!(flags & kDraft)) {
         if (f.valid[0] < kPageRows || f.valid[1] < kPageRows) {
           // rows that do not count: d = m = 0
           const int half = tid >> 6, row = tid & 63;
@@ -554,17 +727,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int o = tid >> 3, g = tid & 7;  // rows 8 o .. + 7 of the block, values 32 i + 8 n + g
         const uint8_t* const page = stage + (o >> 3) * S::kPage;
         const int r = (o & 7) * 8;
-        // (whether f16 holds what the groups stand for: a share of them each)
-        __half2 most = as_half2(0u);
-#pragma unroll
-        for (int k = 0; k < G / 2; ++k) {
-          const int row = r + 2 * (g & 3), j = (g >> 2) * (G / 2) + k;
-          const __half2 dd = __halves2half2(*reinterpret_cast<const __half*>(page + swizzled(72 * HD + 2 * (row * G + j))),
-                                            *reinterpret_cast<const __half*>(page + swizzled(72 * HD + 2 * ((row + 1) * G + j))));
-          const uint32_t mm = *reinterpret_cast<const uint32_t*>(page + swizzled(76 * HD + 4 * ((row >> 1) * G + j)));
-          most = __hmax2(most, __hfma2(dd, as_half2(0x4b804b80u), __habs2(as_half2(mm))));
-        }
-        if (__hisinf(__low2half(most)) || __hisinf(__high2half(most))) v_again[par] = 1;
         if (!free_place()) break;
 #pragma unroll 1
         for (int P = 0; P < PL; ++P) {
@@ -616,54 +778,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        constexpr int C = HD / 64;
-        const int o = tid & 15, x = tid >> 4;  // rows 8 o .. + 7, values 8 (x + 8 c) .. + 7
-        const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head;
-        const int rows = min(max(f.nodes - 8 * o, 0), 8);
-        uint32_t top = 0;
-#pragma unroll 1
-        for (int c = 0; c < C; ++c) {
-          uint4 w[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            w[r] = make_uint4(0, 0, 0, 0);
-            if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + (int64_t)(f.r0 + 8 * o + r) * p.v_row + 8 * (x + 8 * c));
-          }
-#pragma unroll
-          for (int r = 0; r < 8; ++r) top = max(top, top_bits<T>(w[r]));
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
+        uint32_t top = drafted_top<HD, T>(p, f, tid);
         if (lane == 0) v_tops[warp & 3] = top;
         if (!team()) break;
         top = max(max(v_tops[0], v_tops[1]), max(v_tops[2], v_tops[3]));
-        const float lift = lifted_by(lift_of(top));
         if (tid == 0) {
-          v_lift[par] = lift_of(top);
-          if (top > kHalfMax) v_again[par] = 1;
+          v_lift[(flags >> 8) & 3] = lift_of(top);
+          mbar_arrive(&lifted[(flags >> 8) & 3]);
         }
         if (!free_place()) break;
-#pragma unroll 1
-        for (int c = 0; c < C; ++c) {
-          uint4 w[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            w[r] = make_uint4(0, 0, 0, 0);
-            if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + (int64_t)(f.r0 + 8 * o + r) * p.v_row + 8 * (x + 8 * c));
-          }
-          const int e0 = 8 * (x + 8 * c);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint32_t y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float2 a = pair_of<T>((&w[2 * r].x)[k / 2]), b = pair_of<T>((&w[2 * r + 1].x)[k / 2]);
-              y[r] = as_u32(__floats2half2_rn((k & 1 ? a.y : a.x) * lift, (k & 1 ? b.y : b.x) * lift));
-            }
-            const int e = e0 + k;
-            *reinterpret_cast<uint4*>(dst + ((e >> 7) * 2 + (o >> 3)) * S::kERows * 128 + (e & 127) * 128 +
-                                      (((o & 7) ^ (e & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-          }
-        }
+        drafted_values<HD, T>(p, f, tid, lifted_by(lift_of(top)), dst);
         if (!team()) break;  // v_tops is read
       }
       fence_proxy_async_smem();
@@ -691,43 +815,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e = 0; e < 8; ++e) ones[e] = k == 0 ? 0x3c003c00u : k == 1 ? 0x5c005c00u : 0x78007800u;
       tmem_st8(tmem + S::kOnes + 8 * k + sub, ones);
     }
+    bool begins = true;
+    uint32_t turns = 0;  // of the waits for `told`
 #pragma unroll 1
     for (int i = 0;; ++i) {
-      if (!wait(&full[st], phase)) break;
       const Info& f = infos[i % kInfos];
-      const int flags = f.flags, par = f.count & 3;
+      if (begins) {
+        if (!wait(&told[i % kInfos], turns >> (i % kInfos) & 1u)) break;
+        turns ^= 1u << (i % kInfos);
+        if (!(f.flags & kStop)) {
+          const int par = (f.flags >> 8) & 3;
+          if (r == 0) k_again[par] = 0;
+          // S of the segment before has read its queries
+          if (i > 0 && !wait(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
+          queries<HD, NT, T>(p, f, r, qs, lines[par]);
+          fence_proxy_async_smem();
+          if (!team()) break;
+        }
+      }
+      if (!wait(&full[st], phase)) break;
+      const int flags = f.flags, par = (flags >> 8) & 3;
+      begins = flags & kLast;
       if (flags & kStop) {
         // (not before the products have seen the block two before, or they would miss its turn)
         if (i >= 2 && !wait(&s_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
         if (lane == 0) mbar_arrive(&k_full[i & 1]);
         break;
-      }
-      if (flags & kFirst) {
-        if (r == 0) k_again[par] = 0;
-        if (!team()) break;
-        // S of the segment before has read its queries
-        if (i > 0 && !wait(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
-        // kLanes lanes per row, 8 values each; a row is brought to [1, 2) by a power of two
-        constexpr int kLanes = HD / 8 < 32 ? HD / 8 : 32, kAcross = 128 / kLanes;
-        const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // the place among the words of a row of codes
-#pragma unroll 2
-        for (int c = r / kLanes; c < f.n; c += kAcross) {
-          const int column = f.c0 + c, token = column / p.hpk, head = f.kv * p.hpk + column - token * p.hpk;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (c < f.cols)
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(f.r0 + token) * p.q_row + head * p.q_head + 8 * x);
-          uint32_t top = top_bits<T>(v);
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          bool fine;
-          const float s = to_one(top, fine);
-          if (!fine) k_again[par] = 1;
-          uint32_t y[4];
-          scaled_pairs<T>(v, s, y);
-          *reinterpret_cast<uint4*>(qs + (w / 8) * NT * 128 + sw128_off(c, w % 8)) = make_uint4(y[0], y[1], y[2], y[3]);
-          if (x == 0) lines[par][c] = make_float2(c < f.cols ? p.scale / s : 0.f, kBias);
-        }
-        fence_proxy_async_smem();
       }
       const uint32_t dst = tmem + (i % S::kKs) * S::kKCols + sub;
       // the place is free once S(i - kKs) is done
@@ -774,62 +887,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         // drafted rows: to [1, 2) by a power of two each; who sees whom
-        const bool some = r < f.nodes;
-        const T* src = static_cast<const T*>(p.k) + (int64_t)(f.r0 + r) * p.k_row + f.kv * p.k_head;
+        uint8_t* const to = ring + (size_t)st * S::kStage;
         int parent = -1;
-        if (some) {
+        if (r < f.nodes) {
           parent = p.parents ? p.parents[f.r0 + r] : r - 1;
           if (parent < -1 || parent >= r) {
             flag_position(p.err);
             parent = -1;
           }
         }
-        uint32_t top = 0;
-        if (some)
-#pragma unroll 8
-          for (int x = 0; x < HD / 8; ++x) top = max(top, top_bits<T>(reinterpret_cast<const uint4*>(src)[x]));
-        bool fine;
-        const float s = to_one(top, fine);
-        if (!fine) k_again[par] = 1;
-        k_scale[par][r] = 1.f / s;
-        uint4 bits = make_uint4(0, 0, 0, 0);
-        if (some) (&bits.x)[r >> 5] = 1u << (r & 31);
-        seen[par][r] = bits;
         up[r] = parent;
-        bool ok = team();
+        bool ok = free_place();
 #pragma unroll 1
-        for (int n = 1; ok && n < f.nodes; n <<= 1) {  // ancestors up to 2 n rows above
-          uint4 more = make_uint4(0, 0, 0, 0);
-          int next = -1;
-          if (parent >= 0) {
-            more = seen[par][parent];
-            next = up[parent];
-          }
+        for (int first = 0; ok && first < f.nodes; first += 64) {
+          drafted_keys<HD, T>(p, f, r, first, to, k_scale[par]);
           ok = team();
-          bits.x |= more.x;
-          bits.y |= more.y;
-          bits.z |= more.z;
-          bits.w |= more.w;
-          parent = next;
-          seen[par][r] = bits;
-          up[r] = parent;
-          ok = ok && team();
-        }
-        if (!ok || !free_place()) break;
+          if ((r & 64) == first) {
 #pragma unroll 1
-        for (int w0 = 0; w0 < HD / 8; w0 += 4) {  // four words, 16 columns
-          uint32_t y[16];
+            for (int w = 0; w < HD / 8; w += 4) {  // four words, 16 columns
+              uint32_t y[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int w = w0 + k, P = w / (4 * J), t = w % (4 * J) / J, j = P * J + w % J;
-            uint32_t z[4] = {0, 0, 0, 0};
-            if (some) scaled_pairs<T>(reinterpret_cast<const uint4*>(src)[4 * j + t], s, z);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[4 * k + e] = z[e];
+              for (int k = 0; k < 4; ++k) {
+                const uint4 v = *reinterpret_cast<const uint4*>(to + (r & 63) * (2 * HD) + (((w + k) ^ (r & 7)) << 4));
+                y[4 * k] = v.x;
+                y[4 * k + 1] = v.y;
+                y[4 * k + 2] = v.z;
+                y[4 * k + 3] = v.w;
+              }
+              __syncwarp();
+              tmem_st16(dst + 4 * w, y);
+            }
           }
-          __syncwarp();
-          tmem_st16(dst + 4 * w0, y);
+          if (first + 64 < f.nodes) ok = ok && team();
         }
+        if (!ok) break;
+        uint4 bits = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (int node = r < f.nodes ? r : -1; node >= 0; node = up[node]) {
+          const uint32_t bit = 1u << (node & 31);
+          if (node < 64) {
+            if (node < 32) bits.x |= bit; else bits.y |= bit;
+          } else {
+            if (node < 96) bits.z |= bit; else bits.w |= bit;
+          }
+        }
+        seen[par][r] = bits;
+        fence_proxy_async_smem();
       }
       tmem_wait_st();
       tc_fence_before();
@@ -851,19 +954,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0;; ++i) {
       bool ok = wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u);
       const Info& f = infos[i % kInfos];
-      const int flags = ok ? f.flags : kStop;
-      const int par = f.count & 3, cols = f.n >> 1, x0 = h * cols;  // this half: columns x0 .. x0 + cols - 1 of the tile
+      const int4 head = *reinterpret_cast<const int4*>(&f);
+      const int flags = ok ? head.x : kStop, valid = r < 64 ? head.z : head.w;
+      const int par = (flags >> 8) & 3, cols = head.y >> 1, x0 = h * cols;  // this half: columns x0 .. x0 + cols - 1 of the tile
       const bool first = flags & kFirst;
       const uint32_t sc = tmem + S::kSCol + (i & 1) * NT + x0 + sub;
       uint8_t* const dst = ps + (i & 1) * S::kP + (r >> 3) * 1024 + (r & 7) * 128;
-      float2* const line = lines[par] + x0;
+      float* const line = lines[par] + x0;
       tc_fence_after();
       // P's place is free once PV(i - 2) is done
       if (!(flags & kStop) && i >= 2) ok = wait(&p_empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u);
-      const bool plain = !(flags & kDraft) && (r & ~31 & 63) + 32 <= f.valid[r >> 6];  // every row of the warp counts, for all columns
+      const bool plain = !(flags & kDraft) && (r & 32) + 32 <= valid;  // every row of the warp counts, for all columns
       float ks = 1.f, low = 1.f;
       if (flags & kDraft) {
-        ok = ok && wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u);  // (v_lift)
+        ok = ok && wait(&lifted[par], (uint32_t)(f.count >> 2) & 1u);
         ks = k_scale[par][r];
         low = 1.f / lifted_by(v_lift[par]);
       }
@@ -872,11 +976,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_ld8(sc + x, reinterpret_cast<uint32_t(&)[8]>(a));
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float4 ln = *reinterpret_cast<const float4*>(line + x + e);
-          a[e] = fmaf(a[e] * ks, ln.x, ln.y);
-          a[e + 1] = fmaf(a[e + 1] * ks, ln.z, ln.w);
-        }
+        for (int e = 0; e < 8; ++e) a[e] = fmaf(a[e] * ks, line[x + e], line[NT + x + e]);
         if (flags & kDraft) {
           int token = (f.c0 + x0 + x) / p.hpk, sub_head = (f.c0 + x0 + x) - token * p.hpk;
           const uint32_t* bits = reinterpret_cast<const uint32_t*>(seen[par]) + qd;
@@ -888,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++token;
             }
           }
-        } else if ((r & 63) >= f.valid[r >> 6]) {
+        } else if ((r & 63) >= valid) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) a[e] = -INFINITY;
         }
@@ -897,21 +997,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto weights = [&]() {
         float top = -INFINITY;
         if (plain) {
-#pragma unroll 1
-          for (int x = 0; x < cols; x += 8) {
-            uint32_t s[8], w[4];
-            tmem_ld8(sc + x, s);
-            const float4* ln = reinterpret_cast<const float4*>(line + x);
+          auto eight = [&](const uint32_t* sv, int x) {
+            uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 l = ln[e];
-              const float u = fmaf(__uint_as_float(s[2 * e]), l.x, l.y), v = fmaf(__uint_as_float(s[2 * e + 1]), l.z, l.w);
-              top = fmaxf(top, fmaxf(u, v));
-              w[e] = as_u32(__floats2half2_rn(ex2(u), ex2(v)));
+            for (int e = 0; e < 8; e += 4) {
+              const float4 a = *reinterpret_cast<const float4*>(line + x + e), b = *reinterpret_cast<const float4*>(line + NT + x + e);
+              const float2 u = __ffma2_rn(make_float2(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), make_float2(a.x, a.y), make_float2(b.x, b.y));
+              const float2 v = __ffma2_rn(make_float2(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), make_float2(a.z, a.w), make_float2(b.z, b.w));
+              top = fmaxf(top, fmaxf(u.x, u.y));
+              top = fmaxf(top, fmaxf(v.x, v.y));
+              w[e / 2] = as_u32(__floats2half2_rn(ex2(u.x), ex2(u.y)));
+              w[e / 2 + 1] = as_u32(__floats2half2_rn(ex2(v.x), ex2(v.y)));
             }
             const int c = x0 + x;
             *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
+          };
+#pragma unroll 1
+          for (int x = 0; x < cols; x += 16) {
+            uint32_t sv[16];
+            tmem_ld16(sc + x, sv);  // (columns past the last are loaded, and left)
+            tmem_wait_ld();
+            eight(sv, x);
+            if (x + 8 < cols) eight(sv + 8, x + 8);
           }
         } else {
 #pragma unroll 1
@@ -932,12 +1040,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         return top;
       };
       float top = -INFINITY;
-      if (ok && !(flags & kStop) && !first) top = weights();
-      // a new maximum, where a weight would be larger than the lazy ones may be
       if (!ok) dead[h] = 1;
-      const bool grown = any_of_128(bar, first || top > kBias + kLazy);
-      if ((flags & kStop) || *reinterpret_cast<volatile int*>(&dead[h])) break;
-      if (grown) {
+      bool leave = false;
+#pragma unroll 1
+      for (int turn = !ok || (flags & (kStop | kFirst)) ? 1 : 0; turn < 2; ++turn) {
+        if (turn) {
+          // a new maximum, where a weight would be larger than the lazy ones may be
+          const bool grown = any_of_128(bar, first || top > kBias + kLazy);
+          leave = (flags & kStop) || *reinterpret_cast<volatile int*>(&dead[h]);
+          if (leave || !grown) break;
 #pragma unroll 1
         for (int x = 0; x < cols; x += 8) {
           float a[8];
@@ -954,12 +1065,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!first) m = fmaxf(m, 0.f);
           if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
           change[h][r] = ex2(-m);
-          line[r].y -= m;
+          line[NT + r] -= m;
         }
         // (O of the blocks before is complete)
         if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) dead[h] = 1;
         any_of_128(bar, false);
-        if (*reinterpret_cast<volatile int*>(&dead[h])) break;
+        leave = *reinterpret_cast<volatile int*>(&dead[h]);
+        if (leave) break;
         tc_fence_after();
         if (!first) {
 #pragma unroll 1
@@ -976,8 +1088,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           tmem_wait_st();
         }
-        weights();
+        }
+        top = weights();
       }
+      if (leave) break;
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
@@ -985,41 +1099,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(flags & kLast)) continue;
 
       // ---------------- the end of the segment, in this CTA
-      if (!wait(&p_empty[i & 1], (uint32_t)(i >> 1) & 1u)) {
-        dead[h] = 1;  // (the others of this half see it at the next barrier)
-        continue;
-      }
+      // (where the wait gave up, the numbers are not the segment's, and the next vote ends the role)
+      if (!wait(&p_empty[i & 1], (uint32_t)(i >> 1) & 1u)) dead[h] = 1;
       tc_fence_after();
-      const bool alone = flags & kAlone, again = (k_again[par] | v_again[par]) != 0;
+      const bool alone = flags & kAlone;
       const int slot = 2 * blockIdx.x + (flags & kOpens ? 1 : 0);
       const int used = min(cols, f.cols - x0);  // (columns past them are padding)
-      if (!alone) {
-        if (threadIdx.x == 0) {
-          p.again[slot] = again;
-          if (flags & kOpens) p.opened[blockIdx.x] = Opened{f.run, f.seq, f.kv, f.r0, f.len, f.c0, f.cols, 0};
-        }
-        if (qd == 0)
-#pragma unroll 1
-          for (int x = 0; x < cols; x += 8) {
-            uint32_t l[8];
-            __syncwarp();
-            tmem_ld8(tmem + S::kLCol + x0 + x + sub, l);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (lane == e) p.stats[(size_t)slot * NT + x0 + x + e] = make_float2(kBias - line[x + e].y, __uint_as_float(l[e]));
-          }
-      }
-      if (alone && again) {
-        for (int x = qd; x < used; x += 4) {
-          const int token = (f.c0 + x0 + x) / p.hpk;
-          plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + x0 + x) - token * p.hpk);
-        }
-      } else if (qd * 32 < S::kERows) {
+      bool bad = k_again[par] != 0;
+      if (qd * 32 < S::kERows) {
+        const int token0 = (f.c0 + x0) / p.hpk, head0 = (f.c0 + x0) - token0 * p.hpk;
 #pragma unroll 1
         for (int k = 0; k < S::kHalves; ++k) {
           const int e = 128 * k + 32 * qd + lane;
-          int token = (f.c0 + x0) / p.hpk, sub_head = (f.c0 + x0) - token * p.hpk;
-          T* out = static_cast<T*>(p.out) + (f.r0 + token) * p.out_row + (int64_t)(f.kv * p.hpk + sub_head) * p.out_head + e;
+          int sub_head = head0;
+          T* out = static_cast<T*>(p.out) + (f.r0 + token0) * p.out_row + (int64_t)(f.kv * p.hpk + head0) * p.out_head + e;
           float* part = p.parts + ((size_t)slot * NT + x0) * HD + e;
 #pragma unroll 1
           for (int x = 0; x < used; x += 8) {
@@ -1027,21 +1120,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             tmem_ld8_async(tmem + S::kLCol + x0 + x + sub, l);
             tmem_ld8(tmem + S::kOCol + k * NT + x0 + x + sub, o);
+            const int left = used - x;
+            if (alone) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              if (x + c >= used) break;
-              if (alone) {
-                *out = from_f32<T>(__fdividef(__uint_as_float(o[c]), __uint_as_float(l[c])));
+              for (int c = 0; c < 8; ++c) {
+                const float v = __fdividef(__uint_as_float(o[c]), __uint_as_float(l[c]));
+                if (c < left) {
+                  bad |= !(fabsf(v) <= 3.402823466e38f);
+                  *out = from_f32<T>(v);
+                }
                 out += p.out_head;
                 if (++sub_head == p.hpk) {
                   sub_head = 0;
                   out += p.out_row - p.hpk * p.out_head;
                 }
-              } else {
-                part[(size_t)(x + c) * HD] = __uint_as_float(o[c]);
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                if (c < left) {
+                  bad |= !(fabsf(__uint_as_float(o[c])) <= 3.402823466e38f);
+                  part[(x + c) * HD] = __uint_as_float(o[c]);
+                }
+              if (k == 0 && qd == 0) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                  if (lane == c && c < left)
+                    p.stats[(size_t)slot * NT + x0 + x + c] = make_float2(kBias - line[NT + x + c], __uint_as_float(l[c]));
               }
             }
           }
+        }
+      }
+      // what came out not finite, or may owe its value to an infinity of f16, is computed again
+      bad = any_of_128(bar, bad);
+      if (!alone) {
+        if (r == 0) {
+          p.again[2 * slot + h] = bad;
+          if (h == 0 && (flags & kOpens)) p.opened[blockIdx.x] = Opened{f.run, f.seq, f.kv, f.r0, f.len, f.c0, f.cols, 0};
+        }
+      } else if (bad) {
+        for (int x = qd; x < used; x += 4) {
+          const int token = (f.c0 + x0 + x) / p.hpk;
+          plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + x0 + x) - token * p.hpk);
         }
       }
       tc_fence_before();
@@ -1071,7 +1192,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   // the part that starts the segment is its CTA's slot 1, the others slot 0
   auto slot = [&](int i) { return (size_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   int again = 0;
-  for (int i = threadIdx.x & 31; i < f.run; i += 32) again |= p.again[slot(i)];
+  for (int i = threadIdx.x & 31; i < f.run; i += 32) again |= p.again[2 * slot(i)] | p.again[2 * slot(i) + 1];
   if (__any_sync(0xffffffffu, again != 0)) {
     for (int c = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); c < f.cols; c += gridDim.y * (kJoinThreads / 32)) {
       const int token = (f.c0 + c) / p.hpk;
@@ -1152,7 +1273,7 @@ Layout layout_of(const rrr_kv4_cache* c, int sms) {
   Layout l;
   l.stats = ((int64_t)sms * (int64_t)sizeof(Opened) + 255) / 256 * 256;
   l.again = l.stats + slots * 96 * 8;
-  l.parts = l.again + (slots * 4 + 255) / 256 * 256;
+  l.parts = l.again + (slots * 8 + 255) / 256 * 256;
   l.bytes = l.parts + slots * 96 * c->head_dim * 4;
   return l;
 }
