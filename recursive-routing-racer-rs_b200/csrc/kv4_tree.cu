@@ -14,11 +14,15 @@ namespace {
 constexpr int kMaxHpk = 8, kMaxNodes = 128;
 constexpr float kNone = -3e38f;  // the maximum of no rows: finite, so that it may be subtracted from -inf
 constexpr int kRows = 128;       // KV rows of a block: two pages, or the drafted rows
-constexpr int kStart = 2;        // units in front of a segment's blocks
-constexpr int kThreads = 640;
+constexpr int kStart = 4;        // units in front of a segment's blocks
+constexpr int kGroups = 4;       // of four softmax warps each: group h takes the columns 8 h .. + 7 of every 8 kGroups
+constexpr int kKWarp = 4 * kGroups, kVWarp = kKWarp + 4, kSWarp = kVWarp + 4, kLoadWarp = kSWarp + 1, kPVWarp = kSWarp + 2;
+constexpr int kThreads = 32 * (kSWarp + 4);
 constexpr int kInfos = 16;
+constexpr int kNap = 100;        // ns
 constexpr float kBias = 10.f;    // weights are 2^(s - m + kBias), at most 2^(kBias + kLazy)
 constexpr float kLazy = 5.f;
+constexpr uint32_t kF16 = 1u << 4 | (uint32_t)(kRows >> 4) << 24;  // products' descriptor: f16 operands, f32 sums, M = 128
 
 struct TreeParams {
   const uint8_t* pages;
@@ -39,7 +43,7 @@ struct TreeParams {
   // workspace
   struct Opened* opened;  // [CTA]: the segment that it opened and shares
   float2* stats;          // [slot][column]: maximum, sum
-  int* again;             // [slot][half of the columns]
+  int* again;             // [slot][group of columns]
   float* parts;           // [slot][column][value]
 };
 struct Opened {
@@ -115,16 +119,18 @@ __device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* er
 __device__ __forceinline__ bool quick_wait(uint64_t* bar, uint32_t parity, int* err) {
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, err);
 }
-
-// Whether a phase is complete, without waiting
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+// The same for a role that works ahead of the others: asleep between the tries, which would take issue slots from them
+__device__ __noinline__ bool sleep_longer(uint64_t* bar, uint32_t parity, int* err) {
+  bool ok = false;
+#pragma unroll 1
+  for (int k = 0; k < 256 && !ok; ++k) {
+    __nanosleep(kNap);
+    ok = mbar_try_wait(bar, parity);
+  }
+  return __all_sync(0xffffffffu, ok) || warp_wait(bar, parity, err);
+}
+__device__ __forceinline__ bool sleepy_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || sleep_longer(bar, parity, err);
 }
 
 // Bounded barrier of four warps.
@@ -173,6 +179,23 @@ __device__ __forceinline__ void values_of(uint32_t w, __half2 d, __half2 m, uint
 }
 // 128-byte swizzle of an offset from a 1024-byte border
 __device__ __forceinline__ uint32_t swizzled(uint32_t off) { return off ^ (((off >> 7) & 7u) << 4); }
+// N words (a power of two) at p
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
+  }
+}
 template <typename T>
 __device__ __forceinline__ float2 pair_of(uint32_t w) {
   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) return __half22float2(as_half2(w));
@@ -428,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int k_again[4];
   __shared__ uint32_t v_tops[4];
   __shared__ __align__(16) float lines[4][2 * NT];  // of a column c: the argument of a weight's exponential is score * [c] + [NT + c]
-  __shared__ float quad[2][4][NT / 2], change[2][NT / 2];
-  __shared__ int warp_units[kThreads / 32], first_base, first_seq, dead[2];
+  __shared__ float quad[4][NT], change[NT];
+  __shared__ int warp_units[kThreads / 32], first_base, first_seq, dead[kGroups];
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
   uint8_t* const qs = smem;
@@ -445,20 +468,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&p_full[i], 4 * kGroups);
       mbar_init(&p_empty[i], 1);
       mbar_init(&teams[i], 4);
-      dead[i] = 0;
     }
     for (int i = 0; i < S::kVs; ++i) mbar_init(&v_full[i], 4);
-    mbar_init(&o_empty, 8);
+    mbar_init(&o_empty, 4 * kGroups);
+    for (int i = 0; i < kGroups; ++i) dead[i] = 0;
     for (int i = 0; i < kInfos; ++i) mbar_init(&told[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&lifted[i], 1);
-    mbar_init(&fin, 1);
+    mbar_init(&fin, 2);
     fence_mbarrier_init();
     prefetch_map(&map);
   }
-  if (warp == 16) tmem_alloc(&tmem_slot, 512);
+  if (warp == kSWarp) tmem_alloc(&tmem_slot, 512);
   pdl_launch_dependents();
   pdl_wait();
 
@@ -500,19 +523,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   // Every wait is bounded; a role that gave up leaves, and so do those that wait for it.
   auto wait = [&](uint64_t* bar, uint32_t parity) { return quick_wait(bar, parity, p.err); };
+  auto doze = [&](uint64_t* bar, uint32_t parity) { return sleepy_wait(bar, parity, p.err); };
 
   if (u0 >= u1) {
     // nothing to do
-    if (warp == 16) {
+    if (warp == kSWarp || warp == kPVWarp) {
       if (elect_one()) umma_commit(&fin);
       __syncwarp();
     }
-  } else if (warp == 17) {
+  } else if (warp == kLoadWarp) {
     // ---------------- the blocks in order, and the copies of their pages
     int s = first_seq, count = -1, it = 0, st = 0, base = first_base;
     Shape sh = shape_of<NT>(p, s);
     int each = sh.blocks + kStart;
     int g = (u0 - base) / each, blk = max(0, (u0 - base) % each - kStart);
+    int ids_at = 0, id = 0;  // page numbers of the segment
+    int kv = 0, c0 = 0, cols = 0;
     int the = 0, run = 0;  // (of lane 0) the segment's flags, its CTAs
     bool begin = true, stop = false;
     uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
@@ -535,25 +561,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       stop = s >= p.n_seqs || seg0 + blk >= u1;
       const bool draft = blk + 1 == sh.blocks;
       Info& f = infos[it % kInfos];
-      const int kv = stop ? 0 : g / sh.tiles, tile = g - kv * sh.tiles;
       if (begin || stop) {
+        kv = stop ? 0 : g / sh.tiles;
+        c0 = (g - kv * sh.tiles) * sh.per;
+        cols = min(sh.per, sh.nodes * p.hpk - c0);
         // what the segment is, before its first block is there; its rows on their way to L2
         if (lane == 0) {
-          const int c0 = share.cta_of(seg0), c1 = share.cta_of(seg0 + sh.blocks - 1);
+          const int cta0 = share.cta_of(seg0), cta1 = share.cta_of(seg0 + sh.blocks - 1);
           ++count;
-          the = (c0 == c1 ? kAlone : 0) | (c0 == (int)blockIdx.x ? kOpens : 0) | (count & 3) << 8;
-          run = c1 - c0 + 1;
+          the = (cta0 == cta1 ? kAlone : 0) | (cta0 == (int)blockIdx.x ? kOpens : 0) | (count & 3) << 8;
+          run = cta1 - cta0 + 1;
           f.flags = stop ? kStop : the | kFirst;
           f.n = sh.per;
-          f.c0 = tile * sh.per;
-          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.c0 = c0;
+          f.cols = cols;
           f.kv = kv;
           f.r0 = sh.r0;
           mbar_arrive(&told[it % kInfos]);
         }
         if (!stop) {
           constexpr int kLines = HD / 64;
-          const int c0 = tile * sh.per, cols = min(sh.per, sh.nodes * p.hpk - c0);
           for (int x = lane; x < (cols + 2 * sh.nodes) * kLines; x += 32) {
             const int c = x / kLines, part = x % kLines * 64;
             const T* a;
@@ -569,20 +596,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      int page = 0, valid = 0;
-      if (!stop && !draft && lane < 2) {
-        const int at = 2 * blk + lane;
-        valid = min(kPageRows, sh.len - at * kPageRows);
-        if (valid > 0) page = p.table[(int64_t)s * p.table_stride + at];
-        if (valid < 0) valid = 0;
-        if (page < 0 || page >= p.n_pages) {
+      // the numbers of the next 32 pages, one per lane
+      if (!stop && !draft && (begin || 2 * blk + 2 > ids_at + 32)) {
+        ids_at = 2 * blk;
+        const int left = sh.len - (ids_at + lane) * kPageRows;
+        id = left > 0 ? p.table[(int64_t)s * p.table_stride + ids_at + lane] : 0;
+        if (left > 0 && (id < 0 || id >= p.n_pages)) {
           flag_position(p.err);
-          valid = 0;
+          id = -1;
         }
       }
-      if (!wait(&empty[st], phase)) break;
-      const int v0 = __shfl_sync(0xffffffffu, valid, 0), v1 = __shfl_sync(0xffffffffu, valid, 1);
-      const int p0 = __shfl_sync(0xffffffffu, page, 0), p1 = __shfl_sync(0xffffffffu, page, 1);
+      int p0 = 0, p1 = 0, v0 = 0, v1 = 0;
+      if (!stop && !draft) {
+        p0 = __shfl_sync(0xffffffffu, id, 2 * blk - ids_at);
+        p1 = __shfl_sync(0xffffffffu, id, 2 * blk + 1 - ids_at);
+        v0 = p0 < 0 ? 0 : min(kPageRows, sh.len - 2 * blk * kPageRows);
+        v1 = p1 < 0 ? 0 : max(0, min(kPageRows, sh.len - (2 * blk + 1) * kPageRows));
+      }
+      if (!doze(&empty[st], phase)) break;
       if (lane == 0) {
         uint8_t* dst = ring + (size_t)st * S::kStage;
         if (v0 > 0) tma_load_2d(dst, &map, 0, (int)(((int64_t)p0 * p.nkv + kv) * (S::kPage / 128)), &full[st]);
@@ -594,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           f.n = sh.per;
           f.valid[0] = v0;
           f.valid[1] = v1;
-          f.c0 = tile * sh.per;
-          f.cols = min(sh.per, sh.nodes * p.hpk - f.c0);
+          f.c0 = c0;
+          f.cols = cols;
           f.kv = kv;
           f.count = count;
           f.r0 = sh.r0;
@@ -623,13 +654,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int uses = it > i ? (it - i + S::kStages - 1) / S::kStages : 0;
       if (uses) warp_wait(&full[i], (uint32_t)(uses - 1) & 1u, p.err);
     }
-  } else if (warp == 16) {
-    // ---------------- products: S(0), S(1), PV(0), S(2), PV(1), ...
-    const uint32_t fmt = 1u << 4;  // f16 operands, f32 sums; M = 128
-    const uint64_t q_desc = sw128_desc(smem_addr(qs)), v_desc = sw128_desc(smem_addr(vs)), p_desc = sw128_desc_mn(smem_addr(ps), kRows * 128);
-    auto scores = [&](int i) {   // S = K Q^T of block i
-      const uint32_t idesc = fmt | ((uint32_t)(infos[i % kInfos].n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      const uint32_t to = tmem + S::kSCol + (i & 1) * NT, k = tmem + (i % S::kKs) * S::kKCols;
+  } else if (warp == kSWarp) {
+    // ---------------- scores: S = K Q^T of block i, in the place of S(i - 2) once its weights are there
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);  // (known to be the warp's, as what is derived from it)
+    const uint64_t q_desc = sw128_desc(smem_addr(qs));
+#pragma unroll 1
+    for (int i = 0;; ++i) {
+      if (!wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+      if (i >= 2 && !wait(&p_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
+      const int2 f = *reinterpret_cast<const int2*>(&infos[i % kInfos]);  // flags, columns
+      if (f.x & kStop) {
+        if (lane == 0) mbar_arrive(&s_full[i & 1]);
+        break;
+      }
+      const uint32_t odd = __shfl_sync(0xffffffffu, i & 1, 0), n = __shfl_sync(0xffffffffu, f.y, 0);
+      const uint32_t idesc = kF16 | n >> 3 << 17, to = base + S::kSCol + odd * NT, k = base + (S::kKs == 2 ? odd * S::kKCols : 0u);
+      tc_fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
@@ -637,81 +677,70 @@ __global__ void __launch_bounds__(kThreads, 1)
         umma_commit(&s_full[i & 1]);
       }
       __syncwarp();
-    };
-    auto weighed = [&](int i) {  // O^T += V^T P^T of block i, and the sums of the weights
+    }
+    if (elect_one()) umma_commit(&fin);
+    __syncwarp();
+  } else if (warp == kPVWarp) {
+    // ---------------- weighted sums: O^T += V^T P^T of block i, and the sums of the weights
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t v_desc = sw128_desc(smem_addr(vs)), p_desc = sw128_desc_mn(smem_addr(ps), kRows * 128);
+#pragma unroll 1
+    for (int i = 0;; ++i) {
+      if (!wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u)) break;
       const Info& f = infos[i % kInfos];
-      const int flags = f.flags;
-      const uint32_t idesc = fmt | (1u << 16) | ((uint32_t)(f.n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      const uint64_t v = v_desc + (uint32_t)((i % S::kVs) * (S::kV >> 4)), w = p_desc + (uint32_t)((i & 1) * (S::kP >> 4));
-      const uint32_t more = flags & kFirst ? 0u : 1u;
-      const uint32_t ones = tmem + S::kOnes + (flags & kDraft ? 8u * v_lift[(flags >> 8) & 3] : 0u);
+      const int2 head = *reinterpret_cast<const int2*>(&f);
+      if (head.x & kStop) break;
+      if (!wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+      if ((head.x & kFirst) && f.count > 0 && !wait(&o_empty, (uint32_t)(f.count - 1) & 1u)) break;
+      const uint32_t odd = __shfl_sync(0xffffffffu, i & 1, 0), flags = __shfl_sync(0xffffffffu, head.x, 0), n = __shfl_sync(0xffffffffu, head.y, 0);
+      const uint32_t lift = __shfl_sync(0xffffffffu, flags & kDraft ? v_lift[(flags >> 8) & 3] : 0, 0);
+      const uint32_t idesc = kF16 | 1u << 16 | n >> 3 << 17, more = flags & kFirst ? 0u : 1u, ones = base + S::kOnes + 8u * lift;
+      const uint64_t v = v_desc + (S::kVs == 2 ? odd * (S::kV >> 4) : 0u), w = p_desc + odd * (S::kP >> 4);
+      tc_fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kRows / 16; ++kk) {
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h)
-            umma_f16(tmem + S::kOCol + h * NT, v + (((h * 2 + kk / 4) * S::kERows * 128 + 32 * (kk % 4)) >> 4), w + (2048 * kk >> 4), idesc,
+            umma_f16(base + S::kOCol + h * NT, v + (((h * 2 + kk / 4) * S::kERows * 128 + 32 * (kk % 4)) >> 4), w + (2048 * kk >> 4), idesc,
                      kk > 0 ? 1u : more);
-          umma_f16_ta(tmem + S::kLCol, ones, w + (2048 * kk >> 4), idesc, kk > 0 ? 1u : more);
+          umma_f16_ta(base + S::kLCol, ones, w + (2048 * kk >> 4), idesc, kk > 0 ? 1u : more);
         }
         umma_commit(&p_empty[i & 1]);
       }
       __syncwarp();
-    };
-    // S(0), S(1), then in turn, once P(i) is there: S(i + 2), whose place that frees, and PV(i); S later, if its keys are
-    auto have_keys = [&](int i) {
-      const bool ok = wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u);
-      tc_fence_after();
-      return ok;
-    };
-    bool ok = have_keys(0), stop = ok && (infos[0].flags & kStop);
-    int next = 0;  // the block whose scores come next, or the one that says stop
-    if (ok && !stop) scores(next++);
-    if (ok && !stop) {
-      ok = have_keys(1);
-      stop = ok && (infos[1].flags & kStop);
-      if (ok && !stop) scores(next++);
     }
-#pragma unroll 1
-    for (int i = 0; ok && i < next; ++i) {
-      ok = wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u);
-      auto ahead = [&]() {
-        ok = have_keys(next);
-        stop = ok && (infos[next % kInfos].flags & kStop);
-        if (ok && !stop) scores(next++);
-      };
-      const bool early = ok && !stop && __all_sync(0xffffffffu, mbar_test(&k_full[next & 1], (uint32_t)(next >> 1) & 1u));
-      if (early) ahead();
-      ok = ok && wait(&v_full[i % S::kVs], (uint32_t)(i / S::kVs) & 1u);
-      const int flags = infos[i % kInfos].flags, count = infos[i % kInfos].count;
-      ok = ok && (!(flags & kFirst) || count == 0 || wait(&o_empty, (uint32_t)(count - 1) & 1u));
-      if (!ok) break;
-      tc_fence_after();
-      weighed(i);
-      if (!early && !stop) ahead();
-    }
-    if (stop && lane == 0) mbar_arrive(&s_full[next & 1]);
     if (elect_one()) umma_commit(&fin);
     __syncwarp();
-  } else if (warp >= 18) {
+  } else if (warp > kPVWarp) {
     // (no role)
-  } else if (warp >= 12) {
+  } else if (warp >= kVWarp) {
     // ---------------- V: pairs of rows, transposed to rows of values
-    const int tid = threadIdx.x - 12 * 32;
+    const int tid = threadIdx.x - 32 * kVWarp;
+    // of a cached block a thread takes values 32 k + 8 n + g (of each plane) of every kPass-th eight rows. What lies within a
+    // line of the pages is reached by an exclusive or.
+    constexpr int kPass = 128 / (8 * J);
+    const int g = tid & 7, k = (tid >> 3) % J, o0 = tid / (8 * J);
+    const uint32_t pick = k & 1 ? 0x7632 : 0x5410;
     Quartet team{&teams[1], 0, p.err};
     int st = 0;
     uint32_t phase = 0;
 #pragma unroll 1
     for (int i = 0;; ++i) {
-      if (!wait(&full[st], phase)) break;
+      if (!doze(&full[st], phase)) break;
       const Info& f = infos[i % kInfos];
       const int flags = f.flags;
-      if (flags & kStop) break;
+      if (flags & kStop) {
+        // (not before the products have seen the block two before, as above)
+        if (i >= S::kVs && !doze(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u)) break;
+        if (lane == 0) mbar_arrive(&v_full[i % S::kVs]);
+        break;
+      }
       uint8_t* const stage = ring + (size_t)st * S::kStage;
       uint8_t* const dst = vs + (i % S::kVs) * S::kV;
       // the place is free once PV(i - kVs) is done
       auto free_place = [&]() {
-        return i < S::kVs || wait(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u);
+        return i < S::kVs || doze(&p_empty[(i - S::kVs) & 1], (uint32_t)((i - S::kVs) >> 1) & 1u);
       };
       if (!(flags & kDraft)) {
         if (f.valid[0] < kPageRows || f.valid[1] < kPageRows) {
@@ -724,58 +753,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           if (!team()) break;
         }
-        const int o = tid >> 3, g = tid & 7;  // rows 8 o .. + 7 of the block, values 32 i + 8 n + g
-        const uint8_t* const page = stage + (o >> 3) * S::kPage;
-        const int r = (o & 7) * 8;
         if (!free_place()) break;
+        // (the loop stays small: five warps of four roles share a scheduler's instruction cache)
 #pragma unroll 1
-        for (int P = 0; P < PL; ++P) {
-          uint32_t w[4 * J];  // [t][i]
-#pragma unroll
-          for (int u = 0; u < J; ++u) {
-            const uint4 x = *reinterpret_cast<const uint4*>(page + swizzled(40 * HD + P * 1024 * J + (r + g) * 16 * J + 16 * u));
-            w[4 * u] = x.x;
-            w[4 * u + 1] = x.y;
-            w[4 * u + 2] = x.z;
-            w[4 * u + 3] = x.w;
-          }
-          __half2 d[4][J], m[4][J];
+        for (int n = 0; n < 16 * PL / kPass; ++n) {
+          const int P = n / (16 / kPass), o = n % (16 / kPass) * kPass + o0, r = (o & 7) * 8;  // rows 8 o .. + 7
+          const uint8_t* const page = stage + (o >> 3) * S::kPage;
+          const uint32_t codes = swizzled(40 * HD + P * 1024 * J + (r + g) * 16 * J) + 4 * (k % 4);
+          const uint32_t steps = swizzled(72 * HD + 2 * r * G) ^ (HD == 256 ? 8 * P + 4 * (k >> 1) : 4 * (k >> 1));
+          const uint32_t mins = swizzled(76 * HD + 2 * r * G) ^ (HD == 256 ? 16 * P + 4 * k : 4 * k);
+          uint32_t x[4][4];  // [t][n]: nibble n of the halves, the even row's and the odd row's
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            const int row = r + 2 * t;
-            const uint8_t* const da = page + swizzled(72 * HD + 2 * (row * G + P * J));
-            const uint8_t* const db = page + swizzled(72 * HD + 2 * ((row + 1) * G + P * J));
-            const uint8_t* const ma = page + swizzled(76 * HD + 4 * ((row >> 1) * G + P * J));
-            if constexpr (J == 4) {
-              const uint2 a = *reinterpret_cast<const uint2*>(da), b = *reinterpret_cast<const uint2*>(db);
-              const uint4 c = *reinterpret_cast<const uint4*>(ma);
-              d[t][0] = as_half2(__byte_perm(a.x, b.x, 0x5410));
-              d[t][1] = as_half2(__byte_perm(a.x, b.x, 0x7632));
-              d[t][2] = as_half2(__byte_perm(a.y, b.y, 0x5410));
-              d[t][3] = as_half2(__byte_perm(a.y, b.y, 0x7632));
-              m[t][0] = as_half2(c.x);
-              m[t][1] = as_half2(c.y);
-              m[t][2] = as_half2(c.z);
-              m[t][3] = as_half2(c.w);
-            } else {
-              const uint32_t a = *reinterpret_cast<const uint32_t*>(da), b = *reinterpret_cast<const uint32_t*>(db);
-              const uint2 c = *reinterpret_cast<const uint2*>(ma);
-              d[t][0] = as_half2(__byte_perm(a, b, 0x5410));
-              d[t][1] = as_half2(__byte_perm(a, b, 0x7632));
-              m[t][0] = as_half2(c.x);
-              m[t][1] = as_half2(c.y);
-            }
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (codes ^ (4 * J * t)));
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(page + (steps ^ (4 * G * t)));
+            const uint32_t b = *reinterpret_cast<const uint32_t*>(page + (steps ^ (4 * G * t + 2 * G)));
+            const uint32_t m = *reinterpret_cast<const uint32_t*>(page + (mins ^ (4 * G * t)));
+            values_of(w, as_half2(__byte_perm(a, b, pick)), as_half2(m), x[t]);
           }
-          uint8_t* const to = dst + (P * 2 + (o >> 3)) * S::kERows * 128 + g * 128 + (((o & 7) ^ g) << 4);
+          uint8_t* const to = dst + (P * 2 + (o >> 3)) * S::kERows * 128 + (32 * k + g) * 128 + (((o & 7) ^ g) << 4);
 #pragma unroll
-          for (int k = 0; k < J; ++k) {
-            uint32_t x[4][4];  // [t][n]: nibble n of the halves, the even row's and the odd row's
-#pragma unroll
-            for (int t = 0; t < 4; ++t) values_of(w[t * J + k], d[t][k], m[t][k], x[t]);
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-              *reinterpret_cast<uint4*>(to + (32 * k + 8 * n) * 128) = make_uint4(x[0][n], x[1][n], x[2][n], x[3][n]);
-          }
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(to + 8 * e * 128) = make_uint4(x[0][e], x[1][e], x[2][e], x[3][e]);
         }
       } else {
         uint32_t top = drafted_top<HD, T>(p, f, tid);
@@ -801,10 +800,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= 1;
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= kKWarp) {
     // ---------------- K: a row of keys per thread, into TMEM; and the tile's queries
-    const int r = threadIdx.x - 8 * 32;
+    const int r = threadIdx.x - 32 * kKWarp, half = r >> 6, row = r & 63;
     const uint32_t sub = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t k_codes = swizzled(row * 16 * J), k_steps = swizzled(32 * HD + 2 * row * G), k_mins = swizzled(36 * HD + 2 * row * G);
     Quartet team{&teams[0], 0, p.err};
     int st = 0;
     uint32_t phase = 0;
@@ -821,44 +821,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0;; ++i) {
       const Info& f = infos[i % kInfos];
       if (begins) {
-        if (!wait(&told[i % kInfos], turns >> (i % kInfos) & 1u)) break;
+        if (!doze(&told[i % kInfos], turns >> (i % kInfos) & 1u)) break;
         turns ^= 1u << (i % kInfos);
         if (!(f.flags & kStop)) {
           const int par = (f.flags >> 8) & 3;
           if (r == 0) k_again[par] = 0;
           // S of the segment before has read its queries
-          if (i > 0 && !wait(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
+          if (i > 0 && !doze(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
           queries<HD, NT, T>(p, f, r, qs, lines[par]);
           fence_proxy_async_smem();
           if (!team()) break;
         }
       }
-      if (!wait(&full[st], phase)) break;
+      if (!doze(&full[st], phase)) break;
       const int flags = f.flags, par = (flags >> 8) & 3;
       begins = flags & kLast;
       if (flags & kStop) {
         // (not before the products have seen the block two before, or they would miss its turn)
-        if (i >= 2 && !wait(&s_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
+        if (i >= 2 && !doze(&s_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
         if (lane == 0) mbar_arrive(&k_full[i & 1]);
         break;
       }
       const uint32_t dst = tmem + (i % S::kKs) * S::kKCols + sub;
       // the place is free once S(i - kKs) is done
       auto free_place = [&]() {
-        const bool ok = i < S::kKs || wait(&s_full[(i - S::kKs) & 1], (uint32_t)((i - S::kKs) >> 1) & 1u);
+        const bool ok = i < S::kKs || doze(&s_full[(i - S::kKs) & 1], (uint32_t)((i - S::kKs) >> 1) & 1u);
         tc_fence_after();
         return ok;
       };
       if (!(flags & kDraft)) {
-        const int half = r >> 6, row = r & 63;
         const uint8_t* const page = ring + (size_t)st * S::kStage + half * S::kPage;
-        __half2 d[G / 2], m[G / 2], most = as_half2(0u);
+        uint32_t d[G / 2], m[G / 2];
+        load_words<G / 2>(page + k_steps, d);
+        load_words<G / 2>(page + k_mins, m);
+        __half2 most = as_half2(0u);
 #pragma unroll
-        for (int k = 0; k < G / 2; ++k) {
-          d[k] = *reinterpret_cast<const __half2*>(page + swizzled(32 * HD + 2 * (row * G + 2 * k)));
-          m[k] = *reinterpret_cast<const __half2*>(page + swizzled(36 * HD + 2 * (row * G + 2 * k)));
-          most = __hmax2(most, __hfma2(d[k], as_half2(0x4b804b80u), __habs2(m[k])));
-        }
+        for (int k = 0; k < G / 2; ++k) most = __hmax2(most, __hfma2(as_half2(d[k]), as_half2(0x4b804b80u), __habs2(as_half2(m[k]))));
         if (row < f.valid[half] && (__hisinf(__low2half(most)) || __hisinf(__high2half(most)))) k_again[par] = 1;
         if (!free_place()) break;
 #pragma unroll
@@ -867,12 +865,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < J; ++k) {
             const int j = P * J + k;
-            dd[k] = j & 1 ? __high2half2(d[j / 2]) : __low2half2(d[j / 2]);
-            mm[k] = j & 1 ? __high2half2(m[j / 2]) : __low2half2(m[j / 2]);
+            dd[k] = j & 1 ? __high2half2(as_half2(d[j / 2])) : __low2half2(as_half2(d[j / 2]));
+            mm[k] = j & 1 ? __high2half2(as_half2(m[j / 2])) : __low2half2(as_half2(m[j / 2]));
           }
 #pragma unroll 1
           for (int u = 0; u < J; ++u) {  // four words, 16 columns
-            const uint4 x = *reinterpret_cast<const uint4*>(page + swizzled(P * 1024 * J + row * 16 * J + 16 * u));
+            const uint4 x = *reinterpret_cast<const uint4*>(page + ((k_codes + P * 1024 * J) ^ (16 * u)));
             uint32_t y[16];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -947,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    // ---------------- softmax: a KV row per thread, half of the columns
+    // ---------------- softmax: a KV row per thread, a share of the columns
     const int h = warp >> 2, qd = warp & 3, r = threadIdx.x & 127, bar = 1 + h;
     const uint32_t sub = (uint32_t)(32 * qd) << 16;
 #pragma unroll 1
@@ -956,11 +954,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Info& f = infos[i % kInfos];
       const int4 head = *reinterpret_cast<const int4*>(&f);
       const int flags = ok ? head.x : kStop, valid = r < 64 ? head.z : head.w;
-      const int par = (flags >> 8) & 3, cols = head.y >> 1, x0 = h * cols;  // this half: columns x0 .. x0 + cols - 1 of the tile
+      const int par = (flags >> 8) & 3, n = head.y;
       const bool first = flags & kFirst;
-      const uint32_t sc = tmem + S::kSCol + (i & 1) * NT + x0 + sub;
+      const uint32_t sc = tmem + S::kSCol + (i & 1) * NT + sub;
       uint8_t* const dst = ps + (i & 1) * S::kP + (r >> 3) * 1024 + (r & 7) * 128;
-      float* const line = lines[par] + x0;
+      float* const line = lines[par];
       tc_fence_after();
       // P's place is free once PV(i - 2) is done
       if (!(flags & kStop) && i >= 2) ok = wait(&p_empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u);
@@ -978,11 +976,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 8; ++e) a[e] = fmaf(a[e] * ks, line[x + e], line[NT + x + e]);
         if (flags & kDraft) {
-          int token = (f.c0 + x0 + x) / p.hpk, sub_head = (f.c0 + x0 + x) - token * p.hpk;
+          int token = (f.c0 + x) / p.hpk, sub_head = (f.c0 + x) - token * p.hpk;
           const uint32_t* bits = reinterpret_cast<const uint32_t*>(seen[par]) + qd;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            if (x0 + x + e >= f.cols || !((bits[4 * min(token, kMaxNodes - 1)] >> lane) & 1u)) a[e] = -INFINITY;
+            if (x + e >= f.cols || !((bits[4 * min(token, kMaxNodes - 1)] >> lane) & 1u)) a[e] = -INFINITY;
             if (++sub_head == p.hpk) {
               sub_head = 0;
               ++token;
@@ -1009,21 +1007,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               w[e / 2] = as_u32(__floats2half2_rn(ex2(u.x), ex2(u.y)));
               w[e / 2 + 1] = as_u32(__floats2half2_rn(ex2(v.x), ex2(v.y)));
             }
-            const int c = x0 + x;
+            const int c = x;
             *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           };
 #pragma unroll 1
-          for (int x = 0; x < cols; x += 16) {
-            uint32_t sv[16];
-            tmem_ld16(sc + x, sv);  // (columns past the last are loaded, and left)
-            tmem_wait_ld();
+          for (int x = 8 * h; x < n; x += 8 * kGroups) {
+            uint32_t sv[8];
+            tmem_ld8(sc + x, sv);
             eight(sv, x);
-            if (x + 8 < cols) eight(sv + 8, x + 8);
           }
         } else {
 #pragma unroll 1
-          for (int x = 0; x < cols; x += 8) {
+          for (int x = 8 * h; x < n; x += 8 * kGroups) {
             float a[8];
             arguments(x, a);
             uint32_t w[4];
@@ -1032,7 +1028,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               top = fmaxf(top, fmaxf(a[2 * e], a[2 * e + 1]));
               w[e] = as_u32(__floats2half2_rn(ex2(a[2 * e]) * low, ex2(a[2 * e + 1]) * low));
             }
-            const int c = x0 + x;
+            const int c = x;
             *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -1050,22 +1046,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           leave = (flags & kStop) || *reinterpret_cast<volatile int*>(&dead[h]);
           if (leave || !grown) break;
 #pragma unroll 1
-        for (int x = 0; x < cols; x += 8) {
+        for (int x = 8 * h; x < n; x += 8 * kGroups) {
           float a[8];
           arguments(x, a);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float m = redux_max(a[e]);
-            if (lane == 0) quad[h][qd][x + e] = m;
+            if (lane == 0) quad[qd][x + e] = m;
           }
         }
         any_of_128(bar, false);
-        if (r < cols) {
-          float m = fmaxf(fmaxf(quad[h][0][r], quad[h][1][r]), fmaxf(quad[h][2][r], quad[h][3][r])) - kBias;
+        const int mine = 8 * h + r % 8 + r / 8 * 8 * kGroups;  // a column of the group
+        if (mine < n) {
+          float m = fmaxf(fmaxf(quad[0][mine], quad[1][mine]), fmaxf(quad[2][mine], quad[3][mine])) - kBias;
           if (!first) m = fmaxf(m, 0.f);
           if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
-          change[h][r] = ex2(-m);
-          line[NT + r] -= m;
+          change[mine] = ex2(-m);
+          line[NT + mine] -= m;
         }
         // (O of the blocks before is complete)
         if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) dead[h] = 1;
@@ -1077,13 +1074,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int k = -1; k < S::kHalves; ++k)  // the sums of the weights, and O
 #pragma unroll 1
-            for (int x = 0; x < cols; x += 8) {
-              const uint32_t oc = tmem + S::kOCol + k * NT + x0 + x + sub;
+            for (int x = 8 * h; x < n; x += 8 * kGroups) {
+              const uint32_t oc = tmem + S::kOCol + k * NT + x + sub;
               uint32_t o[8];
               __syncwarp();
               tmem_ld8(oc, o);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * change[h][x + e]);
+              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * change[x + e]);
               tmem_st8(oc, o);
             }
           tmem_wait_st();
@@ -1104,24 +1101,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const bool alone = flags & kAlone;
       const int slot = 2 * blockIdx.x + (flags & kOpens ? 1 : 0);
-      const int used = min(cols, f.cols - x0);  // (columns past them are padding)
       bool bad = k_again[par] != 0;
       if (qd * 32 < S::kERows) {
-        const int token0 = (f.c0 + x0) / p.hpk, head0 = (f.c0 + x0) - token0 * p.hpk;
 #pragma unroll 1
         for (int k = 0; k < S::kHalves; ++k) {
           const int e = 128 * k + 32 * qd + lane;
-          int sub_head = head0;
-          T* out = static_cast<T*>(p.out) + (f.r0 + token0) * p.out_row + (int64_t)(f.kv * p.hpk + head0) * p.out_head + e;
-          float* part = p.parts + ((size_t)slot * NT + x0) * HD + e;
 #pragma unroll 1
-          for (int x = 0; x < used; x += 8) {
+          for (int x = 8 * h; x < f.cols; x += 8 * kGroups) {  // (columns past f.cols are padding)
             uint32_t o[8], l[8];
             __syncwarp();
-            tmem_ld8_async(tmem + S::kLCol + x0 + x + sub, l);
-            tmem_ld8(tmem + S::kOCol + k * NT + x0 + x + sub, o);
-            const int left = used - x;
+            tmem_ld8_async(tmem + S::kLCol + x + sub, l);
+            tmem_ld8(tmem + S::kOCol + k * NT + x + sub, o);
+            const int left = f.cols - x;
             if (alone) {
+              const int token = (f.c0 + x) / p.hpk;
+              int sub_head = (f.c0 + x) - token * p.hpk;
+              T* out = static_cast<T*>(p.out) + (f.r0 + token) * p.out_row + (int64_t)(f.kv * p.hpk + sub_head) * p.out_head + e;
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
                 const float v = __fdividef(__uint_as_float(o[c]), __uint_as_float(l[c]));
@@ -1136,17 +1131,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
             } else {
+              float* part = p.parts + ((size_t)slot * NT + x) * HD + e;
 #pragma unroll
               for (int c = 0; c < 8; ++c)
                 if (c < left) {
                   bad |= !(fabsf(__uint_as_float(o[c])) <= 3.402823466e38f);
-                  part[(x + c) * HD] = __uint_as_float(o[c]);
+                  part[c * HD] = __uint_as_float(o[c]);
                 }
               if (k == 0 && qd == 0) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                   if (lane == c && c < left)
-                    p.stats[(size_t)slot * NT + x0 + x + c] = make_float2(kBias - line[NT + x + c], __uint_as_float(l[c]));
+                    p.stats[(size_t)slot * NT + x + c] = make_float2(kBias - line[NT + x + c], __uint_as_float(l[c]));
               }
             }
           }
@@ -1156,14 +1152,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       bad = any_of_128(bar, bad);
       if (!alone) {
         if (r == 0) {
-          p.again[2 * slot + h] = bad;
+          p.again[kGroups * slot + h] = bad;
           if (h == 0 && (flags & kOpens)) p.opened[blockIdx.x] = Opened{f.run, f.seq, f.kv, f.r0, f.len, f.c0, f.cols, 0};
         }
       } else if (bad) {
-        for (int x = qd; x < used; x += 4) {
-          const int token = (f.c0 + x0 + x) / p.hpk;
-          plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + x0 + x) - token * p.hpk);
-        }
+        for (int x = 8 * h; x < f.cols; x += 8 * kGroups)
+          for (int c = x + qd; c < min(x + 8, f.cols); c += 4) {
+            const int token = (f.c0 + c) / p.hpk;
+            plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + c) - token * p.hpk);
+          }
       }
       tc_fence_before();
       __syncwarp();
@@ -1172,7 +1169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == kSWarp) {
     warp_wait(&fin, 0u, p.err);  // no product still runs when its TMEM is freed
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1192,7 +1189,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   // the part that starts the segment is its CTA's slot 1, the others slot 0
   auto slot = [&](int i) { return (size_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   int again = 0;
-  for (int i = threadIdx.x & 31; i < f.run; i += 32) again |= p.again[2 * slot(i)] | p.again[2 * slot(i) + 1];
+  for (int i = threadIdx.x & 31; i < f.run; i += 32)
+    for (int h = 0; h < kGroups; ++h) again |= p.again[kGroups * slot(i) + h];
   if (__any_sync(0xffffffffu, again != 0)) {
     for (int c = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); c < f.cols; c += gridDim.y * (kJoinThreads / 32)) {
       const int token = (f.c0 + c) / p.hpk;
@@ -1273,7 +1271,7 @@ Layout layout_of(const rrr_kv4_cache* c, int sms) {
   Layout l;
   l.stats = ((int64_t)sms * (int64_t)sizeof(Opened) + 255) / 256 * 256;
   l.again = l.stats + slots * 96 * 8;
-  l.parts = l.again + (slots * 8 + 255) / 256 * 256;
+  l.parts = l.again + (slots * 4 * kGroups + 255) / 256 * 256;
   l.bytes = l.parts + slots * 96 * c->head_dim * 4;
   return l;
 }
