@@ -51,8 +51,11 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return r;
 }
 // Eight values of a group of 32, which four neighbouring lanes hold: their codes, value i at bit
-// 4i, and the group's d and m.
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, __half& m16) {
+// 4i, and the group's d and m. With kOff, whether values that are off by up to `off` (the group's)
+// could have this lane's codes, d or m other than these.
+template <bool kOff = false>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, __half& m16, float off = 0.f,
+                                             bool* unsure = nullptr) {
   const float inf = __int_as_float(0x7f800000);
   float lo = least(least(x[0], x[1], x[2]), least(x[3], x[4], x[5]), least(x[6], x[7], x[7]));
   float hi = largest(largest(x[0], x[1], x[2]), largest(x[3], x[4], x[5]), largest(x[6], x[7], x[7]));
@@ -70,19 +73,25 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[8], __half& d16, _
   d16 = finite ? __float2half_rn(fminf(range > 1e6f ? 65504.f : step, 65504.f)) : __ushort_as_half(0x7fff);
   const float d = __half2float(d16), m = __half2float(m16);
   const float inv = d > 0.f ? __fdividef(1.f / 15.f, d) : 0.f;
+  float furthest = 0.f;
   uint32_t w = 0;
-  bool near = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float q = __saturatef(__fmul_rn(__fsub_rn(x[i], m), inv));  // in units of 15, within 0..15
     const float t = fmaf(q, 15.f, 12582912.f);                      // the nearest integer in the low bits
-    near |= fabsf(fmaf(q, 15.f, 12582912.f - t)) > 0.49999f;
+    furthest = fmaxf(furthest, fabsf(fmaf(q, 15.f, 12582912.f - t)));
     w += __float_as_uint(t) << (4 * i);
   }
   // what 12582912's own bits added
   w -= 0x4b400000u + 0xb4000000u + 0x40000000u;
-  if (near && d > 0.f)
+  if (furthest > 0.49999f && d > 0.f)
     w = divided(x[0], x[1], x[2], x[3], m, d) | divided(x[4], x[5], x[6], x[7], m, d) << 16;
+  if (kOff) {
+    auto apart = [](float at, float by) {
+      return __half_as_ushort(__float2half_rn(at - by)) != __half_as_ushort(__float2half_rn(at + by));
+    };
+    *unsure = finite && (apart(lo, off) || apart(step, off * 0.134f) || furthest > fmaf(off, -15.1f * inv, 0.49998f));
+  }
   return w;
 }
 // Argument rules of an rrr_kv4_cache (kv4_rows.cu).

@@ -3,7 +3,10 @@
 // 1284-1300) for packed rows and pages.
 //
 // Mathematics. qk_rows.cu's norm and rotation in 32 bits and kv4_rows.cu's groups of 32 values; the
-// rotated K is quantised from its 32-bit value, without the rounding to a 16-bit row between.
+// rotated K is quantised from its 32-bit value, without the rounding to a 16-bit row between. A
+// code changes by a whole step where a value crosses a border, so that groups which 32 bits do not
+// decide (the step, the minimum or a code within the arithmetic's error of a rounding border: about
+// one group in a hundred) are normed and rotated again in 64 bits, as all others then would be too.
 //
 // A CTA takes up to eight rows of one sequence that lie in eight aligned rows of a page (two rows
 // whose V codes share words are then one warp's), and a share of the heads. The rows' sines and
@@ -85,6 +88,40 @@ __device__ __forceinline__ bool find_rows(const AppendParams& p, int x, Rows& b)
   return true;
 }
 
+// Eight values (from e0) of a key head whose row starts at src, normed and rotated in 64 bits.
+// All lanes of a warp call it together.
+template <int HD, typename TIN>
+__device__ __noinline__ void rotated_in_64_bits(const AppendParams& p, const TIN* src, int pos, int e0, float (&x)[8]) {
+  double inv = 1.0;
+  if (p.k_gamma) {
+    double sq = 0.0;
+    for (int d = 0; d < 8; ++d) {
+      const double v = to_f32(src[e0 + d]);
+      sq += v * v;
+    }
+    for (int k = 1; k < HD / 8; k <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
+    inv = rsqrt(sq / HD + (double)p.eps);
+  }
+  auto value = [&](int e) {
+    const double v = to_f32(src[e]);
+    return p.k_gamma ? v * (double)p.k_gamma[e] * inv : v;
+  };
+#pragma unroll 1
+  for (int d = 0; d < 8; ++d) {
+    const int e = e0 + d, half = p.half_dim;
+    double z = value(e);
+    if (e < 2 * half) {
+      const bool first = p.halves ? e < half : e % 2 == 0;
+      const int f = p.halves ? (first ? e + half : e - half) : e ^ 1, i = p.halves ? min(e, f) : e / 2;
+      double t = p.turns[i], c, s;
+      if (i < p.n_factors) t /= (double)p.factors[i];
+      rope_turn(t, pos, (double)p.attn_factor, c, s);
+      z = z * c + (first ? -s : s) * value(f);
+    }
+    x[d] = (float)z;
+  }
+}
+
 template <int HD, typename TIN, typename TOUT>
 __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   using B = Kv4Block<HD>;
@@ -129,7 +166,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
   const int half = p.half_dim;
   const TIN* qkv = static_cast<const TIN*>(p.qkv);
 
-  // rows of the query or key head at `first` (an offset in qkv's rows), rotated, to put(row, values)
+  // rows of the query or key head at `first` (an offset in qkv's rows), rotated, to put(row, source,
+  // values, largest): no value among those of the lane and their partners was beyond +-largest
   auto rotated = [&](int64_t first, const float* gamma, auto&& put) {
     float gm[8], gp[8];
     const bool paired = p.halves && half % 8 == 0;
@@ -165,6 +203,9 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
 #pragma unroll
           for (int d = 0; d < 8; ++d) x[a][d] = (gm[d] * x[a][d]) * inv;
         }
+        float largest = 0.f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) largest = fmaxf(largest, fabsf(x[a][d]));
         if (!p.halves) {
 #pragma unroll
           for (int d = 0; d < 8; d += 2)
@@ -180,6 +221,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
             for (int d = 0; d < 8; ++d) {
               const float2 w = turn[rr][(hop > 0 ? e0 : e0 + hop) + d];
               const float y = gamma ? (gp[d] * o[a][d]) * inv : o[a][d];
+              largest = fmaxf(largest, fabsf(y));
               x[a][d] = fmaf(y, hop > 0 ? -w.y : w.y, x[a][d] * w.x);
             }
           }
@@ -196,6 +238,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
                 y = (gamma[f] * y) * inv;
                 z = (gamma[e] * z) * inv;
               }
+              largest = fmaxf(largest, fabsf(y));
               z = fmaf(y, e < half ? -w.y : w.y, z * w.x);
 #pragma unroll
               for (int k = 0; k < 8; ++k)
@@ -203,7 +246,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
             }
           }
         }
-        put(r, r < b.n ? source[rr] : -1, x[a]);
+        put(r, r < b.n ? source[rr] : -1, x[a], largest);
       }
     }
   };
@@ -212,7 +255,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
   for (int task = blockIdx.y * kAppendWarps + warp; task < tasks; task += kAppendWarps * gridDim.y) {
     if (task >= 2 * p.nkv) {
       const int h = task - 2 * p.nkv;
-      rotated((int64_t)h * HD, p.q_gamma, [&](int, int row, const float (&x)[8]) {
+      rotated((int64_t)h * HD, p.q_gamma, [&](int, int row, const float (&x)[8], float) {
         if (row >= 0) store_vec<TOUT, 8>(static_cast<TOUT*>(p.q) + row * p.q_stride + (int64_t)h * HD + e0, x);
       });
       continue;
@@ -269,9 +312,21 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
         }
       }
     } else {
-      rotated((int64_t)(p.nh + h) * HD, p.k_gamma, [&](int r, int from, const float (&x)[8]) {
+      // what the 32-bit norm and rotation can be off by, in units of the largest value: of a value
+      // and its partner each 2^-21.7 (angle 2^-23.3, sine 2^-23, factor and products 2^-24 each);
+      // with norms 2^-19.9 more (13 additions of squares, half of which counts, and the root)
+      const float off = fmaxf(fabsf(p.attn_factor), 1.f) * (p.k_gamma ? 1.f / 524288 : 1.f / 1048576);
+      rotated((int64_t)(p.nh + h) * HD, p.k_gamma, [&](int r, int from, float (&x)[8], float largest) {
         __half d, m;
-        const uint32_t w = quantise(x, d, m);
+        bool unsure;
+#pragma unroll
+        for (int k = 1; k < 4; k <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, k));
+        uint32_t w = quantise<true>(x, d, m, off * largest, &unsure);
+        if (__any_sync(0xffffffffu, unsure)) {
+          const int rr = min(r, b.n - 1);
+          rotated_in_64_bits<HD>(p, qkv + (int64_t)max(source[rr], 0) * p.row_stride + (int64_t)(p.nh + h) * HD, place[rr], e0, x);
+          w = quantise(x, d, m);
+        }
         if (from >= 0) {
           const int row = in_page + r;
           reinterpret_cast<uint32_t*>(blk)[B::k_word(row, j, t)] = w;

@@ -73,6 +73,14 @@ __device__ __forceinline__ void rope_turn(double t, int pos, float af, float& c,
   c *= af;
   s *= af;
 }
+// The same in 64 bits
+__device__ __forceinline__ void rope_turn(double t, int pos, double af, double& c, double& s) {
+  t -= floor(t);
+  const unsigned long long a = __double2ull_rd(t * 18446744073709551616.0) * (unsigned long long)(unsigned)pos;
+  sincospi((double)(long long)a * 1.0842021724855044e-19, &s, &c);  // 2 x turns, in [-1, 1]
+  c *= af;
+  s *= af;
+}
 constexpr int kMaxPairs = 64;  // rope_dim / 2
 // turns[i] = theta^(-2i/rope_dim) / 2 pi as a product of two powers: 16 calls of pow and not 64
 inline void rope_turns(double (&turns)[kMaxPairs], float theta, int rope_dim) {

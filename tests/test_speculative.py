@@ -6,10 +6,10 @@ hold the kernels to (a walk and a chain by hand).
 GPU: every operator against its formula in 64 bits (u = 2^-24 is half a step of f32, h(t) half a
 step of the type):
 
-  append  without norms the 32-bit operations are those of rrr_qk_norm_rope with f32 rows and of
-          rrr_kv4_store: bit for bit. With norms a value read back is off by half a step d of its
-          group, by the roundings of m and d to f16 (h16 |m|, 15 h16 d) and by the rotated value's own
-          error, 32 u (|a| + |b|) af.
+  append  the pages are, bit for bit, those of rrr_kv4_store from K in 64 bits rounded to 32; q without norms
+          that of rrr_qk_norm_rope. A value read back is off by half a step d of its group, by the
+          roundings of m and d to f16 (h16 |m|, 15 h16 d) and by the rotated value's own error,
+          32 u (|a| + |b|) af.
   tree    a score carries (hd + 16) u A of the sums (A = sum |q k| scale) and, of a cached row, h16 A:
           its key is rounded to f16 from its code. A weight 2^x is off by twice that (it and the maximum) and
           8 u. Weights are rounded to f16, those of drafted rows to the type, cached values to f16: h16 +
@@ -235,7 +235,8 @@ def append_inputs(rrr, g, rows, nh, nkv, hd, rd, kind, top=1 << 20):
 @pytest.mark.parametrize("kinds", [("f32", "bf16"), ("bf16", "f16"), ("f16", "f32")])
 @pytest.mark.parametrize("new,held", [([1], [1]), ([5, 0, 130, 1], [70, 64, 130, 65]), ([64, 63, 7], [64, 191, 13])])
 def test_kv4_append(rrr, ctx, hd, nh, nkv, rd, halves, kinds, new, held):
-    """Without norms: the bits of rrr_qk_norm_rope (f32) and rrr_kv4_store; and with norms: within a step."""
+    """q without norms: the bits of rrr_qk_norm_rope (f32). The pages: the bits of rrr_kv4_store with K normed and rotated in 64
+    bits and rounded to 32. q with norms: within its rounding and 32 bits' errors. What is read back: within half a step."""
     g, rows, cu = gen(sum(held) + hd), sum(new), cu_of(new)
     qkv, factors, desc = append_inputs(rrr, g, rows, nh, nkv, hd, rd, kinds[0])
     pos = ints([h - n + i for n, h in zip(new, held) for i in range(n)])
@@ -244,21 +245,26 @@ def test_kv4_append(rrr, ctx, hd, nh, nkv, rd, halves, kinds, new, held):
     kv = [torch.empty(rows, nkv, hd, device="cuda") for _ in range(2)]
     q = [torch.full((rows, nh, hd), 7.0, dtype=DT[kinds[1]], device="cuda") for _ in range(2)]
     q32 = torch.empty(rows, nh, hd, device="cuda")
+
+    def store(at, gammas=(None, None)):
+        refs, mags = ref_qk(qkv, at, nh, nkv, hd, rd, 10000.0, 1.25, factors, gammas, float(np.float32(1e-5)), halves)
+        want.c.store(refs[1].float().contiguous(), refs[2].float().contiguous(), cu, lens)
+        return refs, mags
     rrr.qk_norm_rope(ctx, desc, qkv, pos, q32, kv[0], kv[1], halves=halves)
-    want.c.store(kv[0], kv[1], cu, lens)
+    store(pos)
     got.c.append(desc, qkv, cu, lens, q[0], halves=halves)
     assert torch.equal(got.pages, want.pages)
     assert torch.equal(q[0], q32.to(DT[kinds[1]]))
     # the rows' own positions, and without q
     far = (pos.long() * 37 + 11).int()
-    rrr.qk_norm_rope(ctx, desc, qkv, far, q32, kv[0], kv[1], halves=halves)
-    want.c.store(kv[0], kv[1], cu, lens)
+    store(far)
     got.c.append(desc, qkv, cu, lens, positions=far, halves=halves)
     assert torch.equal(got.pages, want.pages)
     # norms
     gammas = [torch.rand(hd, device="cuda", generator=g) + 0.5 for _ in range(2)]
     got.c.append(desc, qkv, cu, lens, q[1], q_gamma=gammas[0], k_gamma=gammas[1], halves=halves)
-    refs, mags = ref_qk(qkv, pos, nh, nkv, hd, rd, 10000.0, 1.25, factors, gammas, 1e-5, halves)
+    refs, mags = store(pos, gammas)
+    assert torch.equal(got.pages, want.pages)
     out = DT[kinds[1]]
     rounding = 0.0 if out == torch.float32 else half_step(out)
     within(q[1], refs[0], refs[0].abs() * rounding * 1.01 + 32 * U * mags[0] + (2.0 ** -25 if out == torch.float16 else 1e-30))
