@@ -207,15 +207,6 @@ __device__ __forceinline__ void cluster_barrier() {
                    : "memory");
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // The CTA's positions are processed in tiles of 8192 / head_dim rows (64 for 128): the K and
 // V rows of a tile (head g) are copied into shared memory with 16-byte cp.async,
 // double-buffered so that the next tile streams in while this one is computed. The first

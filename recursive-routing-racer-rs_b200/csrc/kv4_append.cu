@@ -10,8 +10,10 @@
 //
 // A CTA takes up to eight rows of one sequence that lie in eight aligned rows of a page (two rows
 // whose V codes share words are then one warp's), and a share of the heads. The rows' sines and
-// cosines are computed once, into shared memory; then each warp takes one head of K, V or q at a
-// time: lane (j, t) the values 32j + 8t .. + 7 of a row of K or q, which are one word of codes.
+// cosines are computed once, into shared memory; a warp keeps those of its rows in registers and
+// goes through heads of q and K, whose values it loads some heads ahead: lane (j, t) the values
+// 32j + 8t .. + 7 of a row, which are one word of K's codes. Partners that lie half a rotation away
+// come by shuffles.
 #include "kv4.cuh"
 
 namespace rrr {
@@ -88,51 +90,55 @@ __device__ __forceinline__ bool find_rows(const AppendParams& p, int x, Rows& b)
   return true;
 }
 
-// Eight values (from e0) of a key head whose row starts at src, normed and rotated in 64 bits.
-// All lanes of a warp call it together.
+// Eight values (from e0) of a key head whose row starts at src, normed and rotated in 64 bits; turn:
+// the row's cosines and sines. All lanes of a warp call it together.
 template <int HD, typename TIN>
-__device__ __noinline__ void rotated_in_64_bits(const AppendParams& p, const TIN* src, int pos, int e0, float (&x)[8]) {
+__device__ __forceinline__ void rotated_in_64_bits(const AppendParams& p, const TIN* src, const double2* turn, int e0,
+                                                   float (&x)[8]) {
+  const int half = p.half_dim;
+  float v[8];
+  load_vec<TIN, 8>(src + e0, v);
   double inv = 1.0;
   if (p.k_gamma) {
     double sq = 0.0;
-    for (int d = 0; d < 8; ++d) {
-      const double v = to_f32(src[e0 + d]);
-      sq += v * v;
-    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) sq = fma((double)v[d], (double)v[d], sq);
+#pragma unroll
     for (int k = 1; k < HD / 8; k <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
     inv = rsqrt(sq / HD + (double)p.eps);
   }
-  auto value = [&](int e) {
-    const double v = to_f32(src[e]);
-    return p.k_gamma ? v * (double)p.k_gamma[e] * inv : v;
-  };
-#pragma unroll 1
+#pragma unroll
   for (int d = 0; d < 8; ++d) {
-    const int e = e0 + d, half = p.half_dim;
-    double z = value(e);
+    const int e = e0 + d;
+    double z = (double)v[d] * inv;
+    if (p.k_gamma) z *= (double)p.k_gamma[e];
     if (e < 2 * half) {
-      const bool first = p.halves ? e < half : e % 2 == 0;
+      const bool first = p.halves ? e < half : d % 2 == 0;
       const int f = p.halves ? (first ? e + half : e - half) : e ^ 1, i = p.halves ? min(e, f) : e / 2;
-      double t = p.turns[i], c, s;
-      if (i < p.n_factors) t /= (double)p.factors[i];
-      rope_turn(t, pos, (double)p.attn_factor, c, s);
-      z = z * c + (first ? -s : s) * value(f);
+      const double2 w = turn[i];
+      double y = (double)to_f32(src[f]) * inv;
+      if (p.k_gamma) y *= (double)p.k_gamma[f];
+      z = z * w.x + (first ? -w.y : w.y) * y;
     }
     x[d] = (float)z;
   }
 }
 
 template <int HD, typename TIN, typename TOUT>
-__global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 3) kv4_append_kernel(const __grid_constant__ AppendParams p) {
   using B = Kv4Block<HD>;
   constexpr int G = B::kGroups, kLanes = 4 * G;   // lanes of a row
-  constexpr int kRows = 32 / kLanes, kAhead = kRows >= 4 ? 2 : 4 / kRows;  // rows at once, and in flight
+  constexpr int kRows = 32 / kLanes;              // rows of a warp
+  constexpr int kAhead = 4, kParts = sizeof(TIN) / 2;  // heads whose values are on their way, 16 bytes each
+  __shared__ uint4 ahead[kAppendWarps][kAhead][kParts][32];
   __shared__ Rows found;
   __shared__ int source[kBlockRows], place[kBlockRows];
+  __shared__ double turns[kMaxPairs];
   __shared__ __align__(16) float2 turn[kBlockRows][kMaxPairs];
+  __shared__ __align__(16) double2 turn64[kBlockRows][kMaxPairs];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.half_dim;
   if (warp == 0) {
     Rows b;
     b.n = 0;
@@ -148,194 +154,200 @@ __global__ void __launch_bounds__(32 * kAppendWarps) kv4_append_kernel(const __g
       place[lane] = max(pos, 0);
     }
     if (lane == 0) found = b;
+  } else {
+    for (int i = threadIdx.x - 32; i < half; i += 32 * (kAppendWarps - 1))
+      turns[i] = i < p.n_factors ? p.turns[i] / (double)p.factors[i] : p.turns[i];
   }
   __syncthreads();
   const Rows b = found;
   if (b.n == 0) return;
-  for (int x = threadIdx.x; x < b.n * p.half_dim; x += 32 * kAppendWarps) {
-    const int r = x / p.half_dim, i = x - r * p.half_dim;
-    double t = p.turns[i];
-    if (i < p.n_factors) t /= (double)p.factors[i];
+  for (int x = threadIdx.x; x < b.n * half; x += 32 * kAppendWarps) {
+    const int r = x / half, i = x - r * half;
     float c, s;
-    rope_turn(t, place[r], p.attn_factor, c, s);
+    rope_turn(turns[i], place[r], p.attn_factor, c, s);
     turn[r][i] = make_float2(c, s);
+    double c64, s64;
+    rope_turn(turns[i], place[r], (double)p.attn_factor, c64, s64);
+    turn64[r][i] = make_double2(c64, s64);
   }
   __syncthreads();
   const int in_page = b.at % kPageRows;
   const int j = lane / 4 % G, t = lane % 4, set = lane / kLanes, e0 = 32 * j + 8 * t;
-  const int half = p.half_dim;
   const TIN* qkv = static_cast<const TIN*>(p.qkv);
 
-  // rows of the query or key head at `first` (an offset in qkv's rows), rotated, to put(row, source,
-  // values, largest): no value among those of the lane and their partners was beyond +-largest
-  auto rotated = [&](int64_t first, const float* gamma, auto&& put) {
-    float gm[8], gp[8];
+  // q and K: a warp takes kRows rows and every `stride`th head of them
+  const int sets = (b.n + kRows - 1) / kRows, share = kAppendWarps / sets;  // warps of the same rows
+  if (warp < sets * share) {
+    const int nq = p.q ? p.nh : 0, heads = nq + p.nkv, stride = share * gridDim.y;
+    const int r = warp % sets * kRows + set, rr = min(r, b.n - 1);  // (rows past the last are read as it)
+    const int row = source[rr];
+    const TIN* src = qkv + (int64_t)max(row, 0) * p.row_stride + e0;
     const bool paired = p.halves && half % 8 == 0;
     const int hop = e0 < half ? half : e0 < 2 * half ? -half : 0;  // where the partners lie (paired)
-    if (gamma)
+    float c[8], s[8];  // of the lane's values
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        gm[d] = gamma[e0 + d];
-        gp[d] = paired ? gamma[e0 + hop + d] : 0.f;
-      }
+    for (int d = 0; d < 8; ++d) {
+      const int i = !p.halves ? (e0 + d) / 2 : e0 + d < half ? e0 + d : e0 + d - half;
+      const bool turns_too = e0 + d < 2 * half;
+      const float2 w = turns_too ? turn[rr][i] : make_float2(1.f, 0.f);
+      c[d] = w.x;
+      s[d] = (p.halves ? e0 + d < half : d % 2 == 0) ? -w.y : w.y;
+    }
+    // what the 32-bit norm and rotation can be off by, in units of the largest value: of a value
+    // and its partner each 2^-21.7 (angle 2^-23.3, sine 2^-23, factor and products 2^-24 each);
+    // with norms 2^-19.9 more (13 additions of squares, half of which counts, and the root)
+    const float off = fmaxf(fabsf(p.attn_factor), 1.f) * (p.k_gamma ? 1.f / 524288 : 1.f / 1048576);
+    float gamma[8];
+    const TIN* heads_at = src + (p.q ? 0 : (int64_t)p.nh * HD);
+    int k = warp / sets * gridDim.y + blockIdx.y;
+    auto fetch = [&](int at, int slot) {
+      if (at < heads)
+#pragma unroll
+        for (int n = 0; n < kParts; ++n) cp_async16(&ahead[warp][slot][n][lane], heads_at + (int64_t)at * HD + 8 / kParts * n);
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int a = 0; a < kAhead - 1; ++a) fetch(k + a * stride, a);
 #pragma unroll 1
-    for (int r0 = set; r0 < b.n + set; r0 += kAhead * kRows) {
-      float x[kAhead][8], o[kAhead][8];
+    for (int nth = 0, key = -1; k < heads; k += stride, ++nth) {
+      const bool normed = k >= nq ? p.k_gamma : p.q_gamma;
+      if (key != (k >= nq)) {
+        key = k >= nq;
+        const float* of = key ? p.k_gamma : p.q_gamma;
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int r = min(r0 + a * kRows, b.n - 1);  // (rows past the last are read as it)
-        const TIN* src = qkv + (int64_t)max(source[r], 0) * p.row_stride + first + e0;
-        load_vec<TIN, 8>(src, x[a]);
-        if (paired) load_vec<TIN, 8>(src + hop, o[a]);
+        for (int d = 0; d < 8; ++d) gamma[d] = of ? of[e0 + d] : 1.f;
       }
+      fetch(k + (kAhead - 1) * stride, (nth + kAhead - 1) % kAhead);  // where the last head's values were
+      cp_async_wait<kAhead - 1>();
+      Vec<TIN, 8> now;
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        if (r0 - set + a * kRows >= b.n) break;
-        const int r = r0 + a * kRows, rr = min(r, b.n - 1);
-        float inv = 1.f;
-        if (gamma) {
-          float sq = 0.f;
+      for (int n = 0; n < kParts; ++n)
+        reinterpret_cast<uint4*>(&now)[n] = ahead[warp][nth % kAhead][n][lane];
+      float x[8];
 #pragma unroll
-          for (int d = 0; d < 8; ++d) sq = fmaf(x[a][d], x[a][d], sq);
+      for (int d = 0; d < 8; ++d) x[d] = to_f32(now.v[d]);
+      float inv = 1.f;
+      if (normed) {
+        float sq = 0.f;
 #pragma unroll
-          for (int k = 1; k < kLanes; k <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, k);
-          inv = rsqrtf(fmaf(sq, 1.f / HD, p.eps));
+        for (int d = 0; d < 8; ++d) sq = fmaf(x[d], x[d], sq);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) x[a][d] = (gm[d] * x[a][d]) * inv;
-        }
-        float largest = 0.f;
+        for (int m = 1; m < kLanes; m <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
+        inv = rsqrtf(fmaf(sq, 1.f / HD, p.eps));
 #pragma unroll
-        for (int d = 0; d < 8; ++d) largest = fmaxf(largest, fabsf(x[a][d]));
-        if (!p.halves) {
+        for (int d = 0; d < 8; ++d) x[d] = (gamma[d] * x[d]) * inv;
+      }
+      float largest = 0.f;  // of the lane's values and their partners
+      if (key)
 #pragma unroll
-          for (int d = 0; d < 8; d += 2)
-            if (e0 + d < 2 * half) {
-              const float2 w = turn[rr][(e0 + d) / 2];
-              const float u = x[a][d], v = x[a][d + 1];
-              x[a][d] = fmaf(-v, w.y, u * w.x);
-              x[a][d + 1] = fmaf(u, w.y, v * w.x);
-            }
-        } else if (paired) {
-          if (hop) {
+      for (int d = 0; d < 8; ++d) largest = fmaxf(largest, fabsf(x[d]));
+      if (!p.halves) {
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              const float2 w = turn[rr][(hop > 0 ? e0 : e0 + hop) + d];
-              const float y = gamma ? (gp[d] * o[a][d]) * inv : o[a][d];
-              largest = fmaxf(largest, fabsf(y));
-              x[a][d] = fmaf(y, hop > 0 ? -w.y : w.y, x[a][d] * w.x);
-            }
-          }
-        } else {  // pairs that lie across lanes' borders
-          const TIN* src = qkv + (int64_t)max(source[rr], 0) * p.row_stride + first;
-#pragma unroll 1
-          for (int d = 0; d < 8; ++d) {
-            const int e = e0 + d;
-            if (e < 2 * half) {
-              const int f = e < half ? e + half : e - half;
-              const float2 w = turn[rr][min(e, f)];
-              float y = to_f32(src[f]), z = to_f32(src[e]);
-              if (gamma) {
-                y = (gamma[f] * y) * inv;
-                z = (gamma[e] * z) * inv;
-              }
-              largest = fmaxf(largest, fabsf(y));
-              z = fmaf(y, e < half ? -w.y : w.y, z * w.x);
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (k == d) x[a][k] = z;
-            }
+        for (int d = 0; d < 8; d += 2) {
+          const float u = x[d], v = x[d + 1];
+          if (e0 + d < 2 * half) {
+            x[d] = fmaf(v, s[d], u * c[d]);
+            x[d + 1] = fmaf(u, s[d + 1], v * c[d + 1]);
           }
         }
-        put(r, r < b.n ? source[rr] : -1, x[a], largest);
+      } else if (paired) {
+        float y[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[d] = __shfl_sync(0xffffffffu, x[d], lane + hop / 8);
+        if (key) largest = fmaxf(largest, __shfl_sync(0xffffffffu, largest, lane + hop / 8));
+        if (hop)
+#pragma unroll
+          for (int d = 0; d < 8; ++d) x[d] = fmaf(y[d], s[d], x[d] * c[d]);
+      } else {  // pairs that lie across lanes' borders
+        const TIN* head = src - e0 + (int64_t)(key ? p.nh + k - nq : k) * HD;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const int e = e0 + d;
+          if (e < 2 * half) {
+            const int f = e < half ? e + half : e - half;
+            float y = to_f32(head[f]);
+            if (normed) y = ((key ? p.k_gamma : p.q_gamma)[f] * y) * inv;
+            largest = fmaxf(largest, fabsf(y));
+            x[d] = fmaf(y, s[d], x[d] * c[d]);
+          }
+        }
+      }
+      const bool stored = r < b.n && row >= 0;
+      if (!key) {
+        if (stored) store_vec<TOUT, 8>(static_cast<TOUT*>(p.q) + row * p.q_stride + (int64_t)k * HD + e0, x);
+        continue;
+      }
+#pragma unroll
+      for (int m = 1; m < 4; m <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, m));
+      const int h = k - nq;
+      __half d16, m16;
+      bool unsure;
+      uint32_t w = quantise<true>(x, d16, m16, off * largest, &unsure);
+      if (__any_sync(0xffffffffu, unsure)) {
+        rotated_in_64_bits<HD>(p, src - e0 + (int64_t)(p.nh + h) * HD, turn64[rr], e0, x);
+        w = quantise(x, d16, m16);
+      }
+      if (stored) {
+        uint8_t* blk = p.pages + (b.page * p.nkv + h) * B::kBytes;
+        reinterpret_cast<uint32_t*>(blk)[B::k_word(in_page + r, j, t)] = w;
+        if (t == 0) {
+          reinterpret_cast<__half*>(blk + B::kCodes)[B::scale(in_page + r, j)] = d16;
+          reinterpret_cast<__half*>(blk + B::kCodes + B::kScales)[B::scale(in_page + r, j)] = m16;
+        }
       }
     }
-  };
+  }
 
-  const int tasks = 2 * p.nkv + (p.q ? p.nh : 0);
-  for (int task = blockIdx.y * kAppendWarps + warp; task < tasks; task += kAppendWarps * gridDim.y) {
-    if (task >= 2 * p.nkv) {
-      const int h = task - 2 * p.nkv;
-      rotated((int64_t)h * HD, p.q_gamma, [&](int, int row, const float (&x)[8], float) {
-        if (row >= 0) store_vec<TOUT, 8>(static_cast<TOUT*>(p.q) + row * p.q_stride + (int64_t)h * HD + e0, x);
-      });
-      continue;
-    }
-    const int h = task >> 1;
-    uint8_t* blk = p.pages + (b.page * p.nkv + h) * B::kBytes;
-    if (task & 1) {
-      uint8_t* vb = blk + B::kHalf;
-      const int g = 2 * t;
-      const TIN* src = qkv + (int64_t)(p.nh + p.nkv + h) * HD + 32 * j + g;
-      const int odd_first = in_page & 1, pairs = (b.n + odd_first + 1) / 2;
+  // V: a warp takes a head of kRows pairs of rows whose codes share words
+  const int g = 2 * t, odd_first = in_page & 1, pairs = (b.n + odd_first + 1) / 2, turns_of = (pairs + kRows - 1) / kRows;
+  const int tasks = p.nkv * turns_of, first = (kAppendWarps - 1 - warp) * gridDim.y + blockIdx.y;
 #pragma unroll 1
-      for (int u = set; u < pairs + set; u += kRows) {
-        if (u - set >= pairs) break;
-        const int r = 2 * min(u, pairs - 1) - odd_first, row = in_page + r;  // the pair's even row
-        uint32_t c[2];
-        bool has[2];
+  for (int task = first; task < tasks; task += kAppendWarps * gridDim.y) {
+    const int h = task / turns_of, u = task % turns_of * kRows + set;
+    uint8_t* vb = p.pages + (b.page * p.nkv + h) * B::kBytes + B::kHalf;
+    const TIN* src = qkv + (int64_t)(p.nh + p.nkv + h) * HD + 32 * j + g;
+    const int r = 2 * min(u, pairs - 1) - odd_first, row = in_page + r;  // the pair's even row
+    uint32_t c[2];
+    bool has[2];
+    float v[2][8];
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const int from = source[min(max(r + o, 0), b.n - 1)];
-          has[o] = u < pairs && r + o >= 0 && r + o < b.n && from >= 0;
-          float v[8];
+    for (int o = 0; o < 2; ++o) {
+      const int from = source[min(max(r + o, 0), b.n - 1)];
+      has[o] = u < pairs && r + o >= 0 && r + o < b.n && from >= 0;
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            float two[2];
-            load_vec<TIN, 2>(src + (int64_t)max(from, 0) * p.row_stride + 8 * n, two);
-            v[2 * n] = two[0];
-            v[2 * n + 1] = two[1];
-          }
-          __half d, m;
-          c[o] = quantise(v, d, m);
-          if (t == 0 && has[o]) {
-            reinterpret_cast<__half*>(vb + B::kCodes)[B::scale(row + o, j)] = d;
-            reinterpret_cast<__half*>(vb + B::kCodes + B::kScales)[B::v_min(row + o, j)] = m;
-          }
-        }
-        // nibbles 0, 2, 4, 6 are g's, the others g + 1's: four each to a half word
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t w[2];
-#pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            uint32_t y = (c[o] >> (4 * e)) & 0x0f0f0f0fu;
-            y = (y | y >> 4) & 0x00ff00ffu;
-            w[o] = (y | y >> 8) & 0xffffu;
-          }
-          uint16_t* codes = reinterpret_cast<uint16_t*>(vb);
-          if (has[0] && has[1])
-            reinterpret_cast<uint32_t*>(vb)[B::v_half(row, j, g + e) / 2] = w[0] | w[1] << 16;
-          else if (has[0])
-            codes[B::v_half(row, j, g + e)] = (uint16_t)w[0];
-          else if (has[1])
-            codes[B::v_half(row + 1, j, g + e)] = (uint16_t)w[1];
-        }
+      for (int n = 0; n < 4; ++n) {
+        float two[2];
+        load_vec<TIN, 2>(src + (int64_t)max(from, 0) * p.row_stride + 8 * n, two);
+        v[o][2 * n] = two[0];
+        v[o][2 * n + 1] = two[1];
       }
-    } else {
-      // what the 32-bit norm and rotation can be off by, in units of the largest value: of a value
-      // and its partner each 2^-21.7 (angle 2^-23.3, sine 2^-23, factor and products 2^-24 each);
-      // with norms 2^-19.9 more (13 additions of squares, half of which counts, and the root)
-      const float off = fmaxf(fabsf(p.attn_factor), 1.f) * (p.k_gamma ? 1.f / 524288 : 1.f / 1048576);
-      rotated((int64_t)(p.nh + h) * HD, p.k_gamma, [&](int r, int from, float (&x)[8], float largest) {
-        __half d, m;
-        bool unsure;
+    }
 #pragma unroll
-        for (int k = 1; k < 4; k <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, k));
-        uint32_t w = quantise<true>(x, d, m, off * largest, &unsure);
-        if (__any_sync(0xffffffffu, unsure)) {
-          const int rr = min(r, b.n - 1);
-          rotated_in_64_bits<HD>(p, qkv + (int64_t)max(source[rr], 0) * p.row_stride + (int64_t)(p.nh + h) * HD, place[rr], e0, x);
-          w = quantise(x, d, m);
-        }
-        if (from >= 0) {
-          const int row = in_page + r;
-          reinterpret_cast<uint32_t*>(blk)[B::k_word(row, j, t)] = w;
-          if (t == 0) {
-            reinterpret_cast<__half*>(blk + B::kCodes)[B::scale(row, j)] = d;
-            reinterpret_cast<__half*>(blk + B::kCodes + B::kScales)[B::scale(row, j)] = m;
-          }
-        }
-      });
+    for (int o = 0; o < 2; ++o) {
+      __half d, m;
+      c[o] = quantise(v[o], d, m);
+      if (t == 0 && has[o]) {
+        reinterpret_cast<__half*>(vb + B::kCodes)[B::scale(row + o, j)] = d;
+        reinterpret_cast<__half*>(vb + B::kCodes + B::kScales)[B::v_min(row + o, j)] = m;
+      }
+    }
+    // nibbles 0, 2, 4, 6 are g's, the others g + 1's: four each to a half word
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uint32_t w[2];
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        uint32_t y = (c[o] >> (4 * e)) & 0x0f0f0f0fu;
+        y = (y | y >> 4) & 0x00ff00ffu;
+        w[o] = (y | y >> 8) & 0xffffu;
+      }
+      uint16_t* codes = reinterpret_cast<uint16_t*>(vb);
+      if (has[0] && has[1])
+        reinterpret_cast<uint32_t*>(vb)[B::v_half(row, j, g + e) / 2] = w[0] | w[1] << 16;
+      else if (has[0])
+        codes[B::v_half(row, j, g + e)] = (uint16_t)w[0];
+      else if (has[1])
+        codes[B::v_half(row + 1, j, g + e)] = (uint16_t)w[1];
     }
   }
 }
