@@ -13,10 +13,15 @@
 // relative error of 2^-24 one draw in some fifty would come out as a neighbour. So exponentials and
 // sums are held in 64 bits; an error of 2^-44 leaves one in 10^7.
 //
+// Exponentials. (x - top) c = n + r, n the nearest multiple of 1/16 (the product added to 1.5 2^48 leaves
+// 16 n in the low bits), |r| <= 1/32 from one more fma, exact; 2^n from a table of 16 in shared
+// memory, which fills its 32 banks, and the exponent's bits; 2^r - 1 by a polynomial of degree 5
+// (interpolated at Chebyshev nodes), off by 2^-46.6: eleven operations of 64 bits.
+//
 // A row is cut into chunks of 4 KB at 16-byte borders of memory. First kernel: per chunk the
 // maximum, its first place and the sum of the exponentials under it, one warp each. Trees: a second
-// kernel, one CTA per sequence, walks: it finds a row's chunk from the chunks' sums and the token
-// inside it. Chains with the draft's logits: one CTA per sequence compares, then the chunks of the
+// kernel, one CTA per row, draws the row's token: its chunk from the chunks' sums, then the token
+// inside it; a third, one CTA per sequence, walks. Chains with the draft's logits: one CTA per sequence compares, then the chunks of the
 // row where the chain ends are summed as max(p - q, 0), and one CTA per sequence draws.
 #include <float.h>
 
@@ -57,6 +62,7 @@ struct VerifyParams {
   Stat* q_stats;
   Ending* endings;
   double* rest;   // [n_seqs][rest_chunks]
+  int* drawn;     // [rows]
   int* err;
 };
 
@@ -64,6 +70,40 @@ struct VerifyParams {
 __device__ __forceinline__ float tidy(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 // 2^y, y <= 0
 __device__ __forceinline__ double exp2_of(double y) { return exp2(y); }
+// The exponentials 2^((x - top) c) of values up to `top`; fine: whether they can be taken this way.
+// Values that are 1000 binary orders and more under the top count as such, NaN too.
+struct Powers {
+  double c, top;
+  float lowest;
+  bool fine;
+};
+__device__ __forceinline__ Powers powers_of(float top, double c) {
+  Powers w;
+  w.c = c;
+  w.top = (double)top;
+  w.lowest = __double2float_rd(w.top - 1000. / c);
+  const double span = (w.top - (double)w.lowest) * c;  // (roundings may leave it another one)
+  w.fine = top < INFINITY && w.lowest >= -FLT_MAX && span > 980. && span < 1020.;
+  return w;
+}
+__device__ __forceinline__ double power(const Powers& w, const double* table, float x) {
+  constexpr double kMagic = 422212465065984.;  // 1.5 2^48
+  const double v = (double)fmaxf(x, w.lowest) - w.top;
+  const double t = fma(v, w.c, kMagic);
+  const double r = fma(v, w.c, kMagic - t);
+  double p = fma(r, 0.0013333744338239965, 0.009618317140580765);
+  p = fma(r, p, 0.05550410866027587);
+  p = fma(r, p, 0.24022650691319414);
+  p = fma(r, p, 0.6931471805599453);
+  const int n = __double2loint(t);
+  const double step = table[n & 15];
+  p = fma(step, r * p, step);
+  return __hiloint2double(__double2hiint(p) + ((n & ~15) << 16), __double2loint(p));
+}
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 16) table[threadIdx.x] = exp2(threadIdx.x * 0.0625);
+  __syncthreads();
+}
 // log2(e) / T; 0 for temperature 0 (and, recorded, for one that is none)
 __device__ __forceinline__ double sharpness(const VerifyParams& p, int seq) {
   const float t = p.temperature ? p.temperature[seq] : 1.f;
@@ -103,8 +143,10 @@ __device__ __forceinline__ bool rows_of(const VerifyParams& p, int seq, int& r0,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kStatWarps) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(32 * kStatWarps, 3) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
   constexpr int kVec = 16 / (int)sizeof(T), kSteps = kChunkBytes / 512, kChunk = kChunkBytes / (int)sizeof(T);
+  __shared__ double table[16];
+  fill_table(table);
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -137,28 +179,32 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_stats_kernel(const __g
   }
   const double c = sharpness(p, seq);
   float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kSteps * kVec; ++i) top = fmaxf(top, to_f32(u.v[i]));
+  const float mine = top = fminf(top, FLT_MAX);
+  const bool infinite = __any_sync(0xffffffffu, mine == FLT_MAX);
+  top = warp_max(top);
   int best = INT32_MAX;
-#pragma unroll
-  for (int i = 0; i < kSteps * kVec; ++i) {
-    const float v = tidy(to_f32(u.v[i]));
-    if (v > top) {
-      top = v;
-      best = i;
-    }
-  }
-  if (best < INT32_MAX) best = chunk * kChunk + (best / kVec * 32 + lane) * kVec + best % kVec - shift;
-  const float mine = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (mine < top) best = INT32_MAX;
-  best = __reduce_min_sync(0xffffffffu, best);
   double sum = 0.;
-  if (c != 0. && top > -INFINITY) {
-    const double m = (double)top;
+  if (c == 0.) {
 #pragma unroll
-    for (int i = 0; i < kSteps * kVec; ++i) {
-      const float v = tidy(to_f32(u.v[i]));
-      if (v > -INFINITY) sum += exp2_of(((double)v - m) * c);
+    for (int i = kSteps * kVec - 1; i >= 0; --i)
+      if (to_f32(u.v[i]) >= top) best = i;
+    if (mine < top || top == -INFINITY) best = INT32_MAX;
+    if (best < INT32_MAX) best = chunk * kChunk + (best / kVec * 32 + lane) * kVec + best % kVec - shift;
+    best = __reduce_min_sync(0xffffffffu, best);
+  } else if (top > -INFINITY) {
+    const Powers w = powers_of(top, c);
+    if (w.fine && !infinite) {
+#pragma unroll
+      for (int i = 0; i < kSteps * kVec; ++i) sum += power(w, table, to_f32(u.v[i]));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kSteps * kVec; ++i) {
+        const int at = chunk * kChunk + (i / kVec * 32 + lane) * kVec + i % kVec;
+        const float v = at >= shift && at < shift + p.vocab ? tidy(to_f32(base[at])) : -INFINITY;
+        if (v > -INFINITY) sum += exp2_of(((double)v - (double)top) * c);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -295,35 +341,42 @@ __device__ __forceinline__ int draw_token(Shared& sh, const VerifyParams& p, int
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(kWalkThreads) verify_tokens_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ Shared sh;
-  __shared__ int child;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x;
+  int seq;
+  if (!find_seq(p, row, seq)) return;
+  const int token = draw_token<T>(sh, p, row, sharpness(p, seq), (double)p.uniforms[2 * (int64_t)row + 1]);
+  if (threadIdx.x == 0) p.drawn[row] = token;
+}
+__global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ int child[2];
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.x;
   int r0, n;
   if (!rows_of(p, seq, r0, n)) n = 0;
-  const double c = sharpness(p, seq);
   int at = 0, count = 0, token = -1;
+  if (threadIdx.x == 0) child[0] = INT32_MAX;
   while (count < n) {
-    if (threadIdx.x == 0) {
-      p.path[r0 + count] = at;
-      child = INT32_MAX;
-    }
+    int& next = child[count & 1];
+    if (threadIdx.x == 0) p.path[r0 + count] = at;
+    token = p.drawn[r0 + at];
     ++count;
-    token = draw_token<T>(sh, p, r0 + at, c, (double)p.uniforms[2 * (int64_t)(r0 + at) + 1]);
+    __syncthreads();
+    if (threadIdx.x == 0) child[count & 1] = INT32_MAX;  // (all have read it)
     if (token < 0) break;
     // (a parent lies before its child)
     for (int i = at + 1 + threadIdx.x; i < n; i += kWalkThreads) {
       const int up = p.parents ? p.parents[r0 + i] : i - 1;
       if (up < -1 || up >= i) flag_position(p.err);
-      if (up == at && p.tokens[r0 + i] == token) atomicMin(&child, i);
+      if (up == at && p.tokens[r0 + i] == token) atomicMin(&next, i);
     }
     __syncthreads();
-    const int found = child;
-    __syncthreads();
-    if (found == INT32_MAX) break;
-    at = found;
+    if (next == INT32_MAX) break;
+    at = next;
   }
   if (threadIdx.x == 0) {
     p.counts[seq] = count;
@@ -416,6 +469,8 @@ __device__ __forceinline__ double rest_of(const T* x, const T* y, int i, const E
 }
 template <typename T>
 __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ double table[16];
+  fill_table(table);
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y, lane = threadIdx.x & 31, chunk = blockIdx.x * kStatWarps + (threadIdx.x >> 5);
@@ -427,9 +482,28 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
   const T* x = static_cast<const T*>(p.logits) + (int64_t)(r0 + e.last) * p.logits_stride;
   const T* y = static_cast<const T*>(p.draft) + (int64_t)(r0 + e.last + 1) * p.draft_stride;
   double sum = 0.;
-  const int end = min(p.vocab, (chunk + 1) * kRestChunk);
-#pragma unroll 4
-  for (int i = chunk * kRestChunk + lane; i < end; i += 32) sum += rest_of(x, y, i, e, c);
+  const int first = chunk * kRestChunk, end = min(p.vocab, first + kRestChunk);
+  const Powers wp = powers_of(e.pm, c), wq = powers_of(e.qm, c);
+  // (tops of FLT_MAX may stand for infinities)
+  if (wp.fine && wq.fine && e.pm < FLT_MAX && e.qm < FLT_MAX) {
+    const double sp = 1. / e.pz, sq = 1. / e.qz;
+    constexpr int kStep = 8;
+#pragma unroll 1
+    for (int i0 = first + lane; i0 < end; i0 += 32 * kStep) {
+      float a[kStep], b[kStep];
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) {
+        const int i = i0 + 32 * k;
+        a[k] = i < end ? to_f32(x[i]) : -INFINITY;
+        b[k] = i < end ? to_f32(y[i]) : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) sum += fmax(power(wp, table, a[k]) * sp - power(wq, table, b[k]) * sq, 0.);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = first + lane; i < end; i += 32) sum += rest_of(x, y, i, e, c);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) p.rest[(int64_t)seq * p.rest_chunks + chunk] = sum;
@@ -476,8 +550,12 @@ cudaError_t launch(const LaunchEnv& env, const VerifyParams& p) {
     if (e != cudaSuccess) return e;
   }
   const dim3 seqs((unsigned)p.n_seqs), block(kWalkThreads);
-  if (!p.draft) return rrr_launch_pdl(verify_walk_kernel<T>, seqs, block, 0, env.stream, env.pdl, p);
-  cudaError_t e = rrr_launch_pdl(verify_chain_kernel<T>, seqs, block, 0, env.stream, env.pdl, p);
+  cudaError_t e = cudaSuccess;
+  if (!p.draft) {
+    if (p.rows > 0) e = rrr_launch_pdl(verify_tokens_kernel<T>, dim3((unsigned)p.rows), block, 0, env.stream, env.pdl, p);
+    return e != cudaSuccess ? e : rrr_launch_pdl(verify_walk_kernel, seqs, block, 0, env.stream, env.pdl, p);
+  }
+  e = rrr_launch_pdl(verify_chain_kernel<T>, seqs, block, 0, env.stream, env.pdl, p);
   if (e == cudaSuccess)
     e = rrr_launch_pdl(verify_rest_kernel<T>, dim3((p.rest_chunks + kStatWarps - 1) / kStatWarps, (unsigned)p.n_seqs),
                        dim3(32 * kStatWarps), 0, env.stream, env.pdl, p);
@@ -488,7 +566,7 @@ cudaError_t launch(const LaunchEnv& env, const VerifyParams& p) {
 int64_t padded(int64_t n) { return (n + 255) / 256 * 256; }
 struct Layout {
   int chunks, rest_chunks;
-  int64_t q, endings, rest, bytes;
+  int64_t q, endings, rest, drawn, bytes;
 };
 Layout layout_of(int rows, int vocab, int n_seqs, bool draft) {
   Layout l;
@@ -497,7 +575,8 @@ Layout layout_of(int rows, int vocab, int n_seqs, bool draft) {
   l.q = padded((int64_t)rows * l.chunks * (int64_t)sizeof(Stat));
   l.endings = l.q * (draft ? 2 : 1);
   l.rest = l.endings + (draft ? padded((int64_t)n_seqs * (int64_t)sizeof(Ending)) : 0);
-  l.bytes = l.rest + (draft ? padded((int64_t)n_seqs * l.rest_chunks * 8) : 0);
+  l.drawn = l.rest + (draft ? padded((int64_t)n_seqs * l.rest_chunks * 8) : 0);
+  l.bytes = l.drawn + (draft ? 0 : padded(4 * (int64_t)rows));
   if (l.bytes < 256) l.bytes = 256;
   return l;
 }
@@ -578,7 +657,8 @@ int rrr_verify_drafts(rrr_ctx* ctx, int type, const void* logits, int64_t logits
                        path, counts, next_tokens, rows, vocab, n_seqs,
                        (int)(((int64_t)vocab + 16 / es - 1 + chunk - 1) / chunk), l.rest_chunks,
                        reinterpret_cast<Stat*>(ws), reinterpret_cast<Stat*>(ws + l.q),
-                       reinterpret_cast<Ending*>(ws + l.endings), reinterpret_cast<double*>(ws + l.rest), env.d_err};
+                       reinterpret_cast<Ending*>(ws + l.endings), reinterpret_cast<double*>(ws + l.rest),
+                       reinterpret_cast<int*>(ws + l.drawn), env.d_err};
   cudaError_t e;
   switch (type) {
     case RRR_F32: e = launch<float>(env, p); break;
