@@ -143,7 +143,7 @@ __device__ __forceinline__ bool rows_of(const VerifyParams& p, int seq, int& r0,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kStatWarps, 3) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(32 * kStatWarps, 4) verify_stats_kernel(const __grid_constant__ VerifyParams p) {
   constexpr int kVec = 16 / (int)sizeof(T), kSteps = kChunkBytes / 512, kChunk = kChunkBytes / (int)sizeof(T);
   __shared__ double table[16];
   fill_table(table);
@@ -156,8 +156,6 @@ __global__ void __launch_bounds__(32 * kStatWarps, 3) verify_stats_kernel(const 
   const bool is_q = rows >= p.rows;
   const int row = (int)(is_q ? rows - p.rows : rows);
   if (row >= p.rows || (is_q && !p.draft)) return;
-  int seq;
-  if (!find_seq(p, row, seq) || (is_q && row == p.cu[seq])) return;
   const T* x = is_q ? static_cast<const T*>(p.draft) + row * p.draft_stride
                     : static_cast<const T*>(p.logits) + row * p.logits_stride;
   const int shift = shift_of(x);
@@ -177,11 +175,16 @@ __global__ void __launch_bounds__(32 * kStatWarps, 3) verify_stats_kernel(const 
         u.v[k * kVec + i] = at + i >= shift && at + i < shift + p.vocab ? base[at + i] : from_f32<T>(-INFINITY);
     }
   }
+  int seq;  // (sought while the values are on their way)
+  if (!find_seq(p, row, seq) || (is_q && row == p.cu[seq])) return;
   const double c = sharpness(p, seq);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kSteps * kVec; ++i) top = fmaxf(top, to_f32(u.v[i]));
   const float mine = top = fminf(top, FLT_MAX);
+  // (so that the words and not the values read from them stay in registers)
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) asm volatile("" : "+r"(u.raw[k].x), "+r"(u.raw[k].y), "+r"(u.raw[k].z), "+r"(u.raw[k].w));
   const bool infinite = __any_sync(0xffffffffu, mine == FLT_MAX);
   top = warp_max(top);
   int best = INT32_MAX;
