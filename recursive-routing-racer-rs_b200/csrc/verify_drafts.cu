@@ -30,7 +30,7 @@
 namespace rrr {
 namespace {
 
-constexpr int kStatWarps = 8, kWalkThreads = 256;
+constexpr int kStatWarps = 8, kWalkThreads = 256, kKept = 2048;
 constexpr int kChunkBytes = 4096, kRestChunk = 1024;
 
 struct Stat {  // of one chunk
@@ -219,8 +219,9 @@ __global__ void __launch_bounds__(32 * kStatWarps, 4) verify_stats_kernel(const 
 struct Shared {
   double sums[kWalkThreads / 32];
   float tops[kWalkThreads / 32];
-  int low, high, chunk;
+  int low, high;
   double before;
+  double kept[kKept];  // the weights of a draw, each read by the thread that wrote it
 };
 __device__ __forceinline__ double block_sum_before(Shared& sh, double v, double& total) {  // of the threads before
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -253,32 +254,35 @@ __device__ __forceinline__ float block_max(Shared& sh, float v) {
   __syncthreads();
   return m;
 }
-// The first i < n whose weights up to it, weight(0) + .. + weight(i), exceed u times their total,
-// `before` being what lies before 0 (at, if given, stands in place of u times the total); the last i
-// with a weight where roundings leave none, -1 where there is no weight. *prior: the sum before i.
+// The first i < n whose weights up to it, before + weight(0) + .. + weight(i), exceed the goal; with
+// u >= 0 the goal becomes u times the weights' total. The last i with a weight where roundings leave
+// none, -1 where there is no weight. *prior: the sum before i.
 template <class F>
-__device__ __forceinline__ int draw(Shared& sh, int n, double u, const double* at, double before, F&& weight, double* prior) {
+__device__ __forceinline__ int draw(Shared& sh, int n, double u, double& goal, double before, F&& weight, double* prior) {
   const int per = (n + kWalkThreads - 1) / kWalkThreads;
   const int a = min(n, (int)threadIdx.x * per), b = min(n, a + per);
   double mine = 0., total;
   int last = -1;
+#pragma unroll 4
   for (int i = a; i < b; ++i) {
     const double w = weight(i);
+    if (n <= kKept) sh.kept[i] = w;
     mine += w;
     if (w > 0.) last = i;
   }
+  auto again = [&](int i) { return n <= kKept ? sh.kept[i] : weight(i); };
   if (threadIdx.x == 0) {
     sh.low = INT32_MAX;
     sh.high = -1;
   }
   double upto = before + block_sum_before(sh, mine, total);
-  const double goal = at ? *at : u * total;
+  if (u >= 0.) goal = u * total;
   const double from = upto;
   if (last >= 0) {
     atomicMax(&sh.high, last);
     if (upto + mine > goal) {
       for (int i = a; i < b; ++i) {
-        const double w = weight(i);
+        const double w = again(i);
         upto += w;
         if (w > 0. && upto > goal) {
           atomicMin(&sh.low, i);
@@ -291,7 +295,7 @@ __device__ __forceinline__ int draw(Shared& sh, int n, double u, const double* a
   const int got = sh.low != INT32_MAX ? sh.low : sh.high;
   if (prior && got >= a && got < b) {
     double s = from;
-    for (int i = a; i < got; ++i) s += weight(i);
+    for (int i = a; i < got; ++i) s += again(i);
     sh.before = s;
   }
   __syncthreads();
@@ -324,19 +328,12 @@ __device__ __forceinline__ int draw_token(Shared& sh, const VerifyParams& p, int
     const Stat s = st[i];
     return s.sum > 0. ? s.sum * exp2_of(((double)s.top - m) * c) : 0.;
   };
-  double goal, before, total;
-  {
-    double mine = 0.;
-    const int per = (p.chunks + kWalkThreads - 1) / kWalkThreads;
-    for (int i = min(p.chunks, (int)threadIdx.x * per), b = min(p.chunks, i + per); i < b; ++i) mine += chunk_weight(i);
-    block_sum_before(sh, mine, total);
-    goal = u * total;
-  }
-  const int chunk = draw(sh, p.chunks, 0., &goal, 0., chunk_weight, &before);
+  double goal, before;
+  const int chunk = draw(sh, p.chunks, u, goal, 0., chunk_weight, &before);
   if (chunk < 0) return -1;
   const T* x = static_cast<const T*>(p.logits) + row * p.logits_stride;
   const int first = max(0, chunk * kChunk - shift_of(x)), end = min(p.vocab, (chunk + 1) * kChunk - shift_of(x));
-  const int got = draw(sh, end - first, 0., &goal, before, [&](int i) {
+  const int got = draw(sh, end - first, -1., goal, before, [&](int i) {
     const float v = tidy(to_f32(x[first + i]));
     return v > -INFINITY ? exp2_of(((double)v - m) * c) : 0.;
   }, nullptr);
@@ -392,10 +389,12 @@ __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_
 __device__ __forceinline__ void warp_stats(const Stat* st, int n, double c, float& top, double& sum) {
   const int lane = threadIdx.x & 31;
   top = -INFINITY;
+#pragma unroll 8
   for (int i = lane; i < n; i += 32) top = fmaxf(top, st[i].top);
   top = warp_max(top);
   sum = 0.;
   if (!(top > -INFINITY)) return;
+#pragma unroll 4
   for (int i = lane; i < n; i += 32) {
     const Stat s = st[i];
     if (s.sum > 0.) sum += s.sum * exp2_of(((double)s.top - (double)top) * c);
@@ -412,6 +411,7 @@ __device__ __forceinline__ double share(float x, float top, double sum, double c
 template <typename T>
 __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ int refused;
+  __shared__ Ending ends[kWalkThreads / 32];  // of the drafts that are looked at together
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -426,9 +426,14 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
       const int64_t row = r0 + i;
       const int x = p.tokens[row];
       const Stat* st = p.p_stats + (row - 1) * p.chunks;
-      float pm, qm;
-      double pz, qz;
+      float pm = 0.f, qm = 0.f;
+      double pz = 0., qz = 0.;
       bool stands = false;
+      if (c != 0.) {
+        warp_stats(st, p.chunks, c, pm, pz);
+        warp_stats(p.q_stats + row * p.chunks, p.chunks, c, qm, qz);
+        if (lane == 0) ends[warp] = Ending{pz, qz, pm, qm, i - 1, pz > 0. && qz > 0.};
+      }
       if (x < 0 || x >= p.vocab) {
         // no token: it does not stand
       } else if (c == 0.) {
@@ -438,8 +443,6 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
           if (st[k].top == pm) best = min(best, st[k].best);
         stands = pm > -INFINITY && __reduce_min_sync(0xffffffffu, best) == x;
       } else {
-        warp_stats(st, p.chunks, c, pm, pz);
-        warp_stats(p.q_stats + row * p.chunks, p.chunks, c, qm, qz);
         const double pp = share(to_f32(static_cast<const T*>(p.logits)[(row - 1) * p.logits_stride + x]), pm, pz, c);
         const double q = share(to_f32(static_cast<const T*>(p.draft)[row * p.draft_stride + x]), qm, qz, c);
         stands = (double)p.uniforms[2 * row] * q < pp;
@@ -452,15 +455,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
     if (stop) break;
   }
   const int count = n ? refused : 0;
-  if (warp == 0 && n) {
-    Ending e{0., 0., 0.f, 0.f, count - 1, 0};
-    if (c != 0. && count < n) {
-      warp_stats(p.p_stats + (int64_t)(r0 + count - 1) * p.chunks, p.chunks, c, e.pm, e.pz);
-      warp_stats(p.q_stats + (int64_t)(r0 + count) * p.chunks, p.chunks, c, e.qm, e.qz);
-      e.refused = e.pz > 0. && e.qz > 0.;
-    }
-    if (lane == 0) p.endings[seq] = e;
-  }
+  if (threadIdx.x == 0 && n)
+    p.endings[seq] = c != 0. && count < n ? ends[(count - 1) % (kWalkThreads / 32)] : Ending{0., 0., 0.f, 0.f, count - 1, 0};
   if (threadIdx.x == 0) p.counts[seq] = count;
   for (int i = threadIdx.x; i < n; i += kWalkThreads) p.path[r0 + i] = i < count ? i : -1;
 }
@@ -524,17 +520,13 @@ __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_
     const double c = sharpness(p, seq), u = (double)p.uniforms[2 * (int64_t)(r0 + e.last) + 1];
     if (e.refused) {
       const double* rest = p.rest + (int64_t)seq * p.rest_chunks;
-      double total, mine = 0., before;
-      const int per = (p.rest_chunks + kWalkThreads - 1) / kWalkThreads;
-      for (int i = min(p.rest_chunks, (int)threadIdx.x * per), b = min(p.rest_chunks, i + per); i < b; ++i) mine += rest[i];
-      block_sum_before(sh, mine, total);
-      const double goal = u * total;
-      const int chunk = draw(sh, p.rest_chunks, 0., &goal, 0., [&](int i) { return rest[i]; }, &before);
+      double goal, before;
+      const int chunk = draw(sh, p.rest_chunks, u, goal, 0., [&](int i) { return rest[i]; }, &before);
       if (chunk >= 0) {
         const T* x = static_cast<const T*>(p.logits) + (int64_t)(r0 + e.last) * p.logits_stride;
         const T* y = static_cast<const T*>(p.draft) + (int64_t)(r0 + e.last + 1) * p.draft_stride;
         const int first = chunk * kRestChunk, end = min(p.vocab, first + kRestChunk);
-        const int got = draw(sh, end - first, 0., &goal, before, [&](int i) { return rest_of(x, y, first + i, e, c); }, nullptr);
+        const int got = draw(sh, end - first, -1., goal, before, [&](int i) { return rest_of(x, y, first + i, e, c); }, nullptr);
         if (got >= 0) token = first + got;
       }
     }
