@@ -177,6 +177,30 @@ __device__ __forceinline__ void values_of(uint32_t w, __half2 d, __half2 m, uint
   x[2] = as_u32(__hfma2(__hadd2(as_half2(and_or(v, 0x000f000fu, big)), less), d, m));
   x[3] = as_u32(__hfma2(__hfma2(as_half2(and_or(v, 0x00f000f0u, big)), sixteenth, less64), d, m));
 }
+// d c + m of two groups as the sum of two such values, the first of which f16 holds exactly where the
+// group's values have both signs: d without its last four bits (a multiple of u, as 64 to 127 u), m
+// rounded to a multiple of u, at most 2,048 u in all; and what is left, under 16 u, whose own
+// rounding is 2^-17 of the value.
+__device__ __forceinline__ void split(uint32_t& d, uint32_t& m, uint32_t& d_rest, uint32_t& m_rest) {
+  const uint32_t most = d & 0xfff0fff0u;
+  const float2 all = __half22float2(as_half2(m));
+  auto multiple = [](float x, uint32_t bits) {
+    const uint32_t e = max((bits >> 10) & 31u, 1u);  // u = 2^(e - 21)
+    return rintf(x * __uint_as_float((148u - e) << 23)) * __uint_as_float((e + 106u) << 23);
+  };
+  const __half2 near = __floats2half2_rn(multiple(all.x, d), multiple(all.y, d >> 16));
+  d_rest = as_u32(__hsub2(as_half2(d), as_half2(most)));
+  m_rest = as_u32(__hsub2(as_half2(m), near));
+  d = most;
+  m = as_u32(near);
+}
+// Two weights as f16 and what that leaves of them
+__device__ __forceinline__ void split(float a, float b, uint32_t& w, uint32_t& rest) {
+  const __half2 x = __floats2half2_rn(a, b);
+  const float2 y = __half22float2(x);
+  w = as_u32(x);
+  rest = as_u32(__floats2half2_rn(a - y.x, b - y.y));
+}
 // 128-byte swizzle of an offset from a 1024-byte border
 __device__ __forceinline__ uint32_t swizzled(uint32_t off) { return off ^ (((off >> 7) & 7u) << 4); }
 // N words (a power of two) at p
@@ -438,8 +462,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ TreeParams p) {
   using S = Sizes<HD, NT>;
   constexpr int G = HD / 32, J = G < 4 ? G : 4, PL = G / J;  // groups, groups per plane, planes
+  // f16 rows show what f16 operands lose, bf16 rows do not: with f16 rows cached keys and weights are sums of two f16
+  // each. The two of a block of keys come one after the other; the weights have one place, in two halves.
+  constexpr bool kTwice = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], k_full[2], s_full[2], v_full[S::kVs], p_full[2], p_empty[2], o_empty, fin;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], k_full[2], k_done[2], s_full[2], v_full[S::kVs], p_full[2], p_empty[2], o_empty, fin;
   __shared__ uint64_t told[kInfos];                // that the info of a segment's first block is there, or that there is none
   __shared__ uint64_t lifted[4];                  // v_lift is there, by the segment's number (every segment but the last has drafted rows here)
   __shared__ uint64_t teams[2];                   // of K's and V's warps
@@ -467,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
+      mbar_init(&k_done[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4 * kGroups);
       mbar_init(&p_empty[i], 1);
@@ -658,9 +686,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- scores: S = K Q^T of block i, in the place of S(i - 2) once its weights are there
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);  // (known to be the warp's, as what is derived from it)
     const uint64_t q_desc = sw128_desc(smem_addr(qs));
+    int kc = 0;  // K's operands so far
 #pragma unroll 1
     for (int i = 0;; ++i) {
-      if (!wait(&k_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
+      if (!wait(&k_full[kc & 1], (uint32_t)(kc >> 1) & 1u)) break;
       if (i >= 2 && !wait(&p_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
       const int2 f = *reinterpret_cast<const int2*>(&infos[i % kInfos]);  // flags, columns
       if (f.x & kStop) {
@@ -668,15 +697,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const uint32_t odd = __shfl_sync(0xffffffffu, i & 1, 0), n = __shfl_sync(0xffffffffu, f.y, 0);
-      const uint32_t idesc = kF16 | n >> 3 << 17, to = base + S::kSCol + odd * NT, k = base + (S::kKs == 2 ? odd * S::kKCols : 0u);
-      tc_fence_after();
-      if (elect_one()) {
+      const uint32_t idesc = kF16 | n >> 3 << 17, to = base + S::kSCol + odd * NT;
+      const int times = kTwice && !(f.x & kDraft) ? 2 : 1;
+      bool ok = true;
+#pragma unroll 1
+      for (int t = 0; t < times && ok; ++t, ++kc) {
+        if (t) ok = wait(&k_full[kc & 1], (uint32_t)(kc >> 1) & 1u);
+        if (!ok) break;
+        const uint32_t k = base + (S::kKs == 2 ? __shfl_sync(0xffffffffu, kc & 1, 0) * S::kKCols : 0u);
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          umma_f16_ta(to, k + 8u * kk, q_desc + (((kk / 4) * NT * 128 + 32 * (kk % 4)) >> 4), idesc, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[i & 1]);
+          for (int kk = 0; kk < HD / 16; ++kk)
+            umma_f16_ta(to, k + 8u * kk, q_desc + (((kk / 4) * NT * 128 + 32 * (kk % 4)) >> 4), idesc, t + kk > 0 ? 1u : 0u);
+          if (kTwice) umma_commit(&k_done[kc & 1]);
+          if (t + 1 == times) umma_commit(&s_full[i & 1]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      if (!ok) break;
     }
     if (elect_one()) umma_commit(&fin);
     __syncwarp();
@@ -695,16 +734,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t odd = __shfl_sync(0xffffffffu, i & 1, 0), flags = __shfl_sync(0xffffffffu, head.x, 0), n = __shfl_sync(0xffffffffu, head.y, 0);
       const uint32_t lift = __shfl_sync(0xffffffffu, flags & kDraft ? v_lift[(flags >> 8) & 3] : 0, 0);
       const uint32_t idesc = kF16 | 1u << 16 | n >> 3 << 17, more = flags & kFirst ? 0u : 1u, ones = base + S::kOnes + 8u * lift;
-      const uint64_t v = v_desc + (S::kVs == 2 ? odd * (S::kV >> 4) : 0u), w = p_desc + odd * (S::kP >> 4);
+      const uint64_t v = v_desc + (S::kVs == 2 ? odd * (S::kV >> 4) : 0u), w = p_desc + (kTwice ? 0u : odd * (S::kP >> 4));
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk) {
+        for (int x = 0; x < (kTwice ? 2 : 1) * (kRows / 16); ++x) {
+          const int kk = x % (kRows / 16);
+          const uint64_t part = w + ((x / (kRows / 16) * S::kP + 2048 * kk) >> 4);
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h)
-            umma_f16(base + S::kOCol + h * NT, v + (((h * 2 + kk / 4) * S::kERows * 128 + 32 * (kk % 4)) >> 4), w + (2048 * kk >> 4), idesc,
-                     kk > 0 ? 1u : more);
-          umma_f16_ta(base + S::kLCol, ones, w + (2048 * kk >> 4), idesc, kk > 0 ? 1u : more);
+            umma_f16(base + S::kOCol + h * NT, v + (((h * 2 + kk / 4) * S::kERows * 128 + 32 * (kk % 4)) >> 4), part, idesc,
+                     x > 0 ? 1u : more);
+          umma_f16_ta(base + S::kLCol, ones, part, idesc, x > 0 ? 1u : more);
         }
         umma_commit(&p_empty[i & 1]);
       }
@@ -817,6 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     bool begins = true;
     uint32_t turns = 0;  // of the waits for `told`
+    int kc = 0;          // operands so far
 #pragma unroll 1
     for (int i = 0;; ++i) {
       const Info& f = infos[i % kInfos];
@@ -838,14 +880,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       begins = flags & kLast;
       if (flags & kStop) {
         // (not before the products have seen the block two before, or they would miss its turn)
-        if (i >= 2 && !doze(&s_full[i & 1], (uint32_t)((i - 2) >> 1) & 1u)) break;
-        if (lane == 0) mbar_arrive(&k_full[i & 1]);
+        if (kc >= 2 && !doze(kTwice ? &k_done[kc & 1] : &s_full[kc & 1], (uint32_t)((kc - 2) >> 1) & 1u)) break;
+        if (lane == 0) mbar_arrive(&k_full[kc & 1]);
         break;
       }
-      const uint32_t dst = tmem + (i % S::kKs) * S::kKCols + sub;
-      // the place is free once S(i - kKs) is done
+      uint32_t dst = 0;
+      // the place is free once the products with the operand kKs before are done (kc = i where there is one per block)
       auto free_place = [&]() {
-        const bool ok = i < S::kKs || doze(&s_full[(i - S::kKs) & 1], (uint32_t)((i - S::kKs) >> 1) & 1u);
+        const int last = kc - S::kKs;
+        dst = tmem + (kc % S::kKs) * S::kKCols + sub;
+        const bool ok = last < 0 || doze(kTwice ? &k_done[last & 1] : &s_full[last & 1], (uint32_t)(last >> 1) & 1u);
         tc_fence_after();
         return ok;
       };
@@ -858,31 +902,54 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < G / 2; ++k) most = __hmax2(most, __hfma2(as_half2(d[k]), as_half2(0x4b804b80u), __habs2(as_half2(m[k]))));
         if (row < f.valid[half] && (__hisinf(__low2half(most)) || __hisinf(__high2half(most)))) k_again[par] = 1;
+        uint32_t d_rest[G / 2], m_rest[G / 2];
+        if (kTwice)
+#pragma unroll
+          for (int k = 0; k < G / 2; ++k) split(d[k], m[k], d_rest[k], m_rest[k]);
         if (!free_place()) break;
-#pragma unroll
-        for (int P = 0; P < PL; ++P) {
-          __half2 dd[J], mm[J];
-#pragma unroll
-          for (int k = 0; k < J; ++k) {
-            const int j = P * J + k;
-            dd[k] = j & 1 ? __high2half2(as_half2(d[j / 2])) : __low2half2(as_half2(d[j / 2]));
-            mm[k] = j & 1 ? __high2half2(as_half2(m[j / 2])) : __low2half2(as_half2(m[j / 2]));
-          }
+        bool ok = true;
 #pragma unroll 1
-          for (int u = 0; u < J; ++u) {  // four words, 16 columns
-            const uint4 x = *reinterpret_cast<const uint4*>(page + ((k_codes + P * 1024 * J) ^ (16 * u)));
-            uint32_t y[16];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t z[4];
-              values_of((&x.x)[k], dd[k % J], mm[k % J], z);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[4 * k + e] = z[e];
-            }
+        for (int t = 0; t < (kTwice ? 2 : 1); ++t) {
+          if (kTwice && t) {
+            tmem_wait_st();
+            tc_fence_before();
             __syncwarp();
-            tmem_st16(dst + P * 16 * J + 16 * u, y);
+            if (lane == 0) mbar_arrive(&k_full[kc & 1]);
+            ++kc;
+            ok = free_place();
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < G / 2; ++k) {
+              d[k] = d_rest[k];
+              m[k] = m_rest[k];
+            }
+          }
+#pragma unroll
+          for (int P = 0; P < PL; ++P) {
+            __half2 dd[J], mm[J];
+#pragma unroll
+            for (int k = 0; k < J; ++k) {
+              const int j = P * J + k;
+              dd[k] = j & 1 ? __high2half2(as_half2(d[j / 2])) : __low2half2(as_half2(d[j / 2]));
+              mm[k] = j & 1 ? __high2half2(as_half2(m[j / 2])) : __low2half2(as_half2(m[j / 2]));
+            }
+#pragma unroll 1
+            for (int u = 0; u < J; ++u) {  // four words, 16 columns
+              const uint4 x = *reinterpret_cast<const uint4*>(page + ((k_codes + P * 1024 * J) ^ (16 * u)));
+              uint32_t y[16];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t z[4];
+                values_of((&x.x)[k], dd[k % J], mm[k % J], z);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * k + e] = z[e];
+              }
+              __syncwarp();
+              tmem_st16(dst + P * 16 * J + 16 * u, y);
+            }
           }
         }
+        if (!ok) break;
       } else {
         // drafted rows: to [1, 2) by a power of two each; who sees whom
         uint8_t* const to = ring + (size_t)st * S::kStage;
@@ -936,9 +1003,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&k_full[i & 1]);
+        mbar_arrive(&k_full[kc & 1]);
         mbar_arrive(&empty[st]);
       }
+      ++kc;
       if (++st == S::kStages) {
         st = 0;
         phase ^= 1;
@@ -957,11 +1025,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int par = (flags >> 8) & 3, n = head.y;
       const bool first = flags & kFirst;
       const uint32_t sc = tmem + S::kSCol + (i & 1) * NT + sub;
-      uint8_t* const dst = ps + (i & 1) * S::kP + (r >> 3) * 1024 + (r & 7) * 128;
+      uint8_t* const dst = ps + (kTwice ? 0 : (i & 1) * S::kP) + (r >> 3) * 1024 + (r & 7) * 128;
       float* const line = lines[par];
       tc_fence_after();
-      // P's place is free once PV(i - 2) is done
-      if (!(flags & kStop) && i >= 2) ok = wait(&p_empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u);
+      // P's place is free once PV(i - kPs) is done
+      constexpr int kPs = kTwice ? 1 : 2;
+      if (!(flags & kStop) && i >= kPs) ok = wait(&p_empty[(i - kPs) & 1], (uint32_t)((i - kPs) >> 1) & 1u);
       const bool plain = !(flags & kDraft) && (r & 32) + 32 <= valid;  // every row of the warp counts, for all columns
       float ks = 1.f, low = 1.f;
       if (flags & kDraft) {
@@ -991,12 +1060,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 8; ++e) a[e] = -INFINITY;
         }
       };
+      auto put = [&](int c, const uint32_t (&w)[4], const uint32_t (&rest)[4]) {
+        uint8_t* const to = dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (kTwice) *reinterpret_cast<uint4*>(to + S::kP) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+      };
       // the weights of all columns into P; the largest argument
       auto weights = [&]() {
         float top = -INFINITY;
         if (plain) {
           auto eight = [&](const uint32_t* sv, int x) {
-            uint32_t w[4];
+            uint32_t w[4], rest[4];
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
               const float4 a = *reinterpret_cast<const float4*>(line + x + e), b = *reinterpret_cast<const float4*>(line + NT + x + e);
@@ -1004,12 +1078,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 v = __ffma2_rn(make_float2(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), make_float2(a.z, a.w), make_float2(b.z, b.w));
               top = fmaxf(top, fmaxf(u.x, u.y));
               top = fmaxf(top, fmaxf(v.x, v.y));
-              w[e / 2] = as_u32(__floats2half2_rn(ex2(u.x), ex2(u.y)));
-              w[e / 2 + 1] = as_u32(__floats2half2_rn(ex2(v.x), ex2(v.y)));
+              if (kTwice) {
+                split(ex2(u.x), ex2(u.y), w[e / 2], rest[e / 2]);
+                split(ex2(v.x), ex2(v.y), w[e / 2 + 1], rest[e / 2 + 1]);
+              } else {
+                w[e / 2] = as_u32(__floats2half2_rn(ex2(u.x), ex2(u.y)));
+                w[e / 2 + 1] = as_u32(__floats2half2_rn(ex2(v.x), ex2(v.y)));
+              }
             }
-            const int c = x;
-            *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            put(x, w, rest);
           };
 #pragma unroll 1
           for (int x = 8 * h; x < n; x += 8 * kGroups) {
@@ -1022,15 +1099,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 8 * h; x < n; x += 8 * kGroups) {
             float a[8];
             arguments(x, a);
-            uint32_t w[4];
+            uint32_t w[4], rest[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               top = fmaxf(top, fmaxf(a[2 * e], a[2 * e + 1]));
-              w[e] = as_u32(__floats2half2_rn(ex2(a[2 * e]) * low, ex2(a[2 * e + 1]) * low));
+              split(ex2(a[2 * e]) * low, ex2(a[2 * e + 1]) * low, w[e], rest[e]);
             }
-            const int c = x;
-            *reinterpret_cast<uint4*>(dst + (c >> 6) * (kRows * 128) + ((((c & 63) >> 3) ^ (r & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            put(x, w, rest);
           }
         }
         return top;
