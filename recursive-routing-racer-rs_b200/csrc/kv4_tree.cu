@@ -14,7 +14,7 @@ namespace {
 constexpr int kMaxHpk = 8, kMaxNodes = 128;
 constexpr float kNone = -3e38f;  // the maximum of no rows: finite, so that it may be subtracted from -inf
 constexpr int kRows = 128;       // KV rows of a block: two pages, or the drafted rows
-constexpr int kStart = 4;        // units in front of a segment's blocks
+constexpr int kStart = 6;        // units in front of a segment's blocks
 constexpr int kGroups = 4;       // of four softmax warps each: group h takes the columns 8 h .. + 7 of every 8 kGroups
 constexpr int kKWarp = 4 * kGroups, kVWarp = kKWarp + 4, kSWarp = kVWarp + 4, kLoadWarp = kSWarp + 1, kPVWarp = kSWarp + 2;
 constexpr int kThreads = 32 * (kSWarp + 4);
@@ -340,38 +340,45 @@ __device__ __noinline__ void plain_row(const TreeParams& p, int seq, int r0, int
   store_vec<T, D>(static_cast<T*>(p.out) + row * p.out_row + head * p.out_head + e0, o);
 }
 
+// What is done once in a segment is kept small: its instructions come from far away each time, which took longer than
+// what they do. So rows are copied as they are to the places of what is made of them, all at once, and each thread then
+// goes through its own 16 bytes in a loop.
+
+// Eight 16-bit values at p, of a row that HD / 8 neighbouring lanes hold, to f16 in the order of K's words, the row brought
+// to [1, 2) by a power of two, which is returned
+template <int HD, typename T>
+__device__ __forceinline__ float row_to_one(uint8_t* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  uint32_t top = top_bits<T>(v);
+#pragma unroll
+  for (int o = 1; o < HD / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float s = to_one(top);
+  uint32_t y[4];
+  scaled_pairs<T>(v, s, y);
+  *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+  return s;
+}
 // The tile's queries into shared memory, in the order of K's words: HD / 8 lanes per row, 8 values each; a row is
 // brought to [1, 2) by a power of two, which its line takes back.
 template <int HD, int NT, typename T>
 __device__ __noinline__ void queries(const TreeParams& p, const Info& f, int r, uint8_t* qs, float* line) {
   constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes;
   const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // the place among the words of a row of codes
-  constexpr int kBatch = 4;
+  uint8_t* const to = qs + (w / 8) * NT * 128;
 #pragma unroll 1
-  for (int c0 = r / kLanes; c0 < f.n; c0 += kBatch * kAcross) {
-    uint4 v[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int c = c0 + k * kAcross, column = f.c0 + c, token = column / p.hpk, head = f.kv * p.hpk + column - token * p.hpk;
-      v[k] = make_uint4(0, 0, 0, 0);
-      if (c < f.cols)
-        v[k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(f.r0 + token) * p.q_row + head * p.q_head + 8 * x);
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int c = c0 + k * kAcross;
-      uint32_t top = top_bits<T>(v[k]);
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (c >= f.n) break;
-      const float s = to_one(top);
-      uint32_t y[4];
-      scaled_pairs<T>(v[k], s, y);
-      *reinterpret_cast<uint4*>(qs + (w / 8) * NT * 128 + sw128_off(c, w % 8)) = make_uint4(y[0], y[1], y[2], y[3]);
-      if (x == 0) {
-        line[c] = c < f.cols ? p.scale / s : 0.f;
-        line[NT + c] = kBias;
-      }
+  for (int c = r / kLanes; c < f.n; c += kAcross) {
+    const int column = f.c0 + min(c, f.cols - 1), token = column / p.hpk, head = f.kv * p.hpk + column - token * p.hpk;
+    cp_async16_or_zero(to + sw128_off(c, w % 8),
+                       static_cast<const T*>(p.q) + (int64_t)(f.r0 + token) * p.q_row + head * p.q_head + 8 * x, c < f.cols);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+#pragma unroll 1
+  for (int c = r / kLanes; c < f.n; c += kAcross) {
+    const float s = row_to_one<HD, T>(to + sw128_off(c, w % 8));
+    if (x == 0) {
+      line[c] = c < f.cols ? p.scale / s : 0.f;
+      line[NT + c] = kBias;
     }
   }
 }
@@ -379,69 +386,55 @@ __device__ __noinline__ void queries(const TreeParams& p, const Info& f, int r, 
 // They go to shared memory, from where their threads take them to TMEM.
 template <int HD, typename T>
 __device__ __noinline__ void drafted_keys(const TreeParams& p, const Info& f, int r, int first, uint8_t* to, float* scales) {
-  constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes, kBatch = 4;
+  constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes;
   const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J, rows = min(f.nodes - first, 64);
   const T* src = static_cast<const T*>(p.k) + (int64_t)(f.r0 + first) * p.k_row + f.kv * p.k_head + 8 * x;
+  const int own = r / kLanes, end = own + rows;  // (whole warps go through the loops)
 #pragma unroll 1
-  for (int c0 = r / kLanes; c0 < 64; c0 += kBatch * kAcross) {
-    if (c0 - r / kLanes >= rows) break;
-    uint4 v[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      v[k] = make_uint4(0, 0, 0, 0);
-      if (c0 + k * kAcross < rows) v[k] = *reinterpret_cast<const uint4*>(src + (c0 + k * kAcross) * p.k_row);
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int c = c0 + k * kAcross;
-      uint32_t top = top_bits<T>(v[k]);
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float s = to_one(top);
-      uint32_t y[4];
-      scaled_pairs<T>(v[k], s, y);
-      *reinterpret_cast<uint4*>(to + c * (2 * HD) + ((w ^ (c & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-      if (x == 0) scales[first + c] = 1.f / s;
-    }
+  for (int c = own; c < end; c += kAcross)
+    cp_async16_or_zero(to + c * (2 * HD) + ((w ^ (c & 7)) << 4), src + min(c, rows - 1) * p.k_row, c < rows);
+  cp_async_commit();
+  cp_async_wait<0>();
+#pragma unroll 1
+  for (int c = own; c < end; c += kAcross) {
+    const float s = row_to_one<HD, T>(to + c * (2 * HD) + ((w ^ (c & 7)) << 4));
+    if (x == 0) scales[first + c] = 1.f / s;
   }
 }
-// Drafted values: rows 8 o .. + 7 (o = tid % 16), values 8 (tid / 16 + 8 c) .. + 7 of them; the largest of their bits, and the
-// values, lifted, into shared memory
-template <int HD, typename T>
-__device__ __forceinline__ void drafted_eight(const TreeParams& p, const Info& f, int tid, int c, uint4 (&w)[8]) {
-  const int o = tid & 15, rows = min(max(f.nodes - 8 * o, 0), 8);
-  const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head + (int64_t)(f.r0 + 8 * o) * p.v_row + 8 * ((tid >> 4) + 8 * c);
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    w[r] = make_uint4(0, 0, 0, 0);
-    if (r < rows) w[r] = *reinterpret_cast<const uint4*>(src + r * p.v_row);
-  }
+// Drafted values: a thread has rows 8 o .. + 7 (o = tid % 16) of values 8 (tid / 16 + 8 c) .. + 7, eight rows of 16 bytes
+// which become eight values of 16 bytes. The rows into shared memory, to the values' places; the largest of their bits.
+template <int HD>
+__device__ __forceinline__ uint8_t* value_place(uint8_t* dst, int o, int e) {
+  constexpr int kERows = HD < 128 ? HD : 128;
+  return dst + ((e >> 7) * 2 + (o >> 3)) * kERows * 128 + (e & 127) * 128 + (((o & 7) ^ (e & 7)) << 4);
 }
 template <int HD, typename T>
-__device__ __noinline__ uint32_t drafted_top(const TreeParams& p, const Info& f, int tid) {
+__device__ __noinline__ uint32_t drafted_rows(const TreeParams& p, const Info& f, int tid, uint8_t* dst) {
+  const int o = tid & 15, e0 = 8 * (tid >> 4);
+  const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head + (int64_t)f.r0 * p.v_row + e0;
+#pragma unroll 1
+  for (int x = 0; x < HD / 8; ++x) {
+    const int row = 8 * o + x % 8, c = x / 8;
+    cp_async16_or_zero(value_place<HD>(dst, o, e0 + 64 * c + x % 8), src + min(row, f.nodes - 1) * p.v_row + 64 * c, row < f.nodes);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
   uint32_t top = 0;
-#pragma unroll
-  for (int c = 0; c < HD / 64; c += 2) {
-    uint4 w[2][8];
-    drafted_eight<HD, T>(p, f, tid, c, w[0]);
-    if (HD > 64) drafted_eight<HD, T>(p, f, tid, c + 1, w[1]);
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      top = max(top, top_bits<T>(w[0][r]));
-      if (HD > 64) top = max(top, top_bits<T>(w[1][r]));
-    }
-  }
+#pragma unroll 1
+  for (int x = 0; x < HD / 8; ++x)
+    top = max(top, top_bits<T>(*reinterpret_cast<const uint4*>(value_place<HD>(dst, o, e0 + 64 * (x / 8) + x % 8))));
   return __reduce_max_sync(0xffffffffu, top);
 }
+// The values of the rows there, lifted
 template <int HD, typename T>
-__device__ __noinline__ void drafted_values(const TreeParams& p, const Info& f, int tid, float lift, uint8_t* dst) {
-  constexpr int kERows = HD < 128 ? HD : 128;
+__device__ __noinline__ void drafted_values(int tid, float lift, uint8_t* dst) {
   const int o = tid & 15;
 #pragma unroll 1
   for (int c = 0; c < HD / 64; ++c) {
-    uint4 w[8];
-    drafted_eight<HD, T>(p, f, tid, c, w);
     const int e0 = 8 * ((tid >> 4) + 8 * c);
+    uint4 w[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) w[r] = *reinterpret_cast<const uint4*>(value_place<HD>(dst, o, e0 + r));
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       uint32_t y[4];
@@ -450,9 +443,7 @@ __device__ __noinline__ void drafted_values(const TreeParams& p, const Info& f, 
         const float2 a = pair_of<T>((&w[2 * r].x)[k / 2]), b = pair_of<T>((&w[2 * r + 1].x)[k / 2]);
         y[r] = as_u32(__floats2half2_rn((k & 1 ? a.y : a.x) * lift, (k & 1 ? b.y : b.x) * lift));
       }
-      const int e = e0 + k;
-      *reinterpret_cast<uint4*>(dst + ((e >> 7) * 2 + (o >> 3)) * kERows * 128 + (e & 127) * 128 + (((o & 7) ^ (e & 7)) << 4)) =
-          make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(value_place<HD>(dst, o, e0 + k)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
 }
@@ -818,7 +809,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             *reinterpret_cast<uint4*>(to + 8 * e * 128) = make_uint4(x[0][e], x[1][e], x[2][e], x[3][e]);
         }
       } else {
-        uint32_t top = drafted_top<HD, T>(p, f, tid);
+        if (!free_place()) break;
+        uint32_t top = drafted_rows<HD, T>(p, f, tid, dst);
         if (lane == 0) v_tops[warp & 3] = top;
         if (!team()) break;
         top = max(max(v_tops[0], v_tops[1]), max(v_tops[2], v_tops[3]));
@@ -826,8 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           v_lift[(flags >> 8) & 3] = lift_of(top);
           mbar_arrive(&lifted[(flags >> 8) & 3]);
         }
-        if (!free_place()) break;
-        drafted_values<HD, T>(p, f, tid, lifted_by(lift_of(top)), dst);
+        drafted_values<HD, T>(tid, lifted_by(lift_of(top)), dst);
         if (!team()) break;  // v_tops is read
       }
       fence_proxy_async_smem();
