@@ -486,8 +486,8 @@ int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, const void* q, 
  * rrr_kv4_append of those. Lengths, trees and results stay on the device. */
 
 /* Appends QKV rows [Q heads | K heads | V heads] to the cache, in one pass: K heads normed and
- * rotated as by rrr_qk_norm_rope (its a, gammas, eps and halves) and quantised from 32 bits, V heads
- * quantised, as rrr_kv4_store holds them. Sequence s has kv_lens[s] rows afterwards, and its packed
+ * rotated as by rrr_qk_norm_rope (its a, gammas, eps and halves), V heads as they are, quantised as by
+ * rrr_kv4_store: K's codes are those of the norm and rotation in 64 bits, rounded to 32. Sequence s has kv_lens[s] rows afterwards, and its packed
  * rows are its last ones. q not NULL: its rows get the query heads, normed and rotated, in out_type.
  * path and counts not NULL (then q is NULL): of sequence s the counts[s] rows path[cu[s]],
  * path[cu[s] + 1], .. (rows of the sequence) are appended in this order, no others: the accepted

@@ -14,6 +14,11 @@
 // goes through heads of q and K, whose values it loads some heads ahead: lane (j, t) the values
 // 32j + 8t .. + 7 of a row, which are one word of K's codes. Partners that lie half a rotation away
 // come by shuffles.
+//
+// What bounds it. Instructions: 5,949 rows of 48 heads of 128, bf16 with norms, 65 us (151 MB, 23 us at the copy's rate),
+// 260 instructions for eight values of 32 lanes on average, of which K and V take four fifths; 64 single rows 10 us,
+// five dependent trips to memory. The 64-bit rotation takes 9 us of the 65; with sines computed again for each group it took
+// 45.
 #include "kv4.cuh"
 
 namespace rrr {

@@ -1,6 +1,28 @@
 // kv4_tree.cu — attention of drafted rows over the 4-bit KV cache (rrr_attention_tree_kv4): the
 // `attention` dispatch (src/model/phi4.rs:1284-1309, 1680-1688) for the rows of a tree of drafted
 // tokens per sequence, which see the sequence's cached rows and their own ancestors.
+//
+// Mathematics. The columns of a tile are up to 64 or 96 (row, query head) pairs of a sequence and KV
+// head, its blocks 128 cached rows each and at last the drafted ones: S = K Q^T, the weights P =
+// 2^(S scale log2(e) - m + 10) with a column's reference m, O^T += V^T P, and the sums of the weights
+// by a product with ones, so that they are the sums of what V is multiplied by. m is taken
+// over anew where a weight would pass 2^15. Who sees whom in the drafted block is a bit mask per row. A
+// query, and a drafted key, is scaled by a power of two, drafted values together by one, so
+// that f16 operands hold both 16-bit types. A result that is not finite, or a cached group that f16 does
+// not hold, is computed again row by row in 32 bits.
+//
+// Layout. One CTA per SM and an equal run of blocks for each; a sequence's share that crosses the border of two CTAs is
+// joined by a second kernel, in order. Keys are dequantised, a row per thread, straight into TMEM (operand A), values
+// transposed into shared memory, queries lie on the products' N side: so few columns cost few product cycles.
+// 27 warps: one copies pages (TMA), four each dequantise K and V, sixteen take the softmax, one each issues the two
+// products.
+//
+// What bounds it. Not memory (1.3 TB/s) nor the tensor cores, but the roles' instructions and hand-overs: a warp gets one in
+// about ten cycles, a block of 48 columns takes 3,400 cycles and of 96 3,600. Measured on 24 heads over 8 of 128: 64
+// sequences of 16 rows on up to 8,190: 267 us (floor 54 by bytes); 60 rows on 131,000: 215 us (57 by operations). With
+// dequantisation, weights and products left out (before the last two steps) 207 and 125 us remained. Steps on the way: keys through shared memory
+// 15 ms as scalar code; rolled loops 690 -> 464 (the instruction cache), scores ahead of the weighted sums -> 333, two
+// issuing warps and sixteen softmax warps -> 322, small code for what a segment does once -> 267.
 #include <math.h>
 
 #include <type_traits>
@@ -1056,12 +1078,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
         if (kTwice) *reinterpret_cast<uint4*>(to + S::kP) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
       };
-      // the weights of all columns into P; the largest argument
-      auto weights = [&]() {
+      // find: the largest arguments of all columns; otherwise their weights into P, and the largest argument. (One copy
+      // of the general arguments for both.)
+      auto columns = [&](bool find) {
         float top = -INFINITY;
-        if (plain) {
-          auto eight = [&](const uint32_t* sv, int x) {
-            uint32_t w[4], rest[4];
+        if (plain && !find) {
+#pragma unroll 1
+          for (int x = 8 * h; x < n; x += 8 * kGroups) {
+            uint32_t sv[8], w[4], rest[4];
+            tmem_ld8(sc + x, sv);
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
               const float4 a = *reinterpret_cast<const float4*>(line + x + e), b = *reinterpret_cast<const float4*>(line + NT + x + e);
@@ -1078,18 +1103,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             put(x, w, rest);
-          };
-#pragma unroll 1
-          for (int x = 8 * h; x < n; x += 8 * kGroups) {
-            uint32_t sv[8];
-            tmem_ld8(sc + x, sv);
-            eight(sv, x);
           }
-        } else {
+          return top;
+        }
 #pragma unroll 1
-          for (int x = 8 * h; x < n; x += 8 * kGroups) {
-            float a[8];
-            arguments(x, a);
+        for (int x = 8 * h; x < n; x += 8 * kGroups) {
+          float a[8];
+          arguments(x, a);
+          if (find) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float m = redux_max(a[e]);
+              if (lane == 0) quad[qd][x + e] = m;
+            }
+          } else {
             uint32_t w[4], rest[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1104,55 +1131,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       float top = -INFINITY;
       if (!ok) dead[h] = 1;
       bool leave = false;
+      // weights, a vote; where one says so the largest arguments, and weights again
+      bool vote = !ok || (flags & (kStop | kFirst));
 #pragma unroll 1
-      for (int turn = !ok || (flags & (kStop | kFirst)) ? 1 : 0; turn < 2; ++turn) {
-        if (turn) {
+      for (;;) {
+        bool find = false;
+        if (vote) {
           // a new maximum, where a weight would be larger than the lazy ones may be
-          const bool grown = any_of_128(bar, first || top > kBias + kLazy);
+          find = any_of_128(bar, first || top > kBias + kLazy);
           leave = (flags & kStop) || *reinterpret_cast<volatile int*>(&dead[h]);
-          if (leave || !grown) break;
+          if (leave || !find) break;
+        }
 #pragma unroll 1
-        for (int x = 8 * h; x < n; x += 8 * kGroups) {
-          float a[8];
-          arguments(x, a);
+        for (;; find = false) {
+          top = columns(find);
+          if (!find) break;
+          any_of_128(bar, false);
+          const int mine = 8 * h + r % 8 + r / 8 * 8 * kGroups;  // a column of the group
+          if (mine < n) {
+            float m = fmaxf(fmaxf(quad[0][mine], quad[1][mine]), fmaxf(quad[2][mine], quad[3][mine])) - kBias;
+            if (!first) m = fmaxf(m, 0.f);
+            if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
+            change[mine] = ex2(-m);
+            line[NT + mine] -= m;
+          }
+          // (O of the blocks before is complete)
+          if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) dead[h] = 1;
+          any_of_128(bar, false);
+          leave = *reinterpret_cast<volatile int*>(&dead[h]);
+          if (leave) break;
+          tc_fence_after();
+          if (!first) {
+#pragma unroll 1
+            for (int k = -1; k < S::kHalves; ++k)  // the sums of the weights, and O
+#pragma unroll 1
+              for (int x = 8 * h; x < n; x += 8 * kGroups) {
+                const uint32_t oc = tmem + S::kOCol + k * NT + x + sub;
+                uint32_t o[8];
+                __syncwarp();
+                tmem_ld8(oc, o);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float m = redux_max(a[e]);
-            if (lane == 0) quad[qd][x + e] = m;
+                for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * change[x + e]);
+                tmem_st8(oc, o);
+              }
+            tmem_wait_st();
           }
         }
-        any_of_128(bar, false);
-        const int mine = 8 * h + r % 8 + r / 8 * 8 * kGroups;  // a column of the group
-        if (mine < n) {
-          float m = fmaxf(fmaxf(quad[0][mine], quad[1][mine]), fmaxf(quad[2][mine], quad[3][mine])) - kBias;
-          if (!first) m = fmaxf(m, 0.f);
-          if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
-          change[mine] = ex2(-m);
-          line[NT + mine] -= m;
-        }
-        // (O of the blocks before is complete)
-        if (!first && !wait(&p_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) dead[h] = 1;
-        any_of_128(bar, false);
-        leave = *reinterpret_cast<volatile int*>(&dead[h]);
-        if (leave) break;
-        tc_fence_after();
-        if (!first) {
-#pragma unroll 1
-          for (int k = -1; k < S::kHalves; ++k)  // the sums of the weights, and O
-#pragma unroll 1
-            for (int x = 8 * h; x < n; x += 8 * kGroups) {
-              const uint32_t oc = tmem + S::kOCol + k * NT + x + sub;
-              uint32_t o[8];
-              __syncwarp();
-              tmem_ld8(oc, o);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * change[x + e]);
-              tmem_st8(oc, o);
-            }
-          tmem_wait_st();
-        }
-        }
-        top = weights();
+        if (leave || vote) break;
+        vote = true;
       }
       if (leave) break;
       fence_proxy_async_smem();

@@ -23,6 +23,10 @@
 // kernel, one CTA per row, draws the row's token: its chunk from the chunks' sums, then the token
 // inside it; a third, one CTA per sequence, walks. Chains with the draft's logits: one CTA per sequence compares, then the chunks of the
 // row where the chain ends are summed as max(p - q, 0), and one CTA per sequence draws.
+//
+// What bounds it. The 64-bit pipe: eleven operations and one conversion a value, at two cycles a warp each. 48 chains of 5
+// rows and their drafts on 200,064 tokens, f32: 148 us (346 MB, 53 us), of which the first kernel takes 110; 285
+// rows of trees, bf16: 65 us (114 MB, 17 us), 55 of them. CUDA's exp2 took 302 and 327 us.
 #include <float.h>
 
 #include "serve_common.cuh"
