@@ -19,10 +19,10 @@
 //
 // What bounds it. Not memory (1.3 TB/s) nor the tensor cores, but the roles' instructions and hand-overs: a warp gets one in
 // about ten cycles, a block of 48 columns takes 3,400 cycles and of 96 3,600. Measured on 24 heads over 8 of 128: 64
-// sequences of 16 rows on up to 8,190: 267 us (floor 54 by bytes); 60 rows on 131,000: 215 us (57 by operations). With
-// dequantisation, weights and products left out (before the last two steps) 207 and 125 us remained. Steps on the way: keys through shared memory
-// 15 ms as scalar code; rolled loops 690 -> 464 (the instruction cache), scores ahead of the weighted sums -> 333, two
-// issuing warps and sixteen softmax warps -> 322, small code for what a segment does once -> 267.
+// sequences of 16 rows on up to 8,190: 245 us (floor 54 by bytes); 60 rows on 131,000: 222 us (57 by operations). With
+// dequantisation, weights and products left out (before the last two steps) 207 and 125 us remained. Steps, for the 64
+// sequences: scalar products 14.8 ms, tensor cores 690 us, rolled loops 464 (the instruction cache), scores ahead of the
+// weighted sums 333, two issuing warps and sixteen softmax warps 322, small code for what a segment does once 245.
 #include <math.h>
 
 #include <type_traits>
