@@ -180,7 +180,11 @@ __global__ void __launch_bounds__(32 * kStatWarps, 4) verify_stats_kernel(const 
     }
   }
   int seq;  // (sought while the values are on their way)
-  if (!find_seq(p, row, seq) || (is_q && row == p.cu[seq])) return;
+  Stat* const to = (is_q ? p.q_stats : p.p_stats) + (int64_t)row * p.chunks + chunk;
+  if (!find_seq(p, row, seq) || (is_q && row == p.cu[seq])) {
+    if (lane == 0) *to = Stat{0., -INFINITY, INT32_MAX};  // (sequences that overlap may come to it)
+    return;
+  }
   const double c = sharpness(p, seq);
   float top = -INFINITY;
 #pragma unroll
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(32 * kStatWarps, 4) verify_stats_kernel(const 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if (lane == 0) (is_q ? p.q_stats : p.p_stats)[(int64_t)row * p.chunks + chunk] = Stat{sum, top, best};
+  if (lane == 0) *to = Stat{sum, top, best};
 }
 
 // ---- one CTA of kWalkThreads threads per sequence
@@ -351,7 +355,10 @@ __global__ void __launch_bounds__(kWalkThreads) verify_tokens_kernel(const __gri
   pdl_wait();
   const int row = blockIdx.x;
   int seq;
-  if (!find_seq(p, row, seq)) return;
+  if (!find_seq(p, row, seq)) {
+    if (threadIdx.x == 0) p.drawn[row] = -1;
+    return;
+  }
   const int token = draw_token<T>(sh, p, row, sharpness(p, seq), (double)p.uniforms[2 * (int64_t)row + 1]);
   if (threadIdx.x == 0) p.drawn[row] = token;
 }

@@ -724,6 +724,71 @@ def test_verify_drafts_bad_arguments_on_the_device(rrr, ctx):
         assert code == 6 and path[:2] == [0, 2]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("chains", [False, True])
+def test_verify_drafts_of_overlapping_sequences(rrr, ctx, chains):
+    """Row starts that go back: recorded; every token is one of the vocabulary's, or -1, whatever the workspace held."""
+    g, vocab = gen(9), 700
+    logits, u, tokens = normal(g, 6, vocab), torch.rand(6, 2, device="cuda", generator=g), ints([0] * 6)
+    draft = normal(g, 6, vocab) if chains else None
+    for cu in ([0, 4, 2, 6], [2, 6, 0, 5], [5, 6, 1, 1], [0, 6, 3, 6]):
+        for heat in (1.0, 0.0):
+            path, n = torch.full((6,), 77, dtype=torch.int32, device="cuda"), len(cu) - 1
+            counts, following = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+            ws = rrr.verify_workspace(ctx, 6, vocab, n, chains)
+            ws.fill_(0x3F)
+            rrr.verify_drafts(ctx, logits, tokens, ints(cu), u, path, counts, following, ws, draft=draft,
+                              temperature=torch.full((n,), heat, device="cuda"))
+            assert ctx.device_error() == 6
+            assert all(-1 <= t < vocab for t in following.tolist()) and all(0 <= c <= 6 for c in counts.tolist())
+
+
+@pytest.mark.gpu
+def test_steps_on_two_streams_at_once(rrr, ctx):
+    """Each stream has its cache and its workspaces: the bits of the calls made one after another."""
+    hd, nh, nkv, vocab, lens, nodes = 128, 6, 2, 5000, [900, 33, 2000], [7, 1, 12]
+    rng, jobs = np.random.default_rng(3), []
+    for seed in range(2):
+        g, cu, total = gen(40 + seed), cu_of(nodes), sum(nodes)
+        cache = Cache(rrr, ctx, nkv, hd, [n + 16 for n in lens], 3)
+        cache.c.store(normal(g, sum(lens), nkv, hd), normal(g, sum(lens), nkv, hd), cu_of(lens), ints(lens))
+        trees = [random_tree(rng, n, "tree") for n in nodes]
+        qkv, factors, desc = append_inputs(rrr, g, total, nh, nkv, hd, 96, "bf16")
+        logits, _, tokens, u = verify_inputs(g, rng, vocab, trees, "f32", False)
+        jobs.append(dict(cache=cache, cu=cu, parents=ints([p for t in trees for p in t]), lens=ints(lens), qkv=qkv, desc=desc, factors=factors,
+                         q=normal(g, total, nh, hd, dtype=torch.bfloat16), k=normal(g, total, nkv, hd, dtype=torch.bfloat16),
+                         v=normal(g, total, nkv, hd, dtype=torch.bfloat16), logits=logits, tokens=tokens, u=u, after=ints([n + 7 for n in lens]),
+                         path=torch.empty(total, dtype=torch.int32, device="cuda"), pages=cache.pages.clone()))
+    torch.cuda.synchronize()
+
+    def run(j, out):
+        j["cache"].c.attention_tree(j["q"], j["k"], j["v"], j["cu"], j["parents"], j["lens"], out["o"], out["ws"])
+        rrr.verify_drafts(ctx, j["logits"], j["tokens"], j["cu"], j["u"], out["path"], out["counts"], out["next"], out["vws"], parents=j["parents"])
+        j["cache"].c.append(j["desc"], j["qkv"], j["cu"], j["after"], path=out["path"], counts=out["counts"])
+
+    def fresh(j):
+        total, i = j["q"].shape[0], dict(dtype=torch.int32, device="cuda")
+        j["cache"].pages.copy_(j["pages"])
+        return dict(o=torch.zeros_like(j["q"]), ws=j["cache"].c.tree_workspace(nh, total), vws=rrr.verify_workspace(ctx, total, vocab, 3, False),
+                    path=torch.zeros(total, **i), counts=torch.zeros(3, **i), next=torch.zeros(3, **i))
+    want = []
+    for j in jobs:
+        out = fresh(j)
+        run(j, out)
+        want.append([out[x].clone() for x in ("o", "path", "counts", "next")] + [j["cache"].pages.clone()])
+    outs, streams = [fresh(j) for j in jobs], [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for j, out, stream in zip(jobs, outs, streams):
+            with torch.cuda.stream(stream):
+                j["cache"].pages.copy_(j["pages"])
+                run(j, out)
+    torch.cuda.synchronize()
+    for j, out, w in zip(jobs, outs, want):
+        assert all(torch.equal(a, b) for a, b in zip([out[x] for x in ("o", "path", "counts", "next")] + [j["cache"].pages], w))
+    assert ctx.device_error() == 0
+
+
 # ------------------------------------------------------------------ together
 def step_of(rrr, ctx, cache, desc, halves, s, graph=False):
     """One step on device values alone: rotated rows of the trees, their attention, verification, the accepted rows
