@@ -34,7 +34,7 @@ namespace rrr {
 namespace {
 
 constexpr int kMaxHpk = 8, kMaxNodes = 128;
-constexpr float kNone = -3e38f;  // the maximum of no rows: finite, so that it may be subtracted from -inf
+constexpr float kNone = -3e38f;  // the reference of no rows: finite, so that it may be subtracted from -inf
 constexpr int kRows = 128;       // KV rows of a block: two pages, or the drafted rows
 constexpr int kStart = 6;        // units in front of a segment's blocks
 constexpr int kGroups = 4;       // of four softmax warps each: group h takes the columns 8 h .. + 7 of every 8 kGroups
@@ -470,6 +470,21 @@ __device__ __noinline__ void drafted_values(int tid, float lift, uint8_t* dst) {
   }
 }
 
+// The first block from blk on with a row on a page that exists, or else `last`. (A part begins with it, whose rows give the
+// maxima their first values: from 0 on they would only rise, and the weights of scores far below 0 are lost in f16.)
+__device__ __noinline__ int first_with_rows(const TreeParams& p, int seq, int len, int blk, int last) {
+  const int lane = threadIdx.x & 31, pages = (len + kPageRows - 1) / kPageRows;
+#pragma unroll 1
+  for (; blk < last; blk += 16) {
+    const int at = 2 * blk + lane;
+    const int id = at < min(pages, 2 * last) ? p.table[(int64_t)seq * p.table_stride + at] : 0;
+    if (id < 0 || id >= p.n_pages) flag_position(p.err);
+    const unsigned there = __ballot_sync(0xffffffffu, at < min(pages, 2 * last) && id >= 0 && id < p.n_pages);
+    if (there) return blk + (__ffs(there) - 1) / 2;
+  }
+  return last;
+}
+
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ TreeParams p) {
@@ -600,9 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int seg0 = base + g * each + kStart;  // unit of the segment's block 0
       stop = s >= p.n_seqs || seg0 + blk >= u1;
-      const bool draft = blk + 1 == sh.blocks;
       Info& f = infos[it % kInfos];
       if (begin || stop) {
+        if (!stop) blk = first_with_rows(p, s, sh.len, blk, min(sh.blocks, u1 - seg0) - 1);
         kv = stop ? 0 : g / sh.tiles;
         c0 = (g - kv * sh.tiles) * sh.per;
         cols = min(sh.per, sh.nodes * p.hpk - c0);
@@ -637,6 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      const bool draft = blk + 1 == sh.blocks;
       // the numbers of the next 32 pages, one per lane
       if (!stop && !draft && (begin || 2 * blk + 2 > ids_at + 32)) {
         ids_at = 2 * blk;
@@ -1151,7 +1167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (mine < n) {
             float m = fmaxf(fmaxf(quad[0][mine], quad[1][mine]), fmaxf(quad[2][mine], quad[3][mine])) - kBias;
             if (!first) m = fmaxf(m, 0.f);
-            if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, or a score that is not finite)
+            if (!(fabsf(m) < 1e37f)) m = 0.f;  // (no row, of which the second kernel knows by the sum, or a score that is not finite)
             change[mine] = ex2(-m);
             line[NT + mine] -= m;
           }
@@ -1307,7 +1323,10 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
       }
       float next = top;
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (!(st[k].y > 0.f)) st[k].x = kNone;  // (no row of this part counts for the column)
+        next = fmaxf(next, st[k].x);
+      }
       const float keep = ex2(top - next);
       top = next;
       sum *= keep;
