@@ -472,10 +472,35 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
   for (int i = threadIdx.x; i < n; i += kWalkThreads) p.path[r0 + i] = i < count ? i : -1;
 }
 
-// max(p - q, 0) of token i where a chain ends
-template <typename T>
-__device__ __forceinline__ double rest_of(const T* x, const T* y, int i, const Ending& e, double c) {
-  return fmax(share(to_f32(x[i]), e.pm, e.pz, c) - share(to_f32(y[i]), e.qm, e.qz, c), 0.);
+// max(p - q, 0) of tokens where a chain ends, from their logits. The sums of chunks and the draw inside one are of the same
+// terms, so that a chunk with a sum has a term to be drawn. power() gives values 1000 binary orders under the top, masked ones
+// too, 2^-1000: beside a p of 2^-940 and more that is no q, and a smaller p is taken as it is, 0 where it is masked.
+struct Rest {
+  Powers wp, wq;
+  double sp, sq;
+  float faint, none;  // x whose p is under 2^-940 of the top's, and 0 in 64 bits
+  bool fast;
+};
+__device__ __forceinline__ Rest rest_from(const Ending& e, double c) {
+  Rest r;
+  r.wp = powers_of(e.pm, c);
+  r.wq = powers_of(e.qm, c);
+  r.sp = 1. / e.pz;
+  r.sq = 1. / e.qz;
+  r.faint = __double2float_ru(r.wp.top - 940. / c);
+  r.none = __double2float_rd(r.wp.top - 1080. / c);
+  // (tops of FLT_MAX may stand for infinities)
+  r.fast = r.wp.fine && r.wq.fine && e.pm < FLT_MAX && e.qm < FLT_MAX;
+  return r;
+}
+__device__ __noinline__ double rest_apart(float x, float y, const Ending& e, double c) {
+  return fmax(share(x, e.pm, e.pz, c) - share(y, e.qm, e.qz, c), 0.);
+}
+// (with r.fast; the products rounded each by itself, so that of equal ones nothing is left)
+__device__ __forceinline__ double rest_of(const Rest& r, const double* table, float x, float y, const Ending& e, double c) {
+  const double d = fmax(__dmul_rn(power(r.wp, table, x), r.sp) - __dmul_rn(power(r.wq, table, y), r.sq), 0.);
+  if (x <= r.faint && x > r.none) return rest_apart(x, y, e, c);
+  return x > r.faint ? d : 0.;
 }
 template <typename T>
 __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __grid_constant__ VerifyParams p) {
@@ -493,10 +518,8 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
   const T* y = static_cast<const T*>(p.draft) + (int64_t)(r0 + e.last + 1) * p.draft_stride;
   double sum = 0.;
   const int first = chunk * kRestChunk, end = min(p.vocab, first + kRestChunk);
-  const Powers wp = powers_of(e.pm, c), wq = powers_of(e.qm, c);
-  // (tops of FLT_MAX may stand for infinities)
-  if (wp.fine && wq.fine && e.pm < FLT_MAX && e.qm < FLT_MAX) {
-    const double sp = 1. / e.pz, sq = 1. / e.qz;
+  const Rest rest = rest_from(e, c);
+  if (rest.fast) {
     constexpr int kStep = 8;
 #pragma unroll 1
     for (int i0 = first + lane; i0 < end; i0 += 32 * kStep) {
@@ -508,11 +531,11 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
         b[k] = i < end ? to_f32(y[i]) : -INFINITY;
       }
 #pragma unroll
-      for (int k = 0; k < kStep; ++k) sum += fmax(power(wp, table, a[k]) * sp - power(wq, table, b[k]) * sq, 0.);
+      for (int k = 0; k < kStep; ++k) sum += rest_of(rest, table, a[k], b[k], e, c);
     }
   } else {
 #pragma unroll 1
-    for (int i = first + lane; i < end; i += 32) sum += rest_of(x, y, i, e, c);
+    for (int i = first + lane; i < end; i += 32) sum += rest_apart(to_f32(x[i]), to_f32(y[i]), e, c);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -521,6 +544,8 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
 template <typename T>
 __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ Shared sh;
+  __shared__ double table[16];
+  fill_table(table);
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.x;
@@ -537,7 +562,11 @@ __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_
         const T* x = static_cast<const T*>(p.logits) + (int64_t)(r0 + e.last) * p.logits_stride;
         const T* y = static_cast<const T*>(p.draft) + (int64_t)(r0 + e.last + 1) * p.draft_stride;
         const int first = chunk * kRestChunk, end = min(p.vocab, first + kRestChunk);
-        const int got = draw(sh, end - first, -1., goal, before, [&](int i) { return rest_of(x, y, first + i, e, c); }, nullptr);
+        const Rest terms = rest_from(e, c);
+        const int got = draw(sh, end - first, -1., goal, before, [&](int i) {
+          const float v = to_f32(x[first + i]), w = to_f32(y[first + i]);
+          return terms.fast ? rest_of(terms, table, v, w, e, c) : rest_apart(v, w, e, c);
+        }, nullptr);
         if (got >= 0) token = first + got;
       }
     }

@@ -1,5 +1,5 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
-sequence without any row that exists.
+sequence without any row that exists, tokens that both distributions mask.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
 import math
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_serving import DT, U, Cache, cu_of, gen, half_step, ints, normal, within
-from test_speculative import H16, ref_tree
+from test_speculative import H16, check_verify, ref_tree
 
 
 # ------------------------------------------------------------------ tree
@@ -59,3 +59,46 @@ def test_attention_tree_of_rows_behind_missing_pages(rrr, ctx, hd, kind, low, ma
         bound = (2 * torch.expm1(2 * (hd + 16) * U * A) + 2 * H16 + h + 64 * U) * top
         within(out[r], ref, ref.abs() * h * 1.01 + bound[..., None] + 2.0 ** -25)
         a += n
+
+
+# ------------------------------------------------------------------ verify
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("mask", ["inf", "nan", "lowest"])
+def test_verify_drafts_of_masked_tokens(rrr, ctx, kind, mask):
+    """Tokens that target and draft both mask are never drawn, and a refused draft's rest is drawn from its own tokens at u = 0
+    too, wherever the distributions' sums lie."""
+    t, vocab = DT[kind], 6000
+    none = {"inf": -math.inf, "nan": math.nan, "lowest": torch.finfo(t).min}[mask]
+
+    def row(at):
+        x = torch.full((vocab,), none, device="cuda", dtype=torch.float32).to(t)
+        for i, p in at.items():
+            x[i] = p
+        return x
+    log = math.log
+    for first in (1500, 3, 2047):  # tokens a < b < c, those before them masked by both
+        a, b, c = first, 3500, 5200
+        cases = [({a: log(0.4), b: log(0.6)}, {a: log(0.5), c: log(0.5)}, c),  # b alone is left
+                 ({a: 0.0, b: 9.0}, {a: 1.0, c: 30.0}, c), ({a: -7.0, b: -7.0, 4999: -9.0}, {a: -5.0, c: -5.0}, c),
+                 ({a: 0.0, b: 0.0}, {a: 3.0, c: 0.0}, c), ({b: 0.0}, {c: 0.0}, c), ({a: 0.0, b: 3.0}, {a: 0.0, b: 0.0}, a)]
+        for p, q, token in cases:
+            for u1 in (0.0, 2.0 ** -24, 0.5):
+                u = torch.tensor([[0.0, u1], [1 - 2.0 ** -24, u1]], device="cuda")
+                for heat in (1.0, 3.0):
+                    check_verify(rrr, ctx, torch.stack([row(p), row(p)]), torch.stack([row(q), row(q)]), ints([0, token]), u,
+                                 [[-1, 0]], [heat])
+                check_verify(rrr, ctx, torch.stack([row(p), row(q)]), None, ints([0, token]), u, [[-1, 0]], [1.0])
+
+
+@pytest.mark.gpu
+def test_verify_drafts_of_faint_tokens(rrr, ctx):
+    """Weights of 2^-1010 are weights: at u = 0 the first of them is drawn."""
+    vocab = 6000
+    x, y = (torch.full((2, vocab), -math.inf, device="cuda") for _ in range(2))
+    x[:, 1200], x[:, 3000], x[:, 3001] = -700.0, 0.0, -1.0  # e^-700 = 2^-1010
+    y[:, 3000], y[:, 5000] = 0.0, 1.0
+    u = torch.tensor([[0.0, 0.0], [0.5, 0.0]], device="cuda")
+    got = check_verify(rrr, ctx, x, y, ints([0, 5000]), u, [[-1, 0]], [1.0])
+    assert got[2] == [1200]
+    assert check_verify(rrr, ctx, x, None, ints([0, 5]), u, [[-1, 0]], [1.0])[2] == [1200]
