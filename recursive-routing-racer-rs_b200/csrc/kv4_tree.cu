@@ -293,7 +293,7 @@ struct Sizes {
   static constexpr int kVs = HD > 128 ? 1 : 2;      // places for V
   static constexpr int kP = (NT + 63) / 64 * kRows * 128;
   static constexpr int kFixed = kQ + kVs * kV + 2 * kP;
-  static constexpr int kStatic = 17 * 1024;         // more than the static shared memory
+  static constexpr int kStatic = 18 * 1024;         // more than the static shared memory
   static constexpr int kFit = (227 * 1024 - kStatic - 1024 - kFixed) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kFixed + kStages * kStage + 1024;
@@ -485,6 +485,37 @@ __device__ __noinline__ int first_with_rows(const TreeParams& p, int seq, int le
   return last;
 }
 
+// The segments of a CTA's own whose bits are set, in 32 bits, a warp per column. All warps come here when the roles are done:
+// the rows may take longer than a role waits.
+constexpr int kBits = 1024;  // segments of a CTA with a bit each; those from the last on share it
+template <int HD, int NT, typename T>
+__device__ __noinline__ void compute_again(const TreeParams& p, int s, int base, int units, const uint32_t* bits) {
+  const int warp = threadIdx.x >> 5;
+  const Share share{units / (int)gridDim.x, units % (int)gridDim.x};
+  const int u0 = share.first(blockIdx.x), u1 = share.first(blockIdx.x + 1);
+  Shape sh = shape_of<NT>(p, s);
+  int each = sh.blocks + kStart, g = (u0 - base) / each, blk = max(0, (u0 - base) % each - kStart);
+#pragma unroll 1
+  for (int count = 0; base + g * each + kStart + blk < u1; ++count, blk = 0) {
+    const int seg0 = base + g * each + kStart, bit = min(count, kBits - 1), cta = (int)blockIdx.x;
+    if (((bits[bit >> 5] >> (bit & 31)) & 1u) && share.cta_of(seg0) == cta && share.cta_of(seg0 + sh.blocks - 1) == cta) {
+      const int kv = g / sh.tiles, c0 = (g - kv * sh.tiles) * sh.per, end = min(c0 + sh.per, sh.nodes * p.hpk);
+#pragma unroll 1
+      for (int c = c0 + warp; c < end; c += kThreads / 32)
+        plain_row<HD, T>(p, s, sh.r0, sh.len, sh.r0 + c / p.hpk, kv, kv * p.hpk + c % p.hpk);
+    }
+    if (++g >= sh.tiles * p.nkv) {
+      g = 0;
+      base += units_of(p, sh);
+      do {
+        if (++s >= p.n_seqs) return;
+        sh = shape_of<NT>(p, s);
+      } while (sh.nodes == 0);
+      each = sh.blocks + kStart;
+    }
+  }
+}
+
 template <int HD, int NT, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ TreeParams p) {
@@ -507,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t v_tops[4];
   __shared__ __align__(16) float lines[4][2 * NT];  // of a column c: the argument of a weight's exponential is score * [c] + [NT + c]
   __shared__ float quad[4][NT], change[NT];
-  __shared__ int warp_units[kThreads / 32], first_base, first_seq, dead[kGroups];
+  __shared__ int warp_units[kThreads / 32], first_base, first_seq, all_units, dead[kGroups];
+  __shared__ uint32_t again[kBits / 32];  // a bit per segment of the CTA's own that f16 did not hold
   __shared__ uint32_t tmem_slot;
   uint8_t* smem = smem_dyn + ((1024u - (smem_addr(smem_dyn) & 1023u)) & 1023u);
   uint8_t* const qs = smem;
@@ -537,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbarrier_init();
     prefetch_map(&map);
   }
+  if (threadIdx.x < kBits / 32) again[threadIdx.x] = 0;
   if (warp == kSWarp) tmem_alloc(&tmem_slot, 512);
   pdl_launch_dependents();
   pdl_wait();
@@ -575,6 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     first_seq = s;
     first_base = base;
+    all_units = U;
   }
   __syncthreads();
   // Every wait is bounded; a role that gave up leaves, and so do those that wait for it.
@@ -1256,19 +1290,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // what came out not finite, or may owe its value to an infinity of f16, is computed again
+      // what came out not finite, or may owe its value to an infinity of f16, is computed again: by the CTA at its end, or by
+      // the second kernel
       bad = any_of_128(bar, bad);
       if (!alone) {
         if (r == 0) {
           p.again[kGroups * slot + h] = bad;
           if (h == 0 && (flags & kOpens)) p.opened[blockIdx.x] = Opened{f.run, f.seq, f.kv, f.r0, f.len, f.c0, f.cols, 0};
         }
-      } else if (bad) {
-        for (int x = 8 * h; x < f.cols; x += 8 * kGroups)
-          for (int c = x + qd; c < min(x + 8, f.cols); c += 4) {
-            const int token = (f.c0 + c) / p.hpk;
-            plain_row<HD, T>(p, f.seq, f.r0, f.len, f.r0 + token, f.kv, f.kv * p.hpk + (f.c0 + c) - token * p.hpk);
-          }
+      } else if (bad && r == 0) {
+        const int bit = min(f.count, kBits - 1);
+        atomicOr(&again[bit >> 5], 1u << (bit & 31));
       }
       tc_fence_before();
       __syncwarp();
@@ -1282,6 +1314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (__any_sync(0xffffffffu, again[lane] != 0)) compute_again<HD, NT, T>(p, first_seq, first_base, all_units, again);
 }
 
 // Joins the parts of the segment that a CTA opened and others share, in the order of the CTAs; where f16 did not hold

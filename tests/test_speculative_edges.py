@@ -1,5 +1,5 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
-sequence without any row that exists, tokens that both distributions mask.
+sequence without any row that exists, rows that are computed again, tokens that both distributions mask.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
 import math
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from test_serving import DT, U, Cache, cu_of, gen, half_step, ints, normal, within
-from test_speculative import H16, check_verify, ref_tree
+from test_speculative import H16, check_verify, compare_tree, ref_tree
 
 
 # ------------------------------------------------------------------ tree
@@ -59,6 +59,46 @@ def test_attention_tree_of_rows_behind_missing_pages(rrr, ctx, hd, kind, low, ma
         bound = (2 * torch.expm1(2 * (hd + 16) * U * A) + 2 * H16 + h + 64 * U) * top
         within(out[r], ref, ref.abs() * h * 1.01 + bound[..., None] + 2.0 ** -25)
         a += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,kind", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+def test_attention_tree_computed_again_outlasts_the_waits(rrr, ctx, hd, kind):
+    """Rows that are computed again take longer than a role may wait for another: every CTA has two sequences of its own, the
+    first of some with an infinity, and all of the others' results are there."""
+    t, g, n, limit_us = DT[kind], gen(hd), 20000, 2000
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    seqs, nodes, per = 2 * sms, 3, -(-n // 64)
+    one = Cache(rrr, ctx, 1, hd, [n], 3)
+    k, v = 0.2 * normal(g, n, 1, hd), normal(g, n, 1, hd)
+    one.c.store(k, v, cu_of([n]), ints([n]))
+    one.c.load(cu_of([n]), ints([n]), k, v)
+    cache = rrr.KV4Cache(ctx, one.pages, one.c.page_table.expand(seqs, per).contiguous(), hd)  # one sequence's rows for all
+    rows = seqs * nodes
+    q, kd, vd = (normal(g, rows, 1, hd, dtype=t) for _ in range(3))
+    bad = list(range(0, seqs, 6))
+    vd[[nodes * s + 1 for s in bad], :, hd // 2] = math.inf  # of row 1: rows 0 and 2 do not see it
+    out, tree = torch.full((rows, 1, hd), 7.0, dtype=t, device="cuda"), [-1, 0, 0]
+    ws = cache.tree_workspace(1, rows)
+    ctx.check(rrr.ffi.lib().rrr_set_wait_limit(ctx.h, limit_us * 1000))
+    try:
+        events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        events[0].record()
+        cache.attention_tree(q, kd, vd, cu_of([nodes] * seqs), ints(tree * seqs), ints([n] * seqs), out, ws)
+        events[1].record()
+        torch.cuda.synchronize()
+    finally:
+        ctx.check(rrr.ffi.lib().rrr_set_wait_limit(ctx.h, 0))
+    assert ctx.device_error() == 0
+    assert events[0].elapsed_time(events[1]) * 1000 > limit_us  # (or the test shows nothing)
+    for s in [*bad[:3], 1, 2, 3, seqs - 2, seqs - 1]:
+        r = slice(nodes * s, nodes * (s + 1))
+        if s in bad:
+            assert bool(out[nodes * s + 1].isfinite().logical_not().any())
+            clean, parents = [nodes * s, nodes * s + 2], [-1, 0]
+        else:
+            clean, parents = list(range(r.start, r.stop)), tree
+        compare_tree(out[clean], q[clean], kd[clean], vd[clean], k, v, [n], [parents], kind, hd ** -0.5)
 
 
 # ------------------------------------------------------------------ verify
