@@ -8,8 +8,8 @@
 // by a product with ones, so that they are the sums of what V is multiplied by. m is taken
 // over anew where a weight would pass 2^15. Who sees whom in the drafted block is a bit mask per row. A
 // query, and a drafted key, is scaled by a power of two, drafted values together by one, so
-// that f16 operands hold both 16-bit types. A result that is not finite, or a cached group that f16 does
-// not hold, is computed again row by row in 32 bits.
+// that f16 operands hold both 16-bit types. A result that is not finite, and one that may owe something to a cached group or
+// a drafted row that f16 does not hold, is computed again row by row in 32 bits.
 //
 // Layout. One CTA per SM and an equal run of blocks for each; a sequence's share that crosses the border of two CTAs is
 // joined by a second kernel, in order. Keys are dequantised, a row per thread, straight into TMEM (operand A), values
@@ -263,10 +263,16 @@ __device__ __forceinline__ float to_one(uint32_t top) {
   const int e = (int)(top >> 23);  // (a subnormal top counts as 2^-126)
   return e == 255 || top == 0 ? 1.f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
 }
-// Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, so that f16 holds them with all their bits (and
-// their rows' weights are divided by it, which have bits to spare)
-__device__ __forceinline__ int lift_of(uint32_t top) { return top >= 0x3b000000u /* 2^-9 */ ? 0 : top >= 0x37000000u /* 2^-17 */ ? 1 : 2; }
+// Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, as far as f16 allows, so that it holds those of rows
+// that are 2^20 times smaller with all their bits too (and their rows' weights are divided by it, which have bits to spare)
+__device__ __forceinline__ int lift_of(uint32_t top) { return top >= 0x43000000u /* 2^7 */ ? 0 : top >= 0x3f800000u /* 1 */ ? 1 : 2; }
 __device__ __forceinline__ float lifted_by(int lift) { return lift == 0 ? 1.f : lift == 1 ? 256.f : 32768.f; }
+// Whether a row of values up to `top` loses bits all the same: its largest is no normal f16. (Who sees that row alone, or with
+// others like it, is computed again.) An f16 row has no bits to lose.
+template <typename T>
+__device__ __forceinline__ bool too_small(uint32_t top, int lift) {
+  return !std::is_same<T, __half>::value && top != 0 && top < (lift == 0 ? 0x38800000u : lift == 1 ? 0x34800000u : 0x31000000u);
+}
 // Eight 16-bit values times s as f16, in the order (0,4) (1,5) (2,6) (3,7) in which a word of K's codes comes apart
 template <typename T>
 __device__ __forceinline__ void scaled_pairs(const uint4& w, float s, uint32_t (&x)[4]) {
@@ -424,14 +430,14 @@ __device__ __noinline__ void drafted_keys(const TreeParams& p, const Info& f, in
   }
 }
 // Drafted values: a thread has rows 8 o .. + 7 (o = tid % 16) of values 8 (tid / 16 + 8 c) .. + 7, eight rows of 16 bytes
-// which become eight values of 16 bytes. The rows into shared memory, to the values' places; the largest of their bits.
+// which become eight values of 16 bytes. The rows into shared memory, to the values' places; the largest bits of row tid.
 template <int HD>
 __device__ __forceinline__ uint8_t* value_place(uint8_t* dst, int o, int e) {
   constexpr int kERows = HD < 128 ? HD : 128;
   return dst + ((e >> 7) * 2 + (o >> 3)) * kERows * 128 + (e & 127) * 128 + (((o & 7) ^ (e & 7)) << 4);
 }
 template <int HD, typename T>
-__device__ __noinline__ uint32_t drafted_rows(const TreeParams& p, const Info& f, int tid, uint8_t* dst) {
+__device__ __noinline__ void drafted_rows(const TreeParams& p, const Info& f, int tid, uint8_t* dst) {
   const int o = tid & 15, e0 = 8 * (tid >> 4);
   const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head + (int64_t)f.r0 * p.v_row + e0;
 #pragma unroll 1
@@ -441,11 +447,13 @@ __device__ __noinline__ uint32_t drafted_rows(const TreeParams& p, const Info& f
   }
   cp_async_commit();
   cp_async_wait<0>();
+}
+template <int HD, typename T>
+__device__ __noinline__ uint32_t row_top(int tid, uint8_t* dst) {
   uint32_t top = 0;
 #pragma unroll 1
-  for (int x = 0; x < HD / 8; ++x)
-    top = max(top, top_bits<T>(*reinterpret_cast<const uint4*>(value_place<HD>(dst, o, e0 + 64 * (x / 8) + x % 8))));
-  return __reduce_max_sync(0xffffffffu, top);
+  for (int e = tid & 7; e < HD; e += 8) top = max(top, top_bits<T>(*reinterpret_cast<const uint4*>(value_place<HD>(dst, tid >> 3, e))));
+  return top;
 }
 // The values of the rows there, lifted
 template <int HD, typename T>
@@ -534,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int up[kMaxNodes];
   __shared__ float k_scale[4][kRows];
   __shared__ int v_lift[4];
-  __shared__ int k_again[4];
+  __shared__ int k_again[4], v_again[4];
   __shared__ uint32_t v_tops[4];
   __shared__ __align__(16) float lines[4][2 * NT];  // of a column c: the argument of a weight's exponential is score * [c] + [NT + c]
   __shared__ float quad[4][NT], change[NT];
@@ -882,16 +890,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         if (!free_place()) break;
-        uint32_t top = drafted_rows<HD, T>(p, f, tid, dst);
-        if (lane == 0) v_tops[warp & 3] = top;
+        drafted_rows<HD, T>(p, f, tid, dst);
+        if (tid == 0) v_again[(flags >> 8) & 3] = 0;
         if (!team()) break;
-        top = max(max(v_tops[0], v_tops[1]), max(v_tops[2], v_tops[3]));
+        const uint32_t mine = row_top<HD, T>(tid, dst), most = __reduce_max_sync(0xffffffffu, mine);
+        if (lane == 0) v_tops[warp & 3] = most;
+        if (!team()) break;
+        const int lift = lift_of(max(max(v_tops[0], v_tops[1]), max(v_tops[2], v_tops[3])));
         if (tid == 0) {
-          v_lift[(flags >> 8) & 3] = lift_of(top);
+          v_lift[(flags >> 8) & 3] = lift;
           mbar_arrive(&lifted[(flags >> 8) & 3]);
         }
-        drafted_values<HD, T>(tid, lifted_by(lift_of(top)), dst);
-        if (!team()) break;  // v_tops is read
+        if (too_small<T>(mine, lift)) v_again[(flags >> 8) & 3] = 1;
+        drafted_values<HD, T>(tid, lifted_by(lift), dst);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -1243,7 +1254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const bool alone = flags & kAlone;
       const int slot = 2 * blockIdx.x + (flags & kOpens ? 1 : 0);
-      bool bad = k_again[par] != 0;
+      bool bad = k_again[par] != 0 || ((flags & kDraft) && v_again[par] != 0);
       if (qd * 32 < S::kERows) {
 #pragma unroll 1
         for (int k = 0; k < S::kHalves; ++k) {

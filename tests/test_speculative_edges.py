@@ -1,5 +1,6 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
-sequence without any row that exists, rows that are computed again, tokens that both distributions mask.
+sequence without any row that exists, rows that are computed again, drafted values of
+very different sizes, tokens that both distributions mask.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
 import math
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 from test_serving import DT, U, Cache, cu_of, gen, half_step, ints, normal, within
-from test_speculative import H16, check_verify, compare_tree, ref_tree
+from test_speculative import H16, ancestors, check_verify, compare_tree, ref_tree
 
 
 # ------------------------------------------------------------------ tree
@@ -99,6 +100,33 @@ def test_attention_tree_computed_again_outlasts_the_waits(rrr, ctx, hd, kind):
         else:
             clean, parents = list(range(r.start, r.stop)), tree
         compare_tree(out[clean], q[clean], kd[clean], vd[clean], k, v, [n], [parents], kind, hd ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 8, 1), (128, 6, 2), (256, 3, 1)])
+@pytest.mark.parametrize("small,large", [(1e-6, 1.0), (1e-4, 1e4), (1e-9, 1.0), (1e-30, 1e-9), (1e-12, 1e30)])
+@pytest.mark.parametrize("n", [0, 70])
+def test_attention_tree_of_small_values_beside_large_ones(rrr, ctx, hd, nh, nkv, small, large, n):
+    """Drafted values of bf16 rows that differ by many powers of two: a row's result owes nothing to the rows that it does not
+    see. (Weights of all equal scores; cached values of zero.)"""
+    t, g = torch.bfloat16, gen(hd)
+    cache = Cache(rrr, ctx, nkv, hd, [max(n, 1)], 3)
+    if n:
+        cache.c.store(torch.zeros(n, nkv, hd, device="cuda"), torch.zeros(n, nkv, hd, device="cuda"), cu_of([n]), ints([n]))
+    tree = [-1, 0, 0, 1, 2, 0]
+    sizes = torch.tensor([small, small, large, small, large, small], device="cuda")[:, None, None]
+    q, k = normal(g, 6, nh, hd, dtype=t), torch.zeros(6, nkv, hd, dtype=t, device="cuda")
+    v = (normal(g, 6, nkv, hd) * sizes).to(t)
+    v[5] = 0  # (nothing at all is no small value)
+    out = torch.empty(6, nh, hd, dtype=t, device="cuda")
+    cache.c.attention_tree(q, k, v, cu_of([6]), ints(tree), ints([n]), out, cache.c.tree_workspace(nh, 6))
+    zero = torch.zeros(n, nkv, hd, dtype=torch.float64, device="cuda")
+    ref, _, _ = ref_tree(q.double(), k.double(), v.double(), zero, zero, tree, hd ** -0.5)
+    h = half_step(t)
+    for i, seen in enumerate(ancestors(tree)):
+        top = float(v[seen].abs().max())
+        within(out[i], ref[i], ref[i].abs() * h * 1.01 + (2 * H16 + 64 * U) * top)
+    assert ctx.device_error() == 0
 
 
 # ------------------------------------------------------------------ verify
