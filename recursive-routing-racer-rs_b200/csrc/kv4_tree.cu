@@ -941,9 +941,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         turns ^= 1u << (i % kInfos);
         if (!(f.flags & kStop)) {
           const int par = (f.flags >> 8) & 3;
-          if (r == 0) k_again[par] = 0;
-          // S of the segment before has read its queries
+          // S of the segment before has read its queries, so that weights three blocks before are there, and the end of a
+          // segment four before, which has read what lies in the same place
           if (i > 0 && !doze(&s_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1u)) break;
+          if (r == 0) k_again[par] = 0;
           queries<HD, NT, T>(p, f, r, qs, lines[par]);
           fence_proxy_async_smem();
           if (!team()) break;

@@ -129,6 +129,28 @@ def test_attention_tree_of_small_values_beside_large_ones(rrr, ctx, hd, nh, nkv,
     assert ctx.device_error() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv", [(64, 4, 2), (128, 3, 1), (256, 2, 1)])
+def test_attention_tree_groups_beyond_f16_among_short_sequences(rrr, ctx, hd, nh, nkv):
+    """Every fourth sequence has a key that f16 does not hold and whose score counts, between sequences of drafted rows alone:
+    what is noted of one segment is read before the fourth one after it takes its place."""
+    g, seqs, nodes = gen(hd), 1200, 2
+    lens = [70 if s % 4 == 0 else 0 for s in range(seqs)]
+    cache, cu = Cache(rrr, ctx, nkv, hd, [70] * seqs, 3), cu_of(lens)
+    k, v = normal(g, sum(lens), nkv, hd) * 1e-4, normal(g, sum(lens), nkv, hd)
+    k[5::70, :, 3], k[5::70, :, 4] = -6e4, 2e5
+    cache.c.store(k, v, cu, ints(lens))
+    cache.c.load(cu, ints(lens), k, v)
+    rows = seqs * nodes
+    q, kd, vd = (normal(g, rows, n, hd, dtype=torch.bfloat16) * s for n, s in ((nh, 1e-4), (nkv, 1.0), (nkv, 1.0)))
+    out = torch.empty(rows, nh, hd, dtype=torch.bfloat16, device="cuda")
+    cache.c.attention_tree(q, kd, vd, cu_of([nodes] * seqs), None, ints(lens), out, cache.c.tree_workspace(nh, rows))
+    some = [s for s in range(seqs) if s % 4 == 0 or s < 40]
+    r = [nodes * s + i for s in some for i in range(nodes)]
+    compare_tree(out[r], q[r], kd[r], vd[r], k, v, [lens[s] for s in some], [[-1, 0]] * len(some), "bf16", hd ** -0.5)
+    assert ctx.device_error() == 0
+
+
 # ------------------------------------------------------------------ verify
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
