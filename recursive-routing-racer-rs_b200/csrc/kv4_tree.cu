@@ -41,6 +41,7 @@ constexpr int kGroups = 4;       // of four softmax warps each: group h takes th
 constexpr int kKWarp = 4 * kGroups, kVWarp = kKWarp + 4, kSWarp = kVWarp + 4, kLoadWarp = kSWarp + 1, kPVWarp = kSWarp + 2;
 constexpr int kThreads = 32 * (kSWarp + 4);
 constexpr int kInfos = 16;
+constexpr int kSumBlocks = 128;  // a power of two: blocks after which the sums in TMEM are moved out
 constexpr int kNap = 100;        // ns
 constexpr float kBias = 10.f;    // weights are 2^(s - m + kBias), at most 2^(kBias + kLazy)
 constexpr float kLazy = 5.f;
@@ -67,6 +68,8 @@ struct TreeParams {
   float2* stats;          // [slot][column]: maximum, sum
   int* again;             // [slot][group of columns]
   float* parts;           // [slot][column][value]
+  float2* held_stats;     // [CTA][quarter][column]: reference and sum of the weights moved out
+  float* held;            // [CTA][column][value]
 };
 struct Opened {
   int run, seq, kv, r0, len, c0, cols, pad;  // run: CTAs that share it, 0 for none
@@ -110,13 +113,15 @@ struct Share {
   }
 };
 
-enum { kDraft = 1, kFirst = 2, kLast = 4, kAlone = 8, kStop = 16, kOpens = 32 };
+// kOut: the sums are moved out after it; kAnew: they begin with it; kHeld: some of the segment's have been moved out before
+enum { kDraft = 1, kFirst = 2, kLast = 4, kAlone = 8, kStop = 16, kOpens = 32, kOut = 64, kAnew = 128, kHeld = 1024 };
 struct __align__(16) Info {  // of a block
   int flags;                // and the segment's number modulo 4 from bit 8 on
   int n, valid[2];          // columns with the padding; rows of each page that count
   int c0, cols, kv, count;  // the tile's columns c0 .. c0 + cols - 1 of the sequence's (row, head) pairs; the segment's number in this CTA
   int r0, nodes, seq, len;
   int run;                  // CTAs that share the segment
+  int outs;                 // how often the sums in TMEM have been read so far
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -493,6 +498,45 @@ __device__ __noinline__ int first_with_rows(const TreeParams& p, int seq, int le
   return last;
 }
 
+// The tensor core cuts off what does not fit a sum's 24 bits, eight or sixteen times a block and always towards zero: over
+// 131,000 rows of one CTA's the results of f16 rows lost 4e-4, over 400,000 2.2e-3. So sums of kSumBlocks blocks are added up in
+// memory, and come back to TMEM at the segment's end: sums in TMEM and those held become one, there or here. By the softmax
+// warps, each its own columns and values, a column at a time (eight at once were 12 us slower for 60 rows on 131,000, whose
+// instructions come from far away).
+template <int HD, int NT>
+__device__ __noinline__ void move_sums(const TreeParams& p, const Info& f, const float* line, uint32_t tmem) {
+  using S = Sizes<HD, NT>;
+  const int lane = threadIdx.x & 31, h = threadIdx.x >> 7, qd = (threadIdx.x >> 5) & 3;
+  const bool out = f.flags & kOut, held = f.flags & kHeld;
+  const uint32_t sub = (uint32_t)(32 * qd) << 16;
+  float2* const stats = p.held_stats + (blockIdx.x * 4 + qd) * NT;
+#pragma unroll 1
+  for (int x = 8 * h; x < f.cols; x += x % 8 == 7 ? 8 * kGroups - 7 : 1) {
+    uint32_t l, o;
+    const float2 was = held ? stats[x] : make_float2(kNone, 0.f);
+    __syncwarp();
+    tmem_ld1(tmem + S::kLCol + x + sub, l);
+    const float m = kBias - line[NT + x], keep = ex2(was.x - m), sum = fmaf(was.y, keep, __uint_as_float(l));  // (a reference only rises)
+    if (!out) tmem_st1(tmem + S::kLCol + x + sub, __float_as_uint(sum));
+    else if (lane == 0) stats[x] = make_float2(sum > 0.f ? m : kNone, sum);
+    if (qd * 32 < S::kERows) {
+#pragma unroll 1
+      for (int k = 0; k < S::kHalves; ++k) {
+        float* const to = p.held + ((size_t)blockIdx.x * NT + x) * HD + 128 * k + 32 * qd + lane;
+        const float old = held ? *to : 0.f;
+        __syncwarp();
+        tmem_ld1(tmem + S::kOCol + k * NT + x + sub, o);
+        const float v = fmaf(old, keep, __uint_as_float(o));
+        if (out) *to = v;
+        __syncwarp();
+        if (!out) tmem_st1(tmem + S::kOCol + k * NT + x + sub, __float_as_uint(v));
+      }
+    }
+  }
+  tmem_wait_st();
+  __syncwarp();
+}
+
 // The segments of a CTA's own whose bits are set, in 32 bits, a warp per column. All warps come here when the roles are done:
 // the rows may take longer than a role waits.
 constexpr int kBits = 1024;  // segments of a CTA with a bit each; those from the last on share it
@@ -637,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = (u0 - base) / each, blk = max(0, (u0 - base) % each - kStart);
     int ids_at = 0, id = 0;  // page numbers of the segment
     int kv = 0, c0 = 0, cols = 0;
-    int the = 0, run = 0;  // (of lane 0) the segment's flags, its CTAs
+    int the = 0, run = 0, from = 0, outs = 0;  // (of lane 0) the segment's flags, its CTAs, its first block here
     bool begin = true, stop = false;
     uint32_t phase = 1;  // of the wait for a free stage: the first round finds them free
     for (;; ++it) {
@@ -720,7 +764,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (stop) {
           f.flags = kStop;
         } else {
-          f.flags = the | (draft ? kDraft : 0) | (begin ? kFirst : 0) | (draft || seg0 + blk + 1 >= u1 ? kLast : 0);
+          from = begin ? blk : from;
+          const int nth = (blk - from) % kSumBlocks;
+          const bool last = draft || seg0 + blk + 1 >= u1, out = !last && nth == kSumBlocks - 1;
+          f.flags = the | (draft ? kDraft : 0) | (begin ? kFirst : 0) | (last ? kLast : out ? kOut : 0) |
+                    (nth == 0 ? kAnew : 0);
+          the |= out ? kHeld : 0;
+          f.outs = outs;
+          outs += last || out;
           f.n = sh.per;
           f.valid[0] = v0;
           f.valid[1] = v1;
@@ -801,10 +852,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int2 head = *reinterpret_cast<const int2*>(&f);
       if (head.x & kStop) break;
       if (!wait(&p_full[i & 1], (uint32_t)(i >> 1) & 1u)) break;
-      if ((head.x & kFirst) && f.count > 0 && !wait(&o_empty, (uint32_t)(f.count - 1) & 1u)) break;
+      if ((head.x & kAnew) && f.outs > 0 && !wait(&o_empty, (uint32_t)(f.outs - 1) & 1u)) break;
       const uint32_t odd = __shfl_sync(0xffffffffu, i & 1, 0), flags = __shfl_sync(0xffffffffu, head.x, 0), n = __shfl_sync(0xffffffffu, head.y, 0);
       const uint32_t lift = __shfl_sync(0xffffffffu, flags & kDraft ? v_lift[(flags >> 8) & 3] : 0, 0);
-      const uint32_t idesc = kF16 | 1u << 16 | n >> 3 << 17, more = flags & kFirst ? 0u : 1u, ones = base + S::kOnes + 8u * lift;
+      const uint32_t idesc = kF16 | 1u << 16 | n >> 3 << 17, more = flags & kAnew ? 0u : 1u, ones = base + S::kOnes + 8u * lift;
       const uint64_t v = v_desc + (S::kVs == 2 ? odd * (S::kV >> 4) : 0u), w = p_desc + (kTwice ? 0u : odd * (S::kP >> 4));
       tc_fence_after();
       if (elect_one()) {
@@ -1247,12 +1298,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
-      if (!(flags & kLast)) continue;
+      if (!(flags & (kLast | kOut))) continue;
 
-      // ---------------- the end of the segment, in this CTA
+      // ---------------- the end of the segment, in this CTA, or of what the tensor core sums at a time
       // (where the wait gave up, the numbers are not the segment's, and the next vote ends the role)
       if (!wait(&p_empty[i & 1], (uint32_t)(i >> 1) & 1u)) dead[h] = 1;
       tc_fence_after();
+      if (flags & (kOut | kHeld)) move_sums<HD, NT>(p, f, line, tmem);
+      if (flags & kOut) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty);
+        continue;
+      }
       const bool alone = flags & kAlone;
       const int slot = 2 * blockIdx.x + (flags & kOpens ? 1 : 0);
       bool bad = k_again[par] != 0 || ((flags & kDraft) && v_again[par] != 0);
@@ -1418,16 +1476,18 @@ cudaError_t launch_type(const LaunchEnv& env, int type, const TreeParams& p) {
   return type == RRR_F16 ? launch<HD, 64, __half>(env, p) : launch<HD, 64, __nv_bfloat16>(env, p);
 }
 
-// The workspace: segments opened, statistics, flags, parts; for the widest tiles
+// The workspace: segments opened, statistics, flags, sums moved out, parts; for the widest tiles
 struct Layout {
-  int64_t stats, again, parts, bytes;
+  int64_t stats, again, held_stats, held, parts, bytes;
 };
 Layout layout_of(const rrr_kv4_cache* c, int sms) {
   const int64_t slots = 2 * (int64_t)sms;
   Layout l;
   l.stats = ((int64_t)sms * (int64_t)sizeof(Opened) + 255) / 256 * 256;
   l.again = l.stats + slots * 96 * 8;
-  l.parts = l.again + (slots * 4 * kGroups + 255) / 256 * 256;
+  l.held_stats = l.again + (slots * 4 * kGroups + 255) / 256 * 256;
+  l.held = l.held_stats + (int64_t)sms * 4 * 96 * 8;
+  l.parts = l.held + (int64_t)sms * 96 * c->head_dim * 4;
   l.bytes = l.parts + slots * 96 * c->head_dim * 4;
   return l;
 }
@@ -1541,6 +1601,8 @@ int rrr_attention_tree_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, const rrr_tree_
   p.stats = reinterpret_cast<float2*>(w + l.stats);
   p.again = reinterpret_cast<int*>(w + l.again);
   p.parts = reinterpret_cast<float*>(w + l.parts);
+  p.held_stats = reinterpret_cast<float2*>(w + l.held_stats);
+  p.held = reinterpret_cast<float*>(w + l.held);
   cudaError_t e;
   switch (hd) {
     case 64: e = launch_type<64>(env, d->type, p); break;

@@ -1,5 +1,5 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
-sequence without any row that exists, rows that are computed again, drafted values of
+sequence without any row that exists, rows that are computed again, very many rows, drafted values of
 very different sizes, tokens that both distributions mask.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
@@ -148,6 +148,65 @@ def test_attention_tree_groups_beyond_f16_among_short_sequences(rrr, ctx, hd, nh
     some = [s for s in range(seqs) if s % 4 == 0 or s < 40]
     r = [nodes * s + i for s in some for i in range(nodes)]
     compare_tree(out[r], q[r], kd[r], vd[r], k, v, [lens[s] for s in some], [[-1, 0]] * len(some), "bf16", hd ** -0.5)
+    assert ctx.device_error() == 0
+
+
+def shared_rows(rrr, ctx, hd, seqs, k, v):
+    """One sequence's rows as those of `seqs`: their cache, and what it holds of k and v."""
+    n = len(k)
+    one = Cache(rrr, ctx, 1, hd, [n], 3)
+    one.c.store(k, v, cu_of([n]), ints([n]))
+    k, v = torch.empty_like(k), torch.empty_like(v)
+    one.c.load(cu_of([n]), ints([n]), k, v)
+    return rrr.KV4Cache(ctx, one.pages, one.c.page_table.expand(seqs, -1).contiguous(), hd), k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh", [(64, 8), (64, 2), (128, 2), (256, 3)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_tree_sums_of_many_rows_by_one_cta(rrr, ctx, hd, nh, kind):
+    """300,000 rows of one CTA's, equal weights, values of one sign in few bits: no rounding but the result's, those of sums of
+    at most 128 blocks (16 cut off a block, 2 u each, in O and in the weights' sum) and of 24 such sums in 32 bits."""
+    t, n, g, nodes = DT[kind], 300000, gen(hd), 2
+    seqs = torch.cuda.get_device_properties(0).multi_processor_count
+    v = (1 + (torch.arange(n, device="cuda") % 13).float() / 16)[:, None, None].expand(n, 1, hd).contiguous()
+    cache, k, v = shared_rows(rrr, ctx, hd, seqs, torch.zeros(n, 1, hd, device="cuda"), v)
+    rows = seqs * nodes
+    q = normal(g, rows, nh, hd, dtype=t)
+    kd, vd = torch.zeros(rows, 1, hd, dtype=t, device="cuda"), torch.ones(rows, 1, hd, dtype=t, device="cuda")
+    out = torch.empty(rows, nh, hd, dtype=t, device="cuda")
+    cache.attention_tree(q, kd, vd, cu_of([nodes] * seqs), None, ints([n] * seqs), out, cache.tree_workspace(nh, rows))
+    total = v[:, 0, 0].double().sum()
+    for i in range(nodes):
+        ref = ((total + i + 1) / (n + i + 1)).expand(seqs, nh, hd)
+        within(out[i::nodes], ref, ref * (half_step(t) * 1.01 + (128 * 16 * 2 + 2 * 24 + 16) * U))
+    assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh", [(64, 8), (128, 3), (256, 2)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("more", [0, 5])
+@pytest.mark.parametrize("rise", [0.25, 2.0, -0.25])
+def test_attention_tree_maxima_that_grow_between_sums(rrr, ctx, hd, nh, kind, more, rise):
+    """Scores that rise (or fall) over 40,000 rows of one CTA's, or of two that share them: what was summed before counts by
+    the maximum that it was summed under. Keys in few bits, so that scores carry the sums' error alone."""
+    t, n, g, nodes = DT[kind], 40000, gen(hd), 3
+    seqs = torch.cuda.get_device_properties(0).multi_processor_count + more
+    k = rise * (torch.arange(n, device="cuda") // 512).float()[:, None, None].expand(n, 1, hd)
+    cache, k, v = shared_rows(rrr, ctx, hd, seqs, k.contiguous(), normal(g, n, 1, hd))
+    rows = seqs * nodes
+    q = torch.full((rows, nh, hd), 1.0 / hd, dtype=t, device="cuda")
+    kd, vd = torch.zeros(rows, 1, hd, dtype=t, device="cuda"), normal(g, rows, 1, hd, dtype=t)
+    out = torch.empty(rows, nh, hd, dtype=t, device="cuda")
+    cache.attention_tree(q, kd, vd, cu_of([nodes] * seqs), None, ints([n] * seqs), out, cache.tree_workspace(nh, rows), scale=1.0)
+    h = half_step(t)
+    for s in (0, 1, seqs // 2, seqs - 2, seqs - 1):
+        r = slice(nodes * s, nodes * (s + 1))
+        ref, A, _ = ref_tree(q[r].double(), kd[r].double(), vd[r].double(), k.double(), v.double(), [-1, 0, 1], 1.0)
+        top = float(max(v.abs().max(), vd[r].abs().max()))
+        bound = (2 * torch.expm1(2 * (hd + 16) * U * A) + 2 * H16 + h + (128 * 16 * 2 + 2 * 3 + 16) * U) * top
+        within(out[r], ref, ref.abs() * h * 1.01 + bound[..., None] + 2.0 ** -25)
     assert ctx.device_error() == 0
 
 
