@@ -6,7 +6,7 @@
 // rotated K is quantised from its 32-bit value, without the rounding to a 16-bit row between. A
 // code changes by a whole step where a value crosses a border, so that groups which 32 bits do not
 // decide (the step, the minimum or a code within the arithmetic's error of a rounding border: about
-// one group in a hundred) are normed and rotated again in 64 bits, as all others then would be too.
+// one group in a hundred; and all groups of a head whose squares leave the range of 32 bits) are normed and rotated again in 64 bits, as all others then would be too.
 //
 // A CTA takes up to eight rows of one sequence that lie in eight aligned rows of a page (two rows
 // whose V codes share words are then one warp's), and a share of the heads. The rows' sines and
@@ -231,14 +231,15 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 3) kv4_append_kernel(const 
       float x[8];
 #pragma unroll
       for (int d = 0; d < 8; ++d) x[d] = to_f32(now.v[d]);
-      float inv = 1.f;
+      float inv = 1.f, ground = 1.f;
       if (normed) {
         float sq = 0.f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) sq = fmaf(x[d], x[d], sq);
 #pragma unroll
         for (int m = 1; m < kLanes; m <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
-        inv = rsqrtf(fmaf(sq, 1.f / HD, p.eps));
+        ground = fmaf(sq, 1.f / HD, p.eps);
+        inv = rsqrtf(ground);
 #pragma unroll
         for (int d = 0; d < 8; ++d) x[d] = (gamma[d] * x[d]) * inv;
       }
@@ -288,6 +289,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 3) kv4_append_kernel(const 
       __half d16, m16;
       bool unsure;
       uint32_t w = quantise<true>(x, d16, m16, off * largest, &unsure);
+      // (and where 32 bits do not hold the squares or the largest values at all)
+      unsure = unsure || !(ground > 7.9e-31f && ground < 1e38f) || !(off * largest < 1e30f);
       if (__any_sync(0xffffffffu, unsure)) {
         rotated_in_64_bits<HD>(p, src - e0 + (int64_t)(p.nh + h) * HD, turn64[rr], e0, x);
         w = quantise(x, d16, m16);

@@ -1,14 +1,15 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
 sequence without any row that exists, rows that are computed again, very many rows, drafted values of
-very different sizes, tokens that both distributions mask.
+very different sizes, tokens that both distributions mask, norms beyond 32 bits' range.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from test_serving import DT, U, Cache, cu_of, gen, half_step, ints, normal, within
+from test_serving import DT, U, Cache, cu_of, gen, half_step, ints, normal, ref_qk, within
 from test_speculative import H16, ancestors, check_verify, compare_tree, ref_tree
 
 
@@ -251,3 +252,25 @@ def test_verify_drafts_of_faint_tokens(rrr, ctx):
     got = check_verify(rrr, ctx, x, y, ints([0, 5000]), u, [[-1, 0]], [1.0])
     assert got[2] == [1200]
     assert check_verify(rrr, ctx, x, None, ints([0, 5]), u, [[-1, 0]], [1.0])[2] == [1200]
+
+
+# ------------------------------------------------------------------ append
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,nh,nkv,rd,halves", [(128, 4, 2, 96, False), (128, 4, 2, 96, True), (64, 2, 2, 36, True), (256, 2, 1, 128, False)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("eps", [0.0, 1e-5])
+def test_kv4_append_norms_beyond_32_bits(rrr, ctx, hd, nh, nkv, rd, halves, kind, eps):
+    """Squares that 32 bits do not hold, on either side: the pages are still those of the norm in 64 bits."""
+    g, n, t = gen(hd), 12, DT[kind]
+    qkv = normal(g, n, (nh + 2 * nkv) * hd)
+    sizes = torch.tensor([1.0, 1e20, 1e-25, 3e18, 1e-19, 1e37, 1e-30, 1.0, 1e-22, 1e19, 1e30, 1e-37], device="cuda")
+    qkv[:, nh * hd:(nh + nkv) * hd] *= sizes[:, None]
+    qkv = qkv.to(t)
+    gammas = [torch.rand(hd, device="cuda", generator=g) + 0.5 for _ in range(2)]
+    desc = rrr.ffi.AttnDesc(nh, nkv, hd, rd, 10000.0, 1.25, None, 0, 100)
+    want, got = (Cache(rrr, ctx, nkv, hd, [n], 3) for _ in range(2))
+    refs, _ = ref_qk(qkv, ints(range(n)), nh, nkv, hd, rd, 10000.0, 1.25, None, gammas, float(np.float32(eps)), halves)
+    want.c.store(refs[1].float().contiguous(), refs[2].float().contiguous(), cu_of([n]), ints([n]))
+    got.c.append(desc, qkv, cu_of([n]), ints([n]), q_gamma=gammas[0], k_gamma=gammas[1], eps=eps, halves=halves)
+    assert torch.equal(got.pages, want.pages)
+    assert ctx.device_error() == 0
