@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 4; ++i) mbar_init(&lifted[i], 1);
     mbar_init(&fin, 2);
     fence_mbarrier_init();
-    prefetch_map(&map);
+    if (p.n_pages > 0) prefetch_map(&map);  // (there is none without pages)
   }
   if (threadIdx.x < kBits / 32) again[threadIdx.x] = 0;
   if (warp == kSWarp) tmem_alloc(&tmem_slot, 512);

@@ -1,5 +1,5 @@
 """What random values of one size do not show of the speculative decoding step's operators (test_speculative.py): parts of a
-sequence without any row that exists, rows that are computed again, very many rows, drafted values of
+sequence without any row that exists, no pages at all, rows that are computed again, very many rows, drafted values of
 very different sizes, tokens that both distributions mask, norms beyond 32 bits' range.
 
 Bounds are those of test_speculative.py, with the roundings that a test's exact values do not make left out."""
@@ -150,6 +150,23 @@ def test_attention_tree_groups_beyond_f16_among_short_sequences(rrr, ctx, hd, nh
     r = [nodes * s + i for s in some for i in range(nodes)]
     compare_tree(out[r], q[r], kd[r], vd[r], k, v, [lens[s] for s in some], [[-1, 0]] * len(some), "bf16", hd ** -0.5)
     assert ctx.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,kind", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("width", [0, 2])
+def test_attention_tree_without_pages(rrr, ctx, hd, kind, width):
+    """A cache that has no page at all: drafted rows see one another; lengths beside 0 are recorded."""
+    t, g, nodes = DT[kind], gen(hd), [3, 0, 5]
+    cache = rrr.KV4Cache(ctx, torch.empty(rrr.KV4Cache.page_shape(0, 1, hd), dtype=torch.uint8, device="cuda"),
+                         torch.zeros(3, width, dtype=torch.int32, device="cuda"), hd)
+    q, k, v = (normal(g, 8, n, hd, dtype=t) for n in (2, 1, 1))
+    none = torch.empty(0, 1, hd, device="cuda")
+    for lens in ([0, 0, 0], [0, 0, 70]):
+        out = torch.empty(8, 2, hd, dtype=t, device="cuda")
+        cache.attention_tree(q, k, v, cu_of(nodes), ints([-1, 0, 0, -1, 0, 1, 1, 3]), ints(lens), out, cache.tree_workspace(2, 8))
+        assert ctx.device_error() == (6 if sum(lens) else 0)
+        compare_tree(out, q, k, v, none, none, [0, 0, 0], [[-1, 0, 0], [], [-1, 0, 1, 1, 3]], kind, hd ** -0.5)
 
 
 def shared_rows(rrr, ctx, hd, seqs, k, v):
