@@ -375,7 +375,8 @@ __device__ __noinline__ void plain_row(const TreeParams& p, int seq, int r0, int
 
 // What is done once in a segment is kept small: its instructions come from far away each time, which took longer than
 // what they do. So rows are copied as they are to the places of what is made of them, all at once, and each thread then
-// goes through its own 16 bytes in a loop.
+// goes through its own 16 bytes in a loop. In place and not as calls, which read the parameters from memory: 64 sequences
+// of 16 rows took 275 us with calls, 245 so.
 
 // Eight 16-bit values at p, of a row that HD / 8 neighbouring lanes hold, to f16 in the order of K's words, the row brought
 // to [1, 2) by a power of two, which is returned
@@ -394,7 +395,7 @@ __device__ __forceinline__ float row_to_one(uint8_t* p) {
 // The tile's queries into shared memory, in the order of K's words: HD / 8 lanes per row, 8 values each; a row is
 // brought to [1, 2) by a power of two, which its line takes back.
 template <int HD, int NT, typename T>
-__device__ __noinline__ void queries(const TreeParams& p, const Info& f, int r, uint8_t* qs, float* line) {
+__device__ __forceinline__ void queries(const TreeParams& p, const Info& f, int r, uint8_t* qs, float* line) {
   constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes;
   const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J;  // the place among the words of a row of codes
   uint8_t* const to = qs + (w / 8) * NT * 128;
@@ -418,7 +419,7 @@ __device__ __noinline__ void queries(const TreeParams& p, const Info& f, int r, 
 // Up to 64 drafted keys from row `first` on: HD / 8 lanes per row, 8 values each; a row is brought to [1, 2) by a power of two.
 // They go to shared memory, from where their threads take them to TMEM.
 template <int HD, typename T>
-__device__ __noinline__ void drafted_keys(const TreeParams& p, const Info& f, int r, int first, uint8_t* to, float* scales) {
+__device__ __forceinline__ void drafted_keys(const TreeParams& p, const Info& f, int r, int first, uint8_t* to, float* scales) {
   constexpr int J = HD < 128 ? HD / 32 : 4, kLanes = HD / 8, kAcross = 128 / kLanes;
   const int x = r % kLanes, j = x / 4, w = (j / J) * 4 * J + (x % 4) * J + j % J, rows = min(f.nodes - first, 64);
   const T* src = static_cast<const T*>(p.k) + (int64_t)(f.r0 + first) * p.k_row + f.kv * p.k_head + 8 * x;
@@ -442,7 +443,7 @@ __device__ __forceinline__ uint8_t* value_place(uint8_t* dst, int o, int e) {
   return dst + ((e >> 7) * 2 + (o >> 3)) * kERows * 128 + (e & 127) * 128 + (((o & 7) ^ (e & 7)) << 4);
 }
 template <int HD, typename T>
-__device__ __noinline__ void drafted_rows(const TreeParams& p, const Info& f, int tid, uint8_t* dst) {
+__device__ __forceinline__ void drafted_rows(const TreeParams& p, const Info& f, int tid, uint8_t* dst) {
   const int o = tid & 15, e0 = 8 * (tid >> 4);
   const T* src = static_cast<const T*>(p.v) + f.kv * p.v_head + (int64_t)f.r0 * p.v_row + e0;
 #pragma unroll 1
@@ -454,7 +455,7 @@ __device__ __noinline__ void drafted_rows(const TreeParams& p, const Info& f, in
   cp_async_wait<0>();
 }
 template <int HD, typename T>
-__device__ __noinline__ uint32_t row_top(int tid, uint8_t* dst) {
+__device__ __forceinline__ uint32_t row_top(int tid, uint8_t* dst) {
   uint32_t top = 0;
 #pragma unroll 1
   for (int e = tid & 7; e < HD; e += 8) top = max(top, top_bits<T>(*reinterpret_cast<const uint4*>(value_place<HD>(dst, tid >> 3, e))));
@@ -462,7 +463,7 @@ __device__ __noinline__ uint32_t row_top(int tid, uint8_t* dst) {
 }
 // The values of the rows there, lifted
 template <int HD, typename T>
-__device__ __noinline__ void drafted_values(int tid, float lift, uint8_t* dst) {
+__device__ __forceinline__ void drafted_values(int tid, float lift, uint8_t* dst) {
   const int o = tid & 15;
 #pragma unroll 1
   for (int c = 0; c < HD / 64; ++c) {
@@ -470,15 +471,20 @@ __device__ __noinline__ void drafted_values(int tid, float lift, uint8_t* dst) {
     uint4 w[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) w[r] = *reinterpret_cast<const uint4*>(value_place<HD>(dst, o, e0 + r));
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t y[4];
+    // two values of the eight rows at a time, the rows' next words in front then
+#pragma unroll 1
+    for (int k = 0; k < 8; k += 2) {
+      uint32_t y[4], z[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float2 a = pair_of<T>((&w[2 * r].x)[k / 2]), b = pair_of<T>((&w[2 * r + 1].x)[k / 2]);
-        y[r] = as_u32(__floats2half2_rn((k & 1 ? a.y : a.x) * lift, (k & 1 ? b.y : b.x) * lift));
+        const float2 a = pair_of<T>(w[2 * r].x), b = pair_of<T>(w[2 * r + 1].x);
+        y[r] = as_u32(__floats2half2_rn(a.x * lift, b.x * lift));
+        z[r] = as_u32(__floats2half2_rn(a.y * lift, b.y * lift));
       }
       *reinterpret_cast<uint4*>(value_place<HD>(dst, o, e0 + k)) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(value_place<HD>(dst, o, e0 + k + 1)) = make_uint4(z[0], z[1], z[2], z[3]);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) w[r] = make_uint4(w[r].y, w[r].z, w[r].w, 0u);
     }
   }
 }
@@ -1470,6 +1476,10 @@ cudaError_t launch(const LaunchEnv& env, const TreeParams& p) {
 }
 template <int HD>
 cudaError_t launch_type(const LaunchEnv& env, int type, const TreeParams& p) {
+  // Tiles of 96 columns where a sequence's (row, query head) pairs do not fit one of 64 on average, since every tile reads
+  // the pages: 32 sequences of 24 rows on up to 4,000, 24 heads on 8 of 128, 109 us (of 64: 164), one of 60 rows on 60,000
+  // 116 (145), 24 of 12 rows, 64 heads on 8 of 64, 87 (119); and where they do fit the smaller tile, whose scores
+  // and sums are fewer: 32 of 16 rows 92 (of 96: 98), 32 of 8 rows of 32 heads, f16, 107 (118). Heads of 256 leave no room in TMEM.
   if constexpr (HD < 256)
     if ((int64_t)p.rows * p.hpk > 64 * (int64_t)p.n_seqs)
       return type == RRR_F16 ? launch<HD, 96, __half>(env, p) : launch<HD, 96, __nv_bfloat16>(env, p);
