@@ -523,7 +523,8 @@ int rrr_attention_tree_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, const rrr_tree_
 
 /* Which drafted rows stand, and the token that follows them. logits: row r is the target's behind
  * row r's token; temperature f32[n_seqs] (NULL: 1); p = softmax(logits / temperature). uniforms
- * f32[rows][2] in [0, 1): an acceptance and a draw for every row. A token is drawn from p as the first
+ * f32[rows][2] in [0, 1): an acceptance and a draw for every row (less, and NaN, counts as 0; a draw
+ * by more is one of the last token). A token is drawn from p as the first
  * i with p_0 + .. + p_i > u; at temperature 0 it is the largest logit's, the first of equals. NaN
  * counts as -inf and +inf as the largest finite value; a row without any value draws -1.
  * draft NULL: from row 0 on, a token is drawn at the row; where a child carries it (the first such

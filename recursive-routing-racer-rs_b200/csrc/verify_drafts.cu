@@ -108,6 +108,11 @@ __device__ __forceinline__ void fill_table(double* table) {
   if (threadIdx.x < 16) table[threadIdx.x] = exp2(threadIdx.x * 0.0625);
   __syncthreads();
 }
+// The number that a row's draft stands by (0) or its token is drawn by (1); none that is negative, and 0 for NaN (draw() takes
+// a negative one for none, and a draft without a chance would stand by it)
+__device__ __forceinline__ double number_of(const VerifyParams& p, int64_t row, int which) {
+  return fmax((double)p.uniforms[2 * row + which], 0.);
+}
 // log2(e) / T; 0 for temperature 0 (and, recorded, for one that is none)
 __device__ __forceinline__ double sharpness(const VerifyParams& p, int seq) {
   const float t = p.temperature ? p.temperature[seq] : 1.f;
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_tokens_kernel(const __gri
     if (threadIdx.x == 0) p.drawn[row] = -1;
     return;
   }
-  const int token = draw_token<T>(sh, p, row, sharpness(p, seq), (double)p.uniforms[2 * (int64_t)row + 1]);
+  const int token = draw_token<T>(sh, p, row, sharpness(p, seq), number_of(p, row, 1));
   if (threadIdx.x == 0) p.drawn[row] = token;
 }
 __global__ void __launch_bounds__(kWalkThreads) verify_walk_kernel(const __grid_constant__ VerifyParams p) {
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
       } else {
         const double pp = share(to_f32(static_cast<const T*>(p.logits)[(row - 1) * p.logits_stride + x]), pm, pz, c);
         const double q = share(to_f32(static_cast<const T*>(p.draft)[row * p.draft_stride + x]), qm, qz, c);
-        stands = (double)p.uniforms[2 * row] * q < pp;
+        stands = number_of(p, row, 0) * q < pp;
       }
       if (!stands && lane == 0) atomicMin(&refused, i);
     }
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_
   if (!rows_of(p, seq, r0, n)) n = 0;
   if (n > 0) {
     const Ending e = p.endings[seq];
-    const double c = sharpness(p, seq), u = (double)p.uniforms[2 * (int64_t)(r0 + e.last) + 1];
+    const double c = sharpness(p, seq), u = number_of(p, r0 + e.last, 1);
     if (e.refused) {
       const double* rest = p.rest + (int64_t)seq * p.rest_chunks;
       double goal, before;

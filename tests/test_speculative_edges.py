@@ -271,6 +271,30 @@ def test_verify_drafts_of_faint_tokens(rrr, ctx):
     assert check_verify(rrr, ctx, x, None, ints([0, 5]), u, [[-1, 0]], [1.0])[2] == [1200]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_verify_drafts_of_numbers_outside_their_range(rrr, ctx, kind):
+    """Numbers that no generator gives draw as the ends of the range do."""
+    g, vocab = gen(2), 5000
+    logits, draft = normal(g, 3, vocab).to(DT[kind]), normal(g, 3, vocab).to(DT[kind])
+    logits[:, ::3] = -math.inf
+    tokens = ints([0, 3, 6])  # (tokens without a chance: the first draft is refused)
+    i = dict(dtype=torch.int32, device="cuda")
+
+    def run(number, draft):
+        u = torch.full((3, 2), number, device="cuda")
+        path, counts, following = torch.zeros(3, **i), torch.zeros(1, **i), torch.zeros(1, **i)
+        ws = rrr.verify_workspace(ctx, 3, vocab, 1, draft is not None)
+        ws.fill_(0x7B)
+        rrr.verify_drafts(ctx, logits, tokens, cu_of([3]), u, path, counts, following, ws, draft=draft)
+        return path.tolist(), counts.tolist(), following.tolist()
+    for y in (None, draft):
+        first, last = run(0.0, y), run(1 - 2.0 ** -24, y)
+        assert all(run(x, y) == first for x in (-1e-3, -5.0, -math.inf, math.nan))
+        assert all(run(x, y)[:2] == last[:2] and run(x, y)[2][0] >= last[2][0] and run(x, y)[2][0] % 3 for x in (1.0, 7.0, math.inf))
+    assert ctx.device_error() == 0
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd,nh,nkv,rd,halves", [(128, 4, 2, 96, False), (128, 4, 2, 96, True), (64, 2, 2, 36, True), (256, 2, 1, 128, False)])
