@@ -481,14 +481,15 @@ int rrr_attention_packed(rrr_ctx* ctx, const rrr_packed_desc* d, const void* q, 
  * in one step. A sequence's packed rows are a tree: row 0 its last token, whose K and V are not
  * cached yet, each other row a drafted token whose parent, parents[cu[s] + i] < i (a row of the
  * sequence, -1 at row 0), is the token before it; parents NULL: chains, parent i - 1. The step:
- * QKV rows (rrr_qk_norm_rope for each row's own position, kv_lens[s] + depth), per layer
- * rrr_attention_tree_kv4; from the logits rrr_verify_drafts says which rows stand; per layer
- * rrr_kv4_append of those. Lengths, trees and results stay on the device. */
+ * QKV rows (rrr_qk_norm_rope for each row's own position, kv_lens[s] + depth, which the caller
+ * makes from parents with the tree), per layer rrr_attention_tree_kv4; from the logits
+ * rrr_verify_drafts says which rows stand; per layer rrr_kv4_append of those. Lengths, trees and
+ * results stay on the device. */
 
 /* Appends QKV rows [Q heads | K heads | V heads] to the cache, in one pass: K heads normed and
  * rotated as by rrr_qk_norm_rope (its a, gammas, eps and halves), V heads as they are, quantised as by
- * rrr_kv4_store: K's codes are those of the norm and rotation in 64 bits, rounded to 32. Sequence s has kv_lens[s] rows afterwards, and its packed
- * rows are its last ones. q not NULL: its rows get the query heads, normed and rotated, in out_type.
+ * rrr_kv4_store: K's codes are those of the norm and rotation in 64 bits, rounded to 32. Sequence s
+ * has kv_lens[s] rows afterwards, and its packed rows are its last ones. q not NULL: its rows get the query heads, normed and rotated, in out_type.
  * path and counts not NULL (then q is NULL): of sequence s the counts[s] rows path[cu[s]],
  * path[cu[s] + 1], .. (rows of the sequence) are appended in this order, no others: the accepted
  * rows of rrr_verify_drafts. A row is rotated for positions[row], or, with positions NULL, for its
@@ -504,7 +505,11 @@ int rrr_kv4_append(rrr_ctx* ctx, const rrr_attn_desc* a, const rrr_kv4_cache* c,
  * at most 8 query heads per KV head. q, k and v are the rows' own, normed and rotated; 16-bit
  * types; scale 0 = 1/sqrt(head_dim). At most 128 rows of a sequence: one with more is left as it was
  * (and recorded). A kv_lens out of range counts as 0, rows on pages that do not exist are left out, and
- * a parent that does not lie before its row is none. Scores and softmax statistics in 32 bits.
+ * a parent that does not lie before its row is none. Scores and softmax statistics in 32 bits, sums
+ * too: those of up to 16,384 rows by the tensor core, which cuts off below the last bit. What they are
+ * of: queries and drafted rows as given; cached values and the weights rounded to f16; cached keys
+ * rounded to f16 with bf16 rows; with f16 rows keys and weights are sums of two f16. A result that is
+ * not finite, or that f16 operands do not give, is computed in 32 bits, a row at a time.
  * Pointers 16-byte aligned, strides multiples of 8 elements; out overlaps no input. workspace:
  * rrr_tree_workspace bytes for this cache and rows (or more of either), whatever they hold; calls that can
  * run at the same time, replays of captured graphs among them, need one each. */
@@ -538,8 +543,9 @@ int rrr_attention_tree_kv4(rrr_ctx* ctx, const rrr_kv4_cache* c, const rrr_tree_
  * path int32[rows]: of each sequence the rows that stand in their order, row 0 first, then -1;
  * counts int32[n_seqs]: how many stand (0 without rows); next_tokens int32[n_seqs]: the token drawn
  * last (-1 without rows). A token outside 0 .. vocab - 1 does not stand. Exponentials and sums are
- * held in 64 bits. A temperature that is negative, infinite or NaN counts as 0. logits and draft: rows of `type`, aligned to
- * their elements. workspace: rrr_verify_workspace bytes, 16-byte aligned, as for rrr_attention_tree_kv4. */
+ * held in 64 bits. A temperature that is negative, infinite or NaN counts as 0 (and is recorded).
+ * logits and draft: rows of `type`, aligned to their elements. workspace: rrr_verify_workspace bytes,
+ * 16-byte aligned, as for rrr_attention_tree_kv4. */
 int rrr_verify_workspace(rrr_ctx* ctx, int rows, int vocab, int n_seqs, int with_draft, int64_t* bytes);
 int rrr_verify_drafts(rrr_ctx* ctx, int type, const void* logits, int64_t logits_stride,
                       const void* draft, int64_t draft_stride, int rows, int vocab, int n_seqs,

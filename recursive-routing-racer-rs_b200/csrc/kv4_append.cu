@@ -6,7 +6,8 @@
 // rotated K is quantised from its 32-bit value, without the rounding to a 16-bit row between. A
 // code changes by a whole step where a value crosses a border, so that groups which 32 bits do not
 // decide (the step, the minimum or a code within the arithmetic's error of a rounding border: about
-// one group in a hundred; and all groups of a head whose squares leave the range of 32 bits) are normed and rotated again in 64 bits, as all others then would be too.
+// one group in a hundred; and all groups of a head whose squares leave the range of 32 bits) are normed
+// and rotated again in 64 bits, as all others then would be too.
 //
 // A CTA takes up to eight rows of one sequence that lie in eight aligned rows of a page (two rows
 // whose V codes share words are then one warp's), and a share of the heads. The rows' sines and
@@ -15,9 +16,9 @@
 // 32j + 8t .. + 7 of a row, which are one word of K's codes. Partners that lie half a rotation away
 // come by shuffles.
 //
-// What bounds it. Instructions: 5,949 rows of 48 heads of 128, bf16 with norms, 65 us (151 MB, 23 us at the copy's rate),
-// 260 instructions for eight values of 32 lanes on average, of which K and V take four fifths; 64 single rows 10 us,
-// five dependent trips to memory. The 64-bit rotation takes 9 us of the 65; with sines computed again for each group it took
+// What bounds it. Instructions: 5,949 rows of 48 heads of 128, bf16 with norms, 60 us (151 MB, 23 us at the copy's rate),
+// 260 instructions for eight values of 32 lanes on average, of which K and V take four fifths; 64 single rows 7.2 us,
+// five dependent trips to memory. The 64-bit rotation takes 9 us of the 60; with sines computed again for each group it took
 // 45.
 #include "kv4.cuh"
 

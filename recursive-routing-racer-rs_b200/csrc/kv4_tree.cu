@@ -19,10 +19,16 @@
 //
 // What bounds it. Not memory (1.3 TB/s) nor the tensor cores, but the roles' instructions and hand-overs: a warp gets one in
 // about ten cycles, a block of 48 columns takes 3,400 cycles and of 96 3,600. Measured on 24 heads over 8 of 128: 64
-// sequences of 16 rows on up to 8,190: 245 us (floor 54 by bytes); 60 rows on 131,000: 222 us (57 by operations). With
-// dequantisation, weights and products left out (before the last two steps) 207 and 125 us remained. Steps, for the 64
-// sequences: scalar products 14.8 ms, tensor cores 690 us, rolled loops 464 (the instruction cache), scores ahead of the
+// sequences of 16 rows on up to 8,190: 245 us (floor 54 by bytes); 60 rows on 131,000: 217-228 us (57 by operations). With
+// dequantisation, weights and products left out (at 322 us for the 64 sequences) 207 and 125 us remained. Steps, for
+// the 64 sequences: scalar products 14.8 ms, tensor cores 690 us, rolled loops 464 (the instruction cache), scores ahead of the
 // weighted sums 333, two issuing warps and sixteen softmax warps 322, small code for what a segment does once 245.
+//
+// What f16 operands round. Queries and drafted keys nothing that their type has, by their scales, nor drafted values (but for
+// rows 2^21 and more below the largest, which are computed again). Cached keys and values d c + m, up to 15 bits and more,
+// and weights to 11 bits each: beside a bf16 result's own rounding that is little: 1.69e-3 to 1.71e-3 against 64
+// bits, 1.65e-3 to 1.66e-3 of it the rounding. Not so for f16 rows, where keys and weights are two f16 each: 2.4e-4 against
+// 2.1e-4; with one each it was 4.3e-4 on 3,000 rows (and 24 trees of up to 33 rows took 108 us against 121).
 #include <math.h>
 
 #include <type_traits>

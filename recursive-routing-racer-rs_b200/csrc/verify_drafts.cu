@@ -21,12 +21,14 @@
 // A row is cut into chunks of 4 KB at 16-byte borders of memory. First kernel: per chunk the
 // maximum, its first place and the sum of the exponentials under it, one warp each. Trees: a second
 // kernel, one CTA per row, draws the row's token: its chunk from the chunks' sums, then the token
-// inside it; a third, one CTA per sequence, walks. Chains with the draft's logits: one CTA per sequence compares, then the chunks of the
-// row where the chain ends are summed as max(p - q, 0), and one CTA per sequence draws.
+// inside it; a third, one CTA per sequence, walks. Chains with the draft's logits: one CTA per sequence
+// compares, then the chunks of the row where the chain ends are summed as max(p - q, 0), and one CTA
+// per sequence draws.
 //
-// What bounds it. The 64-bit pipe: eleven operations and one conversion a value, at two cycles a warp each. 48 chains of 5
-// rows and their drafts on 200,064 tokens, f32: 148 us (346 MB, 53 us), of which the first kernel takes 110; 285
-// rows of trees, bf16: 65 us (114 MB, 17 us), 55 of them. CUDA's exp2 took 302 and 327 us.
+// What bounds it. Issue slots (70 % used) and latencies of the first kernel: 30 warp instructions for 32 values, of which
+// eleven operations and a conversion go to the 64-bit pipe, half busy. 48 chains of 5 rows and their drafts on 200,064
+// tokens, f32: 147 us (346 MB, 53 us), of which the first kernel takes 110, of greedy ones 70; 285 rows of trees, bf16:
+// 72 us (114 MB, 17 us), 60 of them, greedy 31. CUDA's exp2 took 302 and 327 us.
 #include <float.h>
 
 #include "serve_common.cuh"
