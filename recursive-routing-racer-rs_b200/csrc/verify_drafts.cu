@@ -482,6 +482,9 @@ __global__ void __launch_bounds__(kWalkThreads) verify_chain_kernel(const __grid
 // max(p - q, 0) of tokens where a chain ends, from their logits. The sums of chunks and the draw inside one are of the same
 // terms, so that a chunk with a sum has a term to be drawn. power() gives values 1000 binary orders under the top, masked ones
 // too, 2^-1000: beside a p of 2^-940 and more that is no q, and a smaller p is taken as it is, 0 where it is masked.
+// Where the weights under p's and q's maxima are all equal, p and q are, and no rest is left, though their sums may be a rounding
+// apart (rows that begin at other places of 16 bytes are summed in another order). A chunk of such weights alone has its sum with
+// a minus.
 struct Rest {
   Powers wp, wq;
   double sp, sq;
@@ -503,10 +506,17 @@ __device__ __forceinline__ Rest rest_from(const Ending& e, double c) {
 __device__ __noinline__ double rest_apart(float x, float y, const Ending& e, double c) {
   return fmax(share(x, e.pm, e.pz, c) - share(y, e.qm, e.qz, c), 0.);
 }
-// (with r.fast; the products rounded each by itself, so that of equal ones nothing is left)
-__device__ __forceinline__ double rest_of(const Rest& r, const double* table, float x, float y, const Ending& e, double c) {
-  const double d = fmax(__dmul_rn(power(r.wp, table, x), r.sp) - __dmul_rn(power(r.wq, table, y), r.sq), 0.);
-  if (x <= r.faint && x > r.none) return rest_apart(x, y, e, c);
+// (with r.fast; the products rounded each by itself, so that of equal ones nothing is left) differ: bits where weights differ
+__device__ __forceinline__ double rest_of(const Rest& r, const double* table, float x, float y, const Ending& e, double c,
+                                          int& differ) {
+  const double p = power(r.wp, table, x), q = power(r.wq, table, y);
+  differ |= __double2hiint(p) ^ __double2hiint(q);
+  differ |= __double2loint(p) ^ __double2loint(q);
+  const double d = fmax(__dmul_rn(p, r.sp) - __dmul_rn(q, r.sq), 0.);
+  if (x <= r.faint && x > r.none) {
+    differ = 1;
+    return rest_apart(x, y, e, c);
+  }
   return x > r.faint ? d : 0.;
 }
 template <typename T>
@@ -526,6 +536,7 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
   double sum = 0.;
   const int first = chunk * kRestChunk, end = min(p.vocab, first + kRestChunk);
   const Rest rest = rest_from(e, c);
+  int differ = 0;
   if (rest.fast) {
     constexpr int kStep = 8;
 #pragma unroll 1
@@ -538,14 +549,19 @@ __global__ void __launch_bounds__(32 * kStatWarps) verify_rest_kernel(const __gr
         b[k] = i < end ? to_f32(y[i]) : -INFINITY;
       }
 #pragma unroll
-      for (int k = 0; k < kStep; ++k) sum += rest_of(rest, table, a[k], b[k], e, c);
+      for (int k = 0; k < kStep; ++k) sum += rest_of(rest, table, a[k], b[k], e, c, differ);
     }
   } else {
 #pragma unroll 1
-    for (int i = first + lane; i < end; i += 32) sum += rest_apart(to_f32(x[i]), to_f32(y[i]), e, c);
+    for (int i = first + lane; i < end; i += 32) {
+      const float v = tidy(to_f32(x[i])), w = tidy(to_f32(y[i]));
+      differ |= (double)v - (double)e.pm != (double)w - (double)e.qm;
+      sum += rest_apart(v, w, e, c);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (!__any_sync(0xffffffffu, differ)) sum = -sum;
   if (lane == 0) p.rest[(int64_t)seq * p.rest_chunks + chunk] = sum;
 }
 template <typename T>
@@ -564,7 +580,10 @@ __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_
     if (e.refused) {
       const double* rest = p.rest + (int64_t)seq * p.rest_chunks;
       double goal, before;
-      const int chunk = draw(sh, p.rest_chunks, u, goal, 0., [&](int i) { return rest[i]; }, &before);
+      bool differ = false;
+      for (int i = threadIdx.x; i < p.rest_chunks; i += kWalkThreads) differ = differ || !signbit(rest[i]);
+      int chunk = -1;
+      if (__syncthreads_or(differ)) chunk = draw(sh, p.rest_chunks, u, goal, 0., [&](int i) { return fabs(rest[i]); }, &before);
       if (chunk >= 0) {
         const T* x = static_cast<const T*>(p.logits) + (int64_t)(r0 + e.last) * p.logits_stride;
         const T* y = static_cast<const T*>(p.draft) + (int64_t)(r0 + e.last + 1) * p.draft_stride;
@@ -572,7 +591,8 @@ __global__ void __launch_bounds__(kWalkThreads) verify_draw_kernel(const __grid_
         const Rest terms = rest_from(e, c);
         const int got = draw(sh, end - first, -1., goal, before, [&](int i) {
           const float v = to_f32(x[first + i]), w = to_f32(y[first + i]);
-          return terms.fast ? rest_of(terms, table, v, w, e, c) : rest_apart(v, w, e, c);
+          int unused = 0;
+          return terms.fast ? rest_of(terms, table, v, w, e, c, unused) : rest_apart(v, w, e, c);
         }, nullptr);
         if (got >= 0) token = first + got;
       }

@@ -295,6 +295,24 @@ def test_verify_drafts_of_numbers_outside_their_range(rrr, ctx, kind):
     assert ctx.device_error() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [700, 1023, 5001])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_verify_drafts_where_target_and_draft_are_equal(rrr, ctx, vocab, kind):
+    """Equal rows leave no rest, wherever in memory they begin: a draft that cannot stand (no token of the vocabulary, a masked one)
+    is followed by a token of p."""
+    g = gen(vocab)
+    for s in (0.5, 4.0, 20.0):
+        x = s * normal(g, 3, vocab)
+        x[:, 7] = -math.inf
+        x = x.to(DT[kind])
+        for token in (vocab, -1, 7):
+            for u1 in (0.0, 0.129154, 0.5, 0.93, 1 - 2.0 ** -24):
+                u = torch.full((3, 2), u1, device="cuda")
+                for heat in (1.0, 0.6):
+                    check_verify(rrr, ctx, x, x.roll(1, 0), ints([0, token, 3]), u, [[-1, 0, 1]], [heat])
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd,nh,nkv,rd,halves", [(128, 4, 2, 96, False), (128, 4, 2, 96, True), (64, 2, 2, 36, True), (256, 2, 1, 128, False)])
