@@ -28,7 +28,7 @@
 // What bounds it. Issue slots (70 % used) and latencies of the first kernel: 30 warp instructions for 32 values, of which
 // eleven operations and a conversion go to the 64-bit pipe, half busy. 48 chains of 5 rows and their drafts on 200,064
 // tokens, f32: 147 us (346 MB, 53 us), of which the first kernel takes 110, of greedy ones 70; 285 rows of trees, bf16:
-// 72 us (114 MB, 17 us), 60 of them, greedy 31. CUDA's exp2 took 302 and 327 us.
+// 62-72 us (114 MB, 17 us), some 60 of them, greedy 31. CUDA's exp2 took 302 and 327 us.
 #include <float.h>
 
 #include "serve_common.cuh"
