@@ -24,9 +24,9 @@
 // the 64 sequences: scalar products 14.8 ms, tensor cores 690 us, rolled loops 464 (the instruction cache), scores ahead of the
 // weighted sums 333, two issuing warps and sixteen softmax warps 322, small code for what a segment does once 245.
 //
-// What f16 operands round. Queries and drafted keys nothing that their type has, by their scales, nor drafted values (but for
-// rows 2^21 and more below the largest, which are computed again). Cached keys and values d c + m, up to 15 bits and more,
-// and weights to 11 bits each: beside a bf16 result's own rounding that is little: 1.69e-3 to 1.71e-3 against 64
+// What f16 operands round. By their scales queries, drafted keys and drafted values no more than 2^-11 of a row's largest (the
+// rows of values that are too small for that beside others are computed again). Cached keys and values d c + m, up to 15 bits
+// and more, and weights to 11 bits each: beside a bf16 result's own rounding that is little: 1.69e-3 to 1.71e-3 against 64
 // bits, 1.65e-3 to 1.66e-3 of it the rounding. Not so for f16 rows, where keys and weights are two f16 each: 2.4e-4 against
 // 2.1e-4; with one each it was 4.3e-4 on 3,000 rows (and 24 trees of up to 33 rows took 108 us against 121).
 #include <math.h>
@@ -274,11 +274,12 @@ __device__ __forceinline__ float to_one(uint32_t top) {
   const int e = (int)(top >> 23);  // (a subnormal top counts as 2^-126)
   return e == 255 || top == 0 ? 1.f : __uint_as_float((uint32_t)min(max(254 - e, 1), 254) << 23);
 }
-// Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, as far as f16 allows, so that it holds those of rows
-// that are 2^20 times smaller with all their bits too (and their rows' weights are divided by it, which have bits to spare)
+// Drafted values of at most `top` are multiplied by 2^0, 2^8 or 2^15, as far as f16 allows: those of rows that are far
+// smaller (down to 2^-14, 2^-22 or 2^-29) are off by at most 2^-11 of their row's largest then. (And the rows' weights are
+// divided by it, which have bits to spare.)
 __device__ __forceinline__ int lift_of(uint32_t top) { return top >= 0x43000000u /* 2^7 */ ? 0 : top >= 0x3f800000u /* 1 */ ? 1 : 2; }
 __device__ __forceinline__ float lifted_by(int lift) { return lift == 0 ? 1.f : lift == 1 ? 256.f : 32768.f; }
-// Whether a row of values up to `top` loses bits all the same: its largest is no normal f16. (Who sees that row alone, or with
+// Whether a row of values up to `top` loses more all the same: its largest is no normal f16. (Who sees that row alone, or with
 // others like it, is computed again.) An f16 row has no bits to lose.
 template <typename T>
 __device__ __forceinline__ bool too_small(uint32_t top, int lift) {
